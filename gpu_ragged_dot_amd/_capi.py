@@ -72,6 +72,11 @@ class Plan(ctypes.Structure):
                 f"decode_nb={self.decode_nb}, split_k={self.split_k})")
 
 
+class GateSpec(ctypes.Structure):
+    _fields_ = [("top_k", ctypes.c_int), ("clusters", ctypes.c_int), ("top_clusters", ctypes.c_int), ("flags", ctypes.c_int),
+                ("scale", ctypes.c_float)]
+
+
 # every symbol the header declares; checked at load time
 EXPORTS = (
     "rd_abi_version",
@@ -97,6 +102,13 @@ EXPORTS = (
     "rd_moe_dispatch",
     "rd_moe_combine",
     "rd_moe_combine_wgrad",
+    "rd_moe_gate",
+    "rd_moe_gate_grad",
+    "rd_moe_swiglu",
+    "rd_moe_swiglu_grad",
+    "rd_int4_codes_bytes",
+    "rd_int4_pack",
+    "rd_gmm_int4",
 )
 
 
@@ -156,6 +168,20 @@ def _load() -> ctypes.CDLL:
     lib.rd_moe_combine.restype = i
     lib.rd_moe_combine_wgrad.argtypes = [vp, vp, vp, ip, vp, i, i, i, i]
     lib.rd_moe_combine_wgrad.restype = i
+    lib.rd_moe_gate.argtypes = [vp, vp, vp, ip, vp, i, i, ctypes.POINTER(GateSpec), i]
+    lib.rd_moe_gate.restype = i
+    lib.rd_moe_gate_grad.argtypes = [vp, vp, ip, vp, vp, vp, i, i, ctypes.POINTER(GateSpec), i]
+    lib.rd_moe_gate_grad.restype = i
+    lib.rd_moe_swiglu.argtypes = [vp, vp, vp, i, i, i]
+    lib.rd_moe_swiglu.restype = i
+    lib.rd_moe_swiglu_grad.argtypes = [vp, vp, vp, vp, i, i, i]
+    lib.rd_moe_swiglu_grad.restype = i
+    lib.rd_int4_codes_bytes.argtypes = [i, i, i]
+    lib.rd_int4_codes_bytes.restype = sz
+    lib.rd_int4_pack.argtypes = [vp, vp, vp, i, i, i, i]
+    lib.rd_int4_pack.restype = i
+    lib.rd_gmm_int4.argtypes = [vp, vp, vp, vp, vp, ip, vp, i, i, i, i, i, i, i, i, i]
+    lib.rd_gmm_int4.restype = i
     return lib
 
 

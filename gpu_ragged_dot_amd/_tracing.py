@@ -37,7 +37,9 @@ class _Node(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         wanted = [t for t in ctx.operands if t.requires_grad]
-        got = iter(torch.autograd.grad(ctx.results, wanted, grads, retain_graph=True))
+        results = (ctx.results,) if isinstance(ctx.results, torch.Tensor) else ctx.results
+        live = [(t, g) for t, g in zip(results, grads) if t.requires_grad]  # (expert ids have no gradient)
+        got = iter(torch.autograd.grad([t for t, _ in live], wanted, [g for _, g in live], retain_graph=True))
         return (None, *(next(got) if t.requires_grad else None for t in ctx.operands))
 
 

@@ -9,6 +9,7 @@
 #include <cstring>
 
 #include "rd_decode.h"
+#include "rd_int4.h"
 #include "rd_moe.h"
 #include "rd_kernels.h"
 #include "rd_lookup.h"
@@ -1209,6 +1210,106 @@ int rd_moe_combine_wgrad(void* stream, const void* y, const void* dout, const in
   if (!row_of_slot || !dw || (d > 0 && (!y || !dout))) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
   rc = rd::launch_moe_combine_wgrad((hipStream_t)stream, y, dout, row_of_slot, dw, tokens, top_k, d, moe_elem(dtype));
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "moe_combine_wgrad launch");
+}
+
+static int check_gate(const void* logits, const int32_t* ids, const float* weights, int tokens, int experts, const rd_gate_spec* spec,
+                      int dtype, rd::GateSpec* out) {
+  if (!spec) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  const int rc = check_moe(tokens, spec->top_k, 0, dtype);
+  if (rc != RD_OK) return rc;
+  if (experts < 1 || experts > rd::kGateMaxExperts) return fail(RD_ERR_INVALID_ARGUMENT, "experts=%d outside 1..%d", experts, rd::kGateMaxExperts);
+  if (spec->clusters < 1 || spec->clusters > 64 || experts % spec->clusters != 0)
+    return fail(RD_ERR_INVALID_ARGUMENT, "clusters=%d (1..64) do not divide experts=%d", spec->clusters, experts);
+  if (spec->top_clusters < 1 || spec->top_clusters > spec->clusters || spec->top_k > spec->top_clusters * (experts / spec->clusters))
+    return fail(RD_ERR_INVALID_ARGUMENT, "top_clusters=%d of %d clusters hold fewer than top_k=%d experts", spec->top_clusters, spec->clusters, spec->top_k);
+  if ((spec->flags & ~(RD_GATE_SIGMOID | RD_GATE_TOP2 | RD_GATE_RENORMALIZE)) != 0) return fail(RD_ERR_INVALID_ARGUMENT, "unknown gate flags %d", spec->flags);
+  if (!(spec->scale - spec->scale == 0.f) || spec->scale == 0.f) return fail(RD_ERR_INVALID_ARGUMENT, "scale must be finite and not 0");
+  if (tokens > 0 && (!logits || !ids || !weights)) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  *out = rd::GateSpec{tokens, experts, spec->top_k, spec->clusters, spec->top_clusters, (spec->flags & RD_GATE_SIGMOID) != 0,
+                      (spec->flags & RD_GATE_TOP2) != 0, (spec->flags & RD_GATE_RENORMALIZE) != 0, spec->scale, moe_elem(dtype)};
+  return RD_OK;
+}
+
+int rd_moe_gate(void* stream, const void* logits, const float* bias, int32_t* expert_ids, float* weights, int tokens,
+                int experts, const rd_gate_spec* spec, int dtype) {
+  rd::GateSpec p;
+  int rc = check_gate(logits, expert_ids, weights, tokens, experts, spec, dtype, &p);
+  if (rc != RD_OK || tokens == 0) return rc;
+  rc = rd::launch_moe_gate((hipStream_t)stream, logits, bias, expert_ids, weights, p);
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "moe_gate launch");
+}
+
+int rd_moe_gate_grad(void* stream, const void* logits, const int32_t* expert_ids, const float* weights, const float* dweights,
+                     void* dlogits, int tokens, int experts, const rd_gate_spec* spec, int dtype) {
+  rd::GateSpec p;
+  int rc = check_gate(logits, expert_ids, weights, tokens, experts, spec, dtype, &p);
+  if (rc != RD_OK || tokens == 0) return rc;
+  if (!dweights || !dlogits) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  rc = rd::launch_moe_gate_grad((hipStream_t)stream, logits, expert_ids, weights, dweights, dlogits, p);
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "moe_gate_grad launch");
+}
+
+static int check_swiglu(int rows, int f, int dtype) {
+  if (rows < 0 || f < 0 || f >= (1 << 30)) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape rows=%d f=%d", rows, f);
+  return check_moe(0, 1, 0, dtype);
+}
+
+int rd_moe_swiglu(void* stream, const void* y, void* out, int rows, int f, int dtype) {
+  int rc = check_swiglu(rows, f, dtype);
+  if (rc != RD_OK || rows == 0 || f == 0) return rc;
+  if (!y || !out) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  rc = rd::launch_moe_swiglu((hipStream_t)stream, y, out, rows, f, moe_elem(dtype));
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "moe_swiglu launch");
+}
+
+int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, int rows, int f, int dtype) {
+  int rc = check_swiglu(rows, f, dtype);
+  if (rc != RD_OK || rows == 0 || f == 0) return rc;
+  if (!y || !dout || !dy) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  rc = rd::launch_moe_swiglu_grad((hipStream_t)stream, y, dout, dy, rows, f, moe_elem(dtype));
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "moe_swiglu_grad launch");
+}
+
+size_t rd_int4_codes_bytes(int g, int k, int n) {
+  if (g < 0 || k < 0 || n < 0) return 0;
+  return (size_t)g * n * rd::int4_runs(k) * 64;
+}
+
+static int check_int4_weights(const void* codes, int g, int k, int n) {
+  if (g < 1 || k < 0 || n < 0 || k > (1 << 30) || n > (1 << 30)) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape g=%d k=%d n=%d", g, k, n);
+  if ((long long)g * n * rd::int4_runs(k) >= (1ll << 33)) return fail(RD_ERR_INVALID_ARGUMENT, "g*k*n too large");
+  if (k > 0 && n > 0 && (!codes || (reinterpret_cast<uintptr_t>(codes) & 15) != 0))
+    return fail(RD_ERR_INVALID_ARGUMENT, "the codes are null or not 16-byte aligned");
+  return RD_OK;
+}
+
+int rd_int4_pack(void* stream, const uint8_t* q, void* codes, int g, int k, int n, int trans_rhs) {
+  int rc = check_int4_weights(codes, g, k, n);
+  if (rc != RD_OK || k == 0 || n == 0) return rc;
+  if (!q) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  rc = rd::launch_int4_pack((hipStream_t)stream, q, static_cast<uint32_t*>(codes), g, k, n, trans_rhs != 0);
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "int4_pack launch");
+}
+
+int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scales, const uint8_t* zeros,
+                const int32_t* group_sizes, void* y, int m, int k, int n, int g_total, int group_offset, int g_local, int block,
+                int scale_dtype, int dtype) {
+  int rc = check_int4_weights(codes, g_local, k, n);
+  if (rc != RD_OK) return rc;
+  if (m < 0 || m > rd::kInt4MaxRows) return fail(RD_ERR_INVALID_ARGUMENT, "m=%d outside 0..%d", m, rd::kInt4MaxRows);
+  if (g_total < 1 || group_offset < 0 || group_offset > g_total - g_local)
+    return fail(RD_ERR_INVALID_ARGUMENT, "groups [%d, %d + %d) are not within the %d of group_sizes", group_offset, group_offset, g_local, g_total);
+  if (block != 32 && block != 64 && block != 128) return fail(RD_ERR_INVALID_ARGUMENT, "block=%d is none of 32, 64, 128", block);
+  if (dtype != RD_DTYPE_BF16 && dtype != RD_DTYPE_F16) return fail(RD_ERR_INVALID_ARGUMENT, "dtype %d: rows are bfloat16 or float16", dtype);
+  if (scale_dtype != RD_DTYPE_BF16 && scale_dtype != RD_DTYPE_F16 && scale_dtype != RD_DTYPE_F32)
+    return fail(RD_ERR_INVALID_ARGUMENT, "scale dtype %d: scales are bfloat16, float16 or float32", scale_dtype);
+  if (m == 0 || n == 0) return RD_OK;
+  if (!group_sizes || !y || (k > 0 && (!x || !scales))) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  const rd::Int4Problem p = {x, static_cast<const uint32_t*>(codes), scales, zeros, group_sizes, y, m, k, n, g_total, group_offset, g_local,
+                             block, moe_elem(scale_dtype), dtype == RD_DTYPE_F16};
+  if (!rd::int4_grid_fits(p)) return fail(RD_ERR_UNSUPPORTED, "m=%d rows of n=%d in %d groups are more tiles than a launch has", m, n, g_total);
+  rc = rd::launch_gmm_int4((hipStream_t)stream, p);
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "gmm_int4 launch");
 }
 
 }  // extern "C"

@@ -21,4 +21,19 @@ int launch_moe_combine(hipStream_t s, const void* y, const int32_t* row_of_slot,
 int launch_moe_combine_wgrad(hipStream_t s, const void* y, const void* dout, const int32_t* row_of_slot, float* dw,
                              int tokens, int top_k, int d, int elem);
 
+// What rd_moe_gate is asked for (include/ragged_dot_hip.h); elem as above.
+struct GateSpec {
+  int tokens, experts, top_k, clusters, top_clusters;
+  bool sigmoid, top2, renormalize;
+  float scale;
+  int elem;
+};
+constexpr int kGateMaxExperts = 1024;  // sixteen of them to a lane
+int launch_moe_gate(hipStream_t s, const void* logits, const float* bias, int32_t* ids, float* weights, const GateSpec& spec);
+int launch_moe_gate_grad(hipStream_t s, const void* logits, const int32_t* ids, const float* weights, const float* dweights,
+                         void* dlogits, const GateSpec& spec);
+
+int launch_moe_swiglu(hipStream_t s, const void* y, void* out, long long rows, int f, int elem);
+int launch_moe_swiglu_grad(hipStream_t s, const void* y, const void* dout, void* dy, long long rows, int f, int elem);
+
 }  // namespace rd

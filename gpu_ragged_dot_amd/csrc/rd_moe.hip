@@ -9,6 +9,7 @@
 //
 // All of it is integer / byte work bound by HBM: rows move as 16-byte pieces, one work-group per row or token.
 #include "rd_common.h"
+#include "rd_elem.h"
 #include "rd_moe.h"
 
 namespace rd {
@@ -216,15 +217,6 @@ __global__ __launch_bounds__(kRouteSlots) void moe_route_kernel(const int32_t* _
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
-
-template <class T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32<bf16_bits>(bf16_bits v) { return bf16_to_f32(v); }
-template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_f32<f16_t>(f16_t v) { return (float)v; }
-template <class T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ bf16_bits from_f32<bf16_bits>(float v) { return f32_to_bf16(v); }
-template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ f16_t from_f32<f16_t>(float v) { return (f16_t)v; }
 
 constexpr int kRowThreads = 256;
 

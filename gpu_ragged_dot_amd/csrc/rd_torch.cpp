@@ -441,6 +441,164 @@ Tensor moe_combine(const Tensor& y, const std::optional<Tensor>& weights, const 
   return CombineNode::apply(y, w, r);
 }
 
+// ---- expert ids and weights from a router's logits ---------------------------------------------------------------------
+std::tuple<Tensor, Tensor> gate_forward(const Tensor& logits, const Tensor& bias, const rd_gate_spec& spec) {
+  const c10::DeviceGuard guard(logits.device());
+  const auto opts = at::TensorOptions().device(logits.device());
+  const int64_t tokens = logits.size(0);
+  Tensor ids = at::empty({tokens, spec.top_k}, opts.dtype(at::kInt)), weights = at::empty({tokens, spec.top_k}, opts.dtype(at::kFloat));
+  check(rd_moe_gate(stream_of(logits.device()), logits.const_data_ptr(), bias.defined() ? bias.const_data_ptr<float>() : nullptr,
+                    ids.mutable_data_ptr<int32_t>(), weights.mutable_data_ptr<float>(), (int)tokens, (int)logits.size(1), &spec, rows_code(logits)));
+  return {ids, weights};
+}
+
+struct GateHolder : torch::CustomClassHolder {
+  rd_gate_spec spec;
+  explicit GateHolder(const rd_gate_spec& s) : spec(s) {}
+};
+
+struct GateNode : torch::autograd::Function<GateNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const std::optional<Tensor>& bias, const rd_gate_spec& spec) {
+    const auto [ids, weights] = gate_forward(logits, bias.value_or(Tensor()), spec);
+    ctx->save_for_backward({logits, ids, weights});
+    ctx->saved_data["gate"] = c10::IValue::make_capsule(c10::make_intrusive<GateHolder>(spec));
+    ctx->mark_non_differentiable({ids});
+    return {ids, weights};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return in_backward({grads[1]}, [&]() -> variable_list {
+      const auto saved = ctx->get_saved_variables();
+      const Tensor &logits = saved[0], &ids = saved[1], &weights = saved[2];
+      const rd_gate_spec spec = static_cast<GateHolder*>(ctx->saved_data["gate"].toCapsule().get())->spec;
+      check_devices(logits, grads[1]);
+      const c10::DeviceGuard guard(logits.device());
+      const Tensor dw = grads[1].to(at::kFloat).contiguous();
+      Tensor dl = at::empty(logits.sizes(), logits.options().requires_grad(false));
+      check(rd_moe_gate_grad(stream_of(logits.device()), logits.const_data_ptr(), ids.const_data_ptr<int32_t>(), weights.const_data_ptr<float>(),
+                             dw.const_data_ptr<float>(), dl.mutable_data_ptr(), (int)logits.size(0), (int)logits.size(1), &spec, rows_code(logits)));
+      return {dl, Tensor(), Tensor()};
+    });
+  }
+};
+
+std::tuple<Tensor, Tensor> moe_gate(const Tensor& logits_, const std::optional<Tensor>& bias_, int64_t top_k, int64_t clusters, int64_t top_clusters,
+                                    int flags, double scale) {
+  expect_no_tangent(logits_, bias_.value_or(logits_));
+  if (logits_.dim() != 2) throw py::value_error("logits must be [tokens, experts]");
+  if (top_k < 1 || top_k > logits_.size(1)) throw py::value_error("top_k must be within 1.." + std::to_string(logits_.size(1)) + ", the experts");
+  expect_int({logits_.size(0), logits_.size(1), std::abs(clusters), std::abs(top_clusters)});
+  rows_code(logits_);
+  check_devices(logits_, bias_.value_or(logits_));
+  std::optional<Tensor> bias;
+  if (bias_) {
+    if (bias_->numel() != logits_.size(1)) throw py::value_error("bias must have " + std::to_string(logits_.size(1)) + " entries");
+    bias = bias_->detach().reshape({-1}).to(at::kFloat).contiguous();
+  }
+  const rd_gate_spec spec{(int)top_k, (int)clusters, (int)top_clusters, flags, (float)scale};
+  const Tensor logits = logits_.contiguous();
+  if (!wants_grad(logits, logits)) return gate_forward(logits, bias.value_or(Tensor()), spec);
+  const variable_list out = GateNode::apply(logits, bias, spec);
+  return {out[0], out[1]};
+}
+
+// ---- the gated activation ----------------------------------------------------------------------------------------------
+Tensor swiglu_forward(const Tensor& y) {
+  const c10::DeviceGuard guard(y.device());
+  const int64_t f = y.size(1) / 2;
+  Tensor out = at::empty({y.size(0), f}, y.options().requires_grad(false));
+  check(rd_moe_swiglu(stream_of(y.device()), y.const_data_ptr(), out.mutable_data_ptr(), (int)y.size(0), (int)f, rows_code(y)));
+  return out;
+}
+
+struct SwigluNode : torch::autograd::Function<SwigluNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y) {
+    ctx->save_for_backward({y});
+    return swiglu_forward(y);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return in_backward(grads, [&]() -> variable_list {
+      const auto saved = ctx->get_saved_variables();
+      const Tensor& y = saved[0];
+      check_devices(y, grads[0]);
+      same_type(y, grads[0]);
+      const c10::DeviceGuard guard(y.device());
+      const Tensor dout = grads[0].contiguous();
+      Tensor dy = at::empty(y.sizes(), y.options().requires_grad(false));
+      check(rd_moe_swiglu_grad(stream_of(y.device()), y.const_data_ptr(), dout.const_data_ptr(), dy.mutable_data_ptr(), (int)y.size(0),
+                               (int)(y.size(1) / 2), rows_code(y)));
+      return {dy};
+    });
+  }
+};
+
+Tensor moe_swiglu(const Tensor& y_) {
+  expect_no_tangent(y_);
+  if (y_.dim() != 2 || y_.size(1) % 2 != 0) throw py::value_error("y must be [rows, 2 f], the halves gate and up");
+  expect_int({y_.size(0), y_.size(1)});
+  rows_code(y_);
+  check_devices(y_, y_);
+  const Tensor y = y_.contiguous();
+  if (!wants_grad(y, y)) return swiglu_forward(y);
+  return SwigluNode::apply(y);
+}
+
+// ---- products on 4-bit weights -----------------------------------------------------------------------------------------
+Tensor int4_pack(const Tensor& q_, bool trans) {
+  expect(q_.dim() == 3, "q must be [g, k, n], or [g, n, k] with trans_rhs");
+  if (q_.scalar_type() != at::kByte) throw py::type_error("q holds one code 0 .. 15 per byte (uint8)");
+  const int64_t g = q_.size(0), k = q_.size(trans ? 2 : 1), n = q_.size(trans ? 1 : 2);
+  expect_int({g, k, n});
+  check_devices(q_, q_);
+  const Tensor q = q_.contiguous();
+  const c10::DeviceGuard guard(q.device());
+  const int64_t bytes = (int64_t)rd_int4_codes_bytes((int)g, (int)k, (int)n), columns = g * n;
+  Tensor codes = at::empty({g, n, columns ? bytes / columns / 64 : 0, 16}, q.options().dtype(at::kInt));
+  check(rd_int4_pack(stream_of(q.device()), q.const_data_ptr<uint8_t>(), codes.mutable_data_ptr(), (int)g, (int)k, (int)n, trans));
+  return codes;
+}
+
+int scale_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return RD_DTYPE_BF16;
+    case at::kHalf: return RD_DTYPE_F16;
+    case at::kFloat: return RD_DTYPE_F32;
+    default: throw py::type_error("unsupported dtype; scales are bfloat16, float16 or float32");
+  }
+}
+
+Tensor gmm_int4(const Tensor& x_, const Tensor& codes, const Tensor& scales, const std::optional<Tensor>& zeros, int64_t k, int64_t block,
+                const Tensor& gs_, int64_t g_first) {
+  expect_no_tangent(x_, scales);
+  expect(x_.dim() == 2, "x must be [m, k]");
+  if (x_.scalar_type() != at::kBFloat16 && x_.scalar_type() != at::kHalf) throw py::type_error("unsupported dtype; x is bfloat16 or float16");
+  expect(x_.size(1) == k, "contraction mismatch between x and the weights");
+  expect(gs_.dim() == 1, "group_sizes must have one dimension");
+  expect(codes.dim() == 4 && codes.scalar_type() == at::kInt && codes.is_contiguous() && codes.size(2) == (k + 127) / 128 && codes.size(3) == 16,
+         "the codes are not what pack_int4 returns");
+  expect(block == 32 || block == 64 || block == 128, "block is 32, 64 or 128");
+  const int64_t g_local = codes.size(0), n = codes.size(1), g = gs_.numel(), blocks = (k + block - 1) / block;
+  expect(g_first < 0 ? g_local == g : g_first + g_local <= g, "the weights do not hold the groups that group_sizes describes");
+  const auto per_block = [&](const Tensor& t) {
+    return t.dim() == 3 && t.size(0) == g_local && t.size(1) == blocks && t.size(2) == n && t.is_contiguous();
+  };
+  expect(per_block(scales) && (!zeros || per_block(*zeros)), "scales and zeros must be [g, blocks, n] as pack_int4 returns them");
+  const int code = scale_code(scales);
+  if (zeros && zeros->scalar_type() != at::kByte) throw py::type_error("zeros are uint8");
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad(x_, scales), "products on 4-bit weights have no gradient: call them on detached tensors or under torch.no_grad()");
+  expect_int({x_.size(0), k, n, g});
+  check_devices(x_, codes);
+  check_devices(x_, scales);
+  if (zeros) check_devices(x_, *zeros);
+  const at::Device dev = x_.device();
+  const Tensor x = x_.contiguous(), gs = sizes_on(gs_, dev);
+  const c10::DeviceGuard guard(dev);
+  Tensor y = at::empty({x.size(0), n}, x.options().requires_grad(false));
+  check(rd_gmm_int4(stream_of(dev), x.const_data_ptr(), codes.const_data_ptr(), scales.const_data_ptr(), zeros ? zeros->const_data_ptr<uint8_t>() : nullptr,
+                    gs.const_data_ptr<int32_t>(), y.mutable_data_ptr(), (int)x.size(0), (int)k, (int)n, (int)g, (int)(g_first < 0 ? 0 : g_first),
+                    (int)g_local, (int)block, code, x.scalar_type() == at::kHalf ? RD_DTYPE_F16 : RD_DTYPE_BF16));
+  return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_rd_torch, mod) {
@@ -483,4 +641,8 @@ PYBIND11_MODULE(_rd_torch, mod) {
     return dispatch_rows(h, Routing{row_of_slot, slot_of_row, tokens, top_k}, scale.value_or(Tensor()));
   }, unlocked());
   mod.def("moe_combine", &moe_combine, unlocked());
+  mod.def("moe_gate", &moe_gate, unlocked());
+  mod.def("moe_swiglu", &moe_swiglu, unlocked());
+  mod.def("int4_pack", &int4_pack, unlocked());
+  mod.def("gmm_int4", &gmm_int4, unlocked());
 }

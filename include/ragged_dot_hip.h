@@ -229,6 +229,60 @@ int rd_moe_combine(void* stream, const void* y, const int32_t* row_of_slot, cons
 int rd_moe_combine_wgrad(void* stream, const void* y, const void* dout, const int32_t* row_of_slot, float* dw,
                          int tokens, int top_k, int d, int dtype);
 
+/* ---- from a router's logits to expert ids and weights ------------------------------------------------------------------
+ * No counterpart in the reference.  What comes before rd_moe_route and rd_moe_combine.  For every token, over its row l of
+ * `experts` logits (RD_DTYPE_BF16, RD_DTYPE_F32 or RD_DTYPE_F16):
+ *   scores s = softmax(l), or 1 / (1 + exp(-l)) with `sigmoid`; ranks c = s + bias (bias: float32 [experts], or NULL = 0);
+ *   an expert whose logit or bias is -inf is shut: it is never chosen;
+ *   the experts form `clusters` runs of experts / clusters neighbours (1: no clusters), each of which has the largest rank in
+ *   it for a score, or with `top2` the sum of the two largest (a shut one counts -inf); all experts outside the top_clusters
+ *   best clusters are shut;
+ *   expert_ids[token, :] = the top_k largest ranks that are not shut, in falling order; -1 where there are fewer.  rd_moe_route
+ *   drops those, which is how padded rows of a batch are masked: a row of -inf.  Ties of ranks and of clusters go to the lower
+ *   index.  Ranks are compared in 64 bits, or as logits where those decide alone (no bias, no sums of scores);
+ *   weights[token, :] = scale * s[expert_ids], divided by the sum of those s with `renormalize`; 0 for id -1; float32.
+ * A NaN logit ranks first and makes its row's weights NaN (with sigmoid and without renormalize its own weight only), and so
+ * does +inf with softmax; which experts such a row names is not defined, but that they are below `experts` and distinct.
+ * rd_moe_gate_grad: the gradient of the logits for dweights[token, top_k] (float32), with expert_ids and weights as rd_moe_gate
+ * returned them; dlogits has the logits' type.  The choice itself and the bias have no gradient.
+ * 1 <= experts <= 1024, top_k <= 64, 1 <= top_k <= top_clusters * (experts / clusters), clusters <= 64 divides experts, scale finite and not 0. */
+enum rd_gate_flags { RD_GATE_SIGMOID = 1, RD_GATE_TOP2 = 2, RD_GATE_RENORMALIZE = 4 };
+typedef struct rd_gate_spec {
+  int top_k, clusters, top_clusters;
+  int flags; /* RD_GATE_* */
+  float scale;
+} rd_gate_spec;
+int rd_moe_gate(void* stream, const void* logits, const float* bias, int32_t* expert_ids, float* weights, int tokens,
+                int experts, const rd_gate_spec* spec /* host */, int dtype);
+int rd_moe_gate_grad(void* stream, const void* logits, const int32_t* expert_ids, const float* weights, const float* dweights,
+                     void* dlogits, int tokens, int experts, const rd_gate_spec* spec /* host */, int dtype);
+
+/* ---- the gated activation between an expert's two products ---------------------------------------------------------------
+ * No counterpart in the reference.  y is [rows, 2 f], the halves gate and up of every row:
+ *   rd_moe_swiglu:      out[r, :] = gate / (1 + exp(-gate)) * up, [rows, f]
+ *   rd_moe_swiglu_grad: dy[rows, 2 f] for dout[rows, f]
+ * in fp32, rounded once; RD_DTYPE_BF16, RD_DTYPE_F32 or RD_DTYPE_F16. */
+int rd_moe_swiglu(void* stream, const void* y, void* out, int rows, int f, int dtype);
+int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, int rows, int f, int dtype);
+
+/* ---- rd_gmm on 4-bit weights ------------------------------------------------------------------------------------------------
+ * No counterpart in the reference.  y[m, n] = ragged x[m, k] . A with A[e, kk, c] = scale[e, kk / block, c] * (q[e, kk, c] -
+ * zero[e, kk / block, c]), q in 0 .. 15, block 32, 64 or 128 (the last block of a column may be short).
+ *   codes:  rd_int4_codes_bytes(g_local, k, n) bytes, 16-byte aligned, laid out by rd_int4_pack from q, one byte per code (its
+ *           lower four bits), [g, k, n] or with trans_rhs [g, n, k]: word j of piece h of run r of column c,
+ *           codes[e][c][r][h][j], r < ceil(k / 128), h, j < 4, holds the codes of the indices 128 r + 32 j + 8 h + i, i < 8, code
+ *           i at bits 4 (i / 2) + 16 (i % 2); codes past k are 8;
+ *   scales: [g_local, ceil(k / block), n], scale_dtype RD_DTYPE_BF16, RD_DTYPE_F16 or RD_DTYPE_F32;
+ *   zeros:  bytes of the same shape, or NULL: 8 throughout.
+ * x and y are RD_DTYPE_BF16 or RD_DTYPE_F16.  group_sizes, the rows past their sum (zero), clipping at m, group_offset and g_local
+ * are those of rd_gmm_sharded.  fp32 sums, one rounding of the result.  An infinity in x makes its row NaN.
+ * m < 2^25.  No workspace.  No gradients. */
+size_t rd_int4_codes_bytes(int g, int k, int n);
+int rd_int4_pack(void* stream, const uint8_t* q, void* codes, int g, int k, int n, int trans_rhs);
+int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scales, const uint8_t* zeros,
+                const int32_t* group_sizes, void* y, int m, int k, int n, int g_total, int group_offset, int g_local, int block,
+                int scale_dtype, int dtype);
+
 #ifdef __cplusplus
 }
 #endif
