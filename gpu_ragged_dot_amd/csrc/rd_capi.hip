@@ -1272,12 +1272,12 @@ int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, 
 
 size_t rd_int4_codes_bytes(int g, int k, int n) {
   if (g < 0 || k < 0 || n < 0) return 0;
-  return (size_t)g * n * rd::int4_runs(k) * 64;
+  return (size_t)g * rd::int4_strips(n) * rd::int4_runs(k) * 1024;
 }
 
 static int check_int4_weights(const void* codes, int g, int k, int n) {
   if (g < 1 || k < 0 || n < 0 || k > (1 << 30) || n > (1 << 30)) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape g=%d k=%d n=%d", g, k, n);
-  if ((long long)g * n * rd::int4_runs(k) >= (1ll << 33)) return fail(RD_ERR_INVALID_ARGUMENT, "g*k*n too large");
+  if ((long long)g * rd::int4_strips(n) * rd::int4_runs(k) >= (1ll << 29)) return fail(RD_ERR_INVALID_ARGUMENT, "g*k*n too large");
   if (k > 0 && n > 0 && (!codes || (reinterpret_cast<uintptr_t>(codes) & 15) != 0))
     return fail(RD_ERR_INVALID_ARGUMENT, "the codes are null or not 16-byte aligned");
   return RD_OK;
@@ -1301,12 +1301,14 @@ int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scal
     return fail(RD_ERR_INVALID_ARGUMENT, "groups [%d, %d + %d) are not within the %d of group_sizes", group_offset, group_offset, g_local, g_total);
   if (block != 32 && block != 64 && block != 128) return fail(RD_ERR_INVALID_ARGUMENT, "block=%d is none of 32, 64, 128", block);
   if (dtype != RD_DTYPE_BF16 && dtype != RD_DTYPE_F16) return fail(RD_ERR_INVALID_ARGUMENT, "dtype %d: rows are bfloat16 or float16", dtype);
-  if (scale_dtype != RD_DTYPE_BF16 && scale_dtype != RD_DTYPE_F16 && scale_dtype != RD_DTYPE_F32)
-    return fail(RD_ERR_INVALID_ARGUMENT, "scale dtype %d: scales are bfloat16, float16 or float32", scale_dtype);
+  if (scale_dtype != RD_DTYPE_BF16 && scale_dtype != RD_DTYPE_F16)
+    return fail(RD_ERR_INVALID_ARGUMENT, "scale dtype %d: scales are bfloat16 or float16", scale_dtype);
   if (m == 0 || n == 0) return RD_OK;
   if (!group_sizes || !y || (k > 0 && (!x || !scales))) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if ((reinterpret_cast<uintptr_t>(scales) & 7) != 0 || (reinterpret_cast<uintptr_t>(zeros) & 3) != 0)
+    return fail(RD_ERR_INVALID_ARGUMENT, "the scales are not 8-byte aligned or the zeros not 4-byte aligned");
   const rd::Int4Problem p = {x, static_cast<const uint32_t*>(codes), scales, zeros, group_sizes, y, m, k, n, g_total, group_offset, g_local,
-                             block, moe_elem(scale_dtype), dtype == RD_DTYPE_F16};
+                             block, scale_dtype == RD_DTYPE_F16, dtype == RD_DTYPE_F16};
   if (!rd::int4_grid_fits(p)) return fail(RD_ERR_UNSUPPORTED, "m=%d rows of n=%d in %d groups are more tiles than a launch has", m, n, g_total);
   rc = rd::launch_gmm_int4((hipStream_t)stream, p);
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "gmm_int4 launch");

@@ -6,6 +6,7 @@
 // x v over a block, and x itself against ones; then  y += 16 scale (sum x v) - scale (16 + zero) (sum x).  So products are
 // exact, sums are fp32, and nothing is rounded to 16 bits before the result.
 #include "rd_elem.h"
+#include "rd_gemm_rs.h"
 #include "rd_int4.h"
 #include "rd_lookup.h"
 
@@ -13,17 +14,13 @@ namespace rd {
 
 namespace {
 
-// ---- the row tile that a work-group computes -----------------------------------------------------------------------------
-struct RowTile {
-  int group;  // -1: none; g: rows behind the last group
-  int first, rows;
-};
-
-// Row tile t of the groups in order, each cut into tiles of BM rows, then of the rows behind them.  Groups end at row m.
-template <int BM>
-__device__ __forceinline__ RowTile find_row_tile(const int32_t* __restrict__ gs, int g, int m, int t) {
+// ---- which rows a work-group computes ---------------------------------------------------------------------------------------
+// The groups as the waves of a launch see them: sizes that are negative count as 0 and groups end at row m.  kLookupGroups at a
+// time, four per lane: f(chunk of 64 groups, first row and row behind the last one of lane's group) until it returns true.
+template <class F>
+__device__ __forceinline__ void scan_groups(const int32_t* __restrict__ gs, int g, int m, F&& f) {
   const int lane = threadIdx.x & 63;
-  int rows_before = 0, tiles_before = 0;
+  int rows_before = 0;
   for (int base = 0; base < g; base += kLookupGroups) {
     int size[kLookupChunks];
 #pragma unroll
@@ -35,25 +32,52 @@ __device__ __forceinline__ RowTile find_row_tile(const int32_t* __restrict__ gs,
     for (int c = 0; c < kLookupChunks; ++c) {
       if (base + 64 * c >= g) break;
       const int end = imin(rows_before + wave_inclusive_sum(size[c]), m);
-      const int before = __builtin_amdgcn_update_dpp(rows_before, end, 0x138, 0xf, 0xf, false);  // the lane below's: wave_shr:1
-      const int rows = end - before, tiles_own = (rows + BM - 1) / BM;
-      const int tiles = tiles_before + wave_inclusive_sum(tiles_own);
-      const unsigned long long past = __ballot(tiles > t);
-      if (past) {
-        const int l = __ffsll(past) - 1;
-        const int at = t - (__builtin_amdgcn_readlane(tiles, l) - __builtin_amdgcn_readlane(tiles_own, l));
-        const int first = __builtin_amdgcn_readlane(before, l) + at * BM;
-        return {base + 64 * c + l, first, imin(BM, __builtin_amdgcn_readlane(end, l) - first)};
-      }
+      const int first = __builtin_amdgcn_update_dpp(rows_before, end, 0x138, 0xf, 0xf, false);  // the lane below's end: wave_shr:1
+      if (f(base + 64 * c, first, end)) return;
       rows_before = __builtin_amdgcn_readlane(end, 63);
-      tiles_before = __builtin_amdgcn_readlane(tiles, 63);
     }
   }
-  const int first = rows_before + (t - tiles_before) * BM;
-  return {first < m ? g : -1, first, imin(BM, m - first)};
 }
 
-int row_tile_bound(int m, int g, int bm) { return m / bm + imin(g, m) + 1; }
+struct RowTile {
+  int group, first, rows;  // rows 0: none
+};
+
+// Tile t of BM rows of the groups that the weights hold, in order, counting those of at least `least` and at most `most` rows.
+template <int BM>
+__device__ __forceinline__ RowTile find_row_tile(const Int4Problem& p, int least, int most, int t) {
+  RowTile found = {0, 0, 0};
+  int tiles_before = 0;
+  const int lane = threadIdx.x & 63;
+  scan_groups(p.group_sizes, p.g, p.m, [&](int base, int first, int end) {
+    const int e = base + lane - p.g_first, rows = end - first;
+    const int own = e >= 0 && e < p.g_local && rows >= least && rows <= most ? (rows + BM - 1) / BM : 0;
+    const int tiles = tiles_before + wave_inclusive_sum(own);
+    const unsigned long long past = __ballot(tiles > t);
+    if (past) {
+      const int l = __ffsll(past) - 1;
+      const int at = (t - (__builtin_amdgcn_readlane(tiles, l) - __builtin_amdgcn_readlane(own, l))) * BM;
+      const int f = __builtin_amdgcn_readlane(first, l), n = __builtin_amdgcn_readlane(rows, l);
+      found = {base + l, f + at, imin(BM, n - at)};
+      return true;
+    }
+    tiles_before = __builtin_amdgcn_readlane(tiles, 63);
+    return false;
+  });
+  return found;
+}
+
+// The rows of the groups that the weights hold: [first, second); all others are zero.
+__device__ __forceinline__ void held_rows(const Int4Problem& p, int* first_row, int* end_row) {
+  int a = p.g_first == 0 ? 0 : -1, b = -1;
+  scan_groups(p.group_sizes, p.g, p.m, [&](int base, int first, int end) {
+    const int la = p.g_first - base, lb = p.g_first + p.g_local - 1 - base;
+    if (la >= 0 && la < 64) a = __builtin_amdgcn_readlane(first, la);
+    if (lb >= 0 && lb < 64) b = __builtin_amdgcn_readlane(end, lb);
+    return lb < 64;
+  });
+  *first_row = a; *end_row = b;
+}
 
 // ---- arithmetic ----------------------------------------------------------------------------------------------------------
 template <bool HALF>
@@ -62,14 +86,17 @@ __device__ __forceinline__ f32x4_t mfma_16x16x32(u32x4_t a, u32x4_t b, f32x4_t c
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// Eight codes of a word as 1 + q / 16: a code goes to the four highest bits of the fraction, under the exponent of one.
+// Eight codes of a word as 1 + q / 16: a code goes to the four highest bits of the fraction, under the exponent of one.  (The
+// exponent sits in a vector register and the mask in a scalar one: as literals they would take an instruction each.)
 template <bool HALF>
 __device__ __forceinline__ u32x4_t codes_plus_one(uint32_t w) {
   constexpr int AT = HALF ? 6 : 3;  // of 10 and of 7 fraction bits
-  constexpr uint32_t MASK = 0x000f000fu << AT, ONE = HALF ? 0x3c003c00u : 0x3f803f80u;
+  uint32_t mask = 0x000f000fu << AT, one = HALF ? 0x3c003c00u : 0x3f803f80u;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(one));
   u32x4_t v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = ((4 * i <= AT ? w << (AT - 4 * i) : w >> (4 * i - AT)) & MASK) | ONE;
+  for (int i = 0; i < 4; ++i) v[i] = ((4 * i <= AT ? w << (AT - 4 * i) : w >> (4 * i - AT)) & mask) | one;
   return v;
 }
 template <bool HALF>
@@ -78,133 +105,285 @@ __device__ __forceinline__ u32x4_t ones() {
   return u32x4_t{ONE, ONE, ONE, ONE};
 }
 
-__device__ __forceinline__ float load_scale(const void* p, size_t at, int elem) {
-  return elem == 1 ? static_cast<const float*>(p)[at]
-       : elem == 2 ? (float)static_cast<const f16_t*>(p)[at] : bf16_to_f32(static_cast<const bf16_bits*>(p)[at]);
+// Element i of eight of 16 bits, 0 before, set to e.
+__device__ __forceinline__ u32x4_t insert_element(u32x4_t v, int i, uint32_t e) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) v[w] |= i >> 1 == w ? e << (16 * (i & 1)) : 0u;
+  return v;
+}
+
+// A pointer that all lanes share, kept in scalar registers whatever is added to it.
+__device__ __forceinline__ const char* scalar_base(const void* p, size_t offset) {
+  uint64_t b = reinterpret_cast<uint64_t>(p) + offset;
+  asm("" : "+s"(b));
+  return reinterpret_cast<const char*>(b);
+}
+template <class V>
+__device__ __forceinline__ V load_at(const char* base, uint32_t offset) {
+  typedef const __attribute__((address_space(1))) char* global_bytes;
+  typedef V unaligned_t __attribute__((aligned(2)));
+  return *reinterpret_cast<const __attribute__((address_space(1))) unaligned_t*>((global_bytes)base + offset);
+}
+
+__device__ __forceinline__ float scale_to_f32(uint32_t bits, bool half) {
+  const float b = bf16_to_f32((bf16_bits)bits), h = (float)__builtin_bit_cast(f16_t, (uint16_t)bits);
+  return half ? h : b;
 }
 
 // ---- streaming kernel ------------------------------------------------------------------------------------------------------
-constexpr int kInt4Threads = 256, kInt4Waves = 4, kInt4Cols = 64;
+// A work-group computes up to 64 rows of a group x 64 columns.  Its four waves take every fourth run of 128 contraction indices
+// and add up their sums in LDS; a wave has the next run's loads in flight while it multiplies the present one.
+constexpr int kInt4Threads = 256, kInt4Waves = 4, kInt4Cols = 64, kInt4Rows = 64, kInt4Strips = kInt4Cols / kInt4Strip;
 
-// Eight consecutive elements of a row of x from index kk on, zeros from index k on.
-__device__ __forceinline__ u32x4_t load_x(const uint16_t* row, int kk, int k) {
-  if (kk + 8 <= k) return load_any<u32x4_t>(row + kk);
-  alignas(16) uint16_t e[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = kk + i < k ? row[kk + i] : 0;
-  return *reinterpret_cast<u32x4_t*>(e);
-}
+template <int BYTES> struct BlockBits;  // what a run's blocks have of scales or zeros
+template <> struct BlockBits<1> { typedef uint8_t type; };
+template <> struct BlockBits<2> { typedef uint16_t type; };
+template <> struct BlockBits<4> { typedef uint32_t type; };
+template <> struct BlockBits<8> { typedef uint64_t type; };
 
-// 16 rows x 64 columns; the four waves take every fourth run of 128 contraction indices and add up their sums in LDS.
-template <bool HALF, int BLOCK>
-__global__ __launch_bounds__(kInt4Threads) void gmm_int4_stream_kernel(Int4Problem p, int col_tiles) {
-  __shared__ float sums[kInt4Waves][16][kInt4Cols];
+// NT: row tiles of 16
+template <int BLOCK>
+struct Int4Run {
+  static constexpr int PER = kInt4Run / BLOCK;
+  typedef typename BlockBits<2 * PER>::type Scales;
+  typedef typename BlockBits<PER>::type Zeros;
+  u32x4_t codes[kInt4Strips];
+  Scales scales[kInt4Strips];
+  Zeros zeros[kInt4Strips];
+};
+
+template <bool HALF, int BLOCK, bool ZEROS, int NT>
+__device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const RowTile& tile, int c0, float (*sums)[16][kInt4Cols]) {
+  typedef Int4Run<BLOCK> Run;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const RowTile tile = find_row_tile<16>(p.group_sizes, p.g, p.m, blockIdx.x / col_tiles);
-  if (tile.group < 0) return;
-  const int c0 = blockIdx.x % col_tiles * kInt4Cols, cols = imin(kInt4Cols, p.n - c0);
-  const int e = tile.group - p.g_first;
-  const bool held = tile.group < p.g && e >= 0 && e < p.g_local;  // otherwise the rows are zero
-  const int q4 = lane & 15, h = lane >> 4;
-  const int runs = int4_runs(p.k), blocks = (p.k + BLOCK - 1) / BLOCK;
-  f32x4_t y[4];
+  const int q = lane & 15, h = lane >> 4, cols = imin(kInt4Cols, p.n - c0);
+  const int runs = int4_runs(p.k), strips = int4_strips(p.n), e = tile.group - p.g_first;
+  // Every address is a base that all lanes share and an offset of 32 bits; only the columns of scales, cut off at n, and the rows of
+  // x, at the tile's last one, depend on the lane.
+  const size_t codes0 = ((size_t)e * strips + c0 / kInt4Strip) * runs * 1024, scales0 = (size_t)e * runs * p.n + c0;
+  uint32_t column[kInt4Strips], row[NT];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) y[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if (held) {
-    const uint16_t* xrow = static_cast<const uint16_t*>(p.x) + (size_t)(tile.first + imin(q4, tile.rows - 1)) * p.k;
-    const uint32_t* codes = p.codes + (size_t)e * p.n * runs * 16;
-    const size_t scale0 = (size_t)e * blocks * p.n;
-    int col[4];
+  for (int c = 0; c < kInt4Strips; ++c) column[c] = (uint32_t)imin(kInt4Strip * c + q, cols - 1);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) col[c] = c0 + imin(16 * c + q4, cols - 1);
-    for (int r = wave; r < runs; r += kInt4Waves) {
-      u32x4_t w[4], x[4];
+  for (int t = 0; t < NT; ++t) row[t] = (uint32_t)imin(16 * t + q, tile.rows - 1) * (uint32_t)p.k * 2u + 16u * h;
+  const char* x0 = static_cast<const char*>(p.x) + (size_t)tile.first * p.k * 2;
+
+  auto load = [&](int r) {
+    Run d;
+    const size_t at = scales0 + (size_t)r * p.n;
+    const char* scales = scalar_base(p.scales, at * sizeof(typename Run::Scales));
+    const char* zeros = scalar_base(p.zeros, at * sizeof(typename Run::Zeros));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const u32x4_t*>(codes + ((size_t)col[c] * runs + r) * 16 + 4 * h);
+    for (int c = 0; c < kInt4Strips; ++c) {
+      const size_t strip = (size_t)imin(c, (cols - 1) / kInt4Strip) * runs + r;
+      d.codes[c] = load_at<u32x4_t>(scalar_base(p.codes, codes0 + strip * 1024), lane * 16u);
+      d.scales[c] = load_at<typename Run::Scales>(scales, column[c] * (uint32_t)sizeof(typename Run::Scales));
+      if constexpr (ZEROS) d.zeros[c] = *reinterpret_cast<const typename Run::Zeros*>(zeros + column[c] * (uint32_t)sizeof(typename Run::Zeros));
+    }
+    return d;
+  };
+  auto load_x = [&](int r, u32x4_t (&d)[NT][4]) {
+    const char* base = scalar_base(x0, (size_t)r * (2 * kInt4Run));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = load_x(xrow, r * kInt4Run + 32 * j + 8 * h, p.k);
-      constexpr int STEPS = BLOCK / 32;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int b = 0; b < 4 / STEPS; ++b) {
-        const int kb = r * (kInt4Run / BLOCK) + b;
-        if (kb >= blocks) break;
-        f32x4_t xs = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 4; ++j) d[t][j] = load_at<u32x4_t>(base, row[t] + 64u * j);
+  };
+  // Of the run that holds index k: zeros from there on.  A piece that would run past it is read from before it and shifted down.
+  auto load_x_tail = [&](int r, u32x4_t (&d)[NT][4]) {
+    const char* base = x0 + (size_t)r * (2 * kInt4Run);
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) xs = mfma_16x16x32<HALF>(x[b * STEPS + j], ones<HALF>(), xs);
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < STEPS; ++j) v = mfma_16x16x32<HALF>(x[b * STEPS + j], codes_plus_one<HALF>(w[c][b * STEPS + j]), v);
-          const size_t at = scale0 + (size_t)kb * p.n + col[c];
-          const float s = load_scale(p.scales, at, p.scale_elem);
-          const float z = p.zeros ? (float)p.zeros[at] : 8.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[c][i] = __builtin_fmaf(16.f * s, v[i], __builtin_fmaf(-s * (16.f + z), xs[i], y[c][i]));
+      for (int j = 0; j < 4; ++j) {
+        const int past = imax(r * kInt4Run + 32 * j + 8 * h + 8 - p.k, 0);  // elements
+        const char* at = base + 64 * j + row[t];
+        if (p.k >= 8) {
+          d[t][j] = shift_down(load_any<u32x4_t>(at - 2 * past), 2 * imin(past, 8));
+        } else {
+          u32x4_t v = {0, 0, 0, 0};
+#pragma unroll 1
+          for (int i = 0; i < 8 - past; ++i) v = insert_element(v, i, *reinterpret_cast<const uint16_t*>(at + 2 * i));
+          d[t][j] = v;
         }
       }
+  };
+
+  f32x4_t y[NT][kInt4Strips];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int c = 0; c < kInt4Strips; ++c) y[t][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Run& d, const u32x4_t (&xv)[NT][4]) {
+    constexpr int STEPS = BLOCK / 32;
+#pragma unroll
+    for (int b = 0; b < Run::PER; ++b) {
+      f32x4_t xs[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        xs[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) xs[t] = mfma_16x16x32<HALF>(xv[t][b * STEPS + j], ones<HALF>(), xs[t]);
+      }
+#pragma unroll
+      for (int c = 0; c < kInt4Strips; ++c) {
+        f32x4_t v[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) v[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+          const u32x4_t w = codes_plus_one<HALF>(d.codes[c][b * STEPS + j]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) v[t] = mfma_16x16x32<HALF>(xv[t][b * STEPS + j], w, v[t]);
+        }
+        const float s = scale_to_f32((uint32_t)(d.scales[c] >> (16 * b)) & 0xffff, p.scale_half);
+        float plus = 24.f;  // 16 + zero
+        if constexpr (ZEROS) plus = 16.f + (float)((uint32_t)(d.zeros[c] >> (8 * b)) & 0xff);
+        const float s16 = 16.f * s, sz = -s * plus;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[t][c][i] = __builtin_fmaf(s16, v[t][i], __builtin_fmaf(sz, xs[t][i], y[t][c][i]));
+      }
+    }
+  };
+  // (more than 16 rows: x, which is read again and again and comes from the caches, is fetched when it is needed - two runs of
+  // it do not fit the registers that two work-groups on a compute unit leave)
+  const int whole = p.k / kInt4Run, own = (whole - wave + kInt4Waves - 1) / kInt4Waves;  // whole runs; this wave's
+  if (own > 0) {
+    // Work-groups begin at runs of their own: strips lie runs x 1 KB apart, a multiple of 4 KB for most k, and all in step they
+    // would ask a few memory channels at a time.
+    int i = (int)(blockIdx.x % (uint32_t)own);
+    Run now = load(wave + i * kInt4Waves);
+    u32x4_t xv[NT][4];
+    if constexpr (NT == 1) load_x(wave + i * kInt4Waves, xv);
+    for (int left = own; left > 0; --left) {
+      Run next = now;
+      u32x4_t xn[NT][4];
+      const int here = i;
+      if (left > 1) i = i + 1 < own ? i + 1 : 0;
+      if constexpr (NT == 1) load_x(wave + i * kInt4Waves, xn);
+      next = load(wave + i * kInt4Waves);
+      if constexpr (NT > 1) load_x(wave + here * kInt4Waves, xv);
+      multiply(now, xv);
+      now = next;
+      if constexpr (NT == 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xv[0][j] = xn[0][j];
     }
   }
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sums[wave][4 * h + i][16 * c + q4] = y[c][i];
-  __syncthreads();
-  for (int at = threadIdx.x; at < tile.rows * kInt4Cols; at += kInt4Threads) {
-    const int r = at / kInt4Cols, c = at % kInt4Cols;
-    if (c >= cols) continue;
-    const float v = sums[0][r][c] + sums[1][r][c] + sums[2][r][c] + sums[3][r][c];
-    uint16_t* out = static_cast<uint16_t*>(p.y) + (size_t)(tile.first + r) * p.n + c0 + c;
-    if constexpr (HALF) *reinterpret_cast<f16_t*>(out) = (f16_t)v;
-    else *out = f32_to_bf16(v);
+  if (whole < runs && whole % kInt4Waves == wave) {
+    u32x4_t xv[NT][4];
+    load_x_tail(whole, xv);
+    multiply(load(whole), xv);
   }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (16 * t >= tile.rows) break;
+    if (t > 0) __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kInt4Strips; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[wave][4 * h + i][kInt4Strip * c + q] = y[t][c][i];
+    __syncthreads();
+    for (int cell = threadIdx.x; cell < imin(16, tile.rows - 16 * t) * kInt4Cols; cell += kInt4Threads) {
+      const int r = cell / kInt4Cols, c = cell % kInt4Cols;
+      if (c >= cols) continue;
+      const float v = sums[0][r][c] + sums[1][r][c] + sums[2][r][c] + sums[3][r][c];
+      uint16_t* out = static_cast<uint16_t*>(p.y) + (size_t)(tile.first + 16 * t + r) * p.n + c0 + c;
+      if constexpr (HALF) *reinterpret_cast<f16_t*>(out) = (f16_t)v;
+      else *out = f32_to_bf16(v);
+    }
+  }
+}
+
+// Work-groups [0, tiles * col_tiles): a row tile and 64 of its columns; those behind them: 64 rows, of which they zero what is
+// no row of a group that the weights hold.
+// ROWS: of a row tile, 16 or 64.
+template <bool HALF, int BLOCK, bool ZEROS, int ROWS>
+__global__ __launch_bounds__(kInt4Threads, ROWS == 16 ? 4 : 2) void gmm_int4_stream_kernel(Int4Problem p, int tiles, int col_tiles, int most) {
+  __shared__ float sums[kInt4Waves][16][kInt4Cols];
+  if ((int)blockIdx.x >= tiles * col_tiles) {
+    int first, end;
+    held_rows(p, &first, &end);
+    const int r0 = ((int)blockIdx.x - tiles * col_tiles) * kInt4Rows;
+    for (int r = r0; r < imin(r0 + kInt4Rows, p.m); ++r)
+      if (r < first || r >= end)
+        for (int c = threadIdx.x; c < p.n; c += kInt4Threads) static_cast<uint16_t*>(p.y)[(size_t)r * p.n + c] = 0;
+    return;
+  }
+  const RowTile tile = find_row_tile<ROWS>(p, 1, most, blockIdx.x / col_tiles);
+  if (tile.rows == 0) return;
+  const int c0 = blockIdx.x % col_tiles * kInt4Cols;
+  if (ROWS == 16) int4_stream_tile<HALF, BLOCK, ZEROS, 1>(p, tile, c0, sums);
+  else if (tile.rows <= 32) int4_stream_tile<HALF, BLOCK, ZEROS, 2>(p, tile, c0, sums);
+  else int4_stream_tile<HALF, BLOCK, ZEROS, 4>(p, tile, c0, sums);
 }
 
 // ---- laying out the weights --------------------------------------------------------------------------------------------------
 // One word of eight codes per thread.
 __global__ __launch_bounds__(256) void int4_pack_kernel(const uint8_t* __restrict__ q, uint32_t* __restrict__ codes, long long words,
                                                         int k, int n, bool trans_rhs) {
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= words) return;
-  const int j = (int)(at & 3), h = (int)(at >> 2 & 3), runs = int4_runs(k);
-  const long long column = (at >> 4) / runs;
-  const int r = (int)((at >> 4) - column * runs);
-  const long long e = column / n, c = column - e * n;
-  uint32_t w = 0;
+  for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < words; at += (long long)gridDim.x * 256) {
+    const int j = (int)(at & 3), c16 = (int)(at >> 2 & 15), h = (int)(at >> 6 & 3);
+    const int runs = int4_runs(k), strips = int4_strips(n);
+    const long long strip = (at >> 8) / runs;
+    const int r = (int)((at >> 8) - strip * runs);
+    const long long e = strip / strips, c = (strip - e * strips) * kInt4Strip + c16;
+    uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int kk = r * kInt4Run + 32 * j + 8 * h + i;
-    const uint32_t v = kk < k ? q[trans_rhs ? column * k + kk : (e * k + kk) * n + c] & 15u : 8u;
-    w |= v << (4 * (i >> 1) + 16 * (i & 1));
+    for (int i = 0; i < 8; ++i) {
+      const int kk = r * kInt4Run + 32 * j + 8 * h + i;
+      const uint32_t v = kk < k && c < n ? q[trans_rhs ? (e * n + c) * k + kk : (e * k + kk) * n + c] & 15u : 8u;
+      w |= v << (4 * (i >> 1) + 16 * (i & 1));
+    }
+    codes[at] = w;
   }
-  codes[at] = w;
 }
 
-template <bool HALF>
-int stream(hipStream_t s, const Int4Problem& p) {
-  const int col_tiles = (p.n + kInt4Cols - 1) / kInt4Cols;
-  const dim3 grid((unsigned)row_tile_bound(p.m, p.g, 16) * (unsigned)col_tiles);
-  if (p.block == 32) hipLaunchKernelGGL((gmm_int4_stream_kernel<HALF, 32>), grid, dim3(kInt4Threads), 0, s, p, col_tiles);
-  else if (p.block == 64) hipLaunchKernelGGL((gmm_int4_stream_kernel<HALF, 64>), grid, dim3(kInt4Threads), 0, s, p, col_tiles);
-  else hipLaunchKernelGGL((gmm_int4_stream_kernel<HALF, 128>), grid, dim3(kInt4Threads), 0, s, p, col_tiles);
+struct StreamGrid {
+  int rows, tiles, col_tiles;  // rows of a tile; tiles at most, of groups with at most `most` rows
+  long long blocks;
+};
+StreamGrid stream_grid(const Int4Problem& p, int most) {
+  StreamGrid s;
+  s.rows = p.m <= 8 * p.g ? 16 : kInt4Rows;
+  s.tiles = most <= s.rows ? imin(p.g, p.m) : p.m / s.rows + imin(p.g, p.m);
+  s.col_tiles = (p.n + kInt4Cols - 1) / kInt4Cols;
+  s.blocks = (long long)s.tiles * s.col_tiles + (p.m + kInt4Rows - 1) / kInt4Rows;
+  return s;
+}
+
+template <bool HALF, int BLOCK, bool ZEROS>
+int stream(hipStream_t s, const Int4Problem& p, int most) {
+  const StreamGrid g = stream_grid(p, most);
+  const dim3 grid((unsigned)g.blocks);
+  if (g.rows == 16) hipLaunchKernelGGL((gmm_int4_stream_kernel<HALF, BLOCK, ZEROS, 16>), grid, dim3(kInt4Threads), 0, s, p, g.tiles, g.col_tiles, most);
+  else hipLaunchKernelGGL((gmm_int4_stream_kernel<HALF, BLOCK, ZEROS, kInt4Rows>), grid, dim3(kInt4Threads), 0, s, p, g.tiles, g.col_tiles, most);
   return (int)hipGetLastError();
+}
+
+template <bool HALF, int BLOCK>
+int gmm_int4(hipStream_t s, const Int4Problem& p) {
+  return p.zeros ? stream<HALF, BLOCK, true>(s, p, p.m) : stream<HALF, BLOCK, false>(s, p, p.m);
+}
+template <bool HALF>
+int gmm_int4(hipStream_t s, const Int4Problem& p) {
+  return p.block == 32 ? gmm_int4<HALF, 32>(s, p) : p.block == 64 ? gmm_int4<HALF, 64>(s, p) : gmm_int4<HALF, 128>(s, p);
 }
 
 }  // namespace
 
 int launch_int4_pack(hipStream_t s, const uint8_t* q, uint32_t* codes, int g, int k, int n, bool trans_rhs) {
-  const long long words = (long long)g * n * int4_runs(k) * 16;
-  hipLaunchKernelGGL(int4_pack_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, q, codes, words, k, n, trans_rhs);
+  const long long words = (long long)g * int4_strips(n) * int4_runs(k) * 256;
+  hipLaunchKernelGGL(int4_pack_kernel, dim3((unsigned)(words < (1ll << 24) ? (words + 255) / 256 : 1 << 16)), dim3(256), 0, s, q, codes, words, k, n, trans_rhs);
   return (int)hipGetLastError();
 }
 
-bool int4_grid_fits(const Int4Problem& p) {
-  return (long long)row_tile_bound(p.m, p.g, 16) * ((p.n + kInt4Cols - 1) / kInt4Cols) < (1ll << 31) / kInt4Threads;
-}
+bool int4_grid_fits(const Int4Problem& p) { return stream_grid(p, p.m).blocks < (1ll << 31) / kInt4Threads; }
 
 int launch_gmm_int4(hipStream_t s, const Int4Problem& p) {
-  if (p.m == 0 || p.n == 0) return hipSuccess;
-  return p.half ? stream<true>(s, p) : stream<false>(s, p);
+  return p.half ? gmm_int4<true>(s, p) : gmm_int4<false>(s, p);
 }
 
 }  // namespace rd

@@ -551,8 +551,7 @@ Tensor int4_pack(const Tensor& q_, bool trans) {
   check_devices(q_, q_);
   const Tensor q = q_.contiguous();
   const c10::DeviceGuard guard(q.device());
-  const int64_t bytes = (int64_t)rd_int4_codes_bytes((int)g, (int)k, (int)n), columns = g * n;
-  Tensor codes = at::empty({g, n, columns ? bytes / columns / 64 : 0, 16}, q.options().dtype(at::kInt));
+  Tensor codes = at::empty({g, (n + 15) / 16, (k + 127) / 128, 64, 4}, q.options().dtype(at::kInt));
   check(rd_int4_pack(stream_of(q.device()), q.const_data_ptr<uint8_t>(), codes.mutable_data_ptr(), (int)g, (int)k, (int)n, trans));
   return codes;
 }
@@ -561,27 +560,27 @@ int scale_code(const Tensor& t) {
   switch (t.scalar_type()) {
     case at::kBFloat16: return RD_DTYPE_BF16;
     case at::kHalf: return RD_DTYPE_F16;
-    case at::kFloat: return RD_DTYPE_F32;
-    default: throw py::type_error("unsupported dtype; scales are bfloat16, float16 or float32");
+    default: throw py::type_error("unsupported dtype; scales are bfloat16 or float16");
   }
 }
 
-Tensor gmm_int4(const Tensor& x_, const Tensor& codes, const Tensor& scales, const std::optional<Tensor>& zeros, int64_t k, int64_t block,
+Tensor gmm_int4(const Tensor& x_, const Tensor& codes, const Tensor& scales, const std::optional<Tensor>& zeros, int64_t k, int64_t n, int64_t block,
                 const Tensor& gs_, int64_t g_first) {
   expect_no_tangent(x_, scales);
   expect(x_.dim() == 2, "x must be [m, k]");
   if (x_.scalar_type() != at::kBFloat16 && x_.scalar_type() != at::kHalf) throw py::type_error("unsupported dtype; x is bfloat16 or float16");
   expect(x_.size(1) == k, "contraction mismatch between x and the weights");
   expect(gs_.dim() == 1, "group_sizes must have one dimension");
-  expect(codes.dim() == 4 && codes.scalar_type() == at::kInt && codes.is_contiguous() && codes.size(2) == (k + 127) / 128 && codes.size(3) == 16,
-         "the codes are not what pack_int4 returns");
+  const int64_t runs = (k + 127) / 128;
+  expect(codes.dim() == 5 && codes.scalar_type() == at::kInt && codes.is_contiguous() && codes.size(1) == (n + 15) / 16 && codes.size(2) == runs &&
+         codes.size(3) == 64 && codes.size(4) == 4, "the codes are not what pack_int4 returns");
   expect(block == 32 || block == 64 || block == 128, "block is 32, 64 or 128");
-  const int64_t g_local = codes.size(0), n = codes.size(1), g = gs_.numel(), blocks = (k + block - 1) / block;
+  const int64_t g_local = codes.size(0), g = gs_.numel();
   expect(g_first < 0 ? g_local == g : g_first + g_local <= g, "the weights do not hold the groups that group_sizes describes");
   const auto per_block = [&](const Tensor& t) {
-    return t.dim() == 3 && t.size(0) == g_local && t.size(1) == blocks && t.size(2) == n && t.is_contiguous();
+    return t.dim() == 4 && t.size(0) == g_local && t.size(1) == runs && t.size(2) == n && t.size(3) == 128 / block && t.is_contiguous();
   };
-  expect(per_block(scales) && (!zeros || per_block(*zeros)), "scales and zeros must be [g, blocks, n] as pack_int4 returns them");
+  expect(per_block(scales) && (!zeros || per_block(*zeros)), "scales and zeros are not what pack_int4 returns");
   const int code = scale_code(scales);
   if (zeros && zeros->scalar_type() != at::kByte) throw py::type_error("zeros are uint8");
   TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad(x_, scales), "products on 4-bit weights have no gradient: call them on detached tensors or under torch.no_grad()");

@@ -22,10 +22,11 @@ __all__ = ["Int4Weights", "pack_int4", "ragged_dot_int4"]
 
 
 class Int4Weights(NamedTuple):
-    codes: torch.Tensor            # int32 [g, n, ceil(k / 128), 16]  eight codes to a word, in the kernels' order
-    scales: torch.Tensor           # [g, ceil(k / block), n]  bfloat16, float16 or float32
+    codes: torch.Tensor            # int32 [g, ceil(n / 16), ceil(k / 128), 64, 4]  eight codes to a word, in the kernels' order
+    scales: torch.Tensor           # [g, ceil(k / 128), n, 128 / block]  bfloat16 or float16
     zeros: Optional[torch.Tensor]  # uint8, the scales' shape; None = 8
     k: int
+    n: int
     block: int
 
 
@@ -33,7 +34,7 @@ def pack_int4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tenso
               trans_rhs: bool = False) -> Int4Weights:
     """Lays out codes ``q`` (uint8, one of 0 .. 15 per byte) ``[g, k, n]`` with ``scales`` (and ``zeros``)
     ``[g, ceil(k / block), n]``; with ``trans_rhs`` ``[g, n, k]`` and ``[g, n, ceil(k / block)]``, as most checkpoints hold
-    them.  ``block`` is 32, 64 or 128.  Codes above 15 lose their upper bits."""
+    them.  ``block`` is 32, 64 or 128, scales are bfloat16 or float16.  Codes above 15 lose their upper bits."""
     assert q.ndim == 3, f"but {q.ndim=}"
     assert block in (32, 64, 128), f"block is 32, 64 or 128, not {block}"
     g, k, n = (q.shape[0], q.shape[2], q.shape[1]) if trans_rhs else q.shape
@@ -44,10 +45,18 @@ def pack_int4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tenso
     for name, t in (("scales", scales), ("zeros", zeros)):
         if t is not None and tuple(t.shape) != wanted:
             raise ValueError(f"{name} must be {list(wanted)}, not {list(t.shape)}")
-    if scales.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError(f"unsupported dtype {scales.dtype}; scales are bfloat16, float16 or float32")
-    laid_out = lambda t: None if t is None else (t.transpose(1, 2) if trans_rhs else t).detach().contiguous()
-    return Int4Weights(_native.int4_pack(q, bool(trans_rhs)), laid_out(scales), laid_out(zeros), k, int(block))
+    if scales.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"unsupported dtype {scales.dtype}; scales are bfloat16 or float16")
+    runs, per_run = -(-k // 128), 128 // block
+
+    def laid_out(t):  # a run's scales of a column beside each other, zeros past k
+        if t is None:
+            return None
+        out = t.new_zeros((g, n, runs * per_run))
+        out[:, :, :blocks] = t.detach() if trans_rhs else t.detach().transpose(1, 2)
+        return out.view(g, n, runs, per_run).transpose(1, 2).contiguous()
+
+    return Int4Weights(_native.int4_pack(q, bool(trans_rhs)), laid_out(scales), laid_out(zeros), k, n, int(block))
 
 
 def ragged_dot_int4(x: torch.Tensor, weights: Int4Weights, group_sizes, *, group_offset=None) -> torch.Tensor:
@@ -57,7 +66,8 @@ def ragged_dot_int4(x: torch.Tensor, weights: Int4Weights, group_sizes, *, group
     assert x.ndim == 2, f"but {x.ndim=}"
     g_first = -1 if group_offset is None else _group_offset(group_offset)
     assert group_offset is None or g_first >= 0
-    call = lambda x, gs: _native.gmm_int4(x, weights.codes, weights.scales, weights.zeros, weights.k, weights.block, gs, g_first)
+    call = lambda x, gs: _native.gmm_int4(x, weights.codes, weights.scales, weights.zeros, weights.k, weights.n,
+                                          weights.block, gs, g_first)
     if _tracing.active():
         return _tracing.record(call, x, _sizes(group_sizes))
     return call(x, _sizes(group_sizes))

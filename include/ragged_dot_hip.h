@@ -269,11 +269,11 @@ int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, 
  * No counterpart in the reference.  y[m, n] = ragged x[m, k] . A with A[e, kk, c] = scale[e, kk / block, c] * (q[e, kk, c] -
  * zero[e, kk / block, c]), q in 0 .. 15, block 32, 64 or 128 (the last block of a column may be short).
  *   codes:  rd_int4_codes_bytes(g_local, k, n) bytes, 16-byte aligned, laid out by rd_int4_pack from q, one byte per code (its
- *           lower four bits), [g, k, n] or with trans_rhs [g, n, k]: word j of piece h of run r of column c,
- *           codes[e][c][r][h][j], r < ceil(k / 128), h, j < 4, holds the codes of the indices 128 r + 32 j + 8 h + i, i < 8, code
- *           i at bits 4 (i / 2) + 16 (i % 2); codes past k are 8;
- *   scales: [g_local, ceil(k / block), n], scale_dtype RD_DTYPE_BF16, RD_DTYPE_F16 or RD_DTYPE_F32;
- *   zeros:  bytes of the same shape, or NULL: 8 throughout.
+ *           lower four bits), [g, k, n] or with trans_rhs [g, n, k].  In strips of 16 columns and runs of 128 indices, word j of
+ *           piece (h, c), codes[e][strip][run][h][c][j], h, j < 4, c < 16, holds column 16 strip + c and the indices 128 run +
+ *           32 j + 8 h + i, i < 8, code i at bits 4 (i / 2) + 16 (i % 2); codes past k and n are 8;
+ *   scales: [g_local, ceil(k / 128), n, 128 / block], 8-byte aligned, scale_dtype RD_DTYPE_BF16 or RD_DTYPE_F16, 0 past k;
+ *   zeros:  bytes of the same shape, 4-byte aligned, or NULL: 8 throughout.
  * x and y are RD_DTYPE_BF16 or RD_DTYPE_F16.  group_sizes, the rows past their sum (zero), clipping at m, group_offset and g_local
  * are those of rd_gmm_sharded.  fp32 sums, one rounding of the result.  An infinity in x makes its row NaN.
  * m < 2^25.  No workspace.  No gradients. */

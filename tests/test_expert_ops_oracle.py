@@ -117,7 +117,7 @@ def _int4(x=P, codes=P, scales=P, gs=P, y=P, m=4, k=64, n=8, g=2, first=0, local
 @pytest.mark.parametrize("kw", [
     dict(x=None), dict(codes=None), dict(codes=P + 4), dict(scales=None), dict(gs=None), dict(y=None), dict(m=-1), dict(m=1 << 25),
     dict(k=-1), dict(n=-1), dict(g=0, local=0), dict(local=0), dict(first=1), dict(first=-1), dict(first=2 ** 31 - 1), dict(local=3),
-    dict(block=16), dict(block=256), dict(sdtype=3), dict(sdtype=2), dict(dtype=1), dict(dtype=3),
+    dict(block=16), dict(block=256), dict(sdtype=3), dict(sdtype=2), dict(sdtype=1), dict(scales=P + 4), dict(dtype=1), dict(dtype=3),
     dict(g=4096, local=4096, k=1 << 20, n=1 << 20)], ids=lambda kw: ",".join(f"{k}={v}" for k, v in kw.items()))
 def test_int4_refusals(kw):
     assert _int4(**kw) == -1 and _capi.lib.rd_last_error()
@@ -125,7 +125,7 @@ def test_int4_refusals(kw):
 
 def test_int4_sizes():
     lib = _capi.lib
-    assert lib.rd_int4_codes_bytes(2, 128, 3) == 2 * 3 * 64 and lib.rd_int4_codes_bytes(2, 129, 3) == 2 * 3 * 128
+    assert lib.rd_int4_codes_bytes(2, 128, 3) == 2 * 1024 and lib.rd_int4_codes_bytes(2, 129, 17) == 2 * 2 * 2 * 1024
     assert lib.rd_int4_codes_bytes(2, 0, 3) == 0 and lib.rd_int4_codes_bytes(-1, 8, 8) == 0
     assert _int4(m=0) == 0 and _int4(n=0) == 0
     assert lib.rd_int4_pack(None, None, P, 1, 32, 8, 0) == -1 and lib.rd_int4_pack(None, P, P + 2, 1, 32, 8, 0) == -1
@@ -153,7 +153,7 @@ def test_front_end_refusals():
         moe.swiglu(rand(4, 8).double())
     with pytest.raises(RuntimeError, match="ROCm"):
         moe.swiglu(rand(4, 8))
-    q, scales = torch.zeros((2, 64, 8), dtype=torch.uint8), torch.ones((2, 2, 8))
+    q, scales = torch.zeros((2, 64, 8), dtype=torch.uint8), torch.ones((2, 2, 8)).half()
     with pytest.raises(RuntimeError, match="ROCm"):
         rd.pack_int4(q, scales, block=32)
     for bad in (dict(block=16), dict(block=48)):
@@ -166,17 +166,18 @@ def test_front_end_refusals():
     with pytest.raises(TypeError, match="zeros"):
         rd.pack_int4(q, scales, torch.zeros((2, 2, 8)), block=32)
     with pytest.raises(TypeError, match="scales"):
-        rd.pack_int4(q, scales.double(), block=32)
+        rd.pack_int4(q, scales.float(), block=32)
     with pytest.raises(TypeError):
         rd.pack_int4(q.float(), scales, block=32)
-    w = rd.Int4Weights(torch.zeros((2, 8, 1, 16), dtype=torch.int32), scales, None, 64, 32)
+    scales = torch.ones((2, 1, 8, 4)).half()
+    w = rd.Int4Weights(torch.zeros((2, 1, 1, 64, 4), dtype=torch.int32), scales, None, 64, 8, 32)
     gs, x = torch.tensor([1, 3], dtype=torch.int32), rand(4, 64).bfloat16()
     with pytest.raises(RuntimeError, match="ROCm"):
         rd.ragged_dot_int4(x, w, gs)
     for case, error in ((dict(x=x.float()), TypeError), (dict(x=x[:, :32]), AssertionError), (dict(gs=gs[:1]), AssertionError),
                         (dict(w=w._replace(codes=w.codes[:, :, :, :8])), AssertionError), (dict(w=w._replace(block=64)), AssertionError),
-                        (dict(w=w._replace(scales=scales.double())), TypeError), (dict(x=x.clone().requires_grad_()), NotImplementedError),
-                        (dict(w=w._replace(zeros=torch.zeros((2, 2, 8)))), TypeError), (dict(w=w._replace(codes=w.codes.float())), AssertionError)):
+                        (dict(w=w._replace(scales=scales.float())), TypeError), (dict(x=x.clone().requires_grad_()), NotImplementedError),
+                        (dict(w=w._replace(zeros=torch.zeros((2, 1, 8, 4)))), TypeError), (dict(w=w._replace(codes=w.codes.float())), AssertionError)):
         with pytest.raises(error):
             rd.ragged_dot_int4(case.get("x", x), case.get("w", w), case.get("gs", gs))
     with pytest.raises(AssertionError):
@@ -186,7 +187,7 @@ def test_front_end_refusals():
 def test_tangents_are_refused():
     with fwAD.dual_level():
         dual = lambda *s: fwAD.make_dual(torch.randn(*s), torch.randn(*s))
-        w = rd.Int4Weights(torch.zeros((1, 8, 1, 16), dtype=torch.int32), torch.ones((1, 1, 8)), None, 64, 64)
+        w = rd.Int4Weights(torch.zeros((1, 1, 1, 64, 4), dtype=torch.int32), torch.ones((1, 1, 8, 2)), None, 64, 8, 64)
         for call in (lambda: moe.gate(dual(4, 8), 2), lambda: moe.swiglu(dual(4, 8)),
                      lambda: rd.ragged_dot_int4(dual(4, 64).bfloat16(), w, torch.tensor([4]))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
