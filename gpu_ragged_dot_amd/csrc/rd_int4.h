@@ -37,6 +37,10 @@ struct Int4Problem {
 __host__ __device__ inline int int4_runs(int k) { return (k + kInt4Run - 1) / kInt4Run; }
 __host__ __device__ inline int int4_strips(int n) { return (n + kInt4Strip - 1) / kInt4Strip; }
 
+// Groups of at least `least` rows, by 256-column tiles (rd_int4_tile.hip; one object per instance).
+template <bool HALF, int BLOCK>
+int launch_int4_tiles(hipStream_t s, const Int4Problem& p, int least);
+
 bool int4_grid_fits(const Int4Problem& p);  // a launch holds its work-groups
 int launch_int4_pack(hipStream_t s, const uint8_t* q, uint32_t* codes, int g, int k, int n, bool trans_rhs);
 int launch_gmm_int4(hipStream_t s, const Int4Problem& p);

@@ -5,79 +5,18 @@
 // A code becomes the 16-bit number v = 1 + q / 16, exactly, by a shift and an and-or for two of them; the matrix cores sum
 // x v over a block, and x itself against ones; then  y += 16 scale (sum x v) - scale (16 + zero) (sum x).  So products are
 // exact, sums are fp32, and nothing is rounded to 16 bits before the result.
+#include <stdlib.h>
 #include "rd_elem.h"
-#include "rd_gemm_rs.h"
-#include "rd_int4.h"
-#include "rd_lookup.h"
+#include "rd_int4_rows.h"
+#include "rd_int4_tile.h"
 
 namespace rd {
 
 namespace {
 
-// ---- which rows a work-group computes ---------------------------------------------------------------------------------------
-// The groups as the waves of a launch see them: sizes that are negative count as 0 and groups end at row m.  kLookupGroups at a
-// time, four per lane: f(chunk of 64 groups, first row and row behind the last one of lane's group) until it returns true.
-template <class F>
-__device__ __forceinline__ void scan_groups(const int32_t* __restrict__ gs, int g, int m, F&& f) {
-  const int lane = threadIdx.x & 63;
-  int rows_before = 0;
-  for (int base = 0; base < g; base += kLookupGroups) {
-    int size[kLookupChunks];
-#pragma unroll
-    for (int c = 0; c < kLookupChunks; ++c) {
-      const int e = base + 64 * c + lane;
-      size[c] = e < g ? imin(imax(gs[e], 0), m) : 0;
-    }
-#pragma unroll
-    for (int c = 0; c < kLookupChunks; ++c) {
-      if (base + 64 * c >= g) break;
-      const int end = imin(rows_before + wave_inclusive_sum(size[c]), m);
-      const int first = __builtin_amdgcn_update_dpp(rows_before, end, 0x138, 0xf, 0xf, false);  // the lane below's end: wave_shr:1
-      if (f(base + 64 * c, first, end)) return;
-      rows_before = __builtin_amdgcn_readlane(end, 63);
-    }
-  }
-}
-
-struct RowTile {
-  int group, first, rows;  // rows 0: none
-};
-
-// Tile t of BM rows of the groups that the weights hold, in order, counting those of at least `least` and at most `most` rows.
-template <int BM>
-__device__ __forceinline__ RowTile find_row_tile(const Int4Problem& p, int least, int most, int t) {
-  RowTile found = {0, 0, 0};
-  int tiles_before = 0;
-  const int lane = threadIdx.x & 63;
-  scan_groups(p.group_sizes, p.g, p.m, [&](int base, int first, int end) {
-    const int e = base + lane - p.g_first, rows = end - first;
-    const int own = e >= 0 && e < p.g_local && rows >= least && rows <= most ? (rows + BM - 1) / BM : 0;
-    const int tiles = tiles_before + wave_inclusive_sum(own);
-    const unsigned long long past = __ballot(tiles > t);
-    if (past) {
-      const int l = __ffsll(past) - 1;
-      const int at = (t - (__builtin_amdgcn_readlane(tiles, l) - __builtin_amdgcn_readlane(own, l))) * BM;
-      const int f = __builtin_amdgcn_readlane(first, l), n = __builtin_amdgcn_readlane(rows, l);
-      found = {base + l, f + at, imin(BM, n - at)};
-      return true;
-    }
-    tiles_before = __builtin_amdgcn_readlane(tiles, 63);
-    return false;
-  });
-  return found;
-}
-
-// The rows of the groups that the weights hold: [first, second); all others are zero.
-__device__ __forceinline__ void held_rows(const Int4Problem& p, int* first_row, int* end_row) {
-  int a = p.g_first == 0 ? 0 : -1, b = -1;
-  scan_groups(p.group_sizes, p.g, p.m, [&](int base, int first, int end) {
-    const int la = p.g_first - base, lb = p.g_first + p.g_local - 1 - base;
-    if (la >= 0 && la < 64) a = __builtin_amdgcn_readlane(first, la);
-    if (lb >= 0 && lb < 64) b = __builtin_amdgcn_readlane(end, lb);
-    return lb < 64;
-  });
-  *first_row = a; *end_row = b;
-}
+using int4_detail::load_at;
+using int4_detail::scalar_base;
+using int4_detail::scale_to_f32;
 
 // ---- arithmetic ----------------------------------------------------------------------------------------------------------
 template <bool HALF>
@@ -112,41 +51,17 @@ __device__ __forceinline__ u32x4_t insert_element(u32x4_t v, int i, uint32_t e) 
   return v;
 }
 
-// A pointer that all lanes share, kept in scalar registers whatever is added to it.
-__device__ __forceinline__ const char* scalar_base(const void* p, size_t offset) {
-  uint64_t b = reinterpret_cast<uint64_t>(p) + offset;
-  asm("" : "+s"(b));
-  return reinterpret_cast<const char*>(b);
-}
-template <class V>
-__device__ __forceinline__ V load_at(const char* base, uint32_t offset) {
-  typedef const __attribute__((address_space(1))) char* global_bytes;
-  typedef V unaligned_t __attribute__((aligned(2)));
-  return *reinterpret_cast<const __attribute__((address_space(1))) unaligned_t*>((global_bytes)base + offset);
-}
-
-__device__ __forceinline__ float scale_to_f32(uint32_t bits, bool half) {
-  const float b = bf16_to_f32((bf16_bits)bits), h = (float)__builtin_bit_cast(f16_t, (uint16_t)bits);
-  return half ? h : b;
-}
-
 // ---- streaming kernel ------------------------------------------------------------------------------------------------------
 // A work-group computes up to 64 rows of a group x 64 columns.  Its four waves take every fourth run of 128 contraction indices
 // and add up their sums in LDS; a wave has the next run's loads in flight while it multiplies the present one.
 constexpr int kInt4Threads = 256, kInt4Waves = 4, kInt4Cols = 64, kInt4Rows = 64, kInt4Strips = kInt4Cols / kInt4Strip;
 
-template <int BYTES> struct BlockBits;  // what a run's blocks have of scales or zeros
-template <> struct BlockBits<1> { typedef uint8_t type; };
-template <> struct BlockBits<2> { typedef uint16_t type; };
-template <> struct BlockBits<4> { typedef uint32_t type; };
-template <> struct BlockBits<8> { typedef uint64_t type; };
-
 // NT: row tiles of 16
 template <int BLOCK>
 struct Int4Run {
   static constexpr int PER = kInt4Run / BLOCK;
-  typedef typename BlockBits<2 * PER>::type Scales;
-  typedef typename BlockBits<PER>::type Zeros;
+  typedef typename int4_detail::Bits<2 * PER>::type Scales;
+  typedef typename int4_detail::Bits<PER>::type Zeros;
   u32x4_t codes[kInt4Strips];
   Scales scales[kInt4Strips];
   Zeros zeros[kInt4Strips];
@@ -178,7 +93,7 @@ __device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const Row
       const size_t strip = (size_t)imin(c, (cols - 1) / kInt4Strip) * runs + r;
       d.codes[c] = load_at<u32x4_t>(scalar_base(p.codes, codes0 + strip * 1024), lane * 16u);
       d.scales[c] = load_at<typename Run::Scales>(scales, column[c] * (uint32_t)sizeof(typename Run::Scales));
-      if constexpr (ZEROS) d.zeros[c] = *reinterpret_cast<const typename Run::Zeros*>(zeros + column[c] * (uint32_t)sizeof(typename Run::Zeros));
+      if constexpr (ZEROS) d.zeros[c] = load_at<typename Run::Zeros>(zeros, column[c] * (uint32_t)sizeof(typename Run::Zeros));
     }
     return d;
   };
@@ -363,9 +278,18 @@ int stream(hipStream_t s, const Int4Problem& p, int most) {
   return (int)hipGetLastError();
 }
 
+// Groups of more rows than this are left to the tile kernel.
+int kInt4StreamRows() { static int v = getenv("RD_T") ? atoi(getenv("RD_T")) : 32; return v; }
+
 template <bool HALF, int BLOCK>
 int gmm_int4(hipStream_t s, const Int4Problem& p) {
-  return p.zeros ? stream<HALF, BLOCK, true>(s, p, p.m) : stream<HALF, BLOCK, false>(s, p, p.m);
+  int most = p.m;
+  if (p.m > kInt4StreamRows() && p.k >= 8 && p.k <= (1 << 22)) {
+    most = kInt4StreamRows();
+    const int rc = launch_int4_tiles<HALF, BLOCK>(s, p, most + 1);
+    if (rc != hipSuccess) return rc;
+  }
+  return p.zeros ? stream<HALF, BLOCK, true>(s, p, most) : stream<HALF, BLOCK, false>(s, p, most);
 }
 template <bool HALF>
 int gmm_int4(hipStream_t s, const Int4Problem& p) {

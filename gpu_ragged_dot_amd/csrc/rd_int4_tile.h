@@ -1,0 +1,280 @@
+// GEMM core of the ragged product on 4-bit weights, for groups of many rows: y[t, c] = sum_kk x[t, kk] A[kk, c] with A =
+// scale (q - zero) made from its codes (layout in rd_int4.h) on the way into LDS.
+//
+// A tile of BM x 256 held by a 2 x 2 grid of waves, in 64-wide slabs; x goes HBM -> registers -> LDS as in rd_gemm_rs.h, at any
+// pitch and address, two slabs in LDS and two in registers.  A lane owns four pieces of a run of 128 indices (16 bytes, 32 codes,
+// each), with two runs in registers, and turns half of each into 16-bit weights per slab: eight words to 128 bytes of LDS, in the
+// chunk order that the fragment reads undo.  So a code is converted once per row tile and not once per wave.
+//  * A word costs 23 vector instructions (two masks and a shift, eight byte-to-float conversions, eight fused multiply-adds with scale
+//    and -scale zero, four packs), spread a pair of weights at a time over the gaps between matrix-core instructions, which leave
+//    seven issue slots each: 184 a slab beside 64 of those for BM 256.
+//  * The weight is rounded to the rows' type, once: scale (q - zero) itself is exact in fp32 (scale has at most 11 bits, the
+//    difference 5).  Kept exact, as in the streaming kernel, the sums of every block would have to be scaled apart - three vector
+//    instructions per accumulator and block of 128, more than the matrix-core instructions leave.
+#pragma once
+#include "rd_gemm_rs.h"
+#include "rd_int4.h"
+
+namespace rd {
+
+template <int BM_, bool HALF_, int BLOCK_>
+struct Int4TileCfg {
+  typedef typename std::conditional<HALF_, f16_t, bf16_bits>::type Elem;
+  static constexpr bool HALF = HALF_;
+  static constexpr int BM = BM_, BN = 256, BK = 64, BLOCK = BLOCK_, NW = 4, NT = 256;
+  static constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
+  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, SLOT_BYTES = A_BYTES + B_BYTES;
+  static constexpr int EPI_PITCH = WN * 2 + 16, EPI_BYTES = NW * WM * EPI_PITCH;
+  static constexpr int LDS_BYTES = 2 * SLOT_BYTES > EPI_BYTES ? 2 * SLOT_BYTES : EPI_BYTES;
+  static constexpr int PER_RUN = kInt4Run / BLOCK;  // scales of a column per run
+  static_assert(BM % 64 == 0 && LDS_BYTES <= 160 * 1024, "tile shape");
+};
+
+// What a tile reads of the weights.
+struct Int4Columns {
+  const char* codes;   // of the tile's first strip, run 0
+  const char* scales;  // of the group's run 0, column 0
+  const char* zeros;   // the same; where there are none, any memory as large
+  int first, n;        // the tile's first column; columns of the matrix
+  int runs;
+  bool has_zeros, scale_half;
+};
+
+namespace int4_detail {
+template <int V>
+struct Int { static constexpr int value = V; };
+
+template <int BYTES> struct Bits;
+template <> struct Bits<1> { typedef uint8_t type; };
+template <> struct Bits<2> { typedef uint16_t type; };
+template <> struct Bits<4> { typedef uint32_t type; };
+template <> struct Bits<8> { typedef uint64_t type; };
+
+// A pointer that all lanes share, kept in scalar registers whatever is added to it, and a load at a lane's offset from it.
+__device__ __forceinline__ const char* scalar_base(const void* p, size_t offset) {
+  uint64_t b = reinterpret_cast<uint64_t>(p) + offset;
+  asm("" : "+s"(b));
+  return reinterpret_cast<const char*>(b);
+}
+template <class V>
+__device__ __forceinline__ V load_at(const char* base, uint32_t offset) {
+  typedef const __attribute__((address_space(1))) char* global_bytes;
+  typedef V unaligned_t __attribute__((aligned(sizeof(V) < 2 ? 1 : 2)));
+  return *reinterpret_cast<const __attribute__((address_space(1))) unaligned_t*>((global_bytes)base + offset);
+}
+
+__device__ __forceinline__ float scale_to_f32(uint32_t bits, bool half) {
+  const float b = bf16_to_f32((bf16_bits)bits), h = (float)__builtin_bit_cast(f16_t, (uint16_t)bits);
+  return half ? h : b;
+}
+}  // namespace int4_detail
+
+template <class C>
+__device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restrict__ Ap, int lda, int a_lim, const Int4Columns& b, int klen,
+                                                unsigned char* smem, int wave, int lane, f32x16_t (&acc)[C::TM][C::TN]) {
+  using int4_detail::Int;
+  const int wm = wave >> 1, wn = wave & 1;
+  typedef RsLoader<C::BM, C::BK, C::NW, true, typename C::Elem, false> LdA;
+  LdA la;
+  la.init(Ap, lda, a_lim, klen, wave, lane);
+  DldsFragReader<C::BM, C::BK, C::TM, true> fra;
+  DldsFragReader<C::BN, C::BK, C::TN, true> frb;
+  fra.init(wm * C::WM, lane);
+  frb.init(wn * C::WN, lane);
+  const int nk = (klen + C::BK - 1) / C::BK;
+
+  // ---- x: piece q of the loader's slab -> a[SET][q]; a[SET][q] -> LDS ----
+  constexpr int PA = LdA::PER;
+  u32x4_t a[2][PA];
+  auto fetch_a = [&](auto set, int q) { a[decltype(set)::value][q] = la.fetch(q); };
+  auto commit_a = [&](auto set, int slot, int q) { la.commit(smem + slot, q, a[decltype(set)::value][q]); };
+  auto trim_a = [&](auto set, int step, int first, int count) {
+    constexpr int SET = decltype(set)::value;
+    if (step >= nk - 1) {
+      asm volatile("");  // (a branch, not selects in every slab)
+#pragma unroll
+      for (int q = first; q < first + count; ++q) a[SET][q] = la.trim(wave, lane, q, step, a[SET][q]);
+    }
+  };
+
+  // ---- weights: piece i of a run is strip wave + 4 i of the tile, lane 16 h + c its column c and pieces' h ----
+  typedef typename int4_detail::Bits<2 * C::PER_RUN>::type Scales;
+  typedef typename int4_detail::Bits<C::PER_RUN>::type Zeros;
+  u32x4_t codes[2][4];
+  Scales scales[2][4];
+  Zeros zeros[2][4];
+  const int c = lane & 15, h = lane >> 4, last_strip = int4_strips(b.n) - 1 - b.first / kInt4Strip;
+  uint32_t column[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) column[i] = (uint32_t)imin(b.first + kInt4Strip * (wave + 4 * i) + c, b.n - 1);
+  auto fetch_b = [&](auto set, int run, int i) {
+    constexpr int SET = decltype(set)::value;
+    const int r = imin(run, b.runs - 1);  // (behind the last run x is zero)
+    const size_t strip = (size_t)imin(wave + 4 * i, last_strip) * b.runs + r;
+    codes[SET][i] = int4_detail::load_at<u32x4_t>(int4_detail::scalar_base(b.codes, strip * 1024), lane * 16u);
+    const size_t at = (size_t)r * b.n;
+    scales[SET][i] = int4_detail::load_at<Scales>(int4_detail::scalar_base(b.scales, at * sizeof(Scales)), column[i] * (uint32_t)sizeof(Scales));
+    zeros[SET][i] = int4_detail::load_at<Zeros>(int4_detail::scalar_base(b.zeros, at * sizeof(Zeros)), column[i] * (uint32_t)sizeof(Zeros));
+  };
+  // Where a word's weights go: row `column of the tile`, chunk (j & 1) 4 + h, permuted as DldsFragReader reads it.
+  const int b_row = kInt4Strip * wave + c, b_sw = (b_row >> 1) & 7;  // (strips four apart: the permutation repeats)
+  int b_at[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) b_at[j] = C::A_BYTES + b_row * 128 + (((4 * j + h) ^ b_sw) << 4);
+  // Step st of word w (of the slab's half HALF_RUN) of piece i: a pair of weights; with the last one all eight are written.
+  float s = 0.f, sz = 0.f;
+  uint32_t low = 0, high = 0;
+  u32x4_t out;
+  constexpr int kSteps = 4;
+  auto convert = [&](auto set, auto half_run, int slot, int i, int w, int st) {
+    constexpr int SET = decltype(set)::value, J0 = 2 * decltype(half_run)::value;
+    const int j = J0 + w;
+    if (st == 0) {
+      if (w == 0 || C::BLOCK == 32) {
+        const int e = j * 32 / C::BLOCK;
+        s = int4_detail::scale_to_f32((uint32_t)(scales[SET][i] >> (16 * e)) & 0xffff, b.scale_half);
+        const float z = (float)((uint32_t)(zeros[SET][i] >> (8 * e)) & 0xff);
+        sz = -s * (b.has_zeros ? z : 8.f);
+      }
+      const uint32_t word = codes[SET][i][j];
+      low = word & 0x0f0f0f0fu;
+      high = (word >> 4) & 0x0f0f0f0fu;
+      asm("" : "+v"(low), "+v"(high));  // (the compiler would take every code out of the word by itself, an instruction each)
+    }
+    // codes 0, 4, 1, 5 are the bytes of `low`, 2, 6, 3, 7 those of `high`
+    const uint32_t from = (st & 1) ? high : low;
+    const int byte = st >> 1;
+    const float u = (float)((from >> (8 * byte)) & 0xff), v = (float)((from >> (8 * byte + 16)) & 0xff);
+    out[st] = pack_out_x2<C::HALF>(__builtin_fmaf(u, s, sz), __builtin_fmaf(v, s, sz));
+    if (st == kSteps - 1) *reinterpret_cast<u32x4_t*>(smem + slot + b_at[w] + i * 4 * kInt4Strip * 128) = out;
+  };
+
+  constexpr auto part = [](int u) constexpr { return u * PA / 4; };
+  constexpr int HEAD = part(1);
+
+  // ---- slab 0 in LDS, slab 1 in registers with its first quarter written, slab 2 requested; runs 0 and 1 ----
+#pragma unroll
+  for (int i = 0; i < 4; ++i) fetch_b(Int<0>{}, 0, i);
+#pragma unroll
+  for (int q = 0; q < PA; ++q) fetch_a(Int<0>{}, q);
+  la.advance(wave, lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) fetch_b(Int<1>{}, 1, i);
+#pragma unroll
+  for (int q = 0; q < PA; ++q) fetch_a(Int<1>{}, q);
+  la.advance(wave, lane);
+  trim_a(Int<0>{}, 0, 0, PA);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) convert(Int<0>{}, Int<0>{}, 0, i, w, st);
+#pragma unroll
+  for (int q = 0; q < PA; ++q) commit_a(Int<0>{}, 0, q);
+#pragma unroll
+  for (int q = 0; q < PA; ++q) fetch_a(Int<0>{}, q);
+  la.advance(wave, lane);
+  trim_a(Int<1>{}, 1, 0, HEAD);
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) convert(Int<0>{}, Int<1>{}, C::SLOT_BYTES, 0, w, st);
+  fetch_b(Int<0>{}, 2, 0);
+#pragma unroll
+  for (int q = 0; q < HEAD; ++q) commit_a(Int<1>{}, C::SLOT_BYTES, q);
+#pragma unroll
+  for (int q = 0; q < HEAD; ++q) fetch_a(Int<1>{}, q);
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): slab 0 is written
+  __builtin_amdgcn_s_barrier();
+
+  bf16x8_t fa[2][C::TM], fb[2][C::TN];
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i) fa[0][i] = fra.read(smem, i, 0);
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) fb[0][j] = frb.read(smem + C::A_BYTES, j, 0);
+
+  // Slab t, PHASE = t & 3.  Substeps 0 .. 2 write quarters 1 .. 3 of slab t + 1, substep 3, behind the slab's barrier, quarter 0 of
+  // slab t + 2 into the slot that slab t has left.  A piece of x is followed by its load two slabs on, a piece of a run, once its
+  // second half is written, by its load two runs on.
+  auto slab = [&](int t, auto phase) {
+    constexpr int PHASE = decltype(phase)::value, CUR = PHASE & 1, NEXT = 1 - CUR;
+    constexpr int cur_off = CUR * C::SLOT_BYTES, next_off = NEXT * C::SLOT_BYTES;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool last = u == 3;
+      if (last) {  // own reads of slab t returned, own part of slab t + 1 written; behind the barrier slab t + 1 is complete
+        la.advance(wave, lane);
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const unsigned char* ra = smem + (last ? next_off : cur_off);  // fragments of the next substep
+      const int us = last ? 0 : u + 1, quarter = last ? 0 : u + 1;
+      const int first = part(quarter), count = part(quarter + 1) - part(quarter);
+      if (last) trim_a(Int<CUR>{}, t + 2, first, count);
+      else trim_a(Int<NEXT>{}, t + 1, first, count);
+      // ops of the substep: a fragment read and a step of a conversion in turn, then what moves of x and of the runs
+      constexpr int FR = C::TM + C::TN, CV = 2 * kSteps, MF = C::TM * C::TN;
+      const int ops = FR + CV + 2 * count + 1;
+      auto op = [&](int o) {
+        constexpr int BOTH = FR < CV ? FR : CV;
+        const bool paired = o < 2 * BOTH;
+        const int read = paired ? (o % 2 == 0 ? o / 2 : -1) : FR > CV && o < FR + CV ? o - CV : -1;
+        const int conv = paired ? (o % 2 == 1 ? o / 2 : -1) : CV > FR && o < FR + CV ? o - FR : -1;
+        if (read >= 0) {
+          if (read < C::TM) fa[(u + 1) & 1][read] = fra.read(ra, read, us);
+          else fb[(u + 1) & 1][read - C::TM] = frb.read(ra + C::A_BYTES, read - C::TM, us);
+        } else if (conv >= 0) {
+          // slab t + 2: run (t + 2) / 2, half t & 1; slab t + 1: run (t + 1) / 2, half (t + 1) & 1
+          if (last) convert(Int<((PHASE + 2) >> 1) & 1>{}, Int<CUR>{}, cur_off, quarter, conv / kSteps, conv % kSteps);
+          else convert(Int<((PHASE + 1) >> 1) & 1>{}, Int<NEXT>{}, next_off, quarter, conv / kSteps, conv % kSteps);
+        } else if (o < FR + CV + 2 * count) {
+          const int q = first + (o - FR - CV) / 2;
+          const bool write = (o - FR - CV) % 2 == 0;
+          if (last) { if (write) commit_a(Int<CUR>{}, cur_off, q); else fetch_a(Int<CUR>{}, q); }
+          else { if (write) commit_a(Int<NEXT>{}, next_off, q); else fetch_a(Int<NEXT>{}, q); }
+        } else if (last ? CUR == 1 : NEXT == 1) {  // a second half has just been written
+          if (last) fetch_b(Int<((PHASE + 2) >> 1) & 1>{}, ((t + 2) >> 1) + 2, quarter);
+          else fetch_b(Int<((PHASE + 1) >> 1) & 1>{}, ((t + 1) >> 1) + 2, quarter);
+        }
+      };
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
+#pragma unroll
+        for (int o = m * ops / MF; o < (m + 1) * ops / MF; ++o) op(o);
+        const int i = m / C::TN, j = m % C::TN;
+        acc[i][j] = mfma_32x32x16<C::HALF>(fb[u & 1][j], fa[u & 1][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // (an nk that is no multiple of four multiplies up to three slabs of zeros: a way out of the middle of the loop had the compiler
+  // hold two sets of accumulators, 600 registers spilled)
+  for (int t = 0; t < nk; t += 4) {
+    slab(t, Int<0>{});
+    slab(t + 1, Int<1>{});
+    slab(t + 2, Int<2>{});
+    slab(t + 3, Int<3>{});
+  }
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_s_barrier();  // the slots are no longer read by any wave
+}
+
+// rows x min(256, n - first column) of y at Op (row pitch n); klen >= 8.
+template <class C>
+__device__ __forceinline__ void int4_tile(const void* Ap, int lda, int rows, const Int4Columns& b, int klen, void* Op, unsigned char* smem) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  f32x16_t acc[C::TM][C::TN];
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+  int4_tile_kloop<C>(static_cast<const typename C::Elem*>(Ap), lda, rows, b, klen, smem, wave, lane, acc);
+  rs_store16<C>(acc, wave >> 1, wave & 1, wave, lane, rows, imin(C::BN, b.n - b.first), static_cast<typename C::Elem*>(Op), b.n, smem);
+}
+
+}  // namespace rd
