@@ -108,6 +108,7 @@ EXPORTS = (
     "rd_moe_swiglu_grad",
     "rd_int4_codes_bytes",
     "rd_int4_pack",
+    "rd_gmm_int4_workspace_bytes",
     "rd_gmm_int4",
 )
 
@@ -180,7 +181,9 @@ def _load() -> ctypes.CDLL:
     lib.rd_int4_codes_bytes.restype = sz
     lib.rd_int4_pack.argtypes = [vp, vp, vp, i, i, i, i]
     lib.rd_int4_pack.restype = i
-    lib.rd_gmm_int4.argtypes = [vp, vp, vp, vp, vp, ip, vp, i, i, i, i, i, i, i, i, i]
+    lib.rd_gmm_int4_workspace_bytes.argtypes = [i, i, i, i]
+    lib.rd_gmm_int4_workspace_bytes.restype = sz
+    lib.rd_gmm_int4.argtypes = [vp, vp, vp, vp, vp, ip, vp, i, i, i, i, i, i, i, i, i, vp, sz]
     lib.rd_gmm_int4.restype = i
     return lib
 

@@ -1291,9 +1291,14 @@ int rd_int4_pack(void* stream, const uint8_t* q, void* codes, int g, int k, int 
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "int4_pack launch");
 }
 
+size_t rd_gmm_int4_workspace_bytes(int m, int k, int n, int g) {
+  if (m < 0 || k < 0 || n < 0 || g < 1) return 0;
+  return align_up(rd::int4_workspace_bytes(m, k, n, g), 256);
+}
+
 int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scales, const uint8_t* zeros,
                 const int32_t* group_sizes, void* y, int m, int k, int n, int g_total, int group_offset, int g_local, int block,
-                int scale_dtype, int dtype) {
+                int scale_dtype, int dtype, void* workspace, size_t workspace_bytes) {
   int rc = check_int4_weights(codes, g_local, k, n);
   if (rc != RD_OK) return rc;
   if (m < 0 || m > rd::kInt4MaxRows) return fail(RD_ERR_INVALID_ARGUMENT, "m=%d outside 0..%d", m, rd::kInt4MaxRows);
@@ -1307,8 +1312,12 @@ int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scal
   if (!group_sizes || !y || (k > 0 && (!x || !scales))) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
   if ((reinterpret_cast<uintptr_t>(scales) & 7) != 0 || (reinterpret_cast<uintptr_t>(zeros) & 3) != 0)
     return fail(RD_ERR_INVALID_ARGUMENT, "the scales are not 8-byte aligned or the zeros not 4-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail(RD_ERR_WORKSPACE, "workspace misaligned");
+  const size_t needed = rd::int4_workspace_bytes(m, k, n, g_total);
+  float* partials = workspace && needed > 0 && workspace_bytes >= needed ? static_cast<float*>(workspace) : nullptr;
+  int32_t* counters = partials ? reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + rd::kInt4PartialBytes) : nullptr;
   const rd::Int4Problem p = {x, static_cast<const uint32_t*>(codes), scales, zeros, group_sizes, y, m, k, n, g_total, group_offset, g_local,
-                             block, scale_dtype == RD_DTYPE_F16, dtype == RD_DTYPE_F16};
+                             block, scale_dtype == RD_DTYPE_F16, dtype == RD_DTYPE_F16, partials, counters};
   if (!rd::int4_grid_fits(p)) return fail(RD_ERR_UNSUPPORTED, "m=%d rows of n=%d in %d groups are more tiles than a launch has", m, n, g_total);
   rc = rd::launch_gmm_int4((hipStream_t)stream, p);
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "gmm_int4 launch");

@@ -5,7 +5,6 @@
 // A code becomes the 16-bit number v = 1 + q / 16, exactly, by a shift and an and-or for two of them; the matrix cores sum
 // x v over a block, and x itself against ones; then  y += 16 scale (sum x v) - scale (16 + zero) (sum x).  So products are
 // exact, sums are fp32, and nothing is rounded to 16 bits before the result.
-#include <stdlib.h>
 #include "rd_elem.h"
 #include "rd_int4_rows.h"
 #include "rd_int4_tile.h"
@@ -221,6 +220,7 @@ __global__ __launch_bounds__(kInt4Threads, ROWS == 16 ? 4 : 2) void gmm_int4_str
   if ((int)blockIdx.x >= tiles * col_tiles) {
     int first, end;
     held_rows(p, &first, &end);
+    if (p.partials && (int)blockIdx.x == tiles * col_tiles && threadIdx.x < kInt4Slots) p.counters[threadIdx.x] = 0;  // of the tile kernel behind this one
     const int r0 = ((int)blockIdx.x - tiles * col_tiles) * kInt4Rows;
     for (int r = r0; r < imin(r0 + kInt4Rows, p.m); ++r)
       if (r < first || r >= end)
@@ -278,18 +278,29 @@ int stream(hipStream_t s, const Int4Problem& p, int most) {
   return (int)hipGetLastError();
 }
 
-// Groups of more rows than this are left to the tile kernel.
-int kInt4StreamRows() { static int v = getenv("RD_T") ? atoi(getenv("RD_T")) : 32; return v; }
+// Whether groups of more than kInt4Rows rows are left to the tile kernel, a launch of its own.  The sizes are on the device; the rule
+// takes them to be equal, and what each kernel needs for that, us, from rounds of what the device holds at a time: 512 work-groups of
+// 64 rows x 64 columns of the streaming kernel at 8.5 per 1024 indices (half as much for 32 rows), 256 tiles of the other at 1.1 ..
+// 2.0 a slab of 64 by their height.  bf16, blocks of 128, streaming | tiles: 4 groups of 512 x 2048 x 2048 41 | 57, 8 of 256 x
+// 4096 x 4096 129 | 105, 12 of 256 x 1024 x 1536 30 | 43, 32 of 72 x 7168 x 2048 207 | 139, 64 of 128 x 2048 x 1024 74 | 52.  Where the
+// streaming kernel is long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
+bool uses_tiles(int m, int k, int n, int g) {
+  if (m <= kInt4Rows || k < 8 || k > (1 << 22)) return false;
+  const double rows = (double)((m + g - 1) / g), cols64 = (n + 63) / 64, cols256 = (n + 255) / 256;
+  const double rounds = g * ceil(rows / 64) * cols64 / 512;
+  const double streaming = 6 + ceil(rounds) * k * 0.0083 * (rows <= 32 ? 0.55 : 1);
+  if (streaming > 100) return true;
+  if (rows <= kInt4Rows) return false;
+  const double last = rows - 256 * floor(rows / 256), height = last == 0 ? 0 : last <= 64 ? 1.1 : last <= 128 ? 1.3 : last <= 192 ? 1.65 : 2;
+  const double work = g * cols256 * (2 * floor(rows / 256) + height) / 256, least = rows >= 256 ? 2 : height;
+  return 12 + k / 64 * (work > least ? work : least) < streaming;
+}
 
 template <bool HALF, int BLOCK>
 int gmm_int4(hipStream_t s, const Int4Problem& p) {
-  int most = p.m;
-  if (p.m > kInt4StreamRows() && p.k >= 8 && p.k <= (1 << 22)) {
-    most = kInt4StreamRows();
-    const int rc = launch_int4_tiles<HALF, BLOCK>(s, p, most + 1);
-    if (rc != hipSuccess) return rc;
-  }
-  return p.zeros ? stream<HALF, BLOCK, true>(s, p, most) : stream<HALF, BLOCK, false>(s, p, most);
+  const int most = uses_tiles(p.m, p.k, p.n, p.g) ? kInt4Rows : p.m;
+  const int rc = p.zeros ? stream<HALF, BLOCK, true>(s, p, most) : stream<HALF, BLOCK, false>(s, p, most);
+  return rc != hipSuccess || most == p.m ? rc : launch_int4_tiles<HALF, BLOCK>(s, p, most + 1);
 }
 template <bool HALF>
 int gmm_int4(hipStream_t s, const Int4Problem& p) {
@@ -302,6 +313,10 @@ int launch_int4_pack(hipStream_t s, const uint8_t* q, uint32_t* codes, int g, in
   const long long words = (long long)g * int4_strips(n) * int4_runs(k) * 256;
   hipLaunchKernelGGL(int4_pack_kernel, dim3((unsigned)(words < (1ll << 24) ? (words + 255) / 256 : 1 << 16)), dim3(256), 0, s, q, codes, words, k, n, trans_rhs);
   return (int)hipGetLastError();
+}
+
+size_t int4_workspace_bytes(int m, int k, int n, int g) {
+  return uses_tiles(m, k, n, g) && n > 0 ? kInt4PartialBytes + kInt4Slots * sizeof(int32_t) : 0;
 }
 
 bool int4_grid_fits(const Int4Problem& p) { return stream_grid(p, p.m).blocks < (1ll << 31) / kInt4Threads; }

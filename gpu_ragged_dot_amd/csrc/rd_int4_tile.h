@@ -27,16 +27,17 @@ struct Int4TileCfg {
   static constexpr int EPI_PITCH = WN * 2 + 16, EPI_BYTES = NW * WM * EPI_PITCH;
   static constexpr int LDS_BYTES = 2 * SLOT_BYTES > EPI_BYTES ? 2 * SLOT_BYTES : EPI_BYTES;
   static constexpr int PER_RUN = kInt4Run / BLOCK;  // scales of a column per run
+  static constexpr bool DLDS = true;  // (splitk_combine(): four waves with many accumulators take 16 vectors of two pieces at a time)
   static_assert(BM % 64 == 0 && LDS_BYTES <= 160 * 1024, "tile shape");
 };
 
 // What a tile reads of the weights.
 struct Int4Columns {
-  const char* codes;   // of the tile's first strip, run 0
-  const char* scales;  // of the group's run 0, column 0
+  const char* codes;   // of the tile's first strip and first run
+  const char* scales;  // of the group's first run, column 0
   const char* zeros;   // the same; where there are none, any memory as large
   int first, n;        // the tile's first column; columns of the matrix
-  int runs;
+  int runs, stride;    // the tile's runs; runs from one strip to the next
   bool has_zeros, scale_half;
 };
 
@@ -93,7 +94,8 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
     if (step >= nk - 1) {
       asm volatile("");  // (a branch, not selects in every slab)
 #pragma unroll
-      for (int q = first; q < first + count; ++q) a[SET][q] = la.trim(wave, lane, q, step, a[SET][q]);
+      for (int q = 0; q < PA; ++q)
+        if (q >= first && q < first + count) a[SET][q] = la.trim(wave, lane, q, step, a[SET][q]);
     }
   };
 
@@ -110,7 +112,7 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
   auto fetch_b = [&](auto set, int run, int i) {
     constexpr int SET = decltype(set)::value;
     const int r = imin(run, b.runs - 1);  // (behind the last run x is zero)
-    const size_t strip = (size_t)imin(wave + 4 * i, last_strip) * b.runs + r;
+    const size_t strip = (size_t)imin(wave + 4 * i, last_strip) * b.stride + r;
     codes[SET][i] = int4_detail::load_at<u32x4_t>(int4_detail::scalar_base(b.codes, strip * 1024), lane * 16u);
     const size_t at = (size_t)r * b.n;
     scales[SET][i] = int4_detail::load_at<Scales>(int4_detail::scalar_base(b.scales, at * sizeof(Scales)), column[i] * (uint32_t)sizeof(Scales));
@@ -150,7 +152,7 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
   };
 
   constexpr auto part = [](int u) constexpr { return u * PA / 4; };
-  constexpr int HEAD = part(1);
+  constexpr int HEAD = part(1), HEAD_MOST = (PA + 3) / 4;
 
   // ---- slab 0 in LDS, slab 1 in registers with its first quarter written, slab 2 requested; runs 0 and 1 ----
 #pragma unroll
@@ -243,7 +245,8 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
 #pragma unroll
       for (int m = 0; m < MF; ++m) {
 #pragma unroll
-        for (int o = m * ops / MF; o < (m + 1) * ops / MF; ++o) op(o);
+        for (int o = 0; o < FR + CV + 2 * HEAD_MOST + 1; ++o)
+          if (o >= m * ops / MF && o < (m + 1) * ops / MF) op(o);
         const int i = m / C::TN, j = m % C::TN;
         acc[i][j] = mfma_32x32x16<C::HALF>(fb[u & 1][j], fa[u & 1][i], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
@@ -264,7 +267,8 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
 
 // rows x min(256, n - first column) of y at Op (row pitch n); klen >= 8.
 template <class C>
-__device__ __forceinline__ void int4_tile(const void* Ap, int lda, int rows, const Int4Columns& b, int klen, void* Op, unsigned char* smem) {
+__device__ __forceinline__ void int4_tile(const void* Ap, int lda, int rows, const Int4Columns& b, int klen, void* Op, unsigned char* smem,
+                                          const SplitK& sk) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x16_t acc[C::TM][C::TN];
 #pragma unroll
@@ -274,6 +278,7 @@ __device__ __forceinline__ void int4_tile(const void* Ap, int lda, int rows, con
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
   int4_tile_kloop<C>(static_cast<const typename C::Elem*>(Ap), lda, rows, b, klen, smem, wave, lane, acc);
+  if (!splitk_combine<C>(acc, sk, threadIdx.x, smem)) return;
   rs_store16<C>(acc, wave >> 1, wave & 1, wave, lane, rows, imin(C::BN, b.n - b.first), static_cast<typename C::Elem*>(Op), b.n, smem);
 }
 

@@ -276,12 +276,16 @@ int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, 
  *   zeros:  bytes of the same shape, 4-byte aligned, or NULL: 8 throughout.
  * x and y are RD_DTYPE_BF16 or RD_DTYPE_F16.  group_sizes, the rows past their sum (zero), clipping at m, group_offset and g_local
  * are those of rd_gmm_sharded.  fp32 sums, one rounding of the result.  An infinity in x makes its row NaN.
- * m < 2^25.  No workspace.  No gradients. */
+ * m < 2^25.  No gradients.
+ * Workspace (optional): rd_gmm_int4_workspace_bytes() bytes, 256-byte aligned, for fp32 partial sums where tiles that do not fill
+ * the device's last round are cut along k; with NULL or a smaller one none are.  So the last bits of a row may follow from the other
+ * groups' sizes, as in rd_gmm. */
 size_t rd_int4_codes_bytes(int g, int k, int n);
 int rd_int4_pack(void* stream, const uint8_t* q, void* codes, int g, int k, int n, int trans_rhs);
+size_t rd_gmm_int4_workspace_bytes(int m, int k, int n, int g);
 int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scales, const uint8_t* zeros,
                 const int32_t* group_sizes, void* y, int m, int k, int n, int g_total, int group_offset, int g_local, int block,
-                int scale_dtype, int dtype);
+                int scale_dtype, int dtype, void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

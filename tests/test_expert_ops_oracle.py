@@ -110,8 +110,8 @@ def test_swiglu_refusals():
     assert lib.rd_moe_swiglu(None, None, None, 0, 8, 0) == 0 and lib.rd_moe_swiglu(None, None, None, 8, 0, 0) == 0
 
 
-def _int4(x=P, codes=P, scales=P, gs=P, y=P, m=4, k=64, n=8, g=2, first=0, local=2, block=32, sdtype=0, dtype=0):
-    return _capi.lib.rd_gmm_int4(None, x, codes, scales, None, gs, y, m, k, n, g, first, local, block, sdtype, dtype)
+def _int4(x=P, codes=P, scales=P, gs=P, y=P, m=4, k=64, n=8, g=2, first=0, local=2, block=32, sdtype=0, dtype=0, ws=None):
+    return _capi.lib.rd_gmm_int4(None, x, codes, scales, None, gs, y, m, k, n, g, first, local, block, sdtype, dtype, ws, 0)
 
 
 @pytest.mark.parametrize("kw", [
@@ -129,6 +129,7 @@ def test_int4_sizes():
     assert lib.rd_int4_codes_bytes(2, 0, 3) == 0 and lib.rd_int4_codes_bytes(-1, 8, 8) == 0
     assert _int4(m=0) == 0 and _int4(n=0) == 0
     assert lib.rd_int4_pack(None, None, P, 1, 32, 8, 0) == -1 and lib.rd_int4_pack(None, P, P + 2, 1, 32, 8, 0) == -1
+    assert _int4(ws=P + 4) == -3 and lib.rd_gmm_int4_workspace_bytes(8, 64, 64, 2) == 0
     assert _int4(m=(1 << 25) - 1, n=1 << 28, g=2) == -2  # more tiles than a launch has
 
 
