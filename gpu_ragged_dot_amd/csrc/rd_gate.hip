@@ -13,9 +13,10 @@
 //  * a row is held by 16 lanes, four rows to a wave, and its ranks are made in 32 bits, as fixed-point numbers of 23 bits with the
 //    expert's index behind them: one unsigned maximum compares rank and index at once, and since no two keys are equal, the next
 //    smaller one is the largest of key - previous (mod 2^32) - a subtraction and half a three-way maximum per expert, nothing to remove;
-//  * whether that decided what 64 bits would decide shows in the keys: where two neighbours among the chosen and the first one left
-//    out, or two clusters, are closer than the error of 32-bit ranks, the wave does that row again in 64 bits (a row in a thousand on
-//    the sizes above).  16-bit logits that rank by themselves are exact in the key: there ties are ties.
+//  * whether that decided what 64 bits would decide shows in the keys.  Where two neighbours among the chosen and the first one left
+//    out are closer than the error of 32-bit ranks (a row in a thousand on the sizes above), the leading 16 are ranked in 64 bits, one
+//    to a lane; where two clusters are, or softmax ranks with a bias, the wave does its rows again in 64 bits.  16-bit logits that rank
+//    by themselves are exact in the key: there ties are ties.
 #include "rd_elem.h"
 #include "rd_moe.h"
 
@@ -343,9 +344,22 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
       }
       const float norm = p.sigmoid ? 1.f : __builtin_amdgcn_rcpf(row_sum(total));
       if (bias) {
+        float bs[PER];
+        if constexpr (VEC && PER >= 4) {
+#pragma unroll
+          for (int i = 0; i < PER; i += 4) {
+            f32x4_t v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (i < own) v = load_any<f32x4_t>(bias + e0 + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bs[i + e] = v[e];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) bs[i] = i < own ? bias[e0 + i] : -INFINITY;
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const float b = i < own ? bias[e0 + i] : -INFINITY;
+          const float b = bs[i];
           least = b == -INFINITY ? least : fminf(least, b);
           most = fmaxf(most, b);
           odd |= !(b < INFINITY);  // NaN, infinity
@@ -391,32 +405,67 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
     const uint32_t score = !p.top2 ? q1 : q2 ? q1 + q2 : 0u;  // (a sum with a shut expert is -inf)
     const int mine = at / cluster_lanes;
     int ahead = 0;
-    bool close = false;
     for (int q = 0; q < p.clusters; ++q) {
       const uint32_t other = (uint32_t)__shfl((int)score, (lane & 48) + q * cluster_lanes, 64);
       ahead += other > score || (other == score && q < mine) ? 1 : 0;
-      const uint32_t apart = umax(other, score) - umin32(other, score);
-      close |= q != mine && mine < p.clusters && apart <= (p.top2 ? 2 * near : near);
     }
-    // close ones matter on the border of those kept and those not
-    odd |= !exact && close && p.top_clusters < p.clusters;
+    if (!exact && p.top_clusters < p.clusters) {  // the worst of those kept against the best of the others
+      const uint32_t worst = ~row_max(ahead < p.top_clusters && mine < p.clusters ? ~score : 0u);
+      const uint32_t best = row_max(ahead >= p.top_clusters && mine < p.clusters ? score : 0u);
+      odd |= worst - best <= (p.top2 ? 2 * near : near);
+    }
     if (ahead >= p.top_clusters)
 #pragma unroll
       for (int i = 0; i < PER; ++i) key[i] = 0u;
   }
 
-  // ---- the top_k largest keys and the one behind them ----
+  // ---- the top_k largest keys and the one behind them, slot s in lane s ----
   uint32_t previous = ~0u, chosen = 0u;  // (no key is as large: ranks end at 2^23 - 2)
-  for (int s = 0; s <= p.top_k; ++s) {
-    uint32_t below = 0u;  // the largest key - previous, which has wrapped around for every smaller key
+  auto next_key = [&]() {  // the largest key - previous, which has wrapped around for every smaller key
+    uint32_t below = 0u;
 #pragma unroll
     for (int i = 0; i < PER; ++i) below = umax(below, key[i] - previous);
-    const uint32_t next = previous ? row_max(below) + previous : 0u;
-    odd |= !exact && s > 0 && next != 0u && (previous >> kKeyIndexBits) - (next >> kKeyIndexBits) <= near;
-    if (s < p.top_k && at == s) chosen = next;
+    return previous ? row_max(below) + previous : 0u;
+  };
+  bool close = false;
+  for (int s = 0; s <= p.top_k; ++s) {
+    const uint32_t next = next_key();
+    close |= s > 0 && next != 0u && (previous >> kKeyIndexBits) - (next >> kKeyIndexBits) <= near;
+    if (at == s) chosen = next;
     previous = next;
   }
-  int id = chosen ? (int)(kKeyIndexMask - (chosen & kKeyIndexMask)) : -1;
+  close = close && !exact;
+  auto expert_of = [](uint32_t k) { return k ? (int)(kKeyIndexMask - (k & kKeyIndexMask)) : -1; };
+  // Close ones in some row: the leading 16 by their ranks in 64 bits, one to a lane, if the last of them is out of the question.
+  // (Softmax ranks with a bias need the whole row's sum in 64 bits.)
+  if (__ballot(close)) {
+    const uint32_t kth = (uint32_t)__shfl((int)chosen, (lane & 48) + p.top_k - 1, 64);
+    for (int s = p.top_k + 1; s < kRowLanes; ++s) {
+      previous = next_key();
+      if (at == s) chosen = previous;
+    }
+    const bool settled = (!scored || p.sigmoid) && p.top_k < kRowLanes && (previous == 0u || (kth >> kKeyIndexBits) - (previous >> kKeyIndexBits) > near);
+    odd |= close && !settled;
+    const int e = expert_of(chosen);
+    double v = -INFINITY;
+    if (e >= 0) {
+      const float x = to_f32<T>(src[e]);
+      v = scored ? 1.0 / (1.0 + exp(-(double)x)) : (double)x;
+      if (bias) v += bias[e];
+    }
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    int ahead = 0;
+    for (int q = 0; q < kRowLanes; ++q) {
+      const int from = (lane & 48) + q;
+      const uint64_t ob = (uint64_t)(uint32_t)__shfl((int)(uint32_t)bits, from, 64) | (uint64_t)(uint32_t)__shfl((int)(uint32_t)(bits >> 32), from, 64) << 32;
+      const double other = __builtin_bit_cast(double, ob);
+      const int oe = __shfl(e, from, 64);
+      ahead += other > v || (other == v && (oe < e || (oe == e && q < at))) ? 1 : 0;  // (those that are none, among themselves by lane)
+    }
+    const uint32_t sorted = (uint32_t)__builtin_amdgcn_ds_permute(((lane & 48) + ahead) << 2, (int)chosen);
+    if (settled) chosen = sorted;
+  }
+  int id = at < p.top_k ? expert_of(chosen) : -1;
   if (__ballot(odd)) id = choose_wide<T, PER>(src, bias, p, cluster_lanes, scored, at, e0, own, top);
 
   // ---- weights ----
