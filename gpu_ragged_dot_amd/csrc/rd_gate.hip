@@ -555,7 +555,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_grad_kernel(const 
                                                                           const float* __restrict__ weights, const float* __restrict__ dweights,
                                                                           T* __restrict__ dlogits, GateSpec p) {
   constexpr int EPP = 16 / sizeof(T);
-  __shared__ __attribute__((aligned(16))) float rows[kGateThreads / kRowLanes][kRowMaxExperts];
+  __shared__ __attribute__((aligned(16))) float rows[kGateThreads / kRowLanes][kRowMaxExperts + 16];  // (a wave's four rows in banks of their own)
   const int at = threadIdx.x & (kRowLanes - 1), mine = threadIdx.x / kRowLanes;
   const int want = blockIdx.x * (kGateThreads / kRowLanes) + mine, row = imin(want, p.tokens - 1);
   float* d = rows[mine];

@@ -53,7 +53,7 @@ __device__ __forceinline__ u32x4_t insert_element(u32x4_t v, int i, uint32_t e) 
 // ---- streaming kernel ------------------------------------------------------------------------------------------------------
 // A work-group computes up to 64 rows of a group x 64 columns.  Its four waves take every fourth run of 128 contraction indices
 // and add up their sums in LDS; a wave has the next run's loads in flight while it multiplies the present one.
-constexpr int kInt4Threads = 256, kInt4Waves = 4, kInt4Cols = 64, kInt4Rows = 64, kInt4Strips = kInt4Cols / kInt4Strip;
+constexpr int kInt4Threads = 256, kInt4Waves = 4, kInt4Cols = 64, kInt4Rows = 32, kInt4Strips = kInt4Cols / kInt4Strip;
 
 // NT: row tiles of 16
 template <int BLOCK>
@@ -128,68 +128,75 @@ __device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const Row
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int c = 0; c < kInt4Strips; ++c) y[t][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](const Run& d, const u32x4_t (&xv)[NT][4]) {
-    constexpr int STEPS = BLOCK / 32;
+  // A run's blocks, one or two strips at a time; once a fragment of x has met the last strip, the next run's takes its place.
+  auto multiply = [&](const Run& d, u32x4_t (&xv)[NT][4], auto refill, int next_run) {
+    constexpr int STEPS = BLOCK / 32, U = NT == 4 ? 1 : 2;  // strips at a time
+    const char* next = scalar_base(x0, (size_t)next_run * (2 * kInt4Run));
 #pragma unroll
     for (int b = 0; b < Run::PER; ++b) {
       f32x4_t xs[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        xs[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < NT; ++t) xs[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) xs[t] = mfma_16x16x32<HALF>(xv[t][b * STEPS + j], ones<HALF>(), xs[t]);
-      }
+      for (int c = 0; c < kInt4Strips; c += U) {
+        f32x4_t v[U][NT];
 #pragma unroll
-      for (int c = 0; c < kInt4Strips; ++c) {
-        f32x4_t v[NT];
+        for (int j = b * STEPS; j < (b + 1) * STEPS; ++j) {
+          u32x4_t w[U];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) v[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          for (int u = 0; u < U; ++u) w[u] = codes_plus_one<HALF>(d.codes[c + u][j]);
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-          const u32x4_t w = codes_plus_one<HALF>(d.codes[c][b * STEPS + j]);
+          for (int t = 0; t < NT; ++t) {
+            if (c == 0) xs[t] = mfma_16x16x32<HALF>(xv[t][j], ones<HALF>(), xs[t]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) v[t] = mfma_16x16x32<HALF>(xv[t][b * STEPS + j], w, v[t]);
+            for (int u = 0; u < U; ++u) {
+              const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+              v[u][t] = mfma_16x16x32<HALF>(xv[t][j], w[u], j == b * STEPS ? zero : v[u][t]);
+            }
+            if (decltype(refill)::value && c + U == kInt4Strips) xv[t][j] = load_at<u32x4_t>(next, row[t] + 64u * j);
+          }
         }
-        const float s = scale_to_f32((uint32_t)(d.scales[c] >> (16 * b)) & 0xffff, p.scale_half);
-        float plus = 24.f;  // 16 + zero
-        if constexpr (ZEROS) plus = 16.f + (float)((uint32_t)(d.zeros[c] >> (8 * b)) & 0xff);
-        const float s16 = 16.f * s, sz = -s * plus;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int u = 0; u < U; ++u) {
+          const float s = scale_to_f32((uint32_t)(d.scales[c + u] >> (16 * b)) & 0xffff, p.scale_half);
+          float plus = 24.f;  // 16 + zero
+          if constexpr (ZEROS) plus = 16.f + (float)((uint32_t)(d.zeros[c + u] >> (8 * b)) & 0xff);
+          const float s16 = 16.f * s, sz = -s * plus;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[t][c][i] = __builtin_fmaf(s16, v[t][i], __builtin_fmaf(sz, xs[t][i], y[t][c][i]));
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[t][c + u][i] = __builtin_fmaf(s16, v[u][t][i], __builtin_fmaf(sz, xs[t][i], y[t][c + u][i]));
+        }
       }
     }
   };
-  // (more than 16 rows: x, which is read again and again and comes from the caches, is fetched when it is needed - two runs of
-  // it do not fit the registers that two work-groups on a compute unit leave)
   const int whole = p.k / kInt4Run, own = (whole - wave + kInt4Waves - 1) / kInt4Waves;  // whole runs; this wave's
   if (own > 0) {
     // Work-groups begin at runs of their own: strips lie runs x 1 KB apart, a multiple of 4 KB for most k, and all in step they
     // would ask a few memory channels at a time.
     int i = (int)(blockIdx.x % (uint32_t)own);
-    Run now = load(wave + i * kInt4Waves);
+    // two runs in turn, so that nothing that is still on its way is moved from one register to another
+    auto turn = [&]() { i = i + 1 < own ? i + 1 : 0; return wave + i * kInt4Waves; };
+    Run even = load(wave + i * kInt4Waves), odd;
     u32x4_t xv[NT][4];
-    if constexpr (NT == 1) load_x(wave + i * kInt4Waves, xv);
-    for (int left = own; left > 0; --left) {
-      Run next = now;
-      u32x4_t xn[NT][4];
-      const int here = i;
-      if (left > 1) i = i + 1 < own ? i + 1 : 0;
-      if constexpr (NT == 1) load_x(wave + i * kInt4Waves, xn);
-      next = load(wave + i * kInt4Waves);
-      if constexpr (NT > 1) load_x(wave + here * kInt4Waves, xv);
-      multiply(now, xv);
-      now = next;
-      if constexpr (NT == 1)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) xv[0][j] = xn[0][j];
+    load_x(wave + i * kInt4Waves, xv);
+    int left = own;
+    for (; left >= 2; left -= 2) {
+      const int second = turn();
+      odd = load(second);
+      __builtin_amdgcn_sched_barrier(0);  // (the compiler would put these loads off until they are needed)
+      multiply(even, xv, std::true_type(), second);
+      const int third = turn();  // (behind the last run the first one again, for nothing)
+      even = load(third);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(odd, xv, std::true_type(), third);
     }
+    if (left) multiply(even, xv, std::false_type(), 0);
   }
   if (whole < runs && whole % kInt4Waves == wave) {
     u32x4_t xv[NT][4];
     load_x_tail(whole, xv);
-    multiply(load(whole), xv);
+    multiply(load(whole), xv, std::false_type(), whole);
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -215,7 +222,7 @@ __device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const Row
 // no row of a group that the weights hold.
 // ROWS: of a row tile, 16 or 64.
 template <bool HALF, int BLOCK, bool ZEROS, int ROWS>
-__global__ __launch_bounds__(kInt4Threads, ROWS == 16 ? 4 : 2) void gmm_int4_stream_kernel(Int4Problem p, int tiles, int col_tiles, int most) {
+__global__ __launch_bounds__(kInt4Threads, ROWS == 16 ? (ZEROS ? 3 : 4) : 2) void gmm_int4_stream_kernel(Int4Problem p, int tiles, int col_tiles, int most) {
   __shared__ float sums[kInt4Waves][16][kInt4Cols];
   if ((int)blockIdx.x >= tiles * col_tiles) {
     int first, end;
@@ -230,9 +237,7 @@ __global__ __launch_bounds__(kInt4Threads, ROWS == 16 ? 4 : 2) void gmm_int4_str
   const RowTile tile = find_row_tile<ROWS>(p, 1, most, blockIdx.x / col_tiles);
   if (tile.rows == 0) return;
   const int c0 = blockIdx.x % col_tiles * kInt4Cols;
-  if (ROWS == 16) int4_stream_tile<HALF, BLOCK, ZEROS, 1>(p, tile, c0, sums);
-  else if (tile.rows <= 32) int4_stream_tile<HALF, BLOCK, ZEROS, 2>(p, tile, c0, sums);
-  else int4_stream_tile<HALF, BLOCK, ZEROS, 4>(p, tile, c0, sums);
+  int4_stream_tile<HALF, BLOCK, ZEROS, ROWS / 16>(p, tile, c0, sums);
 }
 
 // ---- laying out the weights --------------------------------------------------------------------------------------------------
@@ -278,19 +283,21 @@ int stream(hipStream_t s, const Int4Problem& p, int most) {
   return (int)hipGetLastError();
 }
 
-// Whether groups of more than kInt4Rows rows are left to the tile kernel, a launch of its own.  The sizes are on the device; the rule
+constexpr int kInt4FewRows = 64;
+
+// Whether groups of more than kInt4FewRows rows are left to the tile kernel, a launch of its own.  The sizes are on the device; the rule
 // takes them to be equal, and what each kernel needs for that, us, from rounds of what the device holds at a time: 512 work-groups of
 // 64 rows x 64 columns of the streaming kernel at 8.5 per 1024 indices (half as much for 32 rows), 256 tiles of the other at 1.1 ..
 // 2.0 a slab of 64 by their height.  bf16, blocks of 128, streaming | tiles: 4 groups of 512 x 2048 x 2048 41 | 57, 8 of 256 x
 // 4096 x 4096 129 | 105, 12 of 256 x 1024 x 1536 30 | 43, 32 of 72 x 7168 x 2048 207 | 139, 64 of 128 x 2048 x 1024 74 | 52.  Where the
 // streaming kernel is long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
 bool uses_tiles(int m, int k, int n, int g) {
-  if (m <= kInt4Rows || k < 8 || k > (1 << 22)) return false;
+  if (m <= kInt4FewRows || k < 8 || k > (1 << 22)) return false;
   const double rows = (double)((m + g - 1) / g), cols64 = (n + 63) / 64, cols256 = (n + 255) / 256;
   const double rounds = g * ceil(rows / 64) * cols64 / 512;
   const double streaming = 6 + ceil(rounds) * k * 0.0083 * (rows <= 32 ? 0.55 : 1);
   if (streaming > 100) return true;
-  if (rows <= kInt4Rows) return false;
+  if (rows <= kInt4FewRows) return false;
   const double last = rows - 256 * floor(rows / 256), height = last == 0 ? 0 : last <= 64 ? 1.1 : last <= 128 ? 1.3 : last <= 192 ? 1.65 : 2;
   const double work = g * cols256 * (2 * floor(rows / 256) + height) / 256, least = rows >= 256 ? 2 : height;
   return 12 + k / 64 * (work > least ? work : least) < streaming;
@@ -298,7 +305,7 @@ bool uses_tiles(int m, int k, int n, int g) {
 
 template <bool HALF, int BLOCK>
 int gmm_int4(hipStream_t s, const Int4Problem& p) {
-  const int most = uses_tiles(p.m, p.k, p.n, p.g) ? kInt4Rows : p.m;
+  const int most = uses_tiles(p.m, p.k, p.n, p.g) ? kInt4FewRows : p.m;
   const int rc = p.zeros ? stream<HALF, BLOCK, true>(s, p, most) : stream<HALF, BLOCK, false>(s, p, most);
   return rc != hipSuccess || most == p.m ? rc : launch_int4_tiles<HALF, BLOCK>(s, p, most + 1);
 }
