@@ -51,87 +51,97 @@ __device__ __forceinline__ u32x4_t insert_element(u32x4_t v, int i, uint32_t e) 
 }
 
 // ---- streaming kernel ------------------------------------------------------------------------------------------------------
-// A work-group computes up to 64 rows of a group x 64 columns.  Its four waves take every fourth run of 128 contraction indices
+// A work-group computes up to 32 rows of a group x 64 columns.  Its four waves take every fourth run of 128 contraction indices
 // and add up their sums in LDS; a wave has the next run's loads in flight while it multiplies the present one.
+//
+// What bounds few rows is the stream over the codes, what bounds more of them the addresses that a compute unit's loads touch, one
+// piece of a row of memory per cycle.  A fragment's lanes want 16 bytes of 16 rows of x, 64 pieces a load: read like that, x took
+// 512 of the 640 pieces of a run of 32 rows (texture addresser busy 82 % of the time, matrix cores 20 %).  So x comes in whole
+// rows, 16 lanes to a row's 256 bytes of a run (the tile's last row again for those that it does not have), and goes to the
+// fragments through LDS, a wave's own part of it; and 64 columns' scales come in one load and to their lanes by a permutation.
 constexpr int kInt4Threads = 256, kInt4Waves = 4, kInt4Cols = 64, kInt4Rows = 32, kInt4Strips = kInt4Cols / kInt4Strip;
+constexpr int kInt4RowBytes = 2 * kInt4Run;  // of x in a run
 
-// NT: row tiles of 16
 template <int BLOCK>
 struct Int4Run {
   static constexpr int PER = kInt4Run / BLOCK;
   typedef typename int4_detail::Bits<2 * PER>::type Scales;
   typedef typename int4_detail::Bits<PER>::type Zeros;
   u32x4_t codes[kInt4Strips];
-  Scales scales[kInt4Strips];
-  Zeros zeros[kInt4Strips];
+  Scales scales;  // of column `lane`
+  Zeros zeros;
 };
 
+__device__ __forceinline__ uint32_t from_column(uint32_t v, int lane4) { return (uint32_t)__builtin_amdgcn_ds_bpermute(lane4, (int)v); }
+__device__ __forceinline__ uint64_t from_column(uint64_t v, int lane4) {
+  return (uint64_t)from_column((uint32_t)v, lane4) | (uint64_t)from_column((uint32_t)(v >> 32), lane4) << 32;
+}
+
+// NT: row tiles of 16
 template <bool HALF, int BLOCK, bool ZEROS, int NT>
-__device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const RowTile& tile, int c0, float (*sums)[16][kInt4Cols]) {
+__device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const RowTile& tile, int c0, unsigned char* smem) {
   typedef Int4Run<BLOCK> Run;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane & 15, h = lane >> 4, cols = imin(kInt4Cols, p.n - c0);
   const int runs = int4_runs(p.k), strips = int4_strips(p.n), e = tile.group - p.g_first;
-  // Every address is a base that all lanes share and an offset of 32 bits; only the columns of scales, cut off at n, and the rows of
-  // x, at the tile's last one, depend on the lane.
+  // Every address is a base that all lanes share and an offset of 32 bits.
   const size_t codes0 = ((size_t)e * strips + c0 / kInt4Strip) * runs * 1024, scales0 = (size_t)e * runs * p.n + c0;
-  uint32_t column[kInt4Strips], row[NT];
-#pragma unroll
-  for (int c = 0; c < kInt4Strips; ++c) column[c] = (uint32_t)imin(kInt4Strip * c + q, cols - 1);
-#pragma unroll
-  for (int t = 0; t < NT; ++t) row[t] = (uint32_t)imin(16 * t + q, tile.rows - 1) * (uint32_t)p.k * 2u + 16u * h;
-  const char* x0 = static_cast<const char*>(p.x) + (size_t)tile.first * p.k * 2;
-
+  const uint32_t column = (uint32_t)imin(lane, cols - 1);
   auto load = [&](int r) {
     Run d;
     const size_t at = scales0 + (size_t)r * p.n;
-    const char* scales = scalar_base(p.scales, at * sizeof(typename Run::Scales));
-    const char* zeros = scalar_base(p.zeros, at * sizeof(typename Run::Zeros));
+    d.scales = load_at<typename Run::Scales>(scalar_base(p.scales, at * sizeof(typename Run::Scales)), column * (uint32_t)sizeof(typename Run::Scales));
+    if constexpr (ZEROS) d.zeros = load_at<typename Run::Zeros>(scalar_base(p.zeros, at * sizeof(typename Run::Zeros)), column * (uint32_t)sizeof(typename Run::Zeros));
 #pragma unroll
     for (int c = 0; c < kInt4Strips; ++c) {
       const size_t strip = (size_t)imin(c, (cols - 1) / kInt4Strip) * runs + r;
       d.codes[c] = load_at<u32x4_t>(scalar_base(p.codes, codes0 + strip * 1024), lane * 16u);
-      d.scales[c] = load_at<typename Run::Scales>(scales, column[c] * (uint32_t)sizeof(typename Run::Scales));
-      if constexpr (ZEROS) d.zeros[c] = load_at<typename Run::Zeros>(zeros, column[c] * (uint32_t)sizeof(typename Run::Zeros));
     }
     return d;
   };
-  auto load_x = [&](int r, u32x4_t (&d)[NT][4]) {
-    const char* base = scalar_base(x0, (size_t)r * (2 * kInt4Run));
+  // x: load i is rows 4 i + h, 16 bytes (chunk q) of each to a lane.  In LDS a row's chunks are permuted by its number, so that the 16
+  // rows of a fragment read lie in different banks.
+  constexpr int XL = 4 * NT;
+  unsigned char* mine = smem + wave * (NT * 16 * kInt4RowBytes);
+  const char* x0 = static_cast<const char*>(p.x) + (size_t)tile.first * p.k * 2;
+  const uint32_t four_rows = (uint32_t)p.k * 8u, row0 = (uint32_t)h * (uint32_t)p.k * 2u + 16u * q, row_last = (uint32_t)(tile.rows - 1) * (uint32_t)p.k * 2u + 16u * q;
+  auto fetch_x = [&](int r, u32x4_t (&d)[XL]) {
+    const char* base = scalar_base(x0, (size_t)r * kInt4RowBytes);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) d[t][j] = load_at<u32x4_t>(base, row[t] + 64u * j);
+    for (int i = 0; i < XL; ++i) d[i] = load_at<u32x4_t>(base, umin(row0 + (uint32_t)i * four_rows, row_last));
   };
-  // Of the run that holds index k: zeros from there on.  A piece that would run past it is read from before it and shifted down.
-  auto load_x_tail = [&](int r, u32x4_t (&d)[NT][4]) {
-    const char* base = x0 + (size_t)r * (2 * kInt4Run);
+  // Of the run that holds index k: zeros from there on.  A chunk that would run past it is read from before it and shifted down.
+  auto fetch_x_tail = [&](int r, u32x4_t (&d)[XL]) {
+    const int past = imax(r * kInt4Run + 8 * q + 8 - p.k, 0);  // elements
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int past = imax(r * kInt4Run + 32 * j + 8 * h + 8 - p.k, 0);  // elements
-        const char* at = base + 64 * j + row[t];
-        if (p.k >= 8) {
-          d[t][j] = shift_down(load_any<u32x4_t>(at - 2 * past), 2 * imin(past, 8));
-        } else {
-          u32x4_t v = {0, 0, 0, 0};
+    for (int i = 0; i < XL; ++i) {
+      const char* at = x0 + (size_t)r * kInt4RowBytes + umin(row0 + (uint32_t)i * four_rows, row_last);
+      if (p.k >= 8) {
+        d[i] = shift_down(load_any<u32x4_t>(at - 2 * past), 2 * imin(past, 8));
+      } else {
+        d[i] = u32x4_t{0, 0, 0, 0};
 #pragma unroll 1
-          for (int i = 0; i < 8 - past; ++i) v = insert_element(v, i, *reinterpret_cast<const uint16_t*>(at + 2 * i));
-          d[t][j] = v;
-        }
+        for (int n = 0; n < 8 - past; ++n) d[i] = insert_element(d[i], n, *reinterpret_cast<const uint16_t*>(at + 2 * n));
       }
+    }
   };
+  auto stage_x = [&](const u32x4_t (&d)[XL]) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < XL; ++i)
+      *reinterpret_cast<u32x4_t*>(mine + (4 * i + h) * kInt4RowBytes + ((q ^ ((4 * i + h) & 15)) << 4)) = d[i];
+    __builtin_amdgcn_wave_barrier();
+  };
+  auto fragment = [&](int t, int j) { return *reinterpret_cast<const u32x4_t*>(mine + (16 * t + q) * kInt4RowBytes + (((4 * j + h) ^ q) << 4)); };
 
   f32x4_t y[NT][kInt4Strips];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int c = 0; c < kInt4Strips; ++c) y[t][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // A run's blocks, one or two strips at a time; once a fragment of x has met the last strip, the next run's takes its place.
-  auto multiply = [&](const Run& d, u32x4_t (&xv)[NT][4], auto refill, int next_run) {
-    constexpr int STEPS = BLOCK / 32, U = NT == 4 ? 1 : 2;  // strips at a time
-    const char* next = scalar_base(x0, (size_t)next_run * (2 * kInt4Run));
+  // A run's blocks, two strips at a time.
+  auto multiply = [&](const Run& d) {
+    constexpr int STEPS = BLOCK / 32, U = 2;
 #pragma unroll
     for (int b = 0; b < Run::PER; ++b) {
       f32x4_t xs[NT];
@@ -147,20 +157,22 @@ __device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const Row
           for (int u = 0; u < U; ++u) w[u] = codes_plus_one<HALF>(d.codes[c + u][j]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            if (c == 0) xs[t] = mfma_16x16x32<HALF>(xv[t][j], ones<HALF>(), xs[t]);
+            const u32x4_t x = fragment(t, j);
+            if (c == 0) xs[t] = mfma_16x16x32<HALF>(x, ones<HALF>(), xs[t]);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
               const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-              v[u][t] = mfma_16x16x32<HALF>(xv[t][j], w[u], j == b * STEPS ? zero : v[u][t]);
+              v[u][t] = mfma_16x16x32<HALF>(x, w[u], j == b * STEPS ? zero : v[u][t]);
             }
-            if (decltype(refill)::value && c + U == kInt4Strips) xv[t][j] = load_at<u32x4_t>(next, row[t] + 64u * j);
           }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const float s = scale_to_f32((uint32_t)(d.scales[c + u] >> (16 * b)) & 0xffff, p.scale_half);
+          const int from = (kInt4Strip * (c + u) + q) * 4;
+          typedef typename std::conditional<sizeof(typename Run::Scales) == 8, uint64_t, uint32_t>::type Word;
+          const float s = scale_to_f32((uint32_t)(from_column((Word)d.scales, from) >> (16 * b)) & 0xffff, p.scale_half);
           float plus = 24.f;  // 16 + zero
-          if constexpr (ZEROS) plus = 16.f + (float)((uint32_t)(d.zeros[c + u] >> (8 * b)) & 0xff);
+          if constexpr (ZEROS) plus = 16.f + (float)((from_column((uint32_t)d.zeros, from) >> (8 * b)) & 0xff);
           const float s16 = 16.f * s, sz = -s * plus;
 #pragma unroll
           for (int t = 0; t < NT; ++t)
@@ -171,37 +183,48 @@ __device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const Row
     }
   };
   const int whole = p.k / kInt4Run, own = (whole - wave + kInt4Waves - 1) / kInt4Waves;  // whole runs; this wave's
+  u32x4_t xr[XL];
+#pragma unroll
+  for (int i = 0; i < XL; ++i) xr[i] = u32x4_t{0, 0, 0, 0};
   if (own > 0) {
     // Work-groups begin at runs of their own: strips lie runs x 1 KB apart, a multiple of 4 KB for most k, and all in step they
-    // would ask a few memory channels at a time.
+    // would ask a few memory channels at a time.  Two runs in turn, so that nothing that is still on its way is moved from one
+    // register to another.
     int i = (int)(blockIdx.x % (uint32_t)own);
-    // two runs in turn, so that nothing that is still on its way is moved from one register to another
     auto turn = [&]() { i = i + 1 < own ? i + 1 : 0; return wave + i * kInt4Waves; };
+    fetch_x(wave + i * kInt4Waves, xr);
     Run even = load(wave + i * kInt4Waves), odd;
-    u32x4_t xv[NT][4];
-    load_x(wave + i * kInt4Waves, xv);
     int left = own;
     for (; left >= 2; left -= 2) {
+      stage_x(xr);
       const int second = turn();
+      fetch_x(second, xr);
       odd = load(second);
       __builtin_amdgcn_sched_barrier(0);  // (the compiler would put these loads off until they are needed)
-      multiply(even, xv, std::true_type(), second);
+      multiply(even);
+      stage_x(xr);
       const int third = turn();  // (behind the last run the first one again, for nothing)
+      fetch_x(third, xr);
       even = load(third);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(odd, xv, std::true_type(), third);
+      multiply(odd);
     }
-    if (left) multiply(even, xv, std::false_type(), 0);
+    if (left) {
+      stage_x(xr);
+      multiply(even);
+    }
   }
   if (whole < runs && whole % kInt4Waves == wave) {
-    u32x4_t xv[NT][4];
-    load_x_tail(whole, xv);
-    multiply(load(whole), xv, std::false_type(), whole);
+    const Run last = load(whole);
+    fetch_x_tail(whole, xr);
+    stage_x(xr);
+    multiply(last);
   }
+  float (*sums)[16][kInt4Cols] = reinterpret_cast<float (*)[16][kInt4Cols]>(smem);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (16 * t >= tile.rows) break;
-    if (t > 0) __syncthreads();
+    __syncthreads();
 #pragma unroll
     for (int c = 0; c < kInt4Strips; ++c)
 #pragma unroll
@@ -220,10 +243,10 @@ __device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const Row
 
 // Work-groups [0, tiles * col_tiles): a row tile and 64 of its columns; those behind them: 64 rows, of which they zero what is
 // no row of a group that the weights hold.
-// ROWS: of a row tile, 16 or 64.
+// ROWS: of a row tile, 16 or 32.
 template <bool HALF, int BLOCK, bool ZEROS, int ROWS>
-__global__ __launch_bounds__(kInt4Threads, ROWS == 16 ? (ZEROS ? 3 : 4) : 2) void gmm_int4_stream_kernel(Int4Problem p, int tiles, int col_tiles, int most) {
-  __shared__ float sums[kInt4Waves][16][kInt4Cols];
+__global__ __launch_bounds__(kInt4Threads, ROWS == 16 ? 3 : 2) void gmm_int4_stream_kernel(Int4Problem p, int tiles, int col_tiles, int most) {
+  __shared__ __attribute__((aligned(16))) unsigned char smem[kInt4Waves * ROWS * kInt4RowBytes];
   if ((int)blockIdx.x >= tiles * col_tiles) {
     int first, end;
     held_rows(p, &first, &end);
@@ -237,7 +260,7 @@ __global__ __launch_bounds__(kInt4Threads, ROWS == 16 ? (ZEROS ? 3 : 4) : 2) voi
   const RowTile tile = find_row_tile<ROWS>(p, 1, most, blockIdx.x / col_tiles);
   if (tile.rows == 0) return;
   const int c0 = blockIdx.x % col_tiles * kInt4Cols;
-  int4_stream_tile<HALF, BLOCK, ZEROS, ROWS / 16>(p, tile, c0, sums);
+  int4_stream_tile<HALF, BLOCK, ZEROS, ROWS / 16>(p, tile, c0, smem);
 }
 
 // ---- laying out the weights --------------------------------------------------------------------------------------------------
@@ -268,7 +291,8 @@ struct StreamGrid {
 StreamGrid stream_grid(const Int4Problem& p, int most) {
   StreamGrid s;
   s.rows = p.m <= 8 * p.g ? 16 : kInt4Rows;
-  s.tiles = most <= s.rows ? imin(p.g, p.m) : p.m / s.rows + imin(p.g, p.m);
+  const long long of_few = (long long)imin(p.g, p.m) * ((most + s.rows - 1) / s.rows), of_any = p.m / s.rows + imin(p.g, p.m);
+  s.tiles = (int)(of_few < of_any ? of_few : of_any);
   s.col_tiles = (p.n + kInt4Cols - 1) / kInt4Cols;
   s.blocks = (long long)s.tiles * s.col_tiles + (p.m + kInt4Rows - 1) / kInt4Rows;
   return s;
@@ -283,19 +307,18 @@ int stream(hipStream_t s, const Int4Problem& p, int most) {
   return (int)hipGetLastError();
 }
 
-constexpr int kInt4FewRows = 64;
+// Whether groups of more rows than kInt4FewRows are left to the tile kernel, a launch of its own.  The sizes are on the device; the
+// rule takes them to be equal, and what each kernel needs for that, us, from rounds of what the device holds at a time: 512
+// work-groups of 32 rows x 64 columns of the streaming kernel at 5 per 1024 indices, 256 tiles of the other at 1.1 .. 2.0 a slab of
+// 64 by their height.  bf16, blocks of 128, streaming | tiles: 32 groups of 64 x 7168 x 2048 172 | 120, 128 of 64 x 2048 x 768 86 |
+// 72, 8 of 64 x 4096 x 14336 135 | 160, 64 of 40 x 2048 x 1024 40 | 43, 8 of 40 x 4096 x 4096 35 | 52.  Where the streaming kernel is
+// long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
+constexpr int kInt4FewRows = 48;
 
-// Whether groups of more than kInt4FewRows rows are left to the tile kernel, a launch of its own.  The sizes are on the device; the rule
-// takes them to be equal, and what each kernel needs for that, us, from rounds of what the device holds at a time: 512 work-groups of
-// 64 rows x 64 columns of the streaming kernel at 8.5 per 1024 indices (half as much for 32 rows), 256 tiles of the other at 1.1 ..
-// 2.0 a slab of 64 by their height.  bf16, blocks of 128, streaming | tiles: 4 groups of 512 x 2048 x 2048 41 | 57, 8 of 256 x
-// 4096 x 4096 129 | 105, 12 of 256 x 1024 x 1536 30 | 43, 32 of 72 x 7168 x 2048 207 | 139, 64 of 128 x 2048 x 1024 74 | 52.  Where the
-// streaming kernel is long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
 bool uses_tiles(int m, int k, int n, int g) {
   if (m <= kInt4FewRows || k < 8 || k > (1 << 22)) return false;
   const double rows = (double)((m + g - 1) / g), cols64 = (n + 63) / 64, cols256 = (n + 255) / 256;
-  const double rounds = g * ceil(rows / 64) * cols64 / 512;
-  const double streaming = 6 + ceil(rounds) * k * 0.0083 * (rows <= 32 ? 0.55 : 1);
+  const double streaming = 6 + ceil(g * ceil(rows / 32) * cols64 / 512) * k * 0.005;
   if (streaming > 100) return true;
   if (rows <= kInt4FewRows) return false;
   const double last = rows - 256 * floor(rows / 256), height = last == 0 ? 0 : last <= 64 ? 1.1 : last <= 128 ? 1.3 : last <= 192 ? 1.65 : 2;
