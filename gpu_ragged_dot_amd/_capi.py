@@ -72,6 +72,9 @@ class Plan(ctypes.Structure):
                 f"decode_nb={self.decode_nb}, split_k={self.split_k})")
 
 
+RD_INT4_AUTO, RD_INT4_STREAM, RD_INT4_TILES = 0, 1, 2
+
+
 class GateSpec(ctypes.Structure):
     _fields_ = [("top_k", ctypes.c_int), ("clusters", ctypes.c_int), ("top_clusters", ctypes.c_int), ("flags", ctypes.c_int),
                 ("scale", ctypes.c_float)]
@@ -181,9 +184,9 @@ def _load() -> ctypes.CDLL:
     lib.rd_int4_codes_bytes.restype = sz
     lib.rd_int4_pack.argtypes = [vp, vp, vp, i, i, i, i]
     lib.rd_int4_pack.restype = i
-    lib.rd_gmm_int4_workspace_bytes.argtypes = [i, i, i, i]
+    lib.rd_gmm_int4_workspace_bytes.argtypes = [i, i, i, i, i]
     lib.rd_gmm_int4_workspace_bytes.restype = sz
-    lib.rd_gmm_int4.argtypes = [vp, vp, vp, vp, vp, ip, vp, i, i, i, i, i, i, i, i, i, vp, sz]
+    lib.rd_gmm_int4.argtypes = [vp, vp, vp, vp, vp, ip, vp, i, i, i, i, i, i, i, i, i, i, vp, sz]
     lib.rd_gmm_int4.restype = i
     return lib
 

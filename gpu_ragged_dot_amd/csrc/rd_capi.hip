@@ -1217,6 +1217,7 @@ static int check_gate(const void* logits, const int32_t* ids, const float* weigh
   if (!spec) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
   const int rc = check_moe(tokens, spec->top_k, 0, dtype);
   if (rc != RD_OK) return rc;
+  if (tokens > rd::kGateMaxTokens) return fail(RD_ERR_INVALID_ARGUMENT, "tokens=%d outside 0..%d", tokens, rd::kGateMaxTokens);
   if (experts < 1 || experts > rd::kGateMaxExperts) return fail(RD_ERR_INVALID_ARGUMENT, "experts=%d outside 1..%d", experts, rd::kGateMaxExperts);
   if (spec->clusters < 1 || spec->clusters > 64 || experts % spec->clusters != 0)
     return fail(RD_ERR_INVALID_ARGUMENT, "clusters=%d (1..64) do not divide experts=%d", spec->clusters, experts);
@@ -1276,7 +1277,7 @@ size_t rd_int4_codes_bytes(int g, int k, int n) {
 }
 
 static int check_int4_weights(const void* codes, int g, int k, int n) {
-  if (g < 1 || k < 0 || n < 0 || k > (1 << 30) || n > (1 << 30)) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape g=%d k=%d n=%d", g, k, n);
+  if (g < 1 || k < 0 || n < 0 || k > (1 << 24) || n > (1 << 24)) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape g=%d k=%d n=%d", g, k, n);
   if ((long long)g * rd::int4_strips(n) * rd::int4_runs(k) >= (1ll << 29)) return fail(RD_ERR_INVALID_ARGUMENT, "g*k*n too large");
   if (k > 0 && n > 0 && (!codes || (reinterpret_cast<uintptr_t>(codes) & 15) != 0))
     return fail(RD_ERR_INVALID_ARGUMENT, "the codes are null or not 16-byte aligned");
@@ -1291,14 +1292,14 @@ int rd_int4_pack(void* stream, const uint8_t* q, void* codes, int g, int k, int 
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "int4_pack launch");
 }
 
-size_t rd_gmm_int4_workspace_bytes(int m, int k, int n, int g) {
+size_t rd_gmm_int4_workspace_bytes(int m, int k, int n, int g, int kernel) {
   if (m < 0 || k < 0 || n < 0 || g < 1) return 0;
-  return align_up(rd::int4_workspace_bytes(m, k, n, g), 256);
+  return align_up(rd::int4_workspace_bytes(m, k, n, g, kernel), 256);
 }
 
 int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scales, const uint8_t* zeros,
                 const int32_t* group_sizes, void* y, int m, int k, int n, int g_total, int group_offset, int g_local, int block,
-                int scale_dtype, int dtype, void* workspace, size_t workspace_bytes) {
+                int scale_dtype, int dtype, int kernel, void* workspace, size_t workspace_bytes) {
   int rc = check_int4_weights(codes, g_local, k, n);
   if (rc != RD_OK) return rc;
   if (m < 0 || m > rd::kInt4MaxRows) return fail(RD_ERR_INVALID_ARGUMENT, "m=%d outside 0..%d", m, rd::kInt4MaxRows);
@@ -1308,16 +1309,15 @@ int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scal
   if (dtype != RD_DTYPE_BF16 && dtype != RD_DTYPE_F16) return fail(RD_ERR_INVALID_ARGUMENT, "dtype %d: rows are bfloat16 or float16", dtype);
   if (scale_dtype != RD_DTYPE_BF16 && scale_dtype != RD_DTYPE_F16)
     return fail(RD_ERR_INVALID_ARGUMENT, "scale dtype %d: scales are bfloat16 or float16", scale_dtype);
+  if (kernel < RD_INT4_AUTO || kernel > RD_INT4_TILES) return fail(RD_ERR_INVALID_ARGUMENT, "unknown kernel %d", kernel);
   if (m == 0 || n == 0) return RD_OK;
   if (!group_sizes || !y || (k > 0 && (!x || !scales))) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
-  if ((reinterpret_cast<uintptr_t>(scales) & 7) != 0 || (reinterpret_cast<uintptr_t>(zeros) & 3) != 0)
-    return fail(RD_ERR_INVALID_ARGUMENT, "the scales are not 8-byte aligned or the zeros not 4-byte aligned");
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail(RD_ERR_WORKSPACE, "workspace misaligned");
-  const size_t needed = rd::int4_workspace_bytes(m, k, n, g_total);
+  const size_t needed = rd::int4_workspace_bytes(m, k, n, g_total, kernel);
   float* partials = workspace && needed > 0 && workspace_bytes >= needed ? static_cast<float*>(workspace) : nullptr;
   int32_t* counters = partials ? reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + rd::kInt4PartialBytes) : nullptr;
   const rd::Int4Problem p = {x, static_cast<const uint32_t*>(codes), scales, zeros, group_sizes, y, m, k, n, g_total, group_offset, g_local,
-                             block, scale_dtype == RD_DTYPE_F16, dtype == RD_DTYPE_F16, partials, counters};
+                             block, scale_dtype == RD_DTYPE_F16, dtype == RD_DTYPE_F16, kernel, partials, counters};
   if (!rd::int4_grid_fits(p)) return fail(RD_ERR_UNSUPPORTED, "m=%d rows of n=%d in %d groups are more tiles than a launch has", m, n, g_total);
   rc = rd::launch_gmm_int4((hipStream_t)stream, p);
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "gmm_int4 launch");

@@ -329,7 +329,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
   if (exact) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const uint32_t b = sizeof(T) == 2 ? (sizeof(T) == 2 && !__is_same(T, bf16_bits) ? (uint32_t)__builtin_bit_cast(uint16_t, (f16_t)l[i]) : __builtin_bit_cast(uint32_t, l[i]) >> 16) : 0u;
+      const uint32_t b = __is_same(T, f16_t) ? (uint32_t)__builtin_bit_cast(uint16_t, (f16_t)l[i]) : __builtin_bit_cast(uint32_t, l[i]) >> 16;
       const uint32_t sorted = b == 0x8000u ? 0x8000u : (b & 0x8000u) ? b ^ 0xffffu : b | 0x8000u;  // -0 is 0
       key[i] = l[i] == -INFINITY ? 0u : l[i] != l[i] ? 0xffffu : sorted;
     }
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
       for (int i = 0; i < PER; ++i) key[i] = l[i] == -INFINITY ? 0u : 1u + (uint32_t)fminf(fmaxf((l[i] - low) * per_rank, 0.f), kKeyRanks - 3.f);
     }
   }
-  const uint32_t near = (uint32_t)closest;
+  const uint32_t near = (uint32_t)fminf(closest, 1e9f);  // (twice that fits, too)
 #pragma unroll
   for (int i = 0; i < PER; ++i) key[i] = key[i] ? key[i] << kKeyIndexBits | (kKeyIndexMask - (uint32_t)(e0 + i)) : 0u;
 
@@ -508,8 +508,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_grad_kernel(const T* __
   const int lane = threadIdx.x & 63, row = blockIdx.x * (kGateThreads / 64) + (threadIdx.x >> 6);
   if (row >= p.tokens) return;
   const T* src = logits + (size_t)row * p.experts;
-  const bool slot = lane < p.top_k;
-  const int id = slot ? ids[(size_t)row * p.top_k + lane] : -1;
+  const int given = lane < p.top_k ? ids[(size_t)row * p.top_k + lane] : -1, id = given < p.experts ? given : -1;
   const float w = id >= 0 ? weights[(size_t)row * p.top_k + lane] : 0.f;
   const float q = id >= 0 ? w * dweights[(size_t)row * p.top_k + lane] : 0.f;
   const float Q = wave_sum(q);
@@ -559,8 +558,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_grad_kernel(const 
   const int at = threadIdx.x & (kRowLanes - 1), mine = threadIdx.x / kRowLanes;
   const int want = blockIdx.x * (kGateThreads / kRowLanes) + mine, row = imin(want, p.tokens - 1);
   float* d = rows[mine];
-  const bool slot = at < p.top_k;
-  const int id = slot ? ids[(size_t)row * p.top_k + at] : -1;
+  const int given = at < p.top_k ? ids[(size_t)row * p.top_k + at] : -1, id = given < p.experts ? given : -1;
   const float w = id >= 0 ? weights[(size_t)row * p.top_k + at] : 0.f;
   const float q = id >= 0 ? w * dweights[(size_t)row * p.top_k + at] : 0.f;
   const float Q = row_sum(q);

@@ -32,6 +32,7 @@ struct Int4Problem {
   int block;
   bool scale_half;          // scales are float16, else bfloat16
   bool half;                // x and y are float16
+  int kernel;               // RD_INT4_*
   float* partials;          // kInt4Slots tiles of 256 x 256, or null: no tile is cut along k
   int32_t* counters;        // kInt4Slots, behind them
 };
@@ -39,7 +40,7 @@ struct Int4Problem {
 constexpr int kInt4Slots = 256;  // work-groups of the tile kernel that run at a time, one per compute unit
 constexpr size_t kInt4PartialBytes = (size_t)kInt4Slots * 256 * 256 * sizeof(float);
 // Of the whole workspace; 0: no launch of these sizes is cut.
-size_t int4_workspace_bytes(int m, int k, int n, int g);
+size_t int4_workspace_bytes(int m, int k, int n, int g, int kernel);
 
 __host__ __device__ inline int int4_runs(int k) { return (k + kInt4Run - 1) / kInt4Run; }
 __host__ __device__ inline int int4_strips(int n) { return (n + kInt4Strip - 1) / kInt4Strip; }

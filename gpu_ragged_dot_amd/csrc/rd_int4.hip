@@ -5,6 +5,7 @@
 // A code becomes the 16-bit number v = 1 + q / 16, exactly, by a shift and an and-or for two of them; the matrix cores sum
 // x v over a block, and x itself against ones; then  y += 16 scale (sum x v) - scale (16 + zero) (sum x).  So products are
 // exact, sums are fp32, and nothing is rounded to 16 bits before the result.
+#include "../../include/ragged_dot_hip.h"
 #include "rd_elem.h"
 #include "rd_int4_rows.h"
 #include "rd_int4_tile.h"
@@ -315,8 +316,9 @@ int stream(hipStream_t s, const Int4Problem& p, int most) {
 // long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
 constexpr int kInt4FewRows = 48;
 
-bool uses_tiles(int m, int k, int n, int g) {
-  if (m <= kInt4FewRows || k < 8 || k > (1 << 22)) return false;
+bool uses_tiles(int m, int k, int n, int g, int kernel) {
+  if (m <= kInt4FewRows || k < 8 || k > (1 << 22) || kernel == RD_INT4_STREAM) return false;
+  if (kernel == RD_INT4_TILES) return true;
   const double rows = (double)((m + g - 1) / g), cols64 = (n + 63) / 64, cols256 = (n + 255) / 256;
   const double streaming = 6 + ceil(g * ceil(rows / 32) * cols64 / 512) * k * 0.005;
   if (streaming > 100) return true;
@@ -326,9 +328,15 @@ bool uses_tiles(int m, int k, int n, int g) {
   return 12 + k / 64 * (work > least ? work : least) < streaming;
 }
 
+// Rows of the largest groups that the streaming kernel multiplies.  (float16 does not have the range of bfloat16 scales, and the
+// tiles' weights are of the rows' type.)
+int most_streamed(const Int4Problem& p) {
+  return (!p.half || p.scale_half) && uses_tiles(p.m, p.k, p.n, p.g, p.kernel) ? kInt4FewRows : p.m;
+}
+
 template <bool HALF, int BLOCK>
 int gmm_int4(hipStream_t s, const Int4Problem& p) {
-  const int most = uses_tiles(p.m, p.k, p.n, p.g) ? kInt4FewRows : p.m;
+  const int most = most_streamed(p);
   const int rc = p.zeros ? stream<HALF, BLOCK, true>(s, p, most) : stream<HALF, BLOCK, false>(s, p, most);
   return rc != hipSuccess || most == p.m ? rc : launch_int4_tiles<HALF, BLOCK>(s, p, most + 1);
 }
@@ -345,11 +353,15 @@ int launch_int4_pack(hipStream_t s, const uint8_t* q, uint32_t* codes, int g, in
   return (int)hipGetLastError();
 }
 
-size_t int4_workspace_bytes(int m, int k, int n, int g) {
-  return uses_tiles(m, k, n, g) && n > 0 ? kInt4PartialBytes + kInt4Slots * sizeof(int32_t) : 0;
+size_t int4_workspace_bytes(int m, int k, int n, int g, int kernel) {
+  return uses_tiles(m, k, n, g, kernel) && n > 0 ? kInt4PartialBytes + kInt4Slots * sizeof(int32_t) : 0;
 }
 
-bool int4_grid_fits(const Int4Problem& p) { return stream_grid(p, p.m).blocks < (1ll << 31) / kInt4Threads; }
+// (The tile kernel's work-groups are fewer than rows / 256 and groups come to, times the columns.)
+bool int4_grid_fits(const Int4Problem& p) {
+  const long long tiles = (p.m / 256 + imin(p.g, p.m)) * (long long)((p.n + 255) / 256);
+  return stream_grid(p, most_streamed(p)).blocks < (1ll << 31) / kInt4Threads && tiles < (1ll << 31) / kInt4Threads;
+}
 
 int launch_gmm_int4(hipStream_t s, const Int4Problem& p) {
   return p.half ? gmm_int4<true>(s, p) : gmm_int4<false>(s, p);

@@ -28,6 +28,7 @@ struct GateSpec {
   float scale;
   int elem;
 };
+constexpr int kGateMaxTokens = 1 << 25;  // a launch has a wave to each, and less than 2^32 threads
 constexpr int kGateMaxExperts = 1024;  // sixteen of them to a lane
 int launch_moe_gate(hipStream_t s, const void* logits, const float* bias, int32_t* ids, float* weights, const GateSpec& spec);
 int launch_moe_gate_grad(hipStream_t s, const void* logits, const int32_t* ids, const float* weights, const float* dweights,

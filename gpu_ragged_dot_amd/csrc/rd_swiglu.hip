@@ -43,15 +43,10 @@ template <class T>
 struct Piece {
   static constexpr int PER = 16 / sizeof(T);
   alignas(16) T e[PER];
-  template <bool STREAM>
-  __device__ __forceinline__ void load(const T* p) {
-    const u32x4_t v = load_any<u32x4_t>(p);
-    *reinterpret_cast<u32x4_t*>(e) = v;
-  }
+  __device__ __forceinline__ void load(const T* p) { *reinterpret_cast<u32x4_t*>(e) = load_any<u32x4_t>(p); }
   __device__ __forceinline__ void store(T* p) const { store_any(p, *reinterpret_cast<const u32x4_t*>(e)); }
 };
 
-// What a work-group computes: `count` pieces from `first` on, U of them per thread.
 struct PieceAt {
   long long row;
   int col;
@@ -74,8 +69,8 @@ __global__ __launch_bounds__(kSwigluThreads) void moe_swiglu_kernel(const T* __r
   for (int i = 0; i < U; ++i) {
     if (first + threadIdx.x + i * kSwigluThreads >= pieces) break;
     at[i] = piece_at(row0, in_row + i * kSwigluThreads, per_row, f, PER);
-    g[i].template load<false>(y + at[i].row * 2 * f + at[i].col);
-    u[i].template load<false>(y + at[i].row * 2 * f + f + at[i].col);
+    g[i].load(y + at[i].row * 2 * f + at[i].col);
+    u[i].load(y + at[i].row * 2 * f + f + at[i].col);
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
@@ -99,9 +94,9 @@ __global__ __launch_bounds__(kSwigluThreads) void moe_swiglu_grad_kernel(const T
   for (int i = 0; i < U; ++i) {
     if (first + threadIdx.x + i * kSwigluThreads >= pieces) break;
     at[i] = piece_at(row0, in_row + i * kSwigluThreads, per_row, f, PER);
-    g[i].template load<false>(y + at[i].row * 2 * f + at[i].col);
-    u[i].template load<false>(y + at[i].row * 2 * f + f + at[i].col);
-    d[i].template load<false>(dout + at[i].row * f + at[i].col);
+    g[i].load(y + at[i].row * 2 * f + at[i].col);
+    u[i].load(y + at[i].row * 2 * f + f + at[i].col);
+    d[i].load(dout + at[i].row * f + at[i].col);
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
@@ -141,10 +136,7 @@ __global__ __launch_bounds__(kSwigluThreads) void moe_swiglu_narrow_grad_kernel(
 // Pieces per thread: one while that many work-groups do not fill the device, then several loads in flight.
 constexpr long long kFewPieces = 256ll * kSwigluThreads * 8;
 
-dim3 blocks_for(long long work, int per_block) {
-  const long long b = (work + per_block - 1) / per_block;
-  return dim3((unsigned)b);
-}
+dim3 blocks_for(long long work, int per_block) { return dim3((unsigned)((work + per_block - 1) / per_block)); }
 template <class T>
 long long pieces_of(long long rows, int f) { return rows * ((f + Piece<T>::PER - 1) / Piece<T>::PER); }
 

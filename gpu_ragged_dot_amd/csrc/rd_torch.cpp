@@ -565,7 +565,7 @@ int scale_code(const Tensor& t) {
 }
 
 Tensor gmm_int4(const Tensor& x_, const Tensor& codes, const Tensor& scales, const std::optional<Tensor>& zeros, int64_t k, int64_t n, int64_t block,
-                const Tensor& gs_, int64_t g_first) {
+                const Tensor& gs_, int64_t g_first, int kernel) {
   expect_no_tangent(x_, scales);
   expect(x_.dim() == 2, "x must be [m, k]");
   if (x_.scalar_type() != at::kBFloat16 && x_.scalar_type() != at::kHalf) throw py::type_error("unsupported dtype; x is bfloat16 or float16");
@@ -592,12 +592,12 @@ Tensor gmm_int4(const Tensor& x_, const Tensor& codes, const Tensor& scales, con
   const Tensor x = x_.contiguous(), gs = sizes_on(gs_, dev);
   const c10::DeviceGuard guard(dev);
   Tensor y = at::empty({x.size(0), n}, x.options().requires_grad(false));
-  const size_t ws_bytes = rd_gmm_int4_workspace_bytes((int)x.size(0), (int)k, (int)n, (int)g);
+  const size_t ws_bytes = rd_gmm_int4_workspace_bytes((int)x.size(0), (int)k, (int)n, (int)g, kernel);
   const Tensor ws = ws_bytes ? scratch(ws_bytes, dev) : Tensor();
   check(rd_gmm_int4(stream_of(dev), x.const_data_ptr(), codes.const_data_ptr(), scales.const_data_ptr(), zeros ? zeros->const_data_ptr<uint8_t>() : nullptr,
                     gs.const_data_ptr<int32_t>(), y.mutable_data_ptr(), (int)x.size(0), (int)k, (int)n, (int)g, (int)(g_first < 0 ? 0 : g_first),
                     (int)g_local, (int)block, code, x.scalar_type() == at::kHalf ? RD_DTYPE_F16 : RD_DTYPE_BF16,
-                    ws.defined() ? ws.mutable_data_ptr() : nullptr, ws_bytes));
+                    kernel, ws.defined() ? ws.mutable_data_ptr() : nullptr, ws_bytes));
   return y;
 }
 

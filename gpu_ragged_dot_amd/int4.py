@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import _tracing
+from . import _capi, _tracing
 from ._native import lib as _native
 from .ops import _group_offset, _sizes
 
@@ -61,13 +61,19 @@ def pack_int4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tenso
 
 def ragged_dot_int4(x: torch.Tensor, weights: Int4Weights, group_sizes, *, group_offset=None) -> torch.Tensor:
     """``(m, k) x (g, k, n) -> (m, n)`` on 4-bit weights; rows past ``sum(group_sizes)`` are zero.  ``x`` is bfloat16 or float16,
-    and so is the result, rounded once from fp32.  ``group_offset`` as in ``gmm``: ``weights`` hold the groups from there on, the
-    rows of the others are zero.  No gradient: an ``x`` that requires one raises ``NotImplementedError``."""
+    and so is the result, rounded once from fp32; groups of many rows multiply weights that are rounded to that type, too.
+    ``group_offset`` as in ``gmm``: ``weights`` hold the groups from there on, the rows of the others are zero.  No gradient: an
+    ``x`` that requires one raises ``NotImplementedError``."""
+    return _ragged_dot_int4(x, weights, group_sizes, group_offset)
+
+
+def _ragged_dot_int4(x, weights, group_sizes, group_offset=None, kernel=_capi.RD_INT4_AUTO):
+    """With the choice of the kernel (``rd_int4_kernel`` in the header)."""
     assert x.ndim == 2, f"but {x.ndim=}"
     g_first = -1 if group_offset is None else _group_offset(group_offset)
     assert group_offset is None or g_first >= 0
-    call = lambda x, gs: _native.gmm_int4(x, weights.codes, weights.scales, weights.zeros, weights.k, weights.n,
-                                          weights.block, gs, g_first)
+    call = lambda x, gs: _native.gmm_int4(x, weights.codes, weights.scales, weights.zeros, weights.k, weights.n, weights.block, gs, g_first,
+                                          kernel)
     if _tracing.active():
         return _tracing.record(call, x, _sizes(group_sizes))
     return call(x, _sizes(group_sizes))

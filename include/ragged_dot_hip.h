@@ -245,7 +245,7 @@ int rd_moe_combine_wgrad(void* stream, const void* y, const void* dout, const in
  * does +inf with softmax; which experts such a row names is not defined, but that they are below `experts` and distinct.
  * rd_moe_gate_grad: the gradient of the logits for dweights[token, top_k] (float32), with expert_ids and weights as rd_moe_gate
  * returned them; dlogits has the logits' type.  The choice itself and the bias have no gradient.
- * 1 <= experts <= 1024, top_k <= 64, 1 <= top_k <= top_clusters * (experts / clusters), clusters <= 64 divides experts, scale finite and not 0. */
+ * tokens <= 2^25, 1 <= experts <= 1024, top_k <= 64, 1 <= top_k <= top_clusters * (experts / clusters), clusters <= 64 divides experts, scale finite and not 0. */
 enum rd_gate_flags { RD_GATE_SIGMOID = 1, RD_GATE_TOP2 = 2, RD_GATE_RENORMALIZE = 4 };
 typedef struct rd_gate_spec {
   int top_k, clusters, top_clusters;
@@ -261,7 +261,7 @@ int rd_moe_gate_grad(void* stream, const void* logits, const int32_t* expert_ids
  * No counterpart in the reference.  y is [rows, 2 f], the halves gate and up of every row:
  *   rd_moe_swiglu:      out[r, :] = gate / (1 + exp(-gate)) * up, [rows, f]
  *   rd_moe_swiglu_grad: dy[rows, 2 f] for dout[rows, f]
- * in fp32, rounded once; RD_DTYPE_BF16, RD_DTYPE_F32 or RD_DTYPE_F16. */
+ * in fp32, rounded once; RD_DTYPE_BF16, RD_DTYPE_F32 or RD_DTYPE_F16.  A result does not overlap an argument. */
 int rd_moe_swiglu(void* stream, const void* y, void* out, int rows, int f, int dtype);
 int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, int rows, int f, int dtype);
 
@@ -272,20 +272,25 @@ int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, 
  *           lower four bits), [g, k, n] or with trans_rhs [g, n, k].  In strips of 16 columns and runs of 128 indices, word j of
  *           piece (h, c), codes[e][strip][run][h][c][j], h, j < 4, c < 16, holds column 16 strip + c and the indices 128 run +
  *           32 j + 8 h + i, i < 8, code i at bits 4 (i / 2) + 16 (i % 2); codes past k and n are 8;
- *   scales: [g_local, ceil(k / 128), n, 128 / block], 8-byte aligned, scale_dtype RD_DTYPE_BF16 or RD_DTYPE_F16, 0 past k;
- *   zeros:  bytes of the same shape, 4-byte aligned, or NULL: 8 throughout.
+ *   scales: [g_local, ceil(k / 128), n, 128 / block], scale_dtype RD_DTYPE_BF16 or RD_DTYPE_F16, 0 past k;
+ *   zeros:  bytes of the same shape, or NULL: 8 throughout.
  * x and y are RD_DTYPE_BF16 or RD_DTYPE_F16.  group_sizes, the rows past their sum (zero), clipping at m, group_offset and g_local
- * are those of rd_gmm_sharded.  fp32 sums, one rounding of the result.  An infinity in x makes its row NaN.
- * m < 2^25.  No gradients.
+ * are those of rd_gmm_sharded.  fp32 sums, one rounding of the result.  Groups of many rows are multiplied in tiles whose weights
+ * are rounded once to the rows' type (float16: infinite past its range); with few rows, and for float16 rows with bfloat16 scales (whose range float16 has not), they
+ * are exact.  An infinity in x makes its row NaN or infinite.
+ * kernel: RD_INT4_AUTO, or the one that multiplies groups of any size whatever it costs: RD_INT4_STREAM, or RD_INT4_TILES, which
+ * leaves groups of up to 48 rows to the other (k >= 8 and k <= 2^22; else, and for the types just named, the other does it all).
+ * m < 2^25, k and n <= 2^24.  No gradients.
  * Workspace (optional): rd_gmm_int4_workspace_bytes() bytes, 256-byte aligned, for fp32 partial sums where tiles that do not fill
  * the device's last round are cut along k; with NULL or a smaller one none are.  So the last bits of a row may follow from the other
  * groups' sizes, as in rd_gmm. */
+enum rd_int4_kernel { RD_INT4_AUTO = 0, RD_INT4_STREAM = 1, RD_INT4_TILES = 2 };
 size_t rd_int4_codes_bytes(int g, int k, int n);
 int rd_int4_pack(void* stream, const uint8_t* q, void* codes, int g, int k, int n, int trans_rhs);
-size_t rd_gmm_int4_workspace_bytes(int m, int k, int n, int g);
+size_t rd_gmm_int4_workspace_bytes(int m, int k, int n, int g, int kernel);
 int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scales, const uint8_t* zeros,
                 const int32_t* group_sizes, void* y, int m, int k, int n, int g_total, int group_offset, int g_local, int block,
-                int scale_dtype, int dtype, void* workspace, size_t workspace_bytes);
+                int scale_dtype, int dtype, int kernel, void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -91,7 +91,7 @@ def _gate(spec=(2, 1, 1, 0, 1.0), logits=P, ids=P, weights=P, tokens=4, experts=
     dict(spec=(2, 0, 1, 0, 1.0)), dict(spec=(2, 3, 1, 0, 1.0)), dict(spec=(2, 65, 1, 0, 1.0), experts=130), dict(spec=(2, 2, 0, 0, 1.0)),
     dict(spec=(2, 2, 3, 0, 1.0)), dict(spec=(5, 2, 1, 0, 1.0)), dict(spec=(2, 1, 1, 8, 1.0)), dict(spec=(2, 1, 1, 0, 0.0)),
     dict(spec=(2, 1, 1, 0, float("inf"))), dict(spec=(2, 1, 1, 0, float("nan"))), dict(logits=None), dict(ids=None),
-    dict(weights=None), dict(tokens=-1), dict(experts=0), dict(experts=1025), dict(dtype=_capi.RD_DTYPE_F8E4M3_BF16)],
+    dict(weights=None), dict(tokens=-1), dict(tokens=(1 << 25) + 1), dict(experts=0), dict(experts=1025), dict(dtype=_capi.RD_DTYPE_F8E4M3_BF16)],
     ids=lambda kw: ",".join(f"{k}={v}" for k, v in kw.items()))
 def test_gate_refusals(kw):
     assert _gate(**kw) == -1 and _capi.lib.rd_last_error()
@@ -110,14 +110,14 @@ def test_swiglu_refusals():
     assert lib.rd_moe_swiglu(None, None, None, 0, 8, 0) == 0 and lib.rd_moe_swiglu(None, None, None, 8, 0, 0) == 0
 
 
-def _int4(x=P, codes=P, scales=P, gs=P, y=P, m=4, k=64, n=8, g=2, first=0, local=2, block=32, sdtype=0, dtype=0, ws=None):
-    return _capi.lib.rd_gmm_int4(None, x, codes, scales, None, gs, y, m, k, n, g, first, local, block, sdtype, dtype, ws, 0)
+def _int4(x=P, codes=P, scales=P, gs=P, y=P, m=4, k=64, n=8, g=2, first=0, local=2, block=32, sdtype=0, dtype=0, ws=None, kernel=0):
+    return _capi.lib.rd_gmm_int4(None, x, codes, scales, None, gs, y, m, k, n, g, first, local, block, sdtype, dtype, kernel, ws, 0)
 
 
 @pytest.mark.parametrize("kw", [
     dict(x=None), dict(codes=None), dict(codes=P + 4), dict(scales=None), dict(gs=None), dict(y=None), dict(m=-1), dict(m=1 << 25),
     dict(k=-1), dict(n=-1), dict(g=0, local=0), dict(local=0), dict(first=1), dict(first=-1), dict(first=2 ** 31 - 1), dict(local=3),
-    dict(block=16), dict(block=256), dict(sdtype=3), dict(sdtype=2), dict(sdtype=1), dict(scales=P + 4), dict(dtype=1), dict(dtype=3),
+    dict(block=16), dict(block=256), dict(sdtype=3), dict(sdtype=2), dict(sdtype=1), dict(kernel=3), dict(kernel=-1), dict(k=(1 << 24) + 1), dict(dtype=1), dict(dtype=3),
     dict(g=4096, local=4096, k=1 << 20, n=1 << 20)], ids=lambda kw: ",".join(f"{k}={v}" for k, v in kw.items()))
 def test_int4_refusals(kw):
     assert _int4(**kw) == -1 and _capi.lib.rd_last_error()
@@ -129,8 +129,9 @@ def test_int4_sizes():
     assert lib.rd_int4_codes_bytes(2, 0, 3) == 0 and lib.rd_int4_codes_bytes(-1, 8, 8) == 0
     assert _int4(m=0) == 0 and _int4(n=0) == 0
     assert lib.rd_int4_pack(None, None, P, 1, 32, 8, 0) == -1 and lib.rd_int4_pack(None, P, P + 2, 1, 32, 8, 0) == -1
-    assert _int4(ws=P + 4) == -3 and lib.rd_gmm_int4_workspace_bytes(8, 64, 64, 2) == 0
-    assert _int4(m=(1 << 25) - 1, n=1 << 28, g=2) == -2  # more tiles than a launch has
+    assert _int4(ws=P + 4) == -3 and lib.rd_gmm_int4_workspace_bytes(8, 64, 64, 2, 0) == 0
+    for kernel in (0, 1, 2):  # more tiles than a launch has
+        assert _int4(m=(1 << 25) - 1, n=1 << 24, g=2, kernel=kernel) == -2
 
 
 def test_front_end_refusals():

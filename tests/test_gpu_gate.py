@@ -114,6 +114,59 @@ def test_near_ties_are_decided_in_64_bits(score):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,top_k", [(16, 1), (40, 11), (64, 12), (64, 13), (256, 15), (256, 16), (256, 17), (600, 9)])
+def test_close_float32_logits(score, experts, top_k):
+    """Rows in which a few, some or all logits lie units in the last place apart: what the leading ones settle, and what they do
+    not (more close ones than that)."""
+    gen = torch.Generator().manual_seed(experts + top_k)
+    logits = torch.randn((64, experts), generator=gen)
+    for t in range(64):
+        crowd = torch.randperm(experts, generator=gen)[:1 + t * experts // 64]
+        at = logits[t].topk(min(top_k, experts - 1)).values[-1]  # in the middle of the choice
+        logits[t, crowd] = at + torch.randint(-6, 7, (len(crowd),), generator=gen) * 2.0 ** -23
+    bias = torch.randint(-2, 3, (experts,), generator=gen).float().cuda() * 2.0 ** -22
+    _check(logits.cuda(), top_k, score=score)
+    _check(logits.cuda(), top_k, score=score, bias=bias)
+    _check(logits.cuda(), top_k, score=score, bias=bias * 2.0 ** 22)
+    if experts % 8 == 0 and top_k <= experts // 2:
+        _check(logits.cuda(), top_k, score=score, clusters=8, top_clusters=4)
+        _check(logits.cuda(), top_k, score=score, bias=bias, clusters=8, top_clusters=4, cluster_score="top2")
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_random_calls(seed):
+    """Sizes, clusters, types, scores and biases of every kind at once: small, larger than the scores, of 1e30, -inf."""
+    rng = np.random.default_rng(1000 + seed)
+    experts = int(rng.integers(1, 1025) if seed % 3 else 8 * rng.integers(1, 65))
+    clusters = int(rng.choice([c for c in range(1, 65) if experts % c == 0]))
+    top_clusters = int(rng.integers(1, clusters + 1))
+    top_k = int(rng.integers(1, min(64, top_clusters * (experts // clusters)) + 1))
+    kw = dict(score=str(rng.choice(["softmax", "sigmoid"])), clusters=clusters, top_clusters=top_clusters, cluster_score=str(rng.choice(["max", "top2"])),
+              renormalize=bool(rng.integers(2)), scale=float(rng.choice([1.0, 2.5, -0.5])))
+    dtype = TYPES[seed % 3]
+    logits = _logits(seed, int(rng.integers(1, 80)), experts, dtype)
+    logits[torch.from_numpy(rng.random(logits.shape) < rng.choice([0, 0.1, 0.9])).cuda()] = -torch.inf
+    bias = rng.integers(-9, 10, experts) * rng.choice([0.001, 1.0, 1e6, 1e30], experts if seed % 2 else 1)
+    bias[rng.random(experts) < rng.choice([0, 0.1, 1.0], p=[0.5, 0.4, 0.1])] = -np.inf
+    print(f"gate {tuple(logits.shape)} top {top_k} {dtype} {kw}", flush=True)
+    _check(logits, top_k, bias=torch.from_numpy(bias.astype(np.float32)).cuda() if rng.integers(3) else None, **kw)
+
+
+@pytest.mark.parametrize("experts", [64, 256, 1000])
+def test_biases_that_are_not_finite(experts):
+    """An infinite or NaN bias ranks its expert first and leaves the others' order and all weights finite."""
+    logits = _logits(31, 9, experts, torch.float32)
+    for score in ("softmax", "sigmoid"):
+        for value in (torch.inf, torch.nan):
+            bias = torch.zeros(experts, device="cuda")
+            bias[[5, 40]] = value
+            got, rest = moe.gate(logits, 6, score=score, bias=bias), moe.gate(logits, 8, score=score, bias=torch.zeros(experts, device="cuda"))
+            assert got.weights.isfinite().all()
+            for row, others in zip(got.expert_ids.tolist(), rest.expert_ids.tolist()):
+                assert row[:2] == [5, 40] and row[2:] == [e for e in others if e not in (5, 40)][:4]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_shut_experts_and_rows(score, renormalize):
     logits = _logits(11, 24, 40, torch.float32)
@@ -193,6 +246,10 @@ def test_strided_logits_other_types_of_bias_and_empty_batches():
     assert torch.equal(moe.gate(logits, 4, bias=bias).expert_ids, moe.gate(logits, 4, bias=bias.float()[None]).expert_ids)
     empty = moe.gate(torch.empty((0, 64), device="cuda", requires_grad=True), 4)
     assert empty.expert_ids.shape == (0, 4)
+    learnt = bias.float().requires_grad_()  # moves the choice only: no gradient
+    out = moe.gate(logits.detach().requires_grad_(), 4, bias=learnt)
+    out.weights.sum().backward()
+    assert learnt.grad is None and not out.expert_ids.requires_grad
     with pytest.raises(ValueError, match="bias"):
         moe.gate(logits, 4, bias=bias[:3])
     with pytest.raises(RuntimeError, match="same device"):
