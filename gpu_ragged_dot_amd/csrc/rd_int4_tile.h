@@ -5,13 +5,18 @@
 // pitch and address, two slabs in LDS and two in registers.  A lane owns four pieces of a run of 128 indices (16 bytes, 32 codes,
 // each), with two runs in registers, and turns half of each into 16-bit weights per slab: eight words to 128 bytes of LDS, in the
 // chunk order that the fragment reads undo.  So a code is converted once per row tile and not once per wave.
-//  * A word costs 23 vector instructions (two masks and a shift, eight byte-to-float conversions, eight fused multiply-adds with scale
-//    and -scale zero, four packs), spread a pair of weights at a time over the gaps between matrix-core instructions, which leave
-//    seven issue slots each: 184 a slab beside 64 of those for BM 256.
+//  * A word costs 17 vector instructions (float16 rows: 13).  An and-or makes the float16 numbers 1024 + q or 64 + q of a pair of codes,
+//    for half of the pairs without a shift, and the fused multiply-add of mixed types takes them as they are: scale v - scale (1024 +
+//    zero), whose terms have 22 bits at most, so that the difference is exact.  (A conversion of bytes each: 23.)
+//  * What a wave does beside matrix-core instructions is dealt out over the gaps between them, which leave seven issue slots each, by
+//    the slots that it takes (schedule() below): 400 slots a slab beside 64 instructions of eight, for BM 256.  What bounds the kernel
+//    is the power that the matrix cores draw, first, and these slots.  bf16 (float16), 8 groups of 2048 x 4096 x 14336, us: 1905
+//    (1955) with byte conversions, writes to LDS two lanes to a bank and an op to a gap whatever it takes; 1850 (1845) as it is.
 //  * The weight is rounded to the rows' type, once: scale (q - zero) itself is exact in fp32 (scale has at most 11 bits, the
-//    difference 5).  Kept exact, as in the streaming kernel, the sums of every block would have to be scaled apart - three vector
+//    difference 9).  Kept exact, as in the streaming kernel, the sums of every block would have to be scaled apart - three vector
 //    instructions per accumulator and block of 128, more than the matrix-core instructions leave.
 #pragma once
+#include <utility>
 #include "rd_gemm_rs.h"
 #include "rd_int4.h"
 
@@ -68,6 +73,46 @@ __device__ __forceinline__ float scale_to_f32(uint32_t bits, bool half) {
   const float b = bf16_to_f32((bf16_bits)bits), h = (float)__builtin_bit_cast(f16_t, (uint16_t)bits);
   return half ? h : b;
 }
+
+template <int N, class F, int... I>
+__device__ __forceinline__ void static_for(F&& f, std::integer_sequence<int, I...>) { (f(Int<I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void static_for(F&& f) { static_for<N>(f, std::make_integer_sequence<int, N>{}); }
+
+// What a wave does beside the matrix-core instructions of a substep, an op to a gap behind another by the issue slots that it takes:
+// an instruction of another kind takes one of the seven that a matrix-core instruction leaves, a write to LDS five.
+enum Op { kReadA, kReadB, kConvert, kCommit, kFetch, kRun, kBarrier };
+constexpr int kMaxOps = 32;
+struct Schedule {
+  int count = 0;
+  Op op[kMaxOps] = {};
+  int arg[kMaxOps] = {}, gap[kMaxOps] = {};
+};
+constexpr Schedule schedule(int tm, int tn, int pieces, bool run, bool barrier) {
+  Schedule s;
+  int cost[kMaxOps] = {}, total = 0;
+  auto add = [&](Op op, int arg, int c) { s.op[s.count] = op; s.arg[s.count] = arg; cost[s.count++] = c; total += c; };
+  const int reads = tm + tn;
+  // the first column of A's fragments, B's, A's others: the order in which the next substep wants them
+  auto read = [&](int r) { if (r == 0) add(kReadA, 0, 1); else if (r <= tn) add(kReadB, r - 1, 1); else add(kReadA, r - tn, 1); };
+  int r = 0, moved = 0;
+  const int ahead = barrier ? 3 : 0;  // steps of a conversion before the barrier: time for what was written last
+  for (int c = 0; c < 8; ++c) {
+    if (c == ahead && barrier) add(kBarrier, 0, 1);
+    for (; c >= ahead && r < reads && r * (8 - ahead) <= (c - ahead) * reads; ++r) read(r);
+    add(kConvert, c, c % 4 == 3 ? 9 : 4);
+    for (; c >= ahead && moved < 2 * pieces && moved * (8 - ahead) < (c - ahead + 1) * 2 * pieces; ++moved)
+      add(moved % 2 == 0 ? kCommit : kFetch, moved / 2, 5);
+  }
+  for (; r < reads; ++r) read(r);
+  if (run) add(kRun, 0, 12);
+  int before = 0;
+  for (int o = 0; o < s.count; ++o) {
+    s.gap[o] = (2 * before + cost[o]) * tm * tn / (2 * total);
+    before += cost[o];
+  }
+  return s;
+}
 }  // namespace int4_detail
 
 template <class C>
@@ -99,13 +144,15 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
     }
   };
 
-  // ---- weights: piece i of a run is strip wave + 4 i of the tile, lane 16 h + c its column c and pieces' h ----
+  // ---- weights: piece i of a run is strip wave + 4 i of the tile; a lane has its piece (h, c).  Eight lanes that write to LDS together
+  // have columns two apart, whose chunks are permuted differently: neighbours would be two to a bank ----
   typedef typename int4_detail::Bits<2 * C::PER_RUN>::type Scales;
   typedef typename int4_detail::Bits<C::PER_RUN>::type Zeros;
   u32x4_t codes[2][4];
   Scales scales[2][4];
   Zeros zeros[2][4];
-  const int c = lane & 15, h = lane >> 4, last_strip = int4_strips(b.n) - 1 - b.first / kInt4Strip;
+  const int c = 2 * (lane & 7) + (lane >> 3 & 1), h = lane >> 4, last_strip = int4_strips(b.n) - 1 - b.first / kInt4Strip;
+  const uint32_t piece = (uint32_t)(16 * h + c) * 16u;
   uint32_t column[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) column[i] = (uint32_t)imin(b.first + kInt4Strip * (wave + 4 * i) + c, b.n - 1);
@@ -113,7 +160,7 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
     constexpr int SET = decltype(set)::value;
     const int r = imin(run, b.runs - 1);  // (behind the last run x is zero)
     const size_t strip = (size_t)imin(wave + 4 * i, last_strip) * b.stride + r;
-    codes[SET][i] = int4_detail::load_at<u32x4_t>(int4_detail::scalar_base(b.codes, strip * 1024), lane * 16u);
+    codes[SET][i] = int4_detail::load_at<u32x4_t>(int4_detail::scalar_base(b.codes, strip * 1024), piece);
     const size_t at = (size_t)r * b.n;
     scales[SET][i] = int4_detail::load_at<Scales>(int4_detail::scalar_base(b.scales, at * sizeof(Scales)), column[i] * (uint32_t)sizeof(Scales));
     zeros[SET][i] = int4_detail::load_at<Zeros>(int4_detail::scalar_base(b.zeros, at * sizeof(Zeros)), column[i] * (uint32_t)sizeof(Zeros));
@@ -124,9 +171,14 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
 #pragma unroll
   for (int j = 0; j < 2; ++j) b_at[j] = C::A_BYTES + b_row * 128 + (((4 * j + h) ^ b_sw) << 4);
   // Step st of word w (of the slab's half HALF_RUN) of piece i: a pair of weights; with the last one all eight are written.
-  float s = 0.f, sz = 0.f;
-  uint32_t low = 0, high = 0;
+  float s = 0.f, from1024 = 0.f, from64 = 0.f;
+  uint32_t word = 0;
+  float lo = 0.f, hi = 0.f;
   u32x4_t out;
+  uint32_t mask0 = 0x000f000fu, mask4 = 0x00f000f0u, one0 = 0x64006400u, one4 = 0x54005400u;  // 1024, 64
+  asm("" : "+s"(mask0), "+s"(mask4));
+  asm("" : "+v"(one0), "+v"(one4));
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
   constexpr int kSteps = 4;
   auto convert = [&](auto set, auto half_run, int slot, int i, int w, int st) {
     constexpr int SET = decltype(set)::value, J0 = 2 * decltype(half_run)::value;
@@ -135,19 +187,24 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
       if (w == 0 || C::BLOCK == 32) {
         const int e = j * 32 / C::BLOCK;
         s = int4_detail::scale_to_f32((uint32_t)(scales[SET][i] >> (16 * e)) & 0xffff, b.scale_half);
-        const float z = (float)((uint32_t)(zeros[SET][i] >> (8 * e)) & 0xff);
-        sz = -s * (b.has_zeros ? z : 8.f);
+        const float z = b.has_zeros ? (float)((uint32_t)(zeros[SET][i] >> (8 * e)) & 0xff) : 8.f;
+        from1024 = -s * (1024.f + z);
+        from64 = -s * (64.f + z);
       }
-      const uint32_t word = codes[SET][i][j];
-      low = word & 0x0f0f0f0fu;
-      high = (word >> 4) & 0x0f0f0f0fu;
-      asm("" : "+v"(low), "+v"(high));  // (the compiler would take every code out of the word by itself, an instruction each)
+      word = codes[SET][i][j];
     }
-    // codes 0, 4, 1, 5 are the bytes of `low`, 2, 6, 3, 7 those of `high`
-    const uint32_t from = (st & 1) ? high : low;
-    const int byte = st >> 1;
-    const float u = (float)((from >> (8 * byte)) & 0xff), v = (float)((from >> (8 * byte + 16)) & 0xff);
-    out[st] = pack_out_x2<C::HALF>(__builtin_fmaf(u, s, sz), __builtin_fmaf(v, s, sz));
+    if (st == 2) word >>= 8;
+    const f16x2_t v = __builtin_bit_cast(f16x2_t, (st & 1) ? (word & mask4) | one4 : (word & mask0) | one0);
+    const float from = (st & 1) ? from64 : from1024;
+    if (C::HALF) {
+      const f16x2_t both = {(_Float16)__builtin_fmaf((float)v[0], s, from), (_Float16)__builtin_fmaf((float)v[1], s, from)};
+      out[st] = __builtin_bit_cast(uint32_t, both);
+    } else {
+      if (st > 0) out[st - 1] = pack_out_x2<C::HALF>(lo, hi);
+      lo = __builtin_fmaf((float)v[0], s, from);
+      hi = __builtin_fmaf((float)v[1], s, from);
+      if (st == kSteps - 1) out[st] = pack_out_x2<C::HALF>(lo, hi);
+    }
     if (st == kSteps - 1) *reinterpret_cast<u32x4_t*>(smem + slot + b_at[w] + i * 4 * kInt4Strip * 128) = out;
   };
 
@@ -201,57 +258,42 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
   // second half is written, by its load two runs on.
   auto slab = [&](int t, auto phase) {
     constexpr int PHASE = decltype(phase)::value, CUR = PHASE & 1, NEXT = 1 - CUR;
-    constexpr int cur_off = CUR * C::SLOT_BYTES, next_off = NEXT * C::SLOT_BYTES;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool last = u == 3;
-      if (last) {  // own reads of slab t returned, own part of slab t + 1 written; behind the barrier slab t + 1 is complete
-        la.advance(wave, lane);
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    int4_detail::static_for<4>([&](auto substep) {
+      constexpr int U = decltype(substep)::value, MF = C::TM * C::TN;
+      constexpr bool LAST = U == 3;
+      constexpr int QUARTER = LAST ? 0 : U + 1, FIRST = part(QUARTER), COUNT = part(QUARTER + 1) - FIRST;
+      // what is written: quarter QUARTER of slab t + 2 (LAST) or t + 1, half HALF_RUN of run SET
+      constexpr int SIDE = LAST ? CUR : NEXT, SET = ((PHASE + (LAST ? 2 : 1)) >> 1) & 1, OFF = SIDE * C::SLOT_BYTES;
+      constexpr int4_detail::Schedule plan = int4_detail::schedule(C::TM, C::TN, COUNT, SIDE == 1, LAST);
+      const unsigned char* ra = smem + (LAST ? NEXT : CUR) * C::SLOT_BYTES;  // fragments of the next substep
+      constexpr int US = LAST ? 0 : U + 1;
+      if (LAST) la.advance(wave, lane);
+      trim_a(Int<SIDE>{}, t + (LAST ? 2 : 1), FIRST, COUNT);
+      int4_detail::static_for<MF>([&](auto gap) {
+        constexpr int M = decltype(gap)::value, I = M / C::TN, J = M % C::TN;
+        int4_detail::static_for<int4_detail::kMaxOps>([&](auto index) {
+          constexpr int O = decltype(index)::value;
+          if constexpr (O < plan.count && plan.gap[O] == M) {
+            constexpr int ARG = plan.arg[O];
+            constexpr int4_detail::Op OP = plan.op[O];
+            if constexpr (OP == int4_detail::kReadA) fa[(U + 1) & 1][ARG] = fra.read(ra, ARG, US);
+            if constexpr (OP == int4_detail::kReadB) fb[(U + 1) & 1][ARG] = frb.read(ra + C::A_BYTES, ARG, US);
+            if constexpr (OP == int4_detail::kConvert) convert(Int<SET>{}, Int<SIDE>{}, OFF, QUARTER, ARG / kSteps, ARG % kSteps);
+            if constexpr (OP == int4_detail::kCommit) commit_a(Int<SIDE>{}, OFF, FIRST + ARG);
+            if constexpr (OP == int4_detail::kFetch) fetch_a(Int<SIDE>{}, FIRST + ARG);
+            if constexpr (OP == int4_detail::kRun) fetch_b(Int<SET>{}, ((t + (LAST ? 2 : 1)) >> 1) + 2, QUARTER);
+            if constexpr (OP == int4_detail::kBarrier) {  // own reads of slab t returned, own part of slab t + 1 written; behind it slab t + 1 is complete
+              __builtin_amdgcn_sched_barrier(0);
+              __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+              __builtin_amdgcn_s_barrier();
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        });
+        acc[I][J] = mfma_32x32x16<C::HALF>(fb[U & 1][J], fa[U & 1][I], acc[I][J]);
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      const unsigned char* ra = smem + (last ? next_off : cur_off);  // fragments of the next substep
-      const int us = last ? 0 : u + 1, quarter = last ? 0 : u + 1;
-      const int first = part(quarter), count = part(quarter + 1) - part(quarter);
-      if (last) trim_a(Int<CUR>{}, t + 2, first, count);
-      else trim_a(Int<NEXT>{}, t + 1, first, count);
-      // ops of the substep: a fragment read and a step of a conversion in turn, then what moves of x and of the runs
-      constexpr int FR = C::TM + C::TN, CV = 2 * kSteps, MF = C::TM * C::TN;
-      const int ops = FR + CV + 2 * count + 1;
-      auto op = [&](int o) {
-        constexpr int BOTH = FR < CV ? FR : CV;
-        const bool paired = o < 2 * BOTH;
-        const int read = paired ? (o % 2 == 0 ? o / 2 : -1) : FR > CV && o < FR + CV ? o - CV : -1;
-        const int conv = paired ? (o % 2 == 1 ? o / 2 : -1) : CV > FR && o < FR + CV ? o - FR : -1;
-        if (read >= 0) {
-          if (read < C::TM) fa[(u + 1) & 1][read] = fra.read(ra, read, us);
-          else fb[(u + 1) & 1][read - C::TM] = frb.read(ra + C::A_BYTES, read - C::TM, us);
-        } else if (conv >= 0) {
-          // slab t + 2: run (t + 2) / 2, half t & 1; slab t + 1: run (t + 1) / 2, half (t + 1) & 1
-          if (last) convert(Int<((PHASE + 2) >> 1) & 1>{}, Int<CUR>{}, cur_off, quarter, conv / kSteps, conv % kSteps);
-          else convert(Int<((PHASE + 1) >> 1) & 1>{}, Int<NEXT>{}, next_off, quarter, conv / kSteps, conv % kSteps);
-        } else if (o < FR + CV + 2 * count) {
-          const int q = first + (o - FR - CV) / 2;
-          const bool write = (o - FR - CV) % 2 == 0;
-          if (last) { if (write) commit_a(Int<CUR>{}, cur_off, q); else fetch_a(Int<CUR>{}, q); }
-          else { if (write) commit_a(Int<NEXT>{}, next_off, q); else fetch_a(Int<NEXT>{}, q); }
-        } else if (last ? CUR == 1 : NEXT == 1) {  // a second half has just been written
-          if (last) fetch_b(Int<((PHASE + 2) >> 1) & 1>{}, ((t + 2) >> 1) + 2, quarter);
-          else fetch_b(Int<((PHASE + 1) >> 1) & 1>{}, ((t + 1) >> 1) + 2, quarter);
-        }
-      };
-#pragma unroll
-      for (int m = 0; m < MF; ++m) {
-#pragma unroll
-        for (int o = 0; o < FR + CV + 2 * HEAD_MOST + 1; ++o)
-          if (o >= m * ops / MF && o < (m + 1) * ops / MF) op(o);
-        const int i = m / C::TN, j = m % C::TN;
-        acc[i][j] = mfma_32x32x16<C::HALF>(fb[u & 1][j], fa[u & 1][i], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
+      });
+    });
   };
   // (an nk that is no multiple of four multiplies up to three slabs of zeros: a way out of the middle of the loop had the compiler
   // hold two sets of accumulators, 600 registers spilled)

@@ -272,7 +272,7 @@ int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, 
  *           lower four bits), [g, k, n] or with trans_rhs [g, n, k].  In strips of 16 columns and runs of 128 indices, word j of
  *           piece (h, c), codes[e][strip][run][h][c][j], h, j < 4, c < 16, holds column 16 strip + c and the indices 128 run +
  *           32 j + 8 h + i, i < 8, code i at bits 4 (i / 2) + 16 (i % 2); codes past k and n are 8;
- *   scales: [g_local, ceil(k / 128), n, 128 / block], scale_dtype RD_DTYPE_BF16 or RD_DTYPE_F16, 0 past k;
+ *   scales: [g_local, ceil(k / 128), n, 128 / block], scale_dtype RD_DTYPE_BF16 or RD_DTYPE_F16, below 2^116, 0 past k;
  *   zeros:  bytes of the same shape, or NULL: 8 throughout.
  * x and y are RD_DTYPE_BF16 or RD_DTYPE_F16.  group_sizes, the rows past their sum (zero), clipping at m, group_offset and g_local
  * are those of rd_gmm_sharded.  fp32 sums, one rounding of the result.  Groups of many rows are multiplied in tiles whose weights
