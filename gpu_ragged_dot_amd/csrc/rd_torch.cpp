@@ -8,6 +8,8 @@
 // rd_lookup.h); a decoding step on 13 experts of 512 x 5248: 18.4 -> 8.3 us.  What a call costs the host: 8.6 us a product,
 // 4.4 a dispatch, 0.2 of them for giving up the interpreter lock and taking it again.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
@@ -161,6 +163,13 @@ at::ScalarType out_type(const Tensor& t) { return t.scalar_type() == at::kFloat8
 // (its own buffer per call: the caching allocator hands it back to the stream that used it)
 Tensor scratch(size_t bytes, const at::Device& dev) {
   return at::empty({(int64_t)(bytes < 256 ? 256 : bytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
+}
+
+// at::empty() on a device without the dispatcher's 0.2 us, for calls whose kernels take less than the host's 4 us.  A trace has to see
+// where a result comes from.
+Tensor empty_on(at::IntArrayRef sizes, at::ScalarType type, const at::Device& dev) {
+  if (at::tracer::impl::is_dispatch_enabled()) return at::empty(sizes, at::TensorOptions().dtype(type).device(dev));
+  return Tensor(at::detail::empty_cuda(sizes, type, dev, std::nullopt));
 }
 
 void* stream_of(const at::Device& dev) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream(); }
@@ -444,9 +453,8 @@ Tensor moe_combine(const Tensor& y, const std::optional<Tensor>& weights, const 
 // ---- expert ids and weights from a router's logits ---------------------------------------------------------------------
 std::tuple<Tensor, Tensor> gate_forward(const Tensor& logits, const Tensor& bias, const rd_gate_spec& spec) {
   const c10::DeviceGuard guard(logits.device());
-  const auto opts = at::TensorOptions().device(logits.device());
   const int64_t tokens = logits.size(0);
-  Tensor ids = at::empty({tokens, spec.top_k}, opts.dtype(at::kInt)), weights = at::empty({tokens, spec.top_k}, opts.dtype(at::kFloat));
+  Tensor ids = empty_on({tokens, spec.top_k}, at::kInt, logits.device()), weights = empty_on({tokens, spec.top_k}, at::kFloat, logits.device());
   check(rd_moe_gate(stream_of(logits.device()), logits.const_data_ptr(), bias.defined() ? bias.const_data_ptr<float>() : nullptr,
                     ids.mutable_data_ptr<int32_t>(), weights.mutable_data_ptr<float>(), (int)tokens, (int)logits.size(1), &spec, rows_code(logits)));
   return {ids, weights};
@@ -475,7 +483,7 @@ struct GateNode : torch::autograd::Function<GateNode> {
       check_devices(logits, grads[1]);
       const c10::DeviceGuard guard(logits.device());
       const Tensor dw = grads[1].to(at::kFloat).contiguous();
-      Tensor dl = at::empty(logits.sizes(), logits.options().requires_grad(false));
+      Tensor dl = empty_on(logits.sizes(), logits.scalar_type(), logits.device());
       check(rd_moe_gate_grad(stream_of(logits.device()), logits.const_data_ptr(), ids.const_data_ptr<int32_t>(), weights.const_data_ptr<float>(),
                              dw.const_data_ptr<float>(), dl.mutable_data_ptr(), (int)logits.size(0), (int)logits.size(1), &spec, rows_code(logits)));
       return {dl, Tensor(), Tensor()};
@@ -507,7 +515,7 @@ std::tuple<Tensor, Tensor> moe_gate(const Tensor& logits_, const std::optional<T
 Tensor swiglu_forward(const Tensor& y) {
   const c10::DeviceGuard guard(y.device());
   const int64_t f = y.size(1) / 2;
-  Tensor out = at::empty({y.size(0), f}, y.options().requires_grad(false));
+  Tensor out = empty_on({y.size(0), f}, y.scalar_type(), y.device());
   check(rd_moe_swiglu(stream_of(y.device()), y.const_data_ptr(), out.mutable_data_ptr(), (int)y.size(0), (int)f, rows_code(y)));
   return out;
 }
@@ -525,7 +533,7 @@ struct SwigluNode : torch::autograd::Function<SwigluNode> {
       same_type(y, grads[0]);
       const c10::DeviceGuard guard(y.device());
       const Tensor dout = grads[0].contiguous();
-      Tensor dy = at::empty(y.sizes(), y.options().requires_grad(false));
+      Tensor dy = empty_on(y.sizes(), y.scalar_type(), y.device());
       check(rd_moe_swiglu_grad(stream_of(y.device()), y.const_data_ptr(), dout.const_data_ptr(), dy.mutable_data_ptr(), (int)y.size(0),
                                (int)(y.size(1) / 2), rows_code(y)));
       return {dy};
@@ -593,7 +601,7 @@ Tensor gmm_int4(const Tensor& x_, const Tensor& codes, const Tensor& scales, con
   const at::Device dev = x_.device();
   const Tensor x = x_.contiguous(), gs = sizes_on(gs_, dev);
   const c10::DeviceGuard guard(dev);
-  Tensor y = at::empty({x.size(0), n}, x.options().requires_grad(false));
+  Tensor y = empty_on({x.size(0), n}, x.scalar_type(), dev);
   const size_t ws_bytes = rd_gmm_int4_workspace_bytes((int)x.size(0), (int)k, (int)n, (int)g, kernel);
   const Tensor ws = ws_bytes ? scratch(ws_bytes, dev) : Tensor();
   check(rd_gmm_int4(stream_of(dev), x.const_data_ptr(), codes.const_data_ptr(), scales.const_data_ptr(), zeros ? zeros->const_data_ptr<uint8_t>() : nullptr,

@@ -41,6 +41,8 @@ class Gating(NamedTuple):
     weights: torch.Tensor       # float32 [tokens, top_k]  for ``combine``; 0 where there is no expert
 
 
+_gating = tuple.__new__                         # Gating(*results) without its keyword arguments' 0.2 us
+
 _SCORES = {"softmax": 0, "sigmoid": 1}         # RD_GATE_SIGMOID
 _CLUSTER_SCORES = {"max": 0, "top2": 2}        # RD_GATE_TOP2
 _RENORMALIZE = 4                               # RD_GATE_RENORMALIZE
@@ -61,11 +63,11 @@ def gate(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Opti
     if cluster_score not in _CLUSTER_SCORES:
         raise ValueError(f"cluster_score is one of {sorted(_CLUSTER_SCORES)}, not {cluster_score!r}")
     flags = _SCORES[score] | _CLUSTER_SCORES[cluster_score] | (_RENORMALIZE if renormalize else 0)
-    spec = (int(top_k), int(clusters), int(clusters if top_clusters is None else top_clusters), flags, float(scale))
+    spec = (top_k, clusters, clusters if top_clusters is None else top_clusters, flags, scale)
     if _tracing.active():
         return Gating(*_tracing.record(lambda l, *b: _native.moe_gate(l, b[0] if b else None, *spec), logits,
                                        *(() if bias is None else (bias,))))
-    return Gating(*_native.moe_gate(logits, bias, *spec))
+    return _gating(Gating, _native.moe_gate(logits, bias, *spec))
 
 
 def route(expert_ids: torch.Tensor, num_groups: int) -> Routing:
