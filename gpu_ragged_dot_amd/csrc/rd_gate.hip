@@ -14,9 +14,9 @@
 //    expert's index behind them: one unsigned maximum compares rank and index at once, and since no two keys are equal, the next
 //    smaller one is the largest of key - previous (mod 2^32) - a subtraction and half a three-way maximum per expert, nothing to remove;
 //  * whether that decided what 64 bits would decide shows in the keys.  Where two neighbours among the chosen and the first one left
-//    out are closer than the error of 32-bit ranks (a row in a thousand on the sizes above), the leading 16 are ranked in 64 bits, one
-//    to a lane; where two clusters are, or softmax ranks with a bias, the wave does its rows again in 64 bits.  16-bit logits that rank
-//    by themselves are exact in the key: there ties are ties.
+//    out are closer than the error of 32-bit ranks (a row in a thousand on the sizes above), those, or the leading 16, are ranked in
+//    64 bits, one to a lane; where two clusters are, the wave does its rows again in 64 bits.  16-bit logits that rank by themselves
+//    are exact in the key: there ties are ties.
 // The sizes above take 29 us so; 4096 tokens, where few rows need 64 bits and a wave's latency is most of it, 9.
 #include "rd_elem.h"
 #include "rd_moe.h"
@@ -437,21 +437,33 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
   }
   close = close && !exact;
   auto expert_of = [](uint32_t k) { return k ? (int)(kKeyIndexMask - (k & kKeyIndexMask)) : -1; };
-  // Close ones in some row: the leading 16 by their ranks in 64 bits, one to a lane, if the last of them is out of the question.
-  // (Softmax ranks with a bias need the whole row's sum in 64 bits.)
+  // Close ones in some row: those chosen and the first left out by their ranks in 64 bits, one to a lane; where that one is close
+  // to the last chosen, as many more as there are lanes, if the last of them is out of the question.
   if (__ballot(close)) {
-    const uint32_t kth = (uint32_t)__shfl((int)chosen, (lane & 48) + p.top_k - 1, 64);
-    for (int s = p.top_k + 1; s < kRowLanes; ++s) {
-      previous = next_key();
-      if (at == s) chosen = previous;
-    }
-    const bool settled = (!scored || p.sigmoid) && p.top_k < kRowLanes && (previous == 0u || (kth >> kKeyIndexBits) - (previous >> kKeyIndexBits) > near);
+    const uint32_t kth = (uint32_t)__shfl((int)chosen, (lane & 48) + p.top_k - 1, 64) >> kKeyIndexBits;
+    auto out_of_question = [&]() { return previous == 0u || kth - (previous >> kKeyIndexBits) > near; };
+    if (__ballot(close && !out_of_question()))
+      for (int s = p.top_k + 1; s < kRowLanes; ++s) {
+        previous = next_key();
+        if (at == s) chosen = previous;
+      }
+    const bool settled = out_of_question();
     odd |= close && !settled;
+    double total = 1.0;
+    if (scored && !p.sigmoid) {
+      total = 0.0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float x = i < own ? to_f32<T>(src[e0 + i]) : -INFINITY;
+        if (x > -INFINITY) total += exp((double)x - (double)top);  // (no NaN here: such a row is odd)
+      }
+      total = row_sum(total);
+    }
     const int e = expert_of(chosen);
     double v = -INFINITY;
     if (e >= 0) {
       const float x = to_f32<T>(src[e]);
-      v = scored ? 1.0 / (1.0 + exp(-(double)x)) : (double)x;
+      v = !scored ? (double)x : p.sigmoid ? 1.0 / (1.0 + exp(-(double)x)) : exp((double)x - (double)top) / total;
       if (bias) v += bias[e];
     }
     const uint64_t bits = __builtin_bit_cast(uint64_t, v);
