@@ -15,9 +15,10 @@
 //    smaller one is the largest of key - previous (mod 2^32) - a subtraction and half a three-way maximum per expert, nothing to remove;
 //  * whether that decided what 64 bits would decide shows in the keys.  Where two neighbours among the chosen and the first one left
 //    out are closer than the error of 32-bit ranks (a row in a thousand on the sizes above), those, or the leading 16, are ranked in
-//    64 bits, one to a lane; where two clusters are, the wave does its rows again in 64 bits.  16-bit logits that rank by themselves
-//    are exact in the key: there ties are ties.
-// The sizes above take 29 us so; 4096 tokens, where few rows need 64 bits and a wave's latency is most of it, 9.
+//    64 bits, one to a lane, and clusters by those of their two best.  Rows that this leaves open the wave does again in 64 bits.  16-bit
+//    logits that rank by themselves are exact in the key: there ties are ties.
+// The sizes above take 21 us so (27 with logits from memory), 1250 vector instructions a wave; 4096 tokens, where a wave's latency is most
+// of it, 9.
 #include "rd_elem.h"
 #include "rd_moe.h"
 
@@ -394,6 +395,25 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
 #pragma unroll
   for (int i = 0; i < PER; ++i) key[i] = key[i] ? key[i] << kKeyIndexBits | (kKeyIndexMask - (uint32_t)(e0 + i)) : 0u;
 
+  auto expert_of = [](uint32_t k) { return k ? (int)(kKeyIndexMask - (k & kKeyIndexMask)) : -1; };
+  // The rank of expert e in 64 bits, and the sum that softmax ranks take.
+  auto wide_total = [&]() {
+    if (!scored || p.sigmoid) return 1.0;
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float x = i < own ? to_f32<T>(src[e0 + i]) : -INFINITY;
+      if (x > -INFINITY) total += exp((double)x - (double)top);  // (a row with NaN is odd)
+    }
+    return row_sum(total);
+  };
+  auto wide_rank = [&](int e, double total) -> double {
+    if (e < 0) return -INFINITY;
+    const double x = to_f32<T>(src[e]);
+    const double v = !scored ? x : p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double)top) / total;
+    return bias ? v + bias[e] : v;
+  };
+
   // ---- clusters ----
   if (p.clusters > 1) {
     Two t = {0u, 0u};
@@ -413,7 +433,28 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
     if (!exact && p.top_clusters < p.clusters) {  // the worst of those kept against the best of the others
       const uint32_t worst = ~row_max(ahead < p.top_clusters && mine < p.clusters ? ~score : 0u);
       const uint32_t best = row_max(ahead >= p.top_clusters && mine < p.clusters ? score : 0u);
-      odd |= worst - best <= (p.top2 ? 2 * near : near);
+      const bool close = worst - best <= (p.top2 ? 2 * near : near);
+      // Close ones in some row: by the ranks of each cluster's two best in 64 bits, if no third one comes into question.
+      if (__ballot(close)) {
+        uint32_t third = 0u;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) third = umax(third, key[i] - t.second);
+        if (cluster_lanes >= 2) third = umax(third, from_lane<kSwap1>(third));
+        if (cluster_lanes >= 4) third = umax(third, from_lane<kSwap2>(third));
+        if (cluster_lanes >= 8) third = umax(third, from_lane<kMirror8>(third));
+        third = t.second ? third + t.second : 0u;
+        const bool questionable = third && (p.top2 ? q2 : q1) - (third >> kKeyIndexBits) <= near;
+        odd |= close && row_max(questionable ? 1u : 0u) != 0u;
+        const double total = wide_total();
+        const double v1 = wide_rank(expert_of(t.first), total), v2 = wide_rank(expert_of(t.second), total);
+        const double exact_score = p.top2 ? v1 + v2 : fmax(v1, v2);
+        int exact_ahead = 0;
+        for (int q = 0; q < p.clusters; ++q) {
+          const double other = __shfl(exact_score, (lane & 48) + q * cluster_lanes, 64);
+          exact_ahead += other > exact_score || (other == exact_score && q < mine) ? 1 : 0;
+        }
+        if (close) ahead = exact_ahead;
+      }
     }
     if (ahead >= p.top_clusters)
 #pragma unroll
@@ -436,7 +477,6 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
     previous = next;
   }
   close = close && !exact;
-  auto expert_of = [](uint32_t k) { return k ? (int)(kKeyIndexMask - (k & kKeyIndexMask)) : -1; };
   // Close ones in some row: those chosen and the first left out by their ranks in 64 bits, one to a lane; where that one is close
   // to the last chosen, as many more as there are lanes, if the last of them is out of the question.
   if (__ballot(close)) {
@@ -449,23 +489,8 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
       }
     const bool settled = out_of_question();
     odd |= close && !settled;
-    double total = 1.0;
-    if (scored && !p.sigmoid) {
-      total = 0.0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const float x = i < own ? to_f32<T>(src[e0 + i]) : -INFINITY;
-        if (x > -INFINITY) total += exp((double)x - (double)top);  // (no NaN here: such a row is odd)
-      }
-      total = row_sum(total);
-    }
     const int e = expert_of(chosen);
-    double v = -INFINITY;
-    if (e >= 0) {
-      const float x = to_f32<T>(src[e]);
-      v = !scored ? (double)x : p.sigmoid ? 1.0 / (1.0 + exp(-(double)x)) : exp((double)x - (double)top) / total;
-      if (bias) v += bias[e];
-    }
+    const double v = wide_rank(e, wide_total());
     const uint64_t bits = __builtin_bit_cast(uint64_t, v);
     int ahead = 0;
     for (int q = 0; q < kRowLanes; ++q) {

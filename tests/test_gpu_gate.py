@@ -133,6 +133,27 @@ def test_close_float32_logits(score, experts, top_k):
         _check(logits.cuda(), top_k, score=score, bias=bias, clusters=8, top_clusters=4, cluster_score="top2")
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("cluster_score", ["max", "top2"])
+@pytest.mark.parametrize("experts,clusters,dtype", [(256, 8, torch.float32), (64, 16, torch.float32), (96, 6, torch.float32), (32, 2, torch.float32),
+                                                    (256, 8, torch.bfloat16), (128, 4, torch.float16)])
+def test_close_clusters(score, cluster_score, experts, clusters, dtype):
+    """Clusters whose best experts are those of another one but for units in the last place, or (16-bit types) all the same; in some
+    rows a third expert is as close."""
+    gen = torch.Generator().manual_seed(experts + clusters)
+    size, tokens = experts // clusters, 64
+    logits = 0.3 * torch.randn((tokens, clusters, size), generator=gen)
+    best = 1.5 + torch.rand((tokens, 1, 2), generator=gen) + torch.randint(-4, 5, (tokens, clusters, 2), generator=gen) * 2.0 ** -23
+    logits[:, :, :2] = best
+    logits[::3, :, 2] = best[::3, :, 1] - torch.randint(0, 3, (tokens // 3 + 1, clusters), generator=gen) * 2.0 ** -23
+    order = torch.stack([torch.randperm(size, generator=gen) for _ in range(tokens * clusters)]).view(tokens, clusters, size)
+    logits = logits.gather(2, order).view(tokens, experts).to(dtype).cuda()
+    bias = torch.zeros(experts) + (torch.randint(-1, 2, (clusters, 1), generator=gen) * 2.0 ** -24).expand(clusters, size).reshape(-1)
+    for b in (None, bias.cuda()):
+        for top_clusters in (1, clusters // 2):
+            _check(logits, min(3, size), bias=b, score=score, clusters=clusters, top_clusters=top_clusters, cluster_score=cluster_score)
+
+
 @pytest.mark.parametrize("seed", range(60))
 def test_random_calls(seed):
     """Sizes, clusters, types, scores and biases of every kind at once: small, larger than the scores, of 1e30, -inf."""
