@@ -316,17 +316,18 @@ int stream(hipStream_t s, const Int4Problem& p, int most) {
 
 // Whether groups of more rows than kInt4FewRows are left to the tile kernel, a launch of its own.  The sizes are on the device; the
 // rule takes them to be equal, and what each kernel needs for that, us, from rounds of what the device holds at a time: 512
-// work-groups of 32 rows x 64 columns of the streaming kernel at 5 per 1024 indices, 256 tiles of the other at 1.1 .. 2.0 a slab of
-// 64 by their height.  bf16, blocks of 128, streaming | tiles: 32 groups of 64 x 7168 x 2048 172 | 120, 128 of 64 x 2048 x 768 86 |
-// 72, 8 of 64 x 4096 x 14336 135 | 160, 64 of 40 x 2048 x 1024 40 | 43, 8 of 40 x 4096 x 4096 35 | 52.  Where the streaming kernel is
-// long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
+// work-groups of 32 rows x 64 columns of the streaming kernel at 1 and 4 per 1024 indices, 256 tiles of the other at 1.1 .. 2.0 a slab
+// of 64 by their height.  bf16, blocks of 128, streaming | tiles: 32 groups of 64 x 7168 x 2048 168 | 135, 128 of 64 x 2048 x 768 85 |
+// 81, 8 of 64 x 4096 x 14336 106 | 138, 32 of 128 x 2048 x 768 35 | 47, 17 of about 96 x 328 x 3080 (blocks of 64, zeros) 35 | 24.  Over
+// 250 calls of random and of equal sizes it costs 0.7 % on the faster of the two.  Where the streaming kernel is long at work, groups
+// of very different sizes pay for the other launch, a few us, whatever their mean.
 constexpr int kInt4FewRows = 48;
 
 bool uses_tiles(int m, int k, int n, int g, int kernel) {
   if (m <= kInt4FewRows || k < 8 || k > (1 << 22) || kernel == RD_INT4_STREAM) return false;
   if (kernel == RD_INT4_TILES) return true;
   const double rows = (double)((m + g - 1) / g), cols64 = (n + 63) / 64, cols256 = (n + 255) / 256;
-  const double streaming = 6 + ceil(g * ceil(rows / 32) * cols64 / 512) * k * 0.005;
+  const double streaming = 6 + g * ceil(rows / 32) * cols64 / 512 * (1 + k * 0.004);
   if (streaming > 100) return true;
   if (rows <= kInt4FewRows) return false;
   const double last = rows - 256 * floor(rows / 256), height = last == 0 ? 0 : last <= 64 ? 1.1 : last <= 128 ? 1.3 : last <= 192 ? 1.65 : 2;
