@@ -18,7 +18,7 @@
 namespace rd {
 
 constexpr int kInt4Run = 128, kInt4Strip = 16;
-constexpr int kInt4MaxRows = (1 << 25) - 1;  // the sum of 64 groups' rows, each cut off at m, fits 32 bits
+constexpr int kInt4MaxRows = (1 << 25) - 1;  // 64 times as many fit 32 bits (counted_rows() in rd_int4_rows.h)
 
 struct Int4Problem {
   const void* x;            // [m][k], bfloat16 or float16

@@ -5,6 +5,10 @@
 
 namespace rd {
 
+// What a group's size counts behind `before` rows: negative ones nothing, and none more than the rows that are left.  So the sum
+// of 64 groups and of what lies before them stays below 64 m, and 32 bits hold it (kInt4MaxRows).
+__host__ __device__ __forceinline__ int counted_rows(int size, int before, int m) { return imin(imax(size, 0), m - before); }
+
 // The groups as the waves of a launch see them: sizes that are negative count as 0 and groups end at row m.  kLookupGroups at a
 // time, four per lane: f(chunk of 64 groups, first row and row behind the last one of lane's group) until it returns true.
 template <class F>
@@ -16,12 +20,12 @@ __device__ __forceinline__ void scan_groups(const int32_t* __restrict__ gs, int 
 #pragma unroll
     for (int c = 0; c < kLookupChunks; ++c) {
       const int e = base + 64 * c + lane;
-      size[c] = e < g ? imin(imax(gs[e], 0), m) : 0;
+      size[c] = e < g ? gs[e] : 0;
     }
 #pragma unroll
     for (int c = 0; c < kLookupChunks; ++c) {
       if (base + 64 * c >= g) break;
-      const int end = imin(rows_before + wave_inclusive_sum(size[c]), m);
+      const int end = imin(rows_before + wave_inclusive_sum(counted_rows(size[c], rows_before, m)), m);
       const int first = __builtin_amdgcn_update_dpp(rows_before, end, 0x138, 0xf, 0xf, false);  // the lane below's end: wave_shr:1
       if (f(base + 64 * c, first, end)) return;
       rows_before = __builtin_amdgcn_readlane(end, 63);
