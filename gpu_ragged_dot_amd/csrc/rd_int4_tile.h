@@ -134,10 +134,11 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
   u32x4_t a[2][PA];
   auto fetch_a = [&](auto set, int q) { a[decltype(set)::value][q] = la.fetch(q); };
   auto commit_a = [&](auto set, int slot, int q) { la.commit(smem + slot, q, a[decltype(set)::value][q]); };
-  auto trim_a = [&](auto set, int step, int first, int count) {
+  auto trim_a = [&](auto set, int step, int first, int count, auto&& also) {
     constexpr int SET = decltype(set)::value;
     if (step >= nk - 1) {
       asm volatile("");  // (a branch, not selects in every slab)
+      also();
 #pragma unroll
       for (int q = 0; q < PA; ++q)
         if (q >= first && q < first + count) a[SET][q] = la.trim(wave, lane, q, step, a[SET][q]);
@@ -207,6 +208,22 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
     }
     if (st == kSteps - 1) *reinterpret_cast<u32x4_t*>(smem + slot + b_at[w] + i * 4 * kInt4Strip * 128) = out;
   };
+  // float16 rows: what piece i has of slab `step` past the contraction becomes zero in LDS, behind the writes of convert().  It stands on
+  // the scale of the last block, on which the padding's codes may be infinite in float16 where the operand's are not, and infinite
+  // times x's zeros is NaN.  (bfloat16 holds every weight.)  To be called where trim_a() has its branch.
+  auto trim_b = [&](int step, int slot, int i) {
+    const int left = klen - step * C::BK;
+    if (!C::HALF || left >= C::BK) return;
+    unsigned char* at = smem + slot + i * 4 * kInt4Strip * 128;
+    if (left <= 0) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) *reinterpret_cast<u32x4_t*>(at + b_at[w]) = u32x4_t{0, 0, 0, 0};
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < 16; ++e)
+        if ((e >> 3) * 32 + 8 * h + (e & 7) >= left) *reinterpret_cast<uint16_t*>(at + (e < 8 ? b_at[0] : b_at[1]) + 2 * (e & 7)) = 0;
+    }
+  };
 
   constexpr auto part = [](int u) constexpr { return u * PA / 4; };
   constexpr int HEAD = part(1), HEAD_MOST = (PA + 3) / 4;
@@ -222,19 +239,22 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
 #pragma unroll
   for (int q = 0; q < PA; ++q) fetch_a(Int<1>{}, q);
   la.advance(wave, lane);
-  trim_a(Int<0>{}, 0, 0, PA);
+  trim_a(Int<0>{}, 0, 0, PA, [] {});
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int w = 0; w < 2; ++w)
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) convert(Int<0>{}, Int<0>{}, 0, i, w, st);
+  if (nk == 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) trim_b(0, 0, i);
 #pragma unroll
   for (int q = 0; q < PA; ++q) commit_a(Int<0>{}, 0, q);
 #pragma unroll
   for (int q = 0; q < PA; ++q) fetch_a(Int<0>{}, q);
   la.advance(wave, lane);
-  trim_a(Int<1>{}, 1, 0, HEAD);
+  trim_a(Int<1>{}, 1, 0, HEAD, [] {});
 #pragma unroll
   for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -268,7 +288,7 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
       const unsigned char* ra = smem + (LAST ? NEXT : CUR) * C::SLOT_BYTES;  // fragments of the next substep
       constexpr int US = LAST ? 0 : U + 1;
       if (LAST) la.advance(wave, lane);
-      trim_a(Int<SIDE>{}, t + (LAST ? 2 : 1), FIRST, COUNT);
+      trim_a(Int<SIDE>{}, t + (LAST ? 2 : 1), FIRST, COUNT, [&] { trim_b(t + 1, NEXT * C::SLOT_BYTES, U); });  // (the quarter written last)
       int4_detail::static_for<MF>([&](auto gap) {
         constexpr int M = decltype(gap)::value, I = M / C::TN, J = M % C::TN;
         int4_detail::static_for<int4_detail::kMaxOps>([&](auto index) {
