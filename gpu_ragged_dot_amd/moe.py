@@ -66,7 +66,7 @@ def gate(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Opti
     spec = (top_k, clusters, clusters if top_clusters is None else top_clusters, flags, scale)
     if _tracing.active():
         return Gating(*_tracing.record(lambda l, *b: _native.moe_gate(l, b[0] if b else None, *spec), logits,
-                                       *(() if bias is None else (bias,))))
+                                       *(() if bias is None else (bias.detach(),))))  # (no gradient: it moves the choice alone)
     return _gating(Gating, _native.moe_gate(logits, bias, *spec))
 
 
