@@ -39,6 +39,8 @@ class _Node(torch.autograd.Function):
         wanted = [t for t in ctx.operands if t.requires_grad]
         results = (ctx.results,) if isinstance(ctx.results, torch.Tensor) else ctx.results
         live = [(t, g) for t, g in zip(results, grads) if t.requires_grad]  # (expert ids have no gradient)
+        if not live:
+            raise NotImplementedError("the traced call has no gradient")
         got = iter(torch.autograd.grad([t for t, _ in live], wanted, [g for _, g in live], retain_graph=True))
         return (None, *(next(got) if t.requires_grad else None for t in ctx.operands))
 

@@ -75,5 +75,7 @@ def _ragged_dot_int4(x, weights, group_sizes, group_offset=None, kernel=_capi.RD
     call = lambda x, gs: _native.gmm_int4(x, weights.codes, weights.scales, weights.zeros, weights.k, weights.n, weights.block, gs, g_first,
                                           kernel)
     if _tracing.active():
-        return _tracing.record(call, x, _sizes(group_sizes))
+        # (a trace's node does not know whether its caller wants gradients: it refuses in the backward pass, and not where x asks for
+        # one under torch.no_grad())
+        return _tracing.record(lambda x, gs: call(x.detach(), gs), x, _sizes(group_sizes))
     return call(x, _sizes(group_sizes))
