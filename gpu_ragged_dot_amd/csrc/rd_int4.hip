@@ -92,7 +92,7 @@ __device__ __forceinline__ void int4_stream_tile(const Int4Problem& p, const Row
     Run d;
     const size_t at = scales0 + (size_t)r * p.n;
     d.scales = load_at<typename Run::Scales>(scalar_base(p.scales, at * sizeof(typename Run::Scales)), column * (uint32_t)sizeof(typename Run::Scales));
-    if constexpr (ZEROS) d.zeros = load_at<typename Run::Zeros>(scalar_base(p.zeros, at * sizeof(typename Run::Zeros)), column * (uint32_t)sizeof(typename Run::Zeros));
+    if constexpr (ZEROS) d.zeros = load_at<typename Run::Zeros, 1>(scalar_base(p.zeros, at * sizeof(typename Run::Zeros)), column * (uint32_t)sizeof(typename Run::Zeros));
 #pragma unroll
     for (int c = 0; c < kInt4Strips; ++c) {
       const size_t strip = (size_t)imin(c, (cols - 1) / kInt4Strip) * runs + r;

@@ -62,10 +62,10 @@ __device__ __forceinline__ const char* scalar_base(const void* p, size_t offset)
   asm("" : "+s"(b));
   return reinterpret_cast<const char*>(b);
 }
-template <class V>
+template <class V, int ALIGNED = 2>
 __device__ __forceinline__ V load_at(const char* base, uint32_t offset) {
   typedef const __attribute__((address_space(1))) char* global_bytes;
-  typedef V unaligned_t __attribute__((aligned(sizeof(V) < 2 ? 1 : 2)));
+  typedef V unaligned_t __attribute__((aligned(ALIGNED)));
   return *reinterpret_cast<const __attribute__((address_space(1))) unaligned_t*>((global_bytes)base + offset);
 }
 
@@ -164,7 +164,7 @@ __device__ __forceinline__ void int4_tile_kloop(const typename C::Elem* __restri
     codes[SET][i] = int4_detail::load_at<u32x4_t>(int4_detail::scalar_base(b.codes, strip * 1024), piece);
     const size_t at = (size_t)r * b.n;
     scales[SET][i] = int4_detail::load_at<Scales>(int4_detail::scalar_base(b.scales, at * sizeof(Scales)), column[i] * (uint32_t)sizeof(Scales));
-    zeros[SET][i] = int4_detail::load_at<Zeros>(int4_detail::scalar_base(b.zeros, at * sizeof(Zeros)), column[i] * (uint32_t)sizeof(Zeros));
+    zeros[SET][i] = int4_detail::load_at<Zeros, 1>(int4_detail::scalar_base(b.zeros, at * sizeof(Zeros)), column[i] * (uint32_t)sizeof(Zeros));
   };
   // Where a word's weights go: row `column of the tile`, chunk (j & 1) 4 + h, permuted as DldsFragReader reads it.
   const int b_row = kInt4Strip * wave + c, b_sw = (b_row >> 1) & 7;  // (strips four apart: the permutation repeats)
