@@ -335,10 +335,9 @@ bool uses_tiles(int m, int k, int n, int g, int kernel) {
   return 12 + k / 64 * (work > least ? work : least) < streaming;
 }
 
-// Rows of the largest groups that the streaming kernel multiplies.  (float16 does not have the range of bfloat16 scales, and the
-// tiles' weights are of the rows' type.)
+// Rows of the largest groups that the streaming kernel multiplies.
 int most_streamed(const Int4Problem& p) {
-  return (!p.half || p.scale_half) && uses_tiles(p.m, p.k, p.n, p.g, p.kernel) ? kInt4FewRows : p.m;
+  return int4_tiles_hold(p.half, p.scale_half) && uses_tiles(p.m, p.k, p.n, p.g, p.kernel) ? kInt4FewRows : p.m;
 }
 
 template <bool HALF, int BLOCK>

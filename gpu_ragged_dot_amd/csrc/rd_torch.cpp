@@ -602,7 +602,9 @@ Tensor gmm_int4(const Tensor& x_, const Tensor& codes, const Tensor& scales, con
   const Tensor x = x_.contiguous(), gs = sizes_on(gs_, dev);
   const c10::DeviceGuard guard(dev);
   Tensor y = empty_on({x.size(0), n}, x.scalar_type(), dev);
-  const size_t ws_bytes = rd_gmm_int4_workspace_bytes((int)x.size(0), (int)k, (int)n, (int)g, kernel);
+  // (float16 rows with bfloat16 scales: no tiles, and nothing to cut)
+  const bool streamed = x.scalar_type() == at::kHalf && code == RD_DTYPE_BF16;
+  const size_t ws_bytes = streamed ? 0 : rd_gmm_int4_workspace_bytes((int)x.size(0), (int)k, (int)n, (int)g, kernel);
   const Tensor ws = ws_bytes ? scratch(ws_bytes, dev) : Tensor();
   check(rd_gmm_int4(stream_of(dev), x.const_data_ptr(), codes.const_data_ptr(), scales.const_data_ptr(), zeros ? zeros->const_data_ptr<uint8_t>() : nullptr,
                     gs.const_data_ptr<int32_t>(), y.mutable_data_ptr(), (int)x.size(0), (int)k, (int)n, (int)g, (int)(g_first < 0 ? 0 : g_first),
