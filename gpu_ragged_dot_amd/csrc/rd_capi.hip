@@ -1294,7 +1294,7 @@ int rd_int4_pack(void* stream, const uint8_t* q, void* codes, int g, int k, int 
 
 size_t rd_gmm_int4_workspace_bytes(int m, int k, int n, int g, int kernel) {
   if (m < 0 || k < 0 || n < 0 || g < 1) return 0;
-  return align_up(rd::int4_workspace_bytes(m, k, n, g, kernel), 256);
+  return align_up(rd::int4_workspace_bytes(m, k, n, g, g, kernel), 256);  // (a slice of the groups needs no more)
 }
 
 int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scales, const uint8_t* zeros,
@@ -1313,7 +1313,7 @@ int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scal
   if (m == 0 || n == 0) return RD_OK;
   if (!group_sizes || !y || (k > 0 && (!x || !scales))) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return fail(RD_ERR_WORKSPACE, "workspace misaligned");
-  const size_t needed = rd::int4_tiles_hold(dtype == RD_DTYPE_F16, scale_dtype == RD_DTYPE_F16) ? rd::int4_workspace_bytes(m, k, n, g_total, kernel) : 0;
+  const size_t needed = rd::int4_tiles_hold(dtype == RD_DTYPE_F16, scale_dtype == RD_DTYPE_F16) ? rd::int4_workspace_bytes(m, k, n, g_total, g_local, kernel) : 0;
   float* partials = workspace && needed > 0 && workspace_bytes >= needed ? static_cast<float*>(workspace) : nullptr;
   int32_t* counters = partials ? reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + rd::kInt4PartialBytes) : nullptr;
   const rd::Int4Problem p = {x, static_cast<const uint32_t*>(codes), scales, zeros, group_sizes, y, m, k, n, g_total, group_offset, g_local,

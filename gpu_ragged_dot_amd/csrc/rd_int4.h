@@ -42,7 +42,7 @@ constexpr size_t kInt4PartialBytes = (size_t)kInt4Slots * 256 * 256 * sizeof(flo
 // The tile kernel's weights are of the rows' type, and float16 does not have the range of bfloat16 scales.
 inline bool int4_tiles_hold(bool half, bool scale_half) { return !half || scale_half; }
 // Of the whole workspace, where the tiles hold the weights; 0: no launch of these sizes is cut.
-size_t int4_workspace_bytes(int m, int k, int n, int g, int kernel);
+size_t int4_workspace_bytes(int m, int k, int n, int g, int g_local, int kernel);
 
 __host__ __device__ inline int int4_runs(int k) { return (k + kInt4Run - 1) / kInt4Run; }
 __host__ __device__ inline int int4_strips(int n) { return (n + kInt4Strip - 1) / kInt4Strip; }

@@ -298,7 +298,8 @@ struct StreamGrid {
 StreamGrid stream_grid(const Int4Problem& p, int most) {
   StreamGrid s;
   s.rows = p.m <= 8 * p.g ? 16 : kInt4Rows;
-  const long long of_few = (long long)imin(p.g, p.m) * ((most + s.rows - 1) / s.rows), of_any = p.m / s.rows + imin(p.g, p.m);
+  const int groups = imin(p.g_local, p.m);
+  const long long of_few = (long long)groups * ((most + s.rows - 1) / s.rows), of_any = p.m / s.rows + groups;
   s.tiles = (int)(of_few < of_any ? of_few : of_any);
   s.col_tiles = (p.n + kInt4Cols - 1) / kInt4Cols;
   s.blocks = (long long)s.tiles * s.col_tiles + (p.m + kInt4Rows - 1) / kInt4Rows;
@@ -323,21 +324,22 @@ int stream(hipStream_t s, const Int4Problem& p, int most) {
 // kernel is long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
 constexpr int kInt4FewRows = 48;
 
-bool uses_tiles(int m, int k, int n, int g, int kernel) {
+// `held`: the groups that the weights hold, which is what either kernel multiplies, of the g that the m rows are spread over.
+bool uses_tiles(int m, int k, int n, int g, int held, int kernel) {
   if (m <= kInt4FewRows || k < 8 || k > (1 << 22) || kernel == RD_INT4_STREAM) return false;
   if (kernel == RD_INT4_TILES) return true;
   const double rows = (double)((m + g - 1) / g), cols64 = (n + 63) / 64, cols256 = (n + 255) / 256;
-  const double streaming = 6 + g * ceil(rows / 32) * cols64 / 512 * (1 + k * 0.004);
+  const double streaming = 6 + held * ceil(rows / 32) * cols64 / 512 * (1 + k * 0.004);
   if (streaming > 100) return true;
   if (rows <= kInt4FewRows) return false;
   const double last = rows - 256 * floor(rows / 256), height = last == 0 ? 0 : last <= 64 ? 1.1 : last <= 128 ? 1.3 : last <= 192 ? 1.65 : 2;
-  const double work = g * cols256 * (2 * floor(rows / 256) + height) / 256, least = rows >= 256 ? 2 : height;
+  const double work = held * cols256 * (2 * floor(rows / 256) + height) / 256, least = rows >= 256 ? 2 : height;
   return 12 + k / 64 * (work > least ? work : least) < streaming;
 }
 
 // Rows of the largest groups that the streaming kernel multiplies.
 int most_streamed(const Int4Problem& p) {
-  return int4_tiles_hold(p.half, p.scale_half) && uses_tiles(p.m, p.k, p.n, p.g, p.kernel) ? kInt4FewRows : p.m;
+  return int4_tiles_hold(p.half, p.scale_half) && uses_tiles(p.m, p.k, p.n, p.g, p.g_local, p.kernel) ? kInt4FewRows : p.m;
 }
 
 template <bool HALF, int BLOCK>
@@ -359,13 +361,13 @@ int launch_int4_pack(hipStream_t s, const uint8_t* q, uint32_t* codes, int g, in
   return (int)hipGetLastError();
 }
 
-size_t int4_workspace_bytes(int m, int k, int n, int g, int kernel) {
-  return uses_tiles(m, k, n, g, kernel) && n > 0 ? kInt4PartialBytes + kInt4Slots * sizeof(int32_t) : 0;
+size_t int4_workspace_bytes(int m, int k, int n, int g, int g_local, int kernel) {
+  return uses_tiles(m, k, n, g, g_local, kernel) && n > 0 ? kInt4PartialBytes + kInt4Slots * sizeof(int32_t) : 0;
 }
 
 // (The tile kernel's work-groups are fewer than rows / 256 and groups come to, times the columns.)
 bool int4_grid_fits(const Int4Problem& p) {
-  const long long tiles = (p.m / 256 + imin(p.g, p.m)) * (long long)((p.n + 255) / 256);
+  const long long tiles = (p.m / 256 + imin(p.g_local, p.m)) * (long long)((p.n + 255) / 256);
   return stream_grid(p, most_streamed(p)).blocks < (1ll << 31) / kInt4Threads && tiles < (1ll << 31) / kInt4Threads;
 }
 

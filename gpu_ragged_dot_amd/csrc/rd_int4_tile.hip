@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256, 1) void gmm_int4_tile_kernel(Int4Problem p, in
 template <bool HALF, int BLOCK>
 int launch_int4_tiles(hipStream_t s, const Int4Problem& p, int least) {
   const int col_tiles = (p.n + kTileCols - 1) / kTileCols;
-  const long long tiles = (p.m / kTileRows + imin(p.g, p.m / least)) * (long long)col_tiles;
+  const long long tiles = (p.m / kTileRows + imin(p.g_local, p.m / least)) * (long long)col_tiles;
   const int whole = (int)((tiles + 7) / 8 * 8);
   hipLaunchKernelGGL((gmm_int4_tile_kernel<HALF, BLOCK>), dim3((unsigned)(whole + (p.partials ? kInt4Slots : 0))), dim3(256), 0, s, p, least, col_tiles, whole);
   return (int)hipGetLastError();

@@ -281,7 +281,7 @@ int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, 
  * kernel: RD_INT4_AUTO, or the one that multiplies groups of any size whatever it costs: RD_INT4_STREAM, or RD_INT4_TILES, which
  * leaves groups of up to 48 rows to the other (k >= 8 and k <= 2^22; else, and for the types just named, the other does it all).
  * m < 2^25, k and n <= 2^24.  No gradients.
- * Workspace (optional): rd_gmm_int4_workspace_bytes() bytes, 256-byte aligned, for fp32 partial sums where tiles that do not fill
+ * Workspace (optional): rd_gmm_int4_workspace_bytes() bytes (g: the groups of group_sizes; enough for any slice of them), 256-byte aligned, for fp32 partial sums where tiles that do not fill
  * the device's last round are cut along k; with NULL or a smaller one none are (float16 rows with bfloat16 scales use none).  So the last bits of a row may follow from the other
  * groups' sizes, as in rd_gmm. */
 enum rd_int4_kernel { RD_INT4_AUTO = 0, RD_INT4_STREAM = 1, RD_INT4_TILES = 2 };
