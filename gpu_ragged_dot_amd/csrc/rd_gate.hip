@@ -291,7 +291,7 @@ __device__ __forceinline__ int choose_wide(const T* __restrict__ src, const floa
 }
 
 // PER: experts a lane has registers for; `chunk` (<= PER): experts it holds, chunk * lane and on.  VEC: in whole pieces of 16 bytes.
-// cluster_lanes: lanes that hold a cluster (1, 2, 4, 8 or 16).
+// (PER is such pieces then.)  cluster_lanes: lanes that hold a cluster (1, 2, 4, 8 or 16).
 template <class T, int PER, bool VEC>
 __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __restrict__ logits, const float* __restrict__ bias,
                                                                      int32_t* __restrict__ ids, float* __restrict__ weights, GateSpec p,
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
   const int e0 = at * chunk, own = imin(chunk, p.experts - e0);  // this lane's experts (own <= 0: none)
   constexpr int EPP = 16 / sizeof(T);
   float l[PER];
-  if constexpr (VEC && PER >= EPP) {
+  if constexpr (VEC) {
 #pragma unroll
     for (int i = 0; i < PER; i += EPP) {
       alignas(16) T v[EPP];
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
       const float norm = p.sigmoid ? 1.f : __builtin_amdgcn_rcpf(row_sum(total));
       if (bias) {
         float bs[PER];
-        if constexpr (VEC && PER >= 4) {
+        if constexpr (VEC) {
 #pragma unroll
           for (int i = 0; i < PER; i += 4) {
             f32x4_t v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -654,9 +654,13 @@ template <class T, int PER>
 int gate_rows_t(hipStream_t s, const void* logits, const float* bias, int32_t* ids, float* weights, const GateSpec& p, int chunk, int cluster_lanes) {
   const int rows = kGateThreads / kRowLanes;
   const dim3 grid((p.tokens + rows - 1) / rows);
-  const bool vec = chunk * sizeof(T) % 16 == 0 && (size_t)p.experts * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
-  if (vec) hipLaunchKernelGGL((moe_gate_rows_kernel<T, PER, true>), grid, dim3(kGateThreads), 0, s, (const T*)logits, bias, ids, weights, p, chunk, cluster_lanes);
-  else hipLaunchKernelGGL((moe_gate_rows_kernel<T, PER, false>), grid, dim3(kGateThreads), 0, s, (const T*)logits, bias, ids, weights, p, chunk, cluster_lanes);
+  if constexpr (PER * sizeof(T) >= 16) {
+    if (chunk * sizeof(T) % 16 == 0 && (size_t)p.experts * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0) {
+      hipLaunchKernelGGL((moe_gate_rows_kernel<T, PER, true>), grid, dim3(kGateThreads), 0, s, (const T*)logits, bias, ids, weights, p, chunk, cluster_lanes);
+      return (int)hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((moe_gate_rows_kernel<T, PER, false>), grid, dim3(kGateThreads), 0, s, (const T*)logits, bias, ids, weights, p, chunk, cluster_lanes);
   return (int)hipGetLastError();
 }
 
