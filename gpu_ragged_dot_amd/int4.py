@@ -59,12 +59,13 @@ def pack_int4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tenso
     return Int4Weights(_native.int4_pack(q, bool(trans_rhs)), laid_out(scales), laid_out(zeros), k, n, int(block))
 
 
-def ragged_dot_int4(x: torch.Tensor, weights: Int4Weights, group_sizes, *, group_offset=None) -> torch.Tensor:
+def ragged_dot_int4(x: torch.Tensor, weights: Int4Weights, group_sizes, *, group_offset=None, exact_weights: bool = False) -> torch.Tensor:
     """``(m, k) x (g, k, n) -> (m, n)`` on 4-bit weights; rows past ``sum(group_sizes)`` are zero.  ``x`` is bfloat16 or float16,
-    and so is the result, rounded once from fp32; groups of many rows multiply weights that are rounded to that type, too.
+    and so is the result, rounded once from fp32.  Where the sizes of the call make it cheaper, groups of more than 48 rows multiply
+    weights that are rounded to that type, too; with ``exact_weights`` none do, which takes up to twice as long for long prompts.
     ``group_offset`` as in ``gmm``: ``weights`` hold the groups from there on, the rows of the others are zero.  No gradient: an
     ``x`` that requires one raises ``NotImplementedError``."""
-    return _ragged_dot_int4(x, weights, group_sizes, group_offset)
+    return _ragged_dot_int4(x, weights, group_sizes, group_offset, _capi.RD_INT4_STREAM if exact_weights else _capi.RD_INT4_AUTO)
 
 
 def _ragged_dot_int4(x, weights, group_sizes, group_offset=None, kernel=_capi.RD_INT4_AUTO):
