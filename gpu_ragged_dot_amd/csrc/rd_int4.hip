@@ -320,8 +320,8 @@ int stream(hipStream_t s, const Int4Problem& p, int most) {
 // work-groups of 32 rows x 64 columns of the streaming kernel at 1 and 4 per 1024 indices, 256 tiles of the other at 1.1 .. 2.0 a slab
 // of 64 by their height.  bf16, blocks of 128, streaming | tiles: 32 groups of 64 x 7168 x 2048 168 | 135, 128 of 64 x 2048 x 768 85 |
 // 81, 8 of 64 x 4096 x 14336 106 | 138, 32 of 128 x 2048 x 768 35 | 47, 17 of 96 x 328 x 3080 (blocks of 64, zeros) 35 | 24, where
-// the rule is wrong.  Over 250 calls of random and of equal sizes it costs 0.7 % on the faster of the two.  Where the streaming
-// kernel is long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
+// the rule is wrong.  Over 216 calls of random and of equal sizes it costs 0.7 % on the faster of the two, 35 % at worst (8 of 64 x
+// 4096 x 14336) and more than 12 % in 8 of them.  Where the streaming kernel is long at work, groups of very different sizes pay for the other launch, a few us, whatever their mean.
 constexpr int kInt4FewRows = 48;
 
 // `held`: the groups that the weights hold, which is what either kernel multiplies, of the g that the m rows are spread over.

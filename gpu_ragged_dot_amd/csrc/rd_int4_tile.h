@@ -11,7 +11,8 @@
 //  * What a wave does beside matrix-core instructions is dealt out over the gaps between them, which leave seven issue slots each, by
 //    the slots that it takes (schedule() below): 400 slots a slab beside 64 instructions of eight, for BM 256.  What bounds the kernel
 //    is the power that the matrix cores draw, first, and these slots.  bf16 (float16), 8 groups of 2048 x 4096 x 14336, us: 1905
-//    (1955) with byte conversions, writes to LDS two lanes to a bank and an op to a gap whatever it takes; 1850 (1845) as it is.
+//    (1955) with byte conversions, writes to LDS two lanes to a bank and an op to a gap whatever it takes; 1850 (1845, and 0.4 % for what
+//    trim_b() clears) as it is.
 //  * The weight is rounded to the rows' type, once: scale (q - zero) itself is exact in fp32 (scale has at most 11 bits, the
 //    difference 9).  Kept exact, as in the streaming kernel, the sums of every block would have to be scaled apart - three vector
 //    instructions per accumulator and block of 128, more than the matrix-core instructions leave.

@@ -21,7 +21,9 @@ __device__ __forceinline__ void tile_of(const Int4Problem& p, const RowTile& til
 
 // One work-group runs on a compute unit at a time, so the launch proceeds in rounds of kInt4Slots tiles.  `tiles` of them in the
 // last round, which is not full: over how many work-groups each is cut along k.  us, as measured: a slab of 64 indices 2.0; what a
-// cut costs, 28, and 0.09 for every piece's 256 KB of partial sums through memory and back.
+// cut costs, 28, and 0.09 for every piece's 256 KB of partial sums through memory and back.  A launch uncut | as cut so: 16 tiles of
+// 2048 indices 58 | 45, of 4096 100 | 58, of 14336 310 | 87; 100 tiles 62 | 62, 105 | 90, 331 | 228; 128 tiles 63 | 63, 103 | 101, 338 |
+// 254; 288 tiles, of which 32 are in the last round, 128 | 117, 225 | 195, 710 | 538.
 __device__ __forceinline__ int split_parts(int tiles, int runs) {
   int best = 1;
   float least = 4.0f * runs;

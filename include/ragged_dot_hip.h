@@ -140,7 +140,8 @@ int rd_sched_map_len(int m, int g, int chunk_m);
  * Replaces the "gpu_gmm" pallas_call (gpu_ragged_dot.py:93-165, 217-226).
  *   A is [g, k, n] (trans_rhs = 0) or [g, n, k] (trans_rhs = 1, gpu_ragged_dot.py:139-144, :190).
  *   Rows of group i are [offset_i, offset_i + group_sizes[i]); rows >= sum(group_sizes) of y are set to zero
- *   (:155-165) -- also when every group is empty.  Groups that would run past m are clipped to m.
+ *   (:155-165) -- also when every group is empty.  Groups that would run past m are clipped to m; the sum of group_sizes
+ *   (here and wherever they are taken, but for rd_gmm_int4) is below 2^31.
  * Workspace: rd_gmm_workspace_bytes() bytes, 256-byte aligned; holds the scheduling map, 64 KiB for the order in which
  * the tile walk's blocks are dealt (long groups' among short groups') and, unless the plan says split_k = -1, fp32
  * partial sums (64 MiB for the 256 x 256 tiles, 4-16 MiB for the float32 ones a default plan names).  A smaller workspace that has room for the map is accepted: the call
@@ -275,15 +276,18 @@ int rd_moe_swiglu_grad(void* stream, const void* y, const void* dout, void* dy, 
  *   scales: [g_local, ceil(k / 128), n, 128 / block], scale_dtype RD_DTYPE_BF16 or RD_DTYPE_F16, below 2^116, 0 past k;
  *   zeros:  bytes of the same shape, or NULL: 8 throughout.
  * x and y are RD_DTYPE_BF16 or RD_DTYPE_F16.  group_sizes, the rows past their sum (zero), clipping at m, group_offset and g_local
- * are those of rd_gmm_sharded.  fp32 sums, one rounding of the result.  Groups of many rows are multiplied in tiles whose weights
- * are rounded once to the rows' type (float16: infinite past its range); with few rows, and for float16 rows with bfloat16 scales (whose range float16 has not), they
- * are exact.  An infinity in x makes its row NaN or infinite.
- * kernel: RD_INT4_AUTO, or the one that multiplies groups of any size whatever it costs: RD_INT4_STREAM, or RD_INT4_TILES, which
- * leaves groups of up to 48 rows to the other (k >= 8 and k <= 2^22; else, and for the types just named, the other does it all).
- * m < 2^25, k and n <= 2^24.  No gradients.
- * Workspace (optional): rd_gmm_int4_workspace_bytes() bytes (g: the groups of group_sizes; enough for any slice of them), 256-byte aligned, for fp32 partial sums where tiles that do not fill
- * the device's last round are cut along k; with NULL or a smaller one none are (float16 rows with bfloat16 scales use none).  So the last bits of a row may follow from the other
- * groups' sizes, as in rd_gmm. */
+ * are those of rd_gmm_sharded; sizes may sum up to anything.  fp32 sums, one rounding of the result.  Groups of many rows are
+ * multiplied in tiles whose weights are rounded once to the rows' type (float16: infinite past its range); with few rows, and for
+ * float16 rows with bfloat16 scales (whose range float16 has not), they are exact.  An infinity in x makes its row NaN or infinite.
+ * kernel: RD_INT4_AUTO, or the one that multiplies groups of any size whatever it costs: RD_INT4_STREAM, whose weights are exact, or
+ * RD_INT4_TILES, which leaves groups of up to 48 rows to the other (k >= 8 and k <= 2^22; else, and for the types just named, the
+ * other does it all).
+ * m < 2^25, k and n <= 2^24, and what a launch has of work-groups: the streaming kernel takes one for every 32 rows x 64 columns of
+ * the groups that it multiplies, at most 2^23 (RD_ERR_UNSUPPORTED beyond).  No gradients.
+ * Workspace (optional): rd_gmm_int4_workspace_bytes() bytes (g: the groups of group_sizes; enough for any slice of them), 256-byte
+ * aligned, for fp32 partial sums where tiles that do not fill the device's last round are cut along k; with NULL or a smaller one
+ * none are (float16 rows with bfloat16 scales use none).  So the last bits of a row may follow from the other groups' sizes, as in
+ * rd_gmm. */
 enum rd_int4_kernel { RD_INT4_AUTO = 0, RD_INT4_STREAM = 1, RD_INT4_TILES = 2 };
 size_t rd_int4_codes_bytes(int g, int k, int n);
 int rd_int4_pack(void* stream, const uint8_t* q, void* codes, int g, int k, int n, int trans_rhs);
