@@ -540,7 +540,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_kernel(const T* __
 }
 
 // With q_i = w_i dw_i and Q their sum over a row's choices:
-//   renormalised: dl_i = (q_i - w_i Q / scale) (1 - s_i for sigmoid), chosen ones only;
+//   renormalised: dl_i = (q_i - w_i / scale Q) (1 - s_i for sigmoid), chosen ones only;
 //   sigmoid: dl_i = q_i (1 - s_i);  softmax: dl_j = [j chosen] q_j - s_j Q for every expert.
 template <class T, int PER>
 __global__ __launch_bounds__(kGateThreads) void moe_gate_grad_kernel(const T* __restrict__ logits, const int32_t* __restrict__ ids,
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_grad_kernel(const T* __
   const float q = id >= 0 ? w * dweights[(size_t)row * p.top_k + lane] : 0.f;
   const float Q = wave_sum(q);
   float g = q;
-  if (p.renormalize) g = q - w * (Q / p.scale);
+  if (p.renormalize) g = q - w / p.scale * Q;  // (0 where one choice has it all)
   if (p.sigmoid && id >= 0) g /= 1.f + expf(to_f32<T>(src[id]));
   float d[PER];
 #pragma unroll
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(kGateThreads) void moe_gate_rows_grad_kernel(const 
   const float Q = row_sum(q);
   const T* src = logits + (size_t)row * p.experts;
   float g = q;
-  if (p.renormalize) g = q - w * (Q / p.scale);
+  if (p.renormalize) g = q - w / p.scale * Q;  // (0 where one choice has it all)
   if (p.sigmoid && id >= 0) g /= 1.f + expf(to_f32<T>(src[id]));
   if (!p.sigmoid && !p.renormalize) {
     float top = -INFINITY, sum = 0.f;
