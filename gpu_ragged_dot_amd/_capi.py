@@ -188,6 +188,18 @@ def _load() -> ctypes.CDLL:
     lib.rd_gmm_int4_workspace_bytes.restype = sz
     lib.rd_gmm_int4.argtypes = [vp, vp, vp, vp, vp, ip, vp, i, i, i, i, i, i, i, i, i, i, vp, sz]
     lib.rd_gmm_int4.restype = i
+    lib.rd_float8_rows.argtypes = [vp, vp, vp, vp, i, i, i, i]
+    lib.rd_float8_rows.restype = i
+    lib.rd_float8_weights.argtypes = [vp, vp, vp, vp, i, i, i, i, i]
+    lib.rd_float8_weights.restype = i
+    lib.rd_float8_values.argtypes = [vp, vp, vp, vp, i, i, i, i, i]
+    lib.rd_float8_values.restype = i
+    lib.rd_moe_dispatch_float8.argtypes = [vp, vp, ip, ip, vp, vp, i, i, i, i, i]
+    lib.rd_moe_dispatch_float8.restype = i
+    lib.rd_moe_swiglu_float8.argtypes = [vp, vp, vp, vp, i, i, i, i]
+    lib.rd_moe_swiglu_float8.restype = i
+    lib.rd_gmm_float8.argtypes = [vp, vp, vp, vp, vp, ip, vp, i, i, i, i, i, i, i, i]
+    lib.rd_gmm_float8.restype = i
     return lib
 
 

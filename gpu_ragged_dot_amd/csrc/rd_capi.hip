@@ -9,6 +9,7 @@
 #include <cstring>
 
 #include "rd_decode.h"
+#include "rd_float8.h"
 #include "rd_int4.h"
 #include "rd_moe.h"
 #include "rd_kernels.h"
@@ -1321,6 +1322,93 @@ int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scal
   if (!rd::int4_grid_fits(p)) return fail(RD_ERR_UNSUPPORTED, "m=%d rows of n=%d in %d groups are more tiles than a launch has", m, n, g_total);
   rc = rd::launch_gmm_int4((hipStream_t)stream, p);
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "gmm_int4 launch");
+}
+
+// Sizes and pointers of numbers held as float8: `rows` rows of `cols` of them, in work-groups of 16 blocks of a row.
+static int check_float8(const void* codes, const void* scales, long long rows, int cols, int dtype) {
+  if (rows < 0 || cols < 0 || cols > rd::kF8MaxDim) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape: %lld rows of %d", rows, cols);
+  const int rc = check_moe(0, 1, 0, dtype);
+  if (rc != RD_OK) return rc;
+  if (rows * rd::float8_scale_pitch(cols) >= (1ll << 28) || rows * ((cols + 7) / 8) >= (1ll << 32))
+    return fail(RD_ERR_UNSUPPORTED, "%lld rows of %d are more blocks than a launch has work-groups for", rows, cols);
+  if (rows > 0 && cols > 0 && (!codes || !scales || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) != 0))
+    return fail(RD_ERR_INVALID_ARGUMENT, "the codes or scales are null or not 16-byte aligned");
+  return RD_OK;
+}
+
+int rd_float8_rows(void* stream, const void* x, void* codes, float* scales, int rows, int k, int pow2, int dtype) {
+  int rc = check_float8(codes, scales, rows, k, dtype);
+  if (rc != RD_OK || rows == 0 || k == 0) return rc;
+  if (!x) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  rc = rd::launch_float8_rows((hipStream_t)stream, x, codes, scales, rows, k, false, pow2 != 0, moe_elem(dtype));
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "float8_rows launch");
+}
+
+int rd_moe_swiglu_float8(void* stream, const void* y, void* codes, float* scales, int rows, int f, int pow2, int dtype) {
+  int rc = check_float8(codes, scales, rows, f, dtype);
+  if (rc != RD_OK || rows == 0 || f == 0) return rc;
+  if (!y) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  rc = rd::launch_float8_rows((hipStream_t)stream, y, codes, scales, rows, f, true, pow2 != 0, moe_elem(dtype));
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "moe_swiglu_float8 launch");
+}
+
+int rd_moe_dispatch_float8(void* stream, const void* h, const int32_t* row_of_slot, const int32_t* slot_of_row, void* codes,
+                           float* scales, int tokens, int top_k, int d, int pow2, int dtype) {
+  int rc = check_moe(tokens, top_k, d, dtype);
+  if (rc != RD_OK) return rc;
+  rc = check_float8(codes, scales, (long long)tokens * top_k, d, dtype);
+  if (rc != RD_OK || tokens == 0 || d == 0) return rc;
+  if (!h || !row_of_slot || !slot_of_row) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  rc = rd::launch_float8_dispatch((hipStream_t)stream, h, row_of_slot, slot_of_row, codes, scales, tokens, top_k, d, pow2 != 0, moe_elem(dtype));
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "moe_dispatch_float8 launch");
+}
+
+static int check_float8_weights(const void* codes, const void* scales, int g, int a, int b) {
+  if (g < 1 || a < 0 || b < 0 || a > rd::kF8MaxDim || b > rd::kF8MaxDim) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape g=%d, %d x %d", g, a, b);
+  if ((double)g * rd::float8_blocks(a) * rd::float8_blocks(b) >= (double)(1 << 23)) return fail(RD_ERR_UNSUPPORTED, "%d matrices of %d x %d are more blocks than a launch has work-groups", g, a, b);
+  if (a > 0 && b > 0 && (!codes || !scales || (reinterpret_cast<uintptr_t>(codes) & 15) != 0))
+    return fail(RD_ERR_INVALID_ARGUMENT, "the codes or scales are null, or the codes not 16-byte aligned");
+  return RD_OK;
+}
+
+int rd_float8_weights(void* stream, const void* A, void* codes, float* scales, int g, int a, int b, int pow2, int dtype) {
+  int rc = check_float8_weights(codes, scales, g, a, b);
+  if (rc == RD_OK) rc = check_moe(0, 1, 0, dtype);
+  if (rc != RD_OK || a == 0 || b == 0) return rc;
+  if (!A) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  rc = rd::launch_float8_weights((hipStream_t)stream, A, codes, scales, g, a, b, pow2 != 0, moe_elem(dtype));
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "float8_weights launch");
+}
+
+int rd_float8_values(void* stream, const void* codes, const float* scales, void* out, int g, int a, int b, int height, int dtype) {
+  if ((height != 1 || g != 1) && height != rd::kF8Block) return fail(RD_ERR_INVALID_ARGUMENT, "height=%d is neither 1 (of one matrix) nor %d", height, rd::kF8Block);
+  int rc = height == 1 ? check_float8(codes, scales, a, b, dtype) : check_float8_weights(codes, scales, g, a, b);
+  if (rc == RD_OK) rc = check_moe(0, 1, 0, dtype);
+  if (rc != RD_OK || a == 0 || b == 0) return rc;
+  if (!out) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if ((long long)g * a * ((b + 7) / 8) >= (1ll << 32)) return fail(RD_ERR_UNSUPPORTED, "%d matrices of %d x %d are more than a launch has work-groups for", g, a, b);
+  rc = rd::launch_float8_values((hipStream_t)stream, codes, scales, out, g, a, b, height, moe_elem(dtype));
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "float8_values launch");
+}
+
+int rd_gmm_float8(void* stream, const void* x, const float* x_scales, const void* A, const float* A_scales, const int32_t* group_sizes,
+                  void* y, int m, int k, int n, int g_total, int group_offset, int g_local, int trans_rhs, int dtype) {
+  int rc = check_float8_weights(A, A_scales, g_local, k, n);
+  if (rc == RD_OK) rc = check_moe(0, 1, 0, dtype);
+  if (rc != RD_OK) return rc;
+  if (m < 0 || m > rd::kF8MaxRows) return fail(RD_ERR_INVALID_ARGUMENT, "m=%d outside 0..%d", m, rd::kF8MaxRows);
+  if (g_total < 1 || group_offset < 0 || group_offset > g_total - g_local)
+    return fail(RD_ERR_INVALID_ARGUMENT, "groups [%d, %d + %d) are not within the %d of group_sizes", group_offset, group_offset, g_local, g_total);
+  if (!trans_rhs && (long long)rd::float8_pitch(k) * rd::float8_pitch(n) >= (1ll << 31))
+    return fail(RD_ERR_UNSUPPORTED, "a matrix of %d x %d codes is beyond 2 GiB: store it [n, k]", k, n);
+  if (m == 0 || n == 0) return RD_OK;
+  if (!group_sizes || !y || (k > 0 && (!x || !x_scales))) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(x_scales)) & 15) != 0) return fail(RD_ERR_INVALID_ARGUMENT, "the rows' codes or scales are not 16-byte aligned");
+  const rd::F8Problem p = {static_cast<const uint8_t*>(x), x_scales, static_cast<const uint8_t*>(A), A_scales, group_sizes, y, m, k, n, g_total,
+                           group_offset, g_local, trans_rhs != 0, moe_elem(dtype)};
+  if (!rd::float8_grid_fits(p)) return fail(RD_ERR_UNSUPPORTED, "m=%d rows of n=%d in %d groups are more tiles than a launch has", m, n, g_total);
+  rc = rd::launch_gmm_float8((hipStream_t)stream, p);
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "gmm_float8 launch");
 }
 
 }  // extern "C"

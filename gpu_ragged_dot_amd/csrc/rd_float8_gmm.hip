@@ -1,0 +1,120 @@
+// The ragged product on float8 rows and weights with a scale for each block of 128: which work-group computes which tile.
+#include "rd_elem.h"
+#include "rd_float8_tile.h"
+#include "rd_int4_rows.h"
+
+namespace rd {
+
+namespace {
+
+constexpr int kF8GmmThreads = 256;
+constexpr int kF8ZeroRows = 64;  // rows that a work-group looks after which multiplies nothing
+constexpr int kF8Band = 4;       // row tiles of a band of the walk
+
+constexpr int larger(int a, int b) { return a > b ? a : b; }
+
+// Rows of a tile and columns; a tile of fewer rows runs on the least of the heights that holds it.
+template <bool B_KMAJOR>
+struct F8Tall {
+  static constexpr int BM = 256, BN = 256;
+  typedef F8TileCfg<256, 256, 2, 2, 2, B_KMAJOR> C256;
+  typedef F8TileCfg<128, 256, 2, 2, 3, B_KMAJOR> C128;
+  typedef F8TileCfg<64, 256, 1, 4, 3, B_KMAJOR> C64;
+  static constexpr int LDS_BYTES = larger(C256::LDS_BYTES, larger(C128::LDS_BYTES, C64::LDS_BYTES)), GROUPS = 1;
+  static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
+    if (t.rows <= 64) float8_tile<C64>(t, y, ldy, elem, smem);
+    else if (t.rows <= 128) float8_tile<C128>(t, y, ldy, elem, smem);
+    else float8_tile<C256>(t, y, ldy, elem, smem);
+  }
+};
+template <bool B_KMAJOR>
+struct F8Few {
+  static constexpr int BM = 64, BN = 128;
+  typedef F8TileCfg<64, 128, 1, 4, 3, B_KMAJOR> C64;
+  typedef F8TileCfg<32, 128, 1, 4, 3, B_KMAJOR> C32;
+  static constexpr int LDS_BYTES = larger(C64::LDS_BYTES, C32::LDS_BYTES), GROUPS = 2;
+  static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
+    if (t.rows <= 32) float8_tile<C32>(t, y, ldy, elem, smem);
+    else float8_tile<C64>(t, y, ldy, elem, smem);
+  }
+};
+
+// Work-groups [0, whole): a tile each; those behind them: rows, of which they zero what is no row of a group that the weights hold.
+template <class S, bool B_KMAJOR>
+__global__ __launch_bounds__(kF8GmmThreads, S::GROUPS) void gmm_float8_kernel(F8Problem p, int col_tiles, int whole) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int size = p.elem == 1 ? 4 : 2;
+  if ((int)blockIdx.x >= whole) {
+    int first, end;
+    held_rows(p, &first, &end);
+    const int r0 = ((int)blockIdx.x - whole) * kF8ZeroRows;
+    for (int r = r0; r < imin(r0 + kF8ZeroRows, p.m); ++r)
+      if (r < first || r >= end)
+        for (int c = threadIdx.x; c < p.n; c += kF8GmmThreads) {
+          if (p.elem == 1) static_cast<float*>(p.y)[(size_t)r * p.n + c] = 0.f;
+          else static_cast<uint16_t*>(p.y)[(size_t)r * p.n + c] = 0;
+        }
+    return;
+  }
+  const int positions = count_row_tiles<S::BM>(p, 1, p.m) * col_tiles;
+  if ((int)(blockIdx.x >> 3) >= (positions + 7) / 8) return;  // (the launch holds as many work-groups as there may be tiles)
+  const int at = xcd_contiguous_id(blockIdx.x, positions);
+  if (at < 0) return;
+  int column = 0;
+  const RowTile tile = find_in_walk<S::BM, kF8Band>(p, 1, p.m, col_tiles, at, &column);
+  const int c0 = column * S::BN, kb = float8_blocks(p.k), nb = float8_blocks(p.n);
+  const size_t e = tile.group - p.g_first;
+  F8Tile t;
+  t.lda = kb * kF8Block;
+  t.ldb = B_KMAJOR ? t.lda : nb * kF8Block;
+  t.ldas = float8_scale_pitch(p.k);
+  t.a = p.x + (size_t)tile.first * t.lda;
+  t.a_scales = p.x_scales + (size_t)tile.first * t.ldas;
+  t.b = p.w + e * kb * nb * (kF8Block * kF8Block) + (size_t)c0 * (B_KMAJOR ? t.lda : 1);
+  t.b_block = B_KMAJOR ? 1 : nb;
+  t.b_column = B_KMAJOR ? kb : 1;
+  t.b_scales = p.w_scales + e * kb * nb + (size_t)(c0 / kF8Block) * t.b_column;
+  t.rows = tile.rows;
+  t.cols = imin(S::BN, p.n - c0);
+  t.blocks = kb;
+  S::run(t, static_cast<char*>(p.y) + ((size_t)tile.first * p.n + c0) * size, p.n, p.elem, smem);
+}
+
+// A mean of at most 64 rows to a group: tiles of 64 rows, two work-groups to a compute unit.
+bool few_rows(const F8Problem& p) { return p.m <= 64ll * p.g; }
+
+struct F8Grid {
+  int col_tiles;
+  long long whole, all;
+};
+F8Grid grid_of(const F8Problem& p) {
+  const int bm = few_rows(p) ? 64 : 256, bn = few_rows(p) ? 128 : 256;
+  F8Grid g;
+  g.col_tiles = (p.n + bn - 1) / bn;
+  g.whole = ((p.m / bm + imin(p.g_local, p.m)) * (long long)g.col_tiles + 7) / 8 * 8;
+  g.all = g.whole + (p.m + kF8ZeroRows - 1) / kF8ZeroRows;
+  return g;
+}
+
+template <template <bool> class S, bool B_KMAJOR>
+int launch_t(hipStream_t s, const F8Problem& p) {
+  auto kern = gmm_float8_kernel<S<B_KMAJOR>, B_KMAJOR>;
+  if (S<B_KMAJOR>::LDS_BYTES > 64 * 1024) {
+    const int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, S<B_KMAJOR>::LDS_BYTES);
+    if (rc != hipSuccess) return rc;
+  }
+  const F8Grid g = grid_of(p);
+  hipLaunchKernelGGL(kern, dim3((unsigned)g.all), dim3(kF8GmmThreads), S<B_KMAJOR>::LDS_BYTES, s, p, g.col_tiles, (int)g.whole);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+bool float8_grid_fits(const F8Problem& p) { return grid_of(p).all < (1ll << 31) / kF8GmmThreads; }
+
+int launch_gmm_float8(hipStream_t s, const F8Problem& p) {
+  if (few_rows(p)) return p.trans_rhs ? launch_t<F8Few, true>(s, p) : launch_t<F8Few, false>(s, p);
+  return p.trans_rhs ? launch_t<F8Tall, true>(s, p) : launch_t<F8Tall, false>(s, p);
+}
+
+}  // namespace rd

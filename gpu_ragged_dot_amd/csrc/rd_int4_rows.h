@@ -1,4 +1,5 @@
-// Which rows a work-group of a product on 4-bit weights computes, worked out by each wave from group_sizes.
+// Which rows a work-group of a product on 4-bit or float8 weights computes, worked out by each wave from group_sizes.  P: a problem
+// with group_sizes, g, m and the groups [g_first, g_first + g_local) that the weights hold.
 #pragma once
 #include "rd_int4.h"
 #include "rd_lookup.h"
@@ -38,8 +39,8 @@ struct RowTile {
 };
 
 // Tile t of BM rows of the groups that the weights hold, in order, counting those of at least `least` and at most `most` rows.
-template <int BM>
-__device__ __forceinline__ RowTile find_row_tile(const Int4Problem& p, int least, int most, int t) {
+template <int BM, class P>
+__device__ __forceinline__ RowTile find_row_tile(const P& p, int least, int most, int t) {
   RowTile found = {0, 0, 0};
   int tiles_before = 0;
   const int lane = threadIdx.x & 63;
@@ -62,7 +63,8 @@ __device__ __forceinline__ RowTile find_row_tile(const Int4Problem& p, int least
 }
 
 // The rows of the groups that the weights hold: [first, second); all others are zero.
-__device__ __forceinline__ void held_rows(const Int4Problem& p, int* first_row, int* end_row) {
+template <class P>
+__device__ __forceinline__ void held_rows(const P& p, int* first_row, int* end_row) {
   int a = p.g_first == 0 ? 0 : -1, b = -1;
   scan_groups(p.group_sizes, p.g, p.m, [&](int base, int first, int end) {
     const int la = p.g_first - base, lb = p.g_first + p.g_local - 1 - base;
@@ -74,8 +76,8 @@ __device__ __forceinline__ void held_rows(const Int4Problem& p, int* first_row, 
 }
 
 // Row tiles in all, counted as find_row_tile() counts them.
-template <int BM>
-__device__ __forceinline__ int count_row_tiles(const Int4Problem& p, int least, int most) {
+template <int BM, class P>
+__device__ __forceinline__ int count_row_tiles(const P& p, int least, int most) {
   int tiles = 0;
   const int lane = threadIdx.x & 63;
   scan_groups(p.group_sizes, p.g, p.m, [&](int base, int first, int end) {
@@ -89,8 +91,8 @@ __device__ __forceinline__ int count_row_tiles(const Int4Problem& p, int least, 
 
 // Position `at` of a walk over all row tiles times `columns` column tiles: group after group, in a group bands of BAND row tiles,
 // in a band column after column.  Returns the row tile and its column.
-template <int BM, int BAND>
-__device__ __forceinline__ RowTile find_in_walk(const Int4Problem& p, int least, int most, int columns, int at, int* column) {
+template <int BM, int BAND, class P>
+__device__ __forceinline__ RowTile find_in_walk(const P& p, int least, int most, int columns, int at, int* column) {
   RowTile found = {0, 0, 0};
   int tiles_before = 0;
   const int lane = threadIdx.x & 63;

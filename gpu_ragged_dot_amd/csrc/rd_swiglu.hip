@@ -13,16 +13,6 @@ namespace {
 
 constexpr int kSwigluThreads = 256;
 
-// sig(g) and sig(-g), neither by a difference from one, nor of an exponential that overflows.  16-bit results: exponential and
-// reciprocal of the hardware, good to 2 units of 2^-23 and the rounding of g log2(e).
-template <class T>
-__device__ __forceinline__ void sigmoids(float g, float* of, float* of_minus) {
-  const float t = sizeof(T) == 2 ? __expf(-fabsf(g)) : expf(-fabsf(g));
-  const float r = sizeof(T) == 2 ? __builtin_amdgcn_rcpf(1.f + t) : 1.f / (1.f + t);
-  *of = g >= 0.f ? r : t * r;
-  *of_minus = g >= 0.f ? t * r : r;
-}
-
 template <class T>
 __device__ __forceinline__ float swiglu_of(float g, float u) {
   float a, b;

@@ -613,6 +613,214 @@ Tensor gmm_int4(const Tensor& x_, const Tensor& codes, const Tensor& scales, con
   return y;
 }
 
+// ---- numbers held as float8, and products on them ----------------------------------------------------------------------
+int64_t blocks_of(int64_t k) { return (k + 127) / 128; }
+int64_t padded(int64_t k) { return blocks_of(k) * 128; }
+int64_t scale_pitch(int64_t k) { return (blocks_of(k) + 3) / 4 * 4; }  // of a row's scales
+
+struct Held {  // codes and scales
+  Tensor codes, scales;
+};
+Held held_rows(int64_t rows, int64_t k, const at::Device& dev) {
+  return {empty_on({rows, padded(k)}, at::kFloat8_e4m3fn, dev), empty_on({rows, scale_pitch(k)}, at::kFloat, dev)};
+}
+std::tuple<Tensor, Tensor> both(const Held& h) { return {h.codes, h.scales}; }
+
+// Numbers that a gradient is asked for are refused: what they are held as has none.
+void no_gradient(const Tensor& t) {
+  expect_no_tangent(t);
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad(t, t), "numbers held as float8 have no gradient: call this on detached tensors or under torch.no_grad(), or ragged_dot_float8 on the rows themselves");
+}
+
+Held quantize_rows_of(const Tensor& x_, bool pow2) {
+  if (x_.dim() != 2) throw py::value_error("x must be [rows, k]");
+  expect_int({x_.size(0), x_.size(1)});
+  const int code = rows_code(x_);
+  check_devices(x_, x_);
+  const Tensor x = x_.contiguous();
+  const c10::DeviceGuard guard(x.device());
+  const Held h = held_rows(x.size(0), x.size(1), x.device());
+  check(rd_float8_rows(stream_of(x.device()), x.const_data_ptr(), h.codes.mutable_data_ptr(), h.scales.mutable_data_ptr<float>(), (int)x.size(0),
+                       (int)x.size(1), pow2, code));
+  return h;
+}
+std::tuple<Tensor, Tensor> float8_rows(const Tensor& x, bool pow2) {
+  no_gradient(x);
+  return both(quantize_rows_of(x, pow2));
+}
+
+Held quantize_weights_of(const Tensor& A_, bool pow2) {
+  if (A_.dim() != 3) throw py::value_error("A must be [g, k, n] or [g, n, k]");
+  expect_int({A_.size(0), A_.size(1), A_.size(2)});
+  const int code = rows_code(A_);
+  check_devices(A_, A_);
+  const Tensor A = A_.contiguous();
+  const c10::DeviceGuard guard(A.device());
+  const int64_t g = A.size(0), a = A.size(1), b = A.size(2);
+  const Held h{empty_on({g, padded(a), padded(b)}, at::kFloat8_e4m3fn, A.device()), empty_on({g, blocks_of(a), blocks_of(b)}, at::kFloat, A.device())};
+  check(rd_float8_weights(stream_of(A.device()), A.const_data_ptr(), h.codes.mutable_data_ptr(), h.scales.mutable_data_ptr<float>(), (int)g, (int)a,
+                          (int)b, pow2, code));
+  return h;
+}
+std::tuple<Tensor, Tensor> float8_weights(const Tensor& A, bool pow2) {
+  no_gradient(A);
+  return both(quantize_weights_of(A, pow2));
+}
+
+// What a kernel takes codes and scales to be.
+void check_held_rows(const Held& h, int64_t k) {
+  expect(h.codes.dim() == 2 && h.codes.scalar_type() == at::kFloat8_e4m3fn && h.codes.is_contiguous() && h.codes.size(1) == padded(k) &&
+         h.scales.dim() == 2 && h.scales.scalar_type() == at::kFloat && h.scales.is_contiguous() && h.scales.size(0) == h.codes.size(0) &&
+         h.scales.size(1) == scale_pitch(k), "the rows' codes and scales are not what quantize_rows returns");
+  check_devices(h.codes, h.scales);
+}
+void check_held_weights(const Held& h, int64_t a, int64_t b) {
+  expect(h.codes.dim() == 3 && h.codes.scalar_type() == at::kFloat8_e4m3fn && h.codes.is_contiguous() && h.codes.size(1) == padded(a) &&
+         h.codes.size(2) == padded(b) && h.scales.dim() == 3 && h.scales.scalar_type() == at::kFloat && h.scales.is_contiguous() &&
+         h.scales.size(0) == h.codes.size(0) && h.scales.size(1) == blocks_of(a) && h.scales.size(2) == blocks_of(b),
+         "the weights' codes and scales are not what quantize_weights or pack_float8 returns");
+  check_devices(h.codes, h.scales);
+}
+
+// a = 0: rows of b numbers; else matrices of a x b
+Tensor float8_values(const Tensor& codes, const Tensor& scales, int64_t a, int64_t b, at::ScalarType type) {
+  const Held h{codes, scales};
+  const bool rows = codes.dim() == 2;
+  if (rows) check_held_rows(h, b);
+  else check_held_weights(h, a, b);
+  const c10::DeviceGuard guard(codes.device());
+  Tensor out = rows ? empty_on({codes.size(0), b}, type, codes.device()) : empty_on({codes.size(0), a, b}, type, codes.device());
+  const int code = rows_code(out);
+  expect_int({codes.size(0)});
+  if (out.numel() > 0)
+    check(rd_float8_values(stream_of(codes.device()), codes.const_data_ptr(), scales.const_data_ptr<float>(), out.mutable_data_ptr(),
+                           rows ? 1 : (int)codes.size(0), (int)(rows ? codes.size(0) : a), (int)b, rows ? 1 : 128, code));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> moe_dispatch_float8(const Tensor& h_, const Tensor& row_of_slot, const Tensor& slot_of_row, int64_t tokens, int64_t top_k, bool pow2) {
+  const Routing r{row_of_slot, slot_of_row, tokens, top_k};
+  no_gradient(h_);
+  if (h_.dim() != 2 || h_.size(0) != tokens) throw py::value_error("h must be [" + std::to_string(tokens) + ", d]");
+  expect_int({tokens, top_k, h_.size(1)});
+  check_routing(h_, r, Tensor());
+  const int code = rows_code(h_);
+  const Tensor h = h_.contiguous();
+  const c10::DeviceGuard guard(h.device());
+  const Held x = held_rows(tokens * top_k, h.size(1), h.device());
+  check(rd_moe_dispatch_float8(stream_of(h.device()), h.const_data_ptr(), row_of_slot.const_data_ptr<int32_t>(), slot_of_row.const_data_ptr<int32_t>(),
+                               x.codes.mutable_data_ptr(), x.scales.mutable_data_ptr<float>(), (int)tokens, (int)top_k, (int)h.size(1), pow2, code));
+  return both(x);
+}
+
+std::tuple<Tensor, Tensor> moe_swiglu_float8(const Tensor& y_, bool pow2) {
+  no_gradient(y_);
+  if (y_.dim() != 2 || y_.size(1) % 2 != 0) throw py::value_error("y must be [rows, 2 f], the halves gate and up");
+  expect_int({y_.size(0), y_.size(1)});
+  const int code = rows_code(y_);
+  check_devices(y_, y_);
+  const Tensor y = y_.contiguous();
+  const c10::DeviceGuard guard(y.device());
+  const Held h = held_rows(y.size(0), y.size(1) / 2, y.device());
+  check(rd_moe_swiglu_float8(stream_of(y.device()), y.const_data_ptr(), h.codes.mutable_data_ptr(), h.scales.mutable_data_ptr<float>(), (int)y.size(0),
+                             (int)(y.size(1) / 2), pow2, code));
+  return both(h);
+}
+
+Tensor gmm_held(const Held& x, const Held& A, const Tensor& gs_, int64_t k, int64_t n, bool trans, int64_t g_first, at::ScalarType type) {
+  check_held_rows(x, k);
+  check_held_weights(A, trans ? n : k, trans ? k : n);
+  expect(gs_.dim() == 1, "group_sizes must have one dimension");
+  const int64_t g_local = A.codes.size(0), g = gs_.numel(), m = x.codes.size(0);
+  expect(g_first < 0 ? g_local == g : g_first + g_local <= g, "the weights do not hold the groups that group_sizes describes");
+  expect_int({m, k, n, g});
+  check_devices(x.codes, A.codes);
+  const at::Device dev = x.codes.device();
+  const Tensor gs = sizes_on(gs_, dev);
+  const c10::DeviceGuard guard(dev);
+  Tensor y = empty_on({m, n}, type, dev);
+  check(rd_gmm_float8(stream_of(dev), x.codes.const_data_ptr(), x.scales.const_data_ptr<float>(), A.codes.const_data_ptr(), A.scales.const_data_ptr<float>(),
+                      gs.const_data_ptr<int32_t>(), y.mutable_data_ptr(), (int)m, (int)k, (int)n, (int)g, (int)(g_first < 0 ? 0 : g_first), (int)g_local,
+                      trans, rows_code(y)));
+  return y;
+}
+
+// A product's operands: numbers, or (codes defined) numbers held as float8 already.
+struct Float8Call : torch::CustomClassHolder {
+  bool trans = false, pow2 = false;
+  int64_t g_first = -1, k = 0, n = 0;
+  at::ScalarType type = at::kBFloat16;
+  Held x, A;
+};
+Tensor float8_product(const Float8Call& c, const Tensor& x, const Tensor& gs, const Held& A) {
+  return gmm_held(x.defined() ? quantize_rows_of(x, c.pow2) : c.x, A, gs, c.k, c.n, c.trans, c.g_first, c.type);
+}
+
+// Straight through: the gradient of the product of what the operands are held as, taken for that of the operands themselves.  dx is a
+// product of the same kind, on the cotangent's rows in 8 bits and the weights that the forward product used; dA the 16- or 32-bit product.
+struct Float8Node : torch::autograd::Function<Float8Node> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& A, const Tensor& gs, const c10::intrusive_ptr<Float8Call>& c) {
+    const Tensor sizes = sizes_on(gs, x.device());
+    const Held w = A ? quantize_weights_of(*A, c->pow2) : c->A;
+    ctx->save_for_backward({x, w.codes, w.scales, sizes});
+    ctx->saved_data["call"] = c10::IValue::make_capsule(c);
+    return float8_product(*c, x, sizes, w);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return in_backward(grads, [&]() -> variable_list {
+      const auto saved = ctx->get_saved_variables();
+      const auto call = ctx->saved_data["call"].toCapsule();
+      const Float8Call& c = *static_cast<Float8Call*>(call.get());
+      const Tensor &x = saved[0], &gs = saved[3];
+      check_devices(x, grads[0]);
+      const Tensor dy = grads[0].contiguous();
+      Tensor dx, dA;
+      if (ctx->needs_input_grad(0))
+        dx = gmm_held(quantize_rows_of(dy, c.pow2), {saved[1], saved[2]}, gs, c.n, c.k, !c.trans, c.g_first, x.scalar_type());
+      if (!c.A.codes.defined() && ctx->needs_input_grad(1)) {  // (given as numbers, not as codes)
+        Call t;
+        t.code = rows_code(x); t.g_first = c.g_first;
+        const Tensor d = dy.to(x.scalar_type());
+        dA = c.trans ? tgmm_forward(d, x, gs, t, 2, saved[1].size(0)) : tgmm_forward(x, d, gs, t, 2, saved[1].size(0));
+      }
+      return {dx, dA, Tensor(), Tensor()};
+    });
+  }
+};
+
+// x, A: the operands' numbers, or None where codes and scales are given (a matrix of the weights is [k, n], with trans [n, k]).
+Tensor gmm_float8(const std::optional<Tensor>& x_, const std::optional<Tensor>& x_codes, const std::optional<Tensor>& x_scales, int64_t k,
+                  const std::optional<Tensor>& A_, const std::optional<Tensor>& A_codes, const std::optional<Tensor>& A_scales, int64_t a, int64_t b,
+                  const Tensor& gs, bool trans, int64_t g_first, at::ScalarType type, bool pow2) {
+  const Tensor x = x_.value_or(Tensor()), A = A_.value_or(Tensor());
+  expect_no_tangent(x, A);
+  auto c = c10::make_intrusive<Float8Call>();
+  c->trans = trans; c->pow2 = pow2; c->g_first = g_first; c->type = type;
+  if (x.defined()) {
+    expect(x.dim() == 2, "x must be [m, k]");
+    rows_code(x);
+  } else {
+    c->x = {*x_codes, *x_scales};
+  }
+  if (A.defined()) {
+    expect(A.dim() == 3, "A must be [g, k, n], or [g, n, k] with trans_rhs");
+    rows_code(A);
+    if (x.defined()) same_type(x, A);
+    a = A.size(1); b = A.size(2);
+  } else {
+    c->A = {*A_codes, *A_scales};
+  }
+  c->k = x.defined() ? x.size(1) : k;
+  c->n = trans ? a : b;
+  expect(c->k == (trans ? b : a), "contraction mismatch between x and A");
+  const bool wants_x = x.defined() && wants_grad(x, x), wants_A = A.defined() && wants_grad(A, A);
+  TORCH_CHECK_NOT_IMPLEMENTED(x.defined() || !wants_A, "the gradient of the weights needs the rows themselves, not rows held as float8");
+  const Tensor& on = x.defined() ? x : c->x.codes;
+  check_devices(on, A.defined() ? A : c->A.codes);
+  if (wants_x || wants_A) return Float8Node::apply(x, A.defined() ? std::optional<Tensor>(A) : std::nullopt, gs, c);
+  return float8_product(*c, x, gs, A.defined() ? quantize_weights_of(A, pow2) : c->A);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_rd_torch, mod) {
@@ -659,4 +867,10 @@ PYBIND11_MODULE(_rd_torch, mod) {
   mod.def("moe_swiglu", &moe_swiglu, unlocked());
   mod.def("int4_pack", &int4_pack, unlocked());
   mod.def("gmm_int4", &gmm_int4, unlocked());
+  mod.def("float8_rows", &float8_rows, unlocked());
+  mod.def("float8_weights", &float8_weights, unlocked());
+  mod.def("float8_values", &float8_values, unlocked());
+  mod.def("moe_dispatch_float8", &moe_dispatch_float8, unlocked());
+  mod.def("moe_swiglu_float8", &moe_swiglu_float8, unlocked());
+  mod.def("gmm_float8", &gmm_float8, unlocked());
 }

@@ -1,0 +1,113 @@
+"""``ragged_dot`` on float8 e4m3fn numbers with a scale for each block of 128: 128 neighbours of a row of ``x``, 128 x 128 of an
+expert's matrix.
+
+    weights = quantize_weights(A)                          # once, or pack_float8(codes, scales) from a checkpoint that has them
+    y = ragged_dot_float8(x, weights, group_sizes)         # serving; x: rows, or quantize_rows(x)
+    y = ragged_dot_float8(x, A, group_sizes)               # training: quantises both, differentiable
+
+A block is held as ``q * s`` with ``s = max(largest magnitude, 2^-80) / 448`` in float32 (with ``pow2`` the next power of two) and
+``q = x / s`` rounded to e4m3fn; one that holds an infinity or NaN is NaN throughout.  ``moe.dispatch`` and ``moe.swiglu`` give rows
+held so by themselves.  The reference has no counterpart; the kernels are behind ``rd_float8_*`` and ``rd_gmm_float8`` of the C ABI
+(``include/ragged_dot_hip.h``), the host side in ``csrc/rd_torch.cpp``.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Union
+
+import torch
+
+from . import _tracing
+from ._native import lib as _native
+from .ops import _group_offset, _sizes
+
+__all__ = ["Float8Rows", "Float8Weights", "quantize_rows", "quantize_weights", "pack_float8", "dequantize", "ragged_dot_float8"]
+
+
+class Float8Rows(NamedTuple):
+    codes: torch.Tensor   # float8_e4m3fn [m, 128 ceil(k / 128)], 0 past k
+    scales: torch.Tensor  # float32 [m, ceil(k / 128) rounded up to a multiple of 4]
+    k: int
+
+
+class Float8Weights(NamedTuple):
+    codes: torch.Tensor   # float8_e4m3fn [g, rows, cols], both rounded up to multiples of 128, 0 in the padding
+    scales: torch.Tensor  # float32 [g, rows / 128, cols / 128]
+    rows: int             # of a matrix: k, or n where the products are called with trans_rhs
+    cols: int
+
+
+def quantize_rows(x: torch.Tensor, *, pow2: bool = False) -> Float8Rows:
+    """Rows ``[m, k]`` in bfloat16, float16 or float32 with a scale for each 128 neighbours.  No gradient."""
+    if _tracing.active():
+        return Float8Rows(*_tracing.record(lambda x: _native.float8_rows(x.detach(), pow2), x), int(x.shape[1]))
+    codes, scales = _native.float8_rows(x, pow2)
+    return Float8Rows(codes, scales, x.shape[1])
+
+
+def quantize_weights(A: torch.Tensor, *, pow2: bool = False) -> Float8Weights:
+    """Weights ``[g, k, n]``, or ``[g, n, k]`` for products with ``trans_rhs``, with a scale for each 128 x 128.  No gradient."""
+    if _tracing.active():
+        return Float8Weights(*_tracing.record(lambda A: _native.float8_weights(A.detach(), pow2), A), *map(int, A.shape[1:]))
+    codes, scales = _native.float8_weights(A, pow2)
+    return Float8Weights(codes, scales, *A.shape[1:])
+
+
+def pack_float8(codes: torch.Tensor, scales: torch.Tensor) -> Float8Weights:
+    """Weights as a checkpoint holds them: e4m3fn ``codes`` ``[g, a, b]`` and ``scales`` ``[g, ceil(a / 128), ceil(b / 128)]``, what a
+    code is multiplied with.  Codes are copied only where ``a`` or ``b`` is no multiple of 128."""
+    assert codes.ndim == 3, f"but {codes.ndim=}"
+    if codes.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"unsupported dtype {codes.dtype}; codes are float8_e4m3fn")
+    if not scales.dtype.is_floating_point:
+        raise TypeError(f"unsupported dtype {scales.dtype}; scales are numbers")
+    g, a, b = codes.shape
+    down, across = -(-a // 128), -(-b // 128)
+    if tuple(scales.shape) != (g, down, across):
+        raise ValueError(f"scales must be {[g, down, across]}, not {list(scales.shape)}")
+    codes, scales = codes.detach(), scales.detach()
+    if (a, b) != (128 * down, 128 * across):
+        whole = torch.zeros((g, 128 * down, 128 * across), dtype=torch.uint8, device=codes.device)
+        whole[:, :a, :b] = codes.view(torch.uint8)
+        codes = whole.view(torch.float8_e4m3fn)
+    return Float8Weights(codes.contiguous(), scales.float().contiguous(), a, b)
+
+
+def dequantize(held: Union[Float8Rows, Float8Weights], dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The numbers, ``q * s`` rounded once to ``dtype`` (bfloat16, float16 or float32): ``[m, k]``, or ``[g, rows, cols]``."""
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"unsupported dtype {dtype}; numbers are bfloat16, float16 or float32")
+    size = (0, held.k) if isinstance(held, Float8Rows) else (held.rows, held.cols)
+    if _tracing.active():
+        return _tracing.record(lambda q, s: _native.float8_values(q, s, *size, dtype), held.codes, held.scales)
+    return _native.float8_values(held.codes, held.scales, *size, dtype)
+
+
+def ragged_dot_float8(x: Union[torch.Tensor, Float8Rows], A: Union[torch.Tensor, Float8Weights], group_sizes, *, trans_rhs: bool = False,
+                      out_dtype: Optional[torch.dtype] = None, pow2: bool = False, group_offset=None) -> torch.Tensor:
+    """``(m, k) x (g, k, n) -> (m, n)``, with ``trans_rhs`` from ``(g, n, k)``, on operands held as float8; rows past
+    ``sum(group_sizes)`` are zero.  Operands given as tensors (bfloat16, float16 or float32, both the same) are quantised first, with
+    ``pow2`` to scales that are powers of two.  Sums are fp32, rounded once to ``out_dtype``: that of ``x`` by default, bfloat16 for
+    rows held as float8.  ``group_offset`` as in ``gmm``.
+
+    Differentiable by operands that are tensors, straight through the quantisation: ``dx`` is the product of the output's gradient,
+    quantised too, with the same float8 weights, ``dA`` that of ``trans_ragged_dot`` on ``x`` and the gradient as they are."""
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if isinstance(x, Float8Rows) else x.dtype
+    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"unsupported dtype {out_dtype}; results are bfloat16, float16 or float32")
+    g_first = -1 if group_offset is None else _group_offset(group_offset)
+    assert group_offset is None or g_first >= 0
+    rows = (None, x.codes, x.scales, x.k) if isinstance(x, Float8Rows) else (x, None, None, 0)
+    weights = (None, *A) if isinstance(A, Float8Weights) else (A, None, None, 0, 0)
+    how = (bool(trans_rhs), g_first, out_dtype, bool(pow2))
+    if _tracing.active():
+        present = [t for t in (*rows[:3], *weights[:3]) if t is not None]
+
+        def call(gs, *tensors):
+            it = iter(tensors)
+            r, w = ([None if t is None else next(it) for t in side[:3]] for side in (rows, weights))
+            return _native.gmm_float8(*r, rows[3], *w, *weights[3:], gs, *how)
+
+        return _tracing.record(call, _sizes(group_sizes), *present)
+    return _native.gmm_float8(*rows, *weights, _sizes(group_sizes), *how)

@@ -24,6 +24,7 @@ import torch
 
 from . import _tracing
 from ._native import lib as _native
+from .float8 import Float8Rows
 
 __all__ = ["Gating", "Routing", "gate", "route", "dispatch", "swiglu", "combine"]
 
@@ -91,17 +92,29 @@ def _combine(y, r: Routing, weights):
         return _native.moe_combine(y, weights, r.row_of_slot, r.slot_of_row, r.tokens, r.top_k)
 
 
-def dispatch(h: torch.Tensor, routing: Routing) -> torch.Tensor:
+def dispatch(h: torch.Tensor, routing: Routing, *, float8: bool = False, pow2: bool = False):
     """``x[row] = h[token of row]``: ``[tokens, d] -> [tokens * top_k, d]`` sorted by expert; rows past
-    ``sum(group_sizes)`` are zero."""
+    ``sum(group_sizes)`` are zero.  With ``float8`` the rows are held as ``quantize_rows(..., pow2=pow2)`` holds them, a token's
+    quantised once for all its rows, for ``ragged_dot_float8``; no gradient."""
+    if float8:
+        call = lambda h, rows, slots: _native.moe_dispatch_float8(h, rows, slots, routing.tokens, routing.top_k, pow2)
+        if _tracing.active():
+            held = _tracing.record(lambda h, *r: call(h.detach(), *r), h, routing.row_of_slot, routing.slot_of_row)
+            return Float8Rows(*held, int(h.shape[1]))
+        return Float8Rows(*call(h, routing.row_of_slot, routing.slot_of_row), h.shape[1])
     if _tracing.active():
         return _tracing.record(lambda *t: dispatch(t[0], routing._replace(row_of_slot=t[1], slot_of_row=t[2])),
                                h, routing.row_of_slot, routing.slot_of_row)
     return _native.moe_dispatch(h, routing.row_of_slot, routing.slot_of_row, routing.tokens, routing.top_k)
 
 
-def swiglu(y: torch.Tensor) -> torch.Tensor:
-    """``silu(gate) * up`` of rows ``[gate | up]``: ``[rows, 2 f] -> [rows, f]``, in fp32 and rounded once."""
+def swiglu(y: torch.Tensor, *, float8: bool = False, pow2: bool = False):
+    """``silu(gate) * up`` of rows ``[gate | up]``: ``[rows, 2 f] -> [rows, f]``, in fp32 and rounded once.  With ``float8`` the
+    result is held as ``quantize_rows(..., pow2=pow2)`` would hold the fp32 values, for ``ragged_dot_float8``; no gradient."""
+    if float8:
+        if _tracing.active():
+            return Float8Rows(*_tracing.record(lambda y: _native.moe_swiglu_float8(y.detach(), pow2), y), int(y.shape[1]) // 2)
+        return Float8Rows(*_native.moe_swiglu_float8(y, pow2), y.shape[1] // 2)
     if _tracing.active():
         return _tracing.record(_native.moe_swiglu, y)
     return _native.moe_swiglu(y)
