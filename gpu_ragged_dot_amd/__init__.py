@@ -15,8 +15,9 @@ if _torch is not None and _torch.version.hip is not None:
     from . import moe  # noqa: F401  (gate / route / dispatch / swiglu / combine around ragged_dot)
     from .float8 import Float8Rows, Float8Weights, dequantize, pack_float8, quantize_rows, quantize_weights, ragged_dot_float8
     from .int4 import Int4Weights, pack_int4, ragged_dot_int4
+    from .ortho import orthogonalize
     from .ops import gmm, make_group_metadata, ragged_dot, ragged_dot_vjp, tgmm, trans_ragged_dot
 
 __all__ = ["gmm", "tgmm", "ragged_dot", "trans_ragged_dot", "ragged_dot_vjp", "make_group_metadata",
            "ragged_dot_int4", "pack_int4", "Int4Weights", "ragged_dot_float8", "quantize_rows", "quantize_weights", "pack_float8", "dequantize",
-           "Float8Rows", "Float8Weights", "moe", "CHUNK_M", "DEFAULT_BLOCK_M", "DEFAULT_BLOCK_N", "DEFAULT_BLOCK_K"]
+           "Float8Rows", "Float8Weights", "orthogonalize", "moe", "CHUNK_M", "DEFAULT_BLOCK_M", "DEFAULT_BLOCK_N", "DEFAULT_BLOCK_K"]

@@ -75,6 +75,11 @@ class Plan(ctypes.Structure):
 RD_INT4_AUTO, RD_INT4_STREAM, RD_INT4_TILES = 0, 1, 2
 
 
+class OrthoSpec(ctypes.Structure):
+    """rd_ortho_spec"""
+    _fields_ = [("steps", ctypes.c_int), ("coefficients", ctypes.POINTER(ctypes.c_double)), ("eps", ctypes.c_double), ("scale", ctypes.c_double)]
+
+
 class GateSpec(ctypes.Structure):
     _fields_ = [("top_k", ctypes.c_int), ("clusters", ctypes.c_int), ("top_clusters", ctypes.c_int), ("flags", ctypes.c_int),
                 ("scale", ctypes.c_float)]
@@ -200,6 +205,10 @@ def _load() -> ctypes.CDLL:
     lib.rd_moe_swiglu_float8.restype = i
     lib.rd_gmm_float8.argtypes = [vp, vp, vp, vp, vp, ip, vp, i, i, i, i, i, i, i, i]
     lib.rd_gmm_float8.restype = i
+    lib.rd_orthogonalize_workspace_bytes.argtypes = [i, i, i, i]
+    lib.rd_orthogonalize_workspace_bytes.restype = sz
+    lib.rd_orthogonalize.argtypes = [vp, vp, vp, i, i, i, ctypes.POINTER(OrthoSpec), i, vp, sz]
+    lib.rd_orthogonalize.restype = i
     return lib
 
 

@@ -11,6 +11,7 @@
 #include "rd_decode.h"
 #include "rd_float8.h"
 #include "rd_int4.h"
+#include "rd_ortho.h"
 #include "rd_moe.h"
 #include "rd_kernels.h"
 #include "rd_lookup.h"
@@ -1409,6 +1410,40 @@ int rd_gmm_float8(void* stream, const void* x, const float* x_scales, const void
   if (!rd::float8_grid_fits(p)) return fail(RD_ERR_UNSUPPORTED, "m=%d rows of n=%d in %d groups are more tiles than a launch has", m, n, g_total);
   rc = rd::launch_gmm_float8((hipStream_t)stream, p);
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "gmm_float8 launch");
+}
+
+static int check_ortho(int g, int k, int n, int dtype) {
+  if (g < 0 || k < 0 || n < 0) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape g=%d, %d x %d", g, k, n);
+  const int rc = check_moe(0, 1, 0, dtype);
+  if (rc != RD_OK) return rc;
+  if (g > 0 && k > 0 && n > 0 && (k > (1 << 28) || n > (1 << 28) || !rd::ortho_grid_fits(g, k, n)))
+    return fail(RD_ERR_UNSUPPORTED, "%d matrices of %d x %d are more than a launch has work-groups for", g, k, n);
+  return RD_OK;
+}
+
+size_t rd_orthogonalize_workspace_bytes(int g, int k, int n, int dtype) {
+  if (check_ortho(g, k, n, dtype) != RD_OK || g == 0 || k == 0 || n == 0) return 0;
+  return align_up(rd::ortho_workspace_bytes(g, k, n, moe_elem(dtype)), 256);
+}
+
+int rd_orthogonalize(void* stream, const void* G, void* out, int g, int k, int n, const rd_ortho_spec* spec, int dtype, void* workspace,
+                     size_t workspace_bytes) {
+  int rc = check_ortho(g, k, n, dtype);
+  if (rc != RD_OK) return rc;
+  if (!spec || spec->steps < 0 || spec->steps > rd::kOrthoMaxSteps || (spec->steps > 0 && !spec->coefficients))
+    return fail(RD_ERR_INVALID_ARGUMENT, "no spec, no coefficients, or steps outside 0..%d", rd::kOrthoMaxSteps);
+  for (int i = 0; i < 3 * spec->steps; ++i)
+    if (!(spec->coefficients[i] - spec->coefficients[i] == 0)) return fail(RD_ERR_INVALID_ARGUMENT, "coefficients must be finite");
+  if (!(spec->eps >= 0) || !(spec->eps - spec->eps == 0) || !(spec->scale - spec->scale == 0)) return fail(RD_ERR_INVALID_ARGUMENT, "eps must be finite and not negative, scale finite");
+  if (!(rd::ortho_growth(spec->steps, spec->coefficients) <= 1024))
+    return fail(RD_ERR_INVALID_ARGUMENT, "these coefficients lead singular values beyond 1024: the iteration does not converge");
+  if (g == 0 || k == 0 || n == 0) return RD_OK;
+  if (!G || !out) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || workspace_bytes < rd_orthogonalize_workspace_bytes(g, k, n, dtype))
+    return fail(RD_ERR_WORKSPACE, "workspace too small or misaligned");
+  const rd::OrthoProblem p = {G, out, g, k, n, moe_elem(dtype), spec->steps, spec->coefficients, spec->eps, spec->scale, workspace};
+  rc = rd::launch_orthogonalize((hipStream_t)stream, p);
+  return rc == hipSuccess ? RD_OK : hip_fail(rc, "orthogonalize launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,412 @@
+// Newton-Schulz iteration on a stack of matrices:  X = G / (|G|_F + eps), then `steps` times
+//   A = X X',  B = b A + c A A,  X = a X + B X
+// with X the smaller side down (G or its transpose), which drives the singular values of X towards one.  Three products of matrices
+// per step, of which the first two are symmetric: their tiles on and below the diagonal are computed, and written twice.
+//
+// Numbers are float16 times a power of two per step and matrix kind that the growth of the singular values allows (|X|, |A| and |B|
+// are bounded by polynomials of it), so that 2^15 is reached and 2^-29 of it still has all eleven bits.  float16 and not bfloat16:
+// eleven bits instead of eight at the same rate.  What the tiles add up is fp32.
+//   16-bit G:  X is held in two numbers, hi + lo, of which the products take hi; A and B in one.  Along the small singular values of X
+//              every step multiplies what is there by a = 3.4, the rounding of X included, until after five steps it has grown 485 times:
+//              of an update of low rank X in one number left 2 % of noise, in two less than 0.1 %.  Products of hi alone cost next to
+//              nothing of that, since B is small along small singular values.
+//   float32 G: everything in two numbers and every product in three, hi hi + hi lo + lo hi: 22 bits, as accurate as float32 products.
+#include "rd_elem.h"
+#include "rd_gemm_w4.h"
+#include "rd_ortho.h"
+
+#include <math.h>
+
+namespace rd {
+
+namespace {
+
+constexpr int kOrthoThreads = 256;
+constexpr int kOrthoChunk = 64 * 1024;  // numbers that a work-group adds up the squares of
+typedef uint16_t half_bits;
+
+// ---- norm ----------------------------------------------------------------------------------------------------------------
+// Sums of squares in 64 bits: of 14336 x 4096 float32 numbers 32 bits would keep 1e-5 at worst, and squares of 1e-25 nothing.
+template <class T>
+__global__ __launch_bounds__(kOrthoThreads) void ortho_norm_kernel(const T* __restrict__ G, double* __restrict__ partial, long long size, int chunks) {
+  __shared__ double sums[kOrthoThreads / 64];
+  const long long e = blockIdx.x / chunks;
+  const int chunk = (int)(blockIdx.x - e * chunks);
+  const long long first = (long long)chunk * kOrthoChunk;
+  const int count = (int)(size - first < kOrthoChunk ? size - first : kOrthoChunk);
+  const T* p = G + e * size + first;
+  double sum = 0;
+  constexpr int PER = 16 / sizeof(T);
+  const int whole = count / PER;
+  for (int i = threadIdx.x; i < whole; i += kOrthoThreads) {
+    alignas(16) T v[PER];
+    *reinterpret_cast<u32x4_t*>(v) = load_any<u32x4_t>(p + i * PER);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) { const double d = to_f32<T>(v[j]); sum = fma(d, d, sum); }
+  }
+  for (int i = whole * PER + threadIdx.x; i < count; i += kOrthoThreads) { const double d = to_f32<T>(p[i]); sum = fma(d, d, sum); }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+__device__ __forceinline__ void split(float v, half_bits* hi, half_bits* lo) {
+  const f16_t h = (f16_t)v;
+  *hi = __builtin_bit_cast(half_bits, h);
+  *lo = __builtin_bit_cast(half_bits, (f16_t)(v - (float)h));
+}
+__device__ __forceinline__ float half_to_f32(half_bits b) { return (float)__builtin_bit_cast(f16_t, b); }
+
+// X = G / (norm + eps), 64 x 64 numbers of the padded X per work-group; `tall`: X is the transpose of G.
+template <class T>
+__global__ __launch_bounds__(kOrthoThreads) void ortho_start_kernel(const T* __restrict__ G, const double* __restrict__ partial, int chunks, half_bits* __restrict__ hi,
+                                                                    half_bits* __restrict__ lo, int k, int n, int rp, int cp, bool tall, double eps, float factor) {
+  __shared__ float tile[64][65];
+  const int across = cp / 64, down = rp / 64;
+  const long long e = blockIdx.x / (across * down);
+  const int in_matrix = (int)(blockIdx.x - e * across * down), r0 = in_matrix / across * 64, c0 = in_matrix % across * 64;
+  double sum = 0;
+  for (int i = 0; i < chunks; ++i) sum += partial[e * chunks + i];
+  const float by = (float)((double)factor / (sqrt(sum) + eps + (sum - sum)));  // (NaN for a sum that is no number)
+  const T* g = G + e * k * n;
+  const int x = threadIdx.x & 63, y0 = threadIdx.x >> 6;
+  // read along the rows of G
+  const int gr = tall ? c0 : r0, gc = tall ? r0 : c0;
+#pragma unroll
+  for (int y = y0; y < 64; y += 4) {
+    const int r = gr + y, c = gc + x;
+    const float v = r < k && c < n ? to_f32<T>(g[(long long)r * n + c]) * by : 0.f;
+    if (tall) tile[x][y] = v; else tile[y][x] = v;
+  }
+  __syncthreads();
+  const long long base = e * rp * cp + (long long)r0 * cp + c0;
+#pragma unroll
+  for (int i = threadIdx.x; i < 64 * 8; i += kOrthoThreads) {
+    const int r = i / 8, c = i % 8 * 8;
+    alignas(16) half_bits h[8], l[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) split(tile[r][c + j], &h[j], &l[j]);
+    *reinterpret_cast<u32x4_t*>(hi + base + (long long)r * cp + c) = *reinterpret_cast<const u32x4_t*>(h);
+    *reinterpret_cast<u32x4_t*>(lo + base + (long long)r * cp + c) = *reinterpret_cast<const u32x4_t*>(l);
+  }
+}
+
+// ---- products --------------------------------------------------------------------------------------------------------------
+// Two planes of padded matrices [rows][cols].
+struct Planes {
+  half_bits *hi, *lo;
+  int rows, cols;
+};
+enum OrthoKind { kGram, kSquare, kApply, kLast };
+struct OrthoStep {
+  Planes left, right;  // operands: the product is left right' (kGram, kSquare), or left right
+  Planes add, to;      // result = of_product * product + of_add * add (kGram: no second term)
+  float of_product, of_add;
+  int g, tiles_r, tiles_c, per_matrix;
+  // kLast: the numbers themselves, [k][n]
+  void* out;
+  int k, n, elem;
+  bool tall;
+};
+
+template <class O>
+__device__ __forceinline__ void store_last(O* out, int r, int c, int rows, int cols, const float (&v)[8]) {  // row r, columns c ..
+  if (r >= rows || c >= cols) return;
+  O* to = out + (long long)r * cols + c;
+  alignas(16) O o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = from_f32<O>(v[i]);
+  if (cols - c >= 8) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(o) / 16; ++i) store_any(to + i * (16 / sizeof(O)), reinterpret_cast<const u32x4_t*>(o)[i]);
+  } else {
+    for (int i = 0; i < cols - c; ++i) to[i] = o[i];
+  }
+}
+__device__ __forceinline__ void store_last(const OrthoStep& p, long long e, int r, int c, const float (&v)[8]) {
+  const long long at = e * p.k * p.n;
+  if (p.elem == 1) store_last(static_cast<float*>(p.out) + at, r, c, p.k, p.n, v);
+  else if (p.elem == 2) store_last(static_cast<f16_t*>(p.out) + at, r, c, p.k, p.n, v);
+  else store_last(static_cast<bf16_bits*>(p.out) + at, r, c, p.k, p.n, v);
+}
+
+// A tile BM x BM of the product; PLANES 2: hi hi + hi lo + lo hi.
+template <int BM, int KIND, int PLANES>
+__global__ __launch_bounds__(kOrthoThreads, 1) void ortho_product_kernel(OrthoStep p) {
+  constexpr bool SYMMETRIC = KIND == kGram || KIND == kSquare;
+  typedef W4Cfg<BM, BM, true, SYMMETRIC, BM == 256 ? 5 : 4, true> C;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int id = xcd_contiguous_id(blockIdx.x, p.g * p.per_matrix);
+  if (id < 0) return;
+  const long long e = id / p.per_matrix;
+  const int t = id - (int)e * p.per_matrix;
+  int ti, tj;
+  if (SYMMETRIC) {  // tiles on and below the diagonal, row by row
+    ti = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while (ti * (ti + 1) / 2 > t) --ti;
+    while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+    tj = t - ti * (ti + 1) / 2;
+  } else {
+    ti = t % p.tiles_r;
+    tj = t / p.tiles_r;
+  }
+  const int r0 = ti * BM, c0 = tj * BM, klen = p.left.cols;
+  const int rows = imin(BM, p.left.rows - r0), cols = imin(BM, (SYMMETRIC ? p.right.rows : p.right.cols) - c0);
+  const long long left = e * p.left.rows * p.left.cols + (long long)r0 * p.left.cols;
+  const long long right = e * p.right.rows * p.right.cols + (SYMMETRIC ? (long long)c0 * p.right.cols : c0);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+  const bool live = wm * C::WM < rows && wn * C::WN < cols;
+
+  f32x16_t acc[C::TM][C::TN];
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+#pragma unroll 1
+  for (int term = 0; term < (PLANES == 2 ? 3 : 1); ++term) {
+    const half_bits* a = (term == 2 ? p.left.lo : p.left.hi) + left;
+    const half_bits* b = (term == 1 ? p.right.lo : p.right.hi) + right;
+    if (live) w4_kloop<C, true>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
+    else w4_kloop<C, false>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
+  }
+  if (!live) return;
+
+  // by way of LDS, 32 rows of the wave's columns at a time, for eight neighbours of a row to a lane, or of a column
+  constexpr int PITCH = C::WN + 4;
+  float* patch = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
+  static_assert(C::NW * 32 * PITCH * 4 <= C::LDS_BYTES, "patches");
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i) {
+    const int pr = r0 + wm * C::WM + i * 32, pc = c0 + wn * C::WN;
+    if (pr >= p.left.rows) break;
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4_t v;
+        v[0] = acc[i][j][4 * g]; v[1] = acc[i][j][4 * g + 1]; v[2] = acc[i][j][4 * g + 2]; v[3] = acc[i][j][4 * g + 3];
+        *reinterpret_cast<f32x4_t*>(patch + (lane & 31) * PITCH + j * 32 + 8 * g + 4 * (lane >> 5)) = v;
+      }
+    __builtin_amdgcn_wave_barrier();
+    constexpr int PER_ROW = C::WN / 8, STEP = 64 / PER_ROW;
+    const bool turned = SYMMETRIC ? ti != tj : KIND == kLast && p.tall;
+#pragma unroll
+    for (int s = 0; s < 32; s += STEP) {
+      const int r = s + lane / PER_ROW, c = lane % PER_ROW * 8;
+      float* at = patch + r * PITCH + c;
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = at[q] * p.of_product;
+      if (pc + c >= p.to.cols) continue;
+      const long long cell = e * p.to.rows * p.to.cols + (long long)(pr + r) * p.to.cols + pc + c;
+      if constexpr (KIND != kGram) {
+        alignas(16) half_bits h[8], l[8];
+        *reinterpret_cast<u32x4_t*>(h) = *reinterpret_cast<const u32x4_t*>(p.add.hi + cell);
+        if (PLANES == 2 || KIND != kSquare) *reinterpret_cast<u32x4_t*>(l) = *reinterpret_cast<const u32x4_t*>(p.add.lo + cell);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float old = PLANES == 2 || KIND != kSquare ? half_to_f32(h[q]) + half_to_f32(l[q]) : half_to_f32(h[q]);
+          v[q] = __builtin_fmaf(old, p.of_add, v[q]);
+        }
+      }
+      if constexpr (KIND == kLast) {
+        if (!p.tall) store_last(p, e, pr + r, pc + c, v);
+      } else {
+        alignas(16) half_bits h[8], l[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) split(v[q], &h[q], &l[q]);
+        *reinterpret_cast<u32x4_t*>(p.to.hi + cell) = *reinterpret_cast<const u32x4_t*>(h);
+        if (PLANES == 2 || KIND == kApply) *reinterpret_cast<u32x4_t*>(p.to.lo + cell) = *reinterpret_cast<const u32x4_t*>(l);
+      }
+      if (turned) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) at[q] = v[q];
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (turned) {
+#pragma unroll
+      for (int s = 0; s < C::WN; s += 16) {  // sixteen columns, four times eight of their rows
+        const int c = s + (lane & 15), r = (lane >> 4) * 8;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = patch[(r + q) * PITCH + c];
+        if (pc + c >= p.to.cols) continue;
+        if constexpr (KIND == kLast) {
+          store_last(p, e, pc + c, pr + r, v);
+        } else {
+          const long long cell = e * p.to.rows * p.to.cols + (long long)(pc + c) * p.to.cols + pr + r;
+          alignas(16) half_bits h[8], l[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) split(v[q], &h[q], &l[q]);
+          *reinterpret_cast<u32x4_t*>(p.to.hi + cell) = *reinterpret_cast<const u32x4_t*>(h);
+          if (PLANES == 2) *reinterpret_cast<u32x4_t*>(p.to.lo + cell) = *reinterpret_cast<const u32x4_t*>(l);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
+// no steps: the matrices over their norms
+template <class T>
+__global__ __launch_bounds__(kOrthoThreads) void ortho_divide_kernel(const T* __restrict__ G, const double* __restrict__ partial, T* __restrict__ out, long long size,
+                                                                     int chunks, double eps, double scale) {
+  const long long e = blockIdx.x / chunks, first = (blockIdx.x - e * chunks) * (long long)kOrthoChunk;
+  double sum = 0;
+  for (int i = 0; i < chunks; ++i) sum += partial[e * chunks + i];
+  const float by = (float)(scale / (sqrt(sum) + eps + (sum - sum)));
+  for (long long i = first + threadIdx.x; i < size && i < first + kOrthoChunk; i += kOrthoThreads) out[e * size + i] = from_f32<T>(to_f32<T>(G[e * size + i]) * by);
+}
+
+template <int BM, int KIND, int PLANES>
+int launch_product(hipStream_t s, OrthoStep p) {
+  constexpr bool SYMMETRIC = KIND == kGram || KIND == kSquare;
+  constexpr int LDS = W4Cfg<BM, BM, true, SYMMETRIC, BM == 256 ? 5 : 4, true>::LDS_BYTES;
+  auto kern = ortho_product_kernel<BM, KIND, PLANES>;
+  if (LDS > 64 * 1024) {
+    const int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (rc != hipSuccess) return rc;
+  }
+  p.tiles_r = (p.left.rows + BM - 1) / BM;
+  p.tiles_c = SYMMETRIC ? p.tiles_r : (p.right.cols + BM - 1) / BM;
+  p.per_matrix = SYMMETRIC ? p.tiles_r * (p.tiles_r + 1) / 2 : p.tiles_r * p.tiles_c;
+  hipLaunchKernelGGL(kern, dim3((unsigned)xcd_padded_grid(p.g * p.per_matrix)), dim3(kOrthoThreads), LDS, s, p);
+  return (int)hipGetLastError();
+}
+template <int KIND>
+int launch_product(hipStream_t s, const OrthoStep& p, bool large, bool two) {
+  if (large) return two ? launch_product<256, KIND, 2>(s, p) : launch_product<256, KIND, 1>(s, p);
+  return two ? launch_product<128, KIND, 2>(s, p) : launch_product<128, KIND, 1>(s, p);
+}
+
+struct OrthoSizes {
+  int rp, cp, chunks;
+  size_t norm, x, square;  // bytes of the sums of squares, of one plane of X, and of one of A
+};
+size_t up(size_t b) { return (b + 255) / 256 * 256; }
+OrthoSizes sizes_of(int g, int k, int n) {
+  OrthoSizes z;
+  const int r = k < n ? k : n, c = k < n ? n : k;
+  z.rp = (r + kOrthoPad - 1) / kOrthoPad * kOrthoPad;
+  z.cp = (c + kOrthoPad - 1) / kOrthoPad * kOrthoPad;
+  z.chunks = (int)(((long long)k * n + kOrthoChunk - 1) / kOrthoChunk);
+  z.norm = up((size_t)g * z.chunks * sizeof(double));
+  z.x = up((size_t)g * z.rp * z.cp * 2);
+  z.square = up((size_t)g * z.rp * z.rp * 2);
+  return z;
+}
+
+// The largest |q(x)| for 0 <= x <= limit, of x p(x x) = a x + b x^3 + c x^5 or of b x + c x^2: at the end or where the derivative is 0.
+double largest(double limit, double a, double b, double c) {
+  double top = 0;
+  auto see = [&](double x) { if (x >= 0 && x <= limit) top = fmax(top, fabs(x * (a + x * x * (b + x * x * c)))); };
+  see(limit);
+  const double d = 9 * b * b - 20 * a * c;  // a + 3 b y + 5 c y^2 = 0, y = x^2
+  if (c != 0 && d >= 0) { see(sqrt(fmax(0.0, (-3 * b + sqrt(d)) / (10 * c)))); see(sqrt(fmax(0.0, (-3 * b - sqrt(d)) / (10 * c)))); }
+  else if (b != 0) see(sqrt(fmax(0.0, -a / (3 * b))));
+  return top;
+}
+double largest_square(double limit, double b, double c) {
+  double top = fabs(limit * (b + limit * c));
+  if (c != 0 && -b / (2 * c) >= 0 && -b / (2 * c) <= limit) top = fmax(top, b * b / (4 * fabs(c)));
+  return top;
+}
+// The power of two that takes numbers up to `top` to 2^15 at most, with room for what roundings add.
+int exponent_for(double top) {
+  int e;
+  frexp(fmax(top * 1.01, 0x1p-9), &e);
+  return 15 - e;
+}
+
+template <class T>
+int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
+  const OrthoSizes z = sizes_of(p.g, p.k, p.n);
+  const bool two = sizeof(T) == 4, tall = p.k > p.n;
+  char* ws = static_cast<char*>(p.workspace);
+  double* partial = reinterpret_cast<double*>(ws);
+  ws += z.norm;
+  auto planes = [&](int rows, int cols, size_t bytes, bool lo) {
+    Planes q{reinterpret_cast<half_bits*>(ws), nullptr, rows, cols};
+    ws += bytes;
+    if (lo) { q.lo = reinterpret_cast<half_bits*>(ws); ws += bytes; }
+    return q;
+  };
+  Planes X[2] = {planes(z.rp, z.cp, z.x, true), planes(z.rp, z.cp, z.x, true)};
+  const Planes A = planes(z.rp, z.rp, z.square, two), B = planes(z.rp, z.rp, z.square, two);
+  const long long size = (long long)p.k * p.n;
+  hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3((unsigned)(p.g * z.chunks)), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, size, z.chunks);
+  int rc = (int)hipGetLastError();
+  if (rc != hipSuccess) return rc;
+  if (p.steps == 0) {
+    hipLaunchKernelGGL((ortho_divide_kernel<T>), dim3((unsigned)(p.g * z.chunks)), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, (T*)p.out, size, z.chunks, p.eps, p.scale);
+    return (int)hipGetLastError();
+  }
+  double bound = 1;
+  int ex = exponent_for(bound);
+  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3((unsigned)(p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, z.chunks, X[0].hi, X[0].lo,
+                     p.k, p.n, z.rp, z.cp, tall, p.eps, (float)ldexp(1.0, ex));
+  if ((rc = (int)hipGetLastError()) != hipSuccess) return rc;
+  const bool large = z.rp > 128;
+  for (int i = 0; i < p.steps; ++i) {
+    const double a = p.coefficients[3 * i], b = p.coefficients[3 * i + 1], c = p.coefficients[3 * i + 2];
+    const int ea = exponent_for(bound * bound), eb = exponent_for(largest_square(bound * bound, b, c));
+    OrthoStep t{};
+    t.g = p.g;
+    t.left = t.right = X[i & 1];
+    t.to = A;
+    t.of_product = (float)ldexp(1.0, ea - 2 * ex);
+    if ((rc = launch_product<kGram>(s, t, large, two)) != hipSuccess) return rc;
+    t.left = t.right = t.add = A;
+    t.to = B;
+    t.of_product = (float)ldexp(c, eb - 2 * ea);
+    t.of_add = (float)ldexp(b, eb - ea);
+    if ((rc = launch_product<kSquare>(s, t, large, two)) != hipSuccess) return rc;
+    const bool last = i + 1 == p.steps;
+    const double next = largest(bound, a, b, c);
+    const int en = exponent_for(next);
+    t.left = B;
+    t.right = t.add = X[i & 1];
+    t.to = X[(i + 1) & 1];
+    t.of_product = last ? (float)ldexp(p.scale, -eb - ex) : (float)ldexp(1.0, en - eb - ex);
+    t.of_add = last ? (float)ldexp(a * p.scale, -ex) : (float)ldexp(a, en - ex);
+    t.out = p.out; t.k = p.k; t.n = p.n; t.elem = p.elem; t.tall = tall;
+    if ((rc = last ? launch_product<kLast>(s, t, large, two) : launch_product<kApply>(s, t, large, two)) != hipSuccess) return rc;
+    bound = next;
+    ex = en;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+size_t ortho_workspace_bytes(int g, int k, int n, int elem) {
+  const OrthoSizes z = sizes_of(g, k, n);
+  return z.norm + 4 * z.x + (elem == 1 ? 4 : 2) * z.square;
+}
+
+bool ortho_grid_fits(int g, int k, int n) {
+  const OrthoSizes z = sizes_of(g, k, n);
+  const double groups = (double)g * ((double)z.rp / 64 * z.cp / 64 + z.chunks);
+  // 32-bit offsets of a tile's operands, and a launch's work-groups
+  return groups < (double)(1 << 23) && (double)z.rp * z.cp < (double)(1 << 30);
+}
+
+double ortho_growth(int steps, const double* coefficients) {
+  double bound = 1, top = 1;
+  for (int i = 0; i < steps; ++i) {
+    bound = largest(bound, coefficients[3 * i], coefficients[3 * i + 1], coefficients[3 * i + 2]);
+    top = fmax(top, bound);
+  }
+  return top;
+}
+
+int launch_orthogonalize(hipStream_t s, const OrthoProblem& p) {
+  return p.elem == 1 ? orthogonalize_t<float>(s, p) : p.elem == 2 ? orthogonalize_t<f16_t>(s, p) : orthogonalize_t<bf16_bits>(s, p);
+}
+
+}  // namespace rd

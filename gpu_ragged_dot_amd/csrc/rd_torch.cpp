@@ -15,6 +15,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
+#include <pybind11/stl.h>
 
 #include <limits>
 #include <map>
@@ -22,6 +23,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/ragged_dot_hip.h"
 
@@ -821,6 +823,26 @@ Tensor gmm_float8(const std::optional<Tensor>& x_, const std::optional<Tensor>& 
   return float8_product(*c, x, gs, A.defined() ? quantize_weights_of(A, pow2) : c->A);
 }
 
+// ---- updates orthogonalised --------------------------------------------------------------------------------------------
+Tensor orthogonalize(const Tensor& G_, const std::vector<double>& coefficients, double eps, double scale) {
+  expect_no_tangent(G_);
+  if (G_.dim() != 2 && G_.dim() != 3) throw py::value_error("G must be [k, n] or [g, k, n]");
+  const int code = rows_code(G_);
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad(G_, G_), "an orthogonalised update has no gradient: call this on detached tensors or under torch.no_grad()");
+  const int64_t k = G_.size(-2), n = G_.size(-1), g = G_.dim() == 3 ? G_.size(0) : 1;
+  expect_int({g, k, n});
+  check_devices(G_, G_);
+  const Tensor G = G_.contiguous();
+  const at::Device dev = G.device();
+  const c10::DeviceGuard guard(dev);
+  Tensor out = empty_on(G.sizes(), G.scalar_type(), dev);
+  const size_t bytes = rd_orthogonalize_workspace_bytes((int)g, (int)k, (int)n, code);
+  const Tensor ws = scratch(bytes, dev);
+  const rd_ortho_spec spec{(int)(coefficients.size() / 3), coefficients.data(), eps, scale};
+  check(rd_orthogonalize(stream_of(dev), G.const_data_ptr(), out.mutable_data_ptr(), (int)g, (int)k, (int)n, &spec, code, ws.mutable_data_ptr(), bytes));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_rd_torch, mod) {
@@ -873,4 +895,5 @@ PYBIND11_MODULE(_rd_torch, mod) {
   mod.def("moe_dispatch_float8", &moe_dispatch_float8, unlocked());
   mod.def("moe_swiglu_float8", &moe_swiglu_float8, unlocked());
   mod.def("gmm_float8", &gmm_float8, unlocked());
+  mod.def("orthogonalize", &orthogonalize, unlocked());
 }
