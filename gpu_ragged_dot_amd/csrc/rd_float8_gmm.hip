@@ -7,7 +7,6 @@ namespace rd {
 
 namespace {
 
-constexpr int kF8GmmThreads = 256;
 constexpr int kF8ZeroRows = 64;  // rows that a work-group looks after which multiplies nothing
 constexpr int kF8Band = 4;       // row tiles of a band of the walk
 
@@ -16,11 +15,11 @@ constexpr int larger(int a, int b) { return a > b ? a : b; }
 // Rows of a tile and columns; a tile of fewer rows runs on the least of the heights that holds it.
 template <bool B_KMAJOR>
 struct F8Tall {
-  static constexpr int BM = 256, BN = 256;
-  typedef F8TileCfg<256, 256, 2, 2, 2, B_KMAJOR> C256;
-  typedef F8TileCfg<128, 256, 2, 2, 3, B_KMAJOR> C128;
-  typedef F8TileCfg<64, 256, 1, 4, 3, B_KMAJOR> C64;
-  static constexpr int LDS_BYTES = larger(C256::LDS_BYTES, larger(C128::LDS_BYTES, C64::LDS_BYTES)), GROUPS = 1;
+  static constexpr int BM = 256, BN = 256, NT = 512, WAVES = 2;
+  typedef F8TileCfg<256, 256, 2, 4, 2, B_KMAJOR> C256;
+  typedef F8TileCfg<128, 256, 2, 4, 3, B_KMAJOR> C128;
+  typedef F8TileCfg<64, 256, 2, 4, 3, B_KMAJOR> C64;
+  static constexpr int LDS_BYTES = larger(C256::LDS_BYTES, larger(C128::LDS_BYTES, C64::LDS_BYTES));
   static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
     if (t.rows <= 64) float8_tile<C64>(t, y, ldy, elem, smem);
     else if (t.rows <= 128) float8_tile<C128>(t, y, ldy, elem, smem);
@@ -29,10 +28,10 @@ struct F8Tall {
 };
 template <bool B_KMAJOR>
 struct F8Few {
-  static constexpr int BM = 64, BN = 128;
+  static constexpr int BM = 64, BN = 128, NT = 256, WAVES = 2;
   typedef F8TileCfg<64, 128, 1, 4, 3, B_KMAJOR> C64;
   typedef F8TileCfg<32, 128, 1, 4, 3, B_KMAJOR> C32;
-  static constexpr int LDS_BYTES = larger(C64::LDS_BYTES, C32::LDS_BYTES), GROUPS = 2;
+  static constexpr int LDS_BYTES = larger(C64::LDS_BYTES, C32::LDS_BYTES);
   static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
     if (t.rows <= 32) float8_tile<C32>(t, y, ldy, elem, smem);
     else float8_tile<C64>(t, y, ldy, elem, smem);
@@ -41,7 +40,7 @@ struct F8Few {
 
 // Work-groups [0, whole): a tile each; those behind them: rows, of which they zero what is no row of a group that the weights hold.
 template <class S, bool B_KMAJOR>
-__global__ __launch_bounds__(kF8GmmThreads, S::GROUPS) void gmm_float8_kernel(F8Problem p, int col_tiles, int whole) {
+__global__ __launch_bounds__(S::NT, S::WAVES) void gmm_float8_kernel(F8Problem p, int col_tiles, int whole) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int size = p.elem == 1 ? 4 : 2;
   if ((int)blockIdx.x >= whole) {
@@ -50,7 +49,7 @@ __global__ __launch_bounds__(kF8GmmThreads, S::GROUPS) void gmm_float8_kernel(F8
     const int r0 = ((int)blockIdx.x - whole) * kF8ZeroRows;
     for (int r = r0; r < imin(r0 + kF8ZeroRows, p.m); ++r)
       if (r < first || r >= end)
-        for (int c = threadIdx.x; c < p.n; c += kF8GmmThreads) {
+        for (int c = threadIdx.x; c < p.n; c += S::NT) {
           if (p.elem == 1) static_cast<float*>(p.y)[(size_t)r * p.n + c] = 0.f;
           else static_cast<uint16_t*>(p.y)[(size_t)r * p.n + c] = 0;
         }
@@ -77,6 +76,7 @@ __global__ __launch_bounds__(kF8GmmThreads, S::GROUPS) void gmm_float8_kernel(F8
   t.rows = tile.rows;
   t.cols = imin(S::BN, p.n - c0);
   t.blocks = kb;
+  t.columns = B_KMAJOR ? t.cols : imin(S::BN, t.ldb - c0);
   S::run(t, static_cast<char*>(p.y) + ((size_t)tile.first * p.n + c0) * size, p.n, p.elem, smem);
 }
 
@@ -104,13 +104,13 @@ int launch_t(hipStream_t s, const F8Problem& p) {
     if (rc != hipSuccess) return rc;
   }
   const F8Grid g = grid_of(p);
-  hipLaunchKernelGGL(kern, dim3((unsigned)g.all), dim3(kF8GmmThreads), S<B_KMAJOR>::LDS_BYTES, s, p, g.col_tiles, (int)g.whole);
+  hipLaunchKernelGGL(kern, dim3((unsigned)g.all), dim3(S<B_KMAJOR>::NT), S<B_KMAJOR>::LDS_BYTES, s, p, g.col_tiles, (int)g.whole);
   return (int)hipGetLastError();
 }
 
 }  // namespace
 
-bool float8_grid_fits(const F8Problem& p) { return grid_of(p).all < (1ll << 31) / kF8GmmThreads; }
+bool float8_grid_fits(const F8Problem& p) { return grid_of(p).all < (1ll << 31) / 512; }
 
 int launch_gmm_float8(hipStream_t s, const F8Problem& p) {
   if (few_rows(p)) return p.trans_rhs ? launch_t<F8Few, true>(s, p) : launch_t<F8Few, false>(s, p);
