@@ -87,7 +87,7 @@ struct F8Reader16 {
 template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int STAGES_, bool B_KMAJOR_>
 struct F8TileCfg {
   static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, STAGES = STAGES_;
-  static constexpr bool B_KMAJOR = B_KMAJOR_;
+  static constexpr bool B_KMAJOR = B_KMAJOR_, PINGPONG = WAVES_M == 2 && WAVES_N == 4 && BM == 256;
   static constexpr int NW = WAVES_M * WAVES_N, NT = 64 * NW;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 16, TN = WN / 16;
   static constexpr int A_BYTES = BM * kF8Block, B_BYTES = BN * kF8Block, STAGE_BYTES = A_BYTES + B_BYTES;
@@ -156,87 +156,190 @@ __device__ __forceinline__ void float8_store(const f32x4_t (&acc)[C::TM][C::TN],
   }
 }
 
+// What the K loops share: a wave's part of a tile and its operands' ways to LDS and out of it.
 template <class C>
-__device__ __forceinline__ void float8_tile(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / C::WAVES_N, wn = wave % C::WAVES_N;
+struct F8Wave {
+  int lane, wave, wm, wn;
+  bool live;
   typename C::LdA la;
   typename C::LdB lb;
-  la.init(t.a, t.lda, t.rows, t.blocks, wave, lane);
-  lb.init(t.b, t.ldb, t.columns, t.blocks, wave, lane);
   F8Reader16<C::BM, C::TM, true> fra;
   F8Reader16<C::BN, C::TN, C::B_KMAJOR> frb;
-  fra.init(wm * C::WM, lane);
-  frb.init(wn * C::WN, lane);
-  const bool live = wm * C::WM < t.rows && wn * C::WN < t.cols;
+  __amdgpu_buffer_rsrc_t scale_rsrc;
+  int scale_off, scale_at;
+  const __attribute__((address_space(4))) float* col_scale;  // (read through the scalar cache: no vector load to wait for)
+  unsigned char* smem;
 
+  __device__ __forceinline__ void init(const F8Tile& t, unsigned char* smem_) {
+    smem = smem_;
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wm = wave / C::WAVES_N; wn = wave % C::WAVES_N;
+    la.init(t.a, t.lda, t.rows, t.blocks, wave, lane);
+    lb.init(t.b, t.ldb, t.columns, t.blocks, wave, lane);
+    fra.init(wm * C::WM, lane);
+    frb.init(wn * C::WN, lane);
+    live = wm * C::WM < t.rows && wn * C::WN < t.cols;
+    const int row = wave * 64 + lane;
+    scale_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)t.a_scales, 0, t.rows * t.ldas * 4, kBufferFlags);
+    scale_off = row < t.rows ? row * t.ldas * 4 : -1;
+    scale_at = (wm * C::WM + (lane & 15)) * 16;
+    col_scale = (const __attribute__((address_space(4))) float*)(live ? t.b_scales + (wn * C::WN / kF8Block) * t.b_column : t.b_scales);
+  }
+  // The wave's share of slab `step`, and of the rows' scales of four blocks beside the first of them: 16 bytes a lane, 64 rows a wave.
+  __device__ __forceinline__ void issue(int step) {
+    unsigned char* st = smem + (step % C::STAGES) * C::STAGE_BYTES;
+    if ((step & 3) == 0 && wave < (C::BM + 63) / 64)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(scale_rsrc, (lds_void_ptr)(smem + C::RING_BYTES + ((step >> 2) & 1) * C::SCALE_BYTES + wave * 1024), 16,
+                                               scale_off >= 0 ? scale_off + step * 4 : kOobOffset, 0, 0, 0);
+    la.issue(st, wave);
+    lb.issue(st + C::A_BYTES, wave);
+    la.advance();
+    lb.advance();
+  }
+  __device__ __forceinline__ const unsigned char* slab(int step) const { return smem + (step % C::STAGES) * C::STAGE_BYTES; }
+  __device__ __forceinline__ float row_scale(int step, int tile) const {
+    return *reinterpret_cast<const float*>(smem + C::RING_BYTES + ((step >> 2) & 1) * C::SCALE_BYTES + (step & 3) * 4 + scale_at + tile * 256);
+  }
+};
+
+__device__ __forceinline__ f32x4_t float8_part(const i32x8_t& b, const i32x8_t& a) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ void float8_add(f32x4_t& acc, const f32x4_t& part, float factor) {
+#pragma unroll
+  for (int v = 0; v < 4; ++v) acc[v] = __builtin_fmaf(part[v], factor, acc[v]);
+}
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A barrier per slab, several slabs on their way: tiles of few rows, which wait for their weights.
+template <class C>
+__device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, int b_block, f32x4_t (&acc)[C::TM][C::TN]) {
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s)
+    if (s < nk) u.issue(s);
+  constexpr int L = C::LdA::PER + C::LdB::PER;
+  for (int kt = 0; kt < nk; ++kt) {
+    // (a load of scales makes a wave wait for no less)
+    if (kt + C::STAGES - 2 < nk) wait_vmcnt<(C::STAGES - 2) * L>(); else wait_vmcnt<0>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    phase_barrier();  // slab kt is in LDS, and slab kt - 1 is no longer being read
+    if (kt + C::STAGES - 1 < nk) u.issue(kt + C::STAGES - 1);
+    if (u.live) {
+      const float w = u.col_scale[(long long)kt * b_block];
+      const unsigned char* ra = u.slab(kt);
+      i32x8_t fb[C::TN];
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) fb[j] = u.frb.read(ra + C::A_BYTES, j);
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const i32x8_t fa = u.fra.read(ra, i);
+        const float factor = u.row_scale(kt, i) * w;
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) float8_add(acc[i][j], float8_part(fb[j], fa), factor);
+      }
+    }
+  }
+}
+
+// Two groups of four waves, one of each per SIMD, half a period apart: while one reads the fragments of half of its rows (memory phase),
+// the other multiplies (compute phase); a barrier ends every phase, four phases a slab.  In phases, group 0 reads slab t in 4 t and
+// 4 t + 2 and multiplies in 4 t + 1 and 4 t + 3, group 1 a phase later.  Slab t - 1 was read last in phase 4 t - 1, so both groups
+// request slab t + 1 in phase 4 t, group 1 amid its multiplications, and wait for it in phase 4 t + 3: nearly a slab's time on its way.
+// Inner sums enter the accumulators four instructions later, those of a phase's last row piece at the start of the next compute phase.
+template <class C>
+__device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int b_block, f32x4_t (&acc)[C::TM][C::TN]) {
+  static_assert(C::NW == 8 && C::WAVES_M == 2 && C::STAGES == 2 && C::TM == 8, "two groups of four waves, four row pieces a phase");
+  const int group = u.wave >> 2;
+  i32x8_t fa[4], fb[C::TN];
+  float factor[4], carried = 0.f;
+  f32x4_t part[2][C::TN];
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) part[1][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  constexpr int L = C::LdA::PER + C::LdB::PER;
+
+  u.issue(0);
+  if (nk > 1) { u.issue(1); wait_vmcnt<L>(); } else wait_vmcnt<0>();
+  phase_barrier();
+  if (group == 1) phase_barrier();
+
+  auto read = [&](int kt, auto half, float w) {
+    constexpr int H = decltype(half)::value;
+    const unsigned char* ra = u.slab(kt);
+    if constexpr (H == 0) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) fb[j] = u.frb.read(ra + C::A_BYTES, j);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      fa[i] = u.fra.read(ra, 4 * H + i);
+      factor[i] = u.row_scale(kt, 4 * H + i) * w;
+    }
+  };
+  auto multiply = [&](auto half) {
+    constexpr int H = decltype(half)::value;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        part[i & 1][j] = float8_part(fb[j], fa[i]);
+        float8_add(acc[(4 * H + i + 7) & 7][j], part[(i + 1) & 1][j], i == 0 ? carried : factor[i == 0 ? 0 : i - 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    carried = factor[3];
+  };
+  typedef std::integral_constant<int, 0> First;
+  typedef std::integral_constant<int, 1> Second;
+  for (int kt = 0; kt < nk; ++kt) {
+    const float w = u.live ? u.col_scale[(long long)kt * b_block] : 0.f;
+    if (u.live) read(kt, First(), w);
+    if (group == 0 && kt > 0 && kt + 1 < nk) u.issue(kt + 1);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    phase_barrier();
+    __builtin_amdgcn_s_setprio(1);
+    if (u.live) multiply(First());
+    __builtin_amdgcn_s_setprio(0);
+    phase_barrier();
+    if (u.live) read(kt, Second(), w);
+    if (group == 1) wait_vmcnt<0>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    phase_barrier();
+    if (group == 1 && kt + 2 < nk) u.issue(kt + 2);
+    __builtin_amdgcn_s_setprio(1);
+    if (u.live) multiply(Second());
+    __builtin_amdgcn_s_setprio(0);
+    if (group == 0) wait_vmcnt<0>();
+    phase_barrier();
+  }
+  if (group == 0) phase_barrier();
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) float8_add(acc[7][j], part[1][j], carried);
+}
+
+template <class C>
+__device__ __forceinline__ void float8_tile(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
+  F8Wave<C> u;
+  u.init(t, smem);
   f32x4_t acc[C::TM][C::TN];
 #pragma unroll
   for (int i = 0; i < C::TM; ++i)
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  const int nk = t.blocks;
-  // A row's scales, four blocks at a time: 16 bytes a lane, 64 rows a wave, beside the slab of the first of the four.
-  unsigned char* const scales = smem + C::RING_BYTES;
-  constexpr int SCALE_WAVES = (C::BM + 63) / 64;
-  const int scale_row = wave * 64 + lane;
-  const __amdgpu_buffer_rsrc_t scale_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)t.a_scales, 0, t.rows * t.ldas * 4, kBufferFlags);
-  auto issue_slab = [&](int step) {
-    unsigned char* st = smem + (step % C::STAGES) * C::STAGE_BYTES;
-    if ((step & 3) == 0 && wave < SCALE_WAVES)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(scale_rsrc, (lds_void_ptr)(scales + ((step >> 2) & 1) * C::SCALE_BYTES + wave * 1024), 16,
-                                               scale_row < t.rows ? (scale_row * t.ldas + step) * 4 : kOobOffset, 0, 0, 0);
-    la.issue(st, wave);
-    lb.issue(st + C::A_BYTES, wave);
-    la.advance();
-    lb.advance();
-  };
-  const float* col_scale = t.b_scales + (wn * C::WN / kF8Block) * t.b_column;
-  const int scale_at = (wm * C::WM + (lane & 15)) * 16;
-
-#pragma unroll
-  for (int s = 0; s < C::STAGES - 1; ++s)
-    if (s < nk) issue_slab(s);
-
-  constexpr int L = C::LdA::PER + C::LdB::PER;
-  for (int kt = 0; kt < nk; ++kt) {
-    // (a scale load makes a wave wait for no less)
-    if (kt + C::STAGES - 2 < nk) wait_vmcnt<(C::STAGES - 2) * L>(); else wait_vmcnt<0>();
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();  // slab kt is in LDS, and slab kt - 1 is no longer being read
-    __builtin_amdgcn_sched_barrier(0);
-    if (kt + C::STAGES - 1 < nk) issue_slab(kt + C::STAGES - 1);
-    if (live) {
-      const float w = col_scale[(long long)kt * t.b_block];
-      const unsigned char* ra = smem + (kt % C::STAGES) * C::STAGE_BYTES;
-      const unsigned char* rb = ra + C::A_BYTES;
-      const unsigned char* rs = scales + ((kt >> 2) & 1) * C::SCALE_BYTES + scale_at + (kt & 3) * 4;
-      i32x8_t fb[C::TN];
-#pragma unroll
-      for (int j = 0; j < C::TN; ++j) fb[j] = frb.read(rb, j);
-#pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        const i32x8_t fa = fra.read(ra, i);
-        const float factor = *reinterpret_cast<const float*>(rs + i * 256) * w;
-#pragma unroll
-        for (int j = 0; j < C::TN; ++j) {
-          f32x4_t part = {};
-          part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, part, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-          for (int v = 0; v < 4; ++v) acc[i][j][v] = __builtin_fmaf(part[v], factor, acc[i][j][v]);
-        }
-      }
-    }
+  if (t.blocks > 0) {
+    if constexpr (C::PINGPONG) float8_kloop_pingpong<C>(u, t.blocks, t.b_block, acc);
+    else float8_kloop<C>(u, t.blocks, t.b_block, acc);
   }
   __builtin_amdgcn_s_waitcnt(0xc07f);
-  __builtin_amdgcn_s_barrier();  // the ring is no longer read by any wave
-  if (!live) return;
-  if (elem == 1) float8_store<C, float>(acc, wm, wn, wave, lane, t.rows, t.cols, static_cast<float*>(y), ldy, smem);
-  else if (elem == 2) float8_store<C, f16_t>(acc, wm, wn, wave, lane, t.rows, t.cols, static_cast<f16_t*>(y), ldy, smem);
-  else float8_store<C, bf16_bits>(acc, wm, wn, wave, lane, t.rows, t.cols, static_cast<bf16_bits*>(y), ldy, smem);
+  phase_barrier();  // the ring is no longer read by any wave
+  if (!u.live) return;
+  if (elem == 1) float8_store<C, float>(acc, u.wm, u.wn, u.wave, u.lane, t.rows, t.cols, static_cast<float*>(y), ldy, smem);
+  else if (elem == 2) float8_store<C, f16_t>(acc, u.wm, u.wn, u.wave, u.lane, t.rows, t.cols, static_cast<f16_t*>(y), ldy, smem);
+  else float8_store<C, bf16_bits>(acc, u.wm, u.wn, u.wave, u.lane, t.rows, t.cols, static_cast<bf16_bits*>(y), ldy, smem);
 }
 
 }  // namespace rd
