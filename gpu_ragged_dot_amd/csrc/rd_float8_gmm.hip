@@ -8,7 +8,10 @@ namespace rd {
 namespace {
 
 constexpr int kF8ZeroRows = 64;  // rows that a work-group looks after which multiplies nothing
-constexpr int kF8Band = 4;       // row tiles of a band of the walk
+#ifndef V_BAND
+#define V_BAND 8
+#endif
+constexpr int kF8Band = V_BAND;       // row tiles of a band of the walk
 
 constexpr int larger(int a, int b) { return a > b ? a : b; }
 
@@ -60,7 +63,12 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void gmm_float8_kernel(F8Problem p
   const int at = xcd_contiguous_id(blockIdx.x, positions);
   if (at < 0) return;
   int column = 0;
-  const RowTile tile = find_in_walk<S::BM, kF8Band>(p, 1, p.m, col_tiles, at, &column);
+  RowTile tile = find_in_walk<S::BM, kF8Band>(p, 1, p.m, col_tiles, at, &column);
+  // the same in all lanes, and so in scalar registers: buffer descriptors made of others are read lane by lane in a loop around every load
+  tile.group = __builtin_amdgcn_readfirstlane(tile.group);
+  tile.first = __builtin_amdgcn_readfirstlane(tile.first);
+  tile.rows = __builtin_amdgcn_readfirstlane(tile.rows);
+  column = __builtin_amdgcn_readfirstlane(column);
   const int c0 = column * S::BN, kb = float8_blocks(p.k), nb = float8_blocks(p.n);
   const size_t e = tile.group - p.g_first;
   F8Tile t;

@@ -288,7 +288,9 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int 
       for (int j = 0; j < C::TN; ++j) {
         part[i & 1][j] = float8_part(fb[j], fa[i]);
         float8_add(acc[(4 * H + i + 7) & 7][j], part[(i + 1) & 1][j], i == 0 ? carried : factor[i == 0 ? 0 : i - 1]);
+#ifndef V_NOSB
         __builtin_amdgcn_sched_barrier(0);
+#endif
       }
     }
     carried = factor[3];
