@@ -156,6 +156,9 @@ __device__ __forceinline__ void float8_store(const f32x4_t (&acc)[C::TM][C::TN],
   }
 }
 
+#ifndef V_FIRST
+#define V_FIRST 2
+#endif
 // What the K loops share: a wave's part of a tile and its operands' ways to LDS and out of it.
 template <class C>
 struct F8Wave {
@@ -198,6 +201,17 @@ struct F8Wave {
     lb.advance();
   }
   __device__ __forceinline__ const unsigned char* slab(int step) const { return smem + (step % C::STAGES) * C::STAGE_BYTES; }
+  // A lane's scale of its row in each of four pieces of sixteen rows, 4 h .. 4 h + 3 of the wave's, times w.  A lane reads that of one of the
+  // 64 rows, and halves and quarters of the wave trade theirs (four reads of LDS take as long as two of a fragment).
+  __device__ __forceinline__ void factors(int step, int h, float w, float (&factor)[4]) const {
+    const unsigned char* at = smem + C::RING_BYTES + ((step >> 2) & 1) * C::SCALE_BYTES + (step & 3) * 4;
+    const uint32_t s = __builtin_bit_cast(uint32_t, *reinterpret_cast<const float*>(at + (wm * C::WM + 64 * h + lane) * 16) * w);
+    const auto half = __builtin_amdgcn_permlane32_swap(s, s, false, false);
+    const auto low = __builtin_amdgcn_permlane16_swap(half[0], half[0], false, false), high = __builtin_amdgcn_permlane16_swap(half[1], half[1], false, false);
+    const uint32_t got[4] = {low[0], low[1], high[0], high[1]};  // (a bit cast of a vector's element itself would read element 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) factor[i] = __builtin_bit_cast(float, got[i]);
+  }
   __device__ __forceinline__ float row_scale(int step, int tile) const {
     return *reinterpret_cast<const float*>(smem + C::RING_BYTES + ((step >> 2) & 1) * C::SCALE_BYTES + (step & 3) * 4 + scale_at + tile * 256);
   }
@@ -275,13 +289,15 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int 
       for (int j = 0; j < C::TN; ++j) fb[j] = u.frb.read(ra + C::A_BYTES, j);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fa[i] = u.fra.read(ra, 4 * H + i);
-      factor[i] = u.row_scale(kt, 4 * H + i) * w;
-    }
+    for (int i = 0; i < (H == 0 ? V_FIRST : 4); ++i) fa[i] = u.fra.read(ra, 4 * H + i);
+    u.factors(kt, H, w, factor);
   };
-  auto multiply = [&](auto half) {
+  auto multiply = [&](int kt, auto half) {
     constexpr int H = decltype(half)::value;
+    if constexpr (H == 0) {
+#pragma unroll
+      for (int i = V_FIRST; i < 4; ++i) fa[i] = u.fra.read(u.slab(kt), i);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -304,7 +320,7 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int 
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     phase_barrier();
     __builtin_amdgcn_s_setprio(1);
-    if (u.live) multiply(First());
+    if (u.live) multiply(kt, First());
     __builtin_amdgcn_s_setprio(0);
     phase_barrier();
     if (u.live) read(kt, Second(), w);
@@ -313,7 +329,7 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int 
     phase_barrier();
     if (group == 1 && kt + 2 < nk) u.issue(kt + 2);
     __builtin_amdgcn_s_setprio(1);
-    if (u.live) multiply(Second());
+    if (u.live) multiply(kt, Second());
     __builtin_amdgcn_s_setprio(0);
     if (group == 0) wait_vmcnt<0>();
     phase_barrier();
