@@ -132,11 +132,22 @@ __device__ __forceinline__ void store_last(const OrthoStep& p, long long e, int 
   else store_last(static_cast<bf16_bits*>(p.out) + at, r, c, p.k, p.n, v);
 }
 
-// A tile BM x BM of the product; PLANES 2: hi hi + hi lo + lo hi.
+// Tiles of the products.  Of the symmetric ones they are square; of the others, whose contraction is short and whose results are read and
+// written in two numbers, large ones are 128 x 256, two work-groups to a compute unit: one multiplies while the other stores.
+template <int BM, bool SYMMETRIC>
+struct OrthoTile {
+  static constexpr int ROWS = !SYMMETRIC && BM == 256 ? 128 : BM, GROUPS = ROWS == 256 ? 1 : 2;
+  typedef W4Cfg<ROWS, BM, true, SYMMETRIC, ROWS == 256 ? 5 : BM == 256 ? 3 : 4, true> C;
+};
+
+template <int BM, bool SYMMETRIC>
+constexpr int ortho_groups = OrthoTile<BM, SYMMETRIC>::GROUPS;
+
+// PLANES 2: hi hi + hi lo + lo hi.
 template <int BM, int KIND, int PLANES>
-__global__ __launch_bounds__(kOrthoThreads, 1) void ortho_product_kernel(OrthoStep p) {
+__global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || KIND == kSquare>)) void ortho_product_kernel(OrthoStep p) {
   constexpr bool SYMMETRIC = KIND == kGram || KIND == kSquare;
-  typedef W4Cfg<BM, BM, true, SYMMETRIC, BM == 256 ? 5 : 4, true> C;
+  typedef typename OrthoTile<BM, SYMMETRIC>::C C;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int id = xcd_contiguous_id(blockIdx.x, p.g * p.per_matrix);
   if (id < 0) return;
@@ -152,8 +163,8 @@ __global__ __launch_bounds__(kOrthoThreads, 1) void ortho_product_kernel(OrthoSt
     ti = t % p.tiles_r;
     tj = t / p.tiles_r;
   }
-  const int r0 = ti * BM, c0 = tj * BM, klen = p.left.cols;
-  const int rows = imin(BM, p.left.rows - r0), cols = imin(BM, (SYMMETRIC ? p.right.rows : p.right.cols) - c0);
+  const int r0 = ti * C::BM, c0 = tj * C::BN, klen = p.left.cols;
+  const int rows = imin(C::BM, p.left.rows - r0), cols = imin(C::BN, (SYMMETRIC ? p.right.rows : p.right.cols) - c0);
   const long long left = e * p.left.rows * p.left.cols + (long long)r0 * p.left.cols;
   const long long right = e * p.right.rows * p.right.cols + (SYMMETRIC ? (long long)c0 * p.right.cols : c0);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
@@ -175,14 +186,36 @@ __global__ __launch_bounds__(kOrthoThreads, 1) void ortho_product_kernel(OrthoSt
   }
   if (!live) return;
 
-  // by way of LDS, 32 rows of the wave's columns at a time, for eight neighbours of a row to a lane, or of a column
+  // by way of LDS, 32 rows of the wave's columns at a time, for eight neighbours of a row to a lane, or of a column; what is added is
+  // requested before, a piece ahead where registers allow
   constexpr int PITCH = C::WN + 4;
   float* patch = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
   static_assert(C::NW * 32 * PITCH * 4 <= C::LDS_BYTES, "patches");
+  constexpr int PER_ROW = C::WN / 8, STEP = 64 / PER_ROW, ITER = 32 / STEP;
+  constexpr bool ADDS = KIND != kGram, ADDS_LO = ADDS && (PLANES == 2 || KIND != kSquare);
+  const bool turned = SYMMETRIC ? ti != tj : KIND == kLast && p.tall;
+  const int own_r = lane / PER_ROW, own_c = lane % PER_ROW * 8, pc = c0 + wn * C::WN;
+  const bool inside = pc + own_c < p.to.cols;
+  const long long matrix = e * p.to.rows * p.to.cols, own = matrix + (long long)(r0 + wm * C::WM + own_r) * p.to.cols + pc + own_c;
+  constexpr int AHEAD = SYMMETRIC ? 1 : 0;  // (the sums of the others leave no registers for two; the other work-group fills the wait)
+  u32x4_t add_hi[AHEAD + 1][ADDS ? ITER : 1], add_lo[AHEAD + 1][ADDS_LO ? ITER : 1];
+  auto request = [&](int i) {
+    if constexpr (ADDS) {
+      if (!inside || r0 + wm * C::WM + i * 32 >= p.left.rows) return;
+#pragma unroll
+      for (int t = 0; t < ITER; ++t) {
+        const long long cell = own + (long long)(i * 32 + t * STEP) * p.to.cols;
+        add_hi[i & AHEAD][t] = *reinterpret_cast<const u32x4_t*>(p.add.hi + cell);
+        if constexpr (ADDS_LO) add_lo[i & AHEAD][t] = *reinterpret_cast<const u32x4_t*>(p.add.lo + cell);
+      }
+    }
+  };
+  if constexpr (AHEAD > 0) request(0);
 #pragma unroll
   for (int i = 0; i < C::TM; ++i) {
-    const int pr = r0 + wm * C::WM + i * 32, pc = c0 + wn * C::WN;
+    const int pr = r0 + wm * C::WM + i * 32;
     if (pr >= p.left.rows) break;
+    if (AHEAD == 0 || i + 1 < C::TM) request(i + AHEAD);
 #pragma unroll
     for (int j = 0; j < C::TN; ++j)
 #pragma unroll
@@ -192,39 +225,37 @@ __global__ __launch_bounds__(kOrthoThreads, 1) void ortho_product_kernel(OrthoSt
         *reinterpret_cast<f32x4_t*>(patch + (lane & 31) * PITCH + j * 32 + 8 * g + 4 * (lane >> 5)) = v;
       }
     __builtin_amdgcn_wave_barrier();
-    constexpr int PER_ROW = C::WN / 8, STEP = 64 / PER_ROW;
-    const bool turned = SYMMETRIC ? ti != tj : KIND == kLast && p.tall;
+    if (inside) {
 #pragma unroll
-    for (int s = 0; s < 32; s += STEP) {
-      const int r = s + lane / PER_ROW, c = lane % PER_ROW * 8;
-      float* at = patch + r * PITCH + c;
-      float v[8];
+      for (int t = 0; t < ITER; ++t) {
+        float* at = patch + (t * STEP + own_r) * PITCH + own_c;
+        float v[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = at[q] * p.of_product;
-      if (pc + c >= p.to.cols) continue;
-      const long long cell = e * p.to.rows * p.to.cols + (long long)(pr + r) * p.to.cols + pc + c;
-      if constexpr (KIND != kGram) {
-        alignas(16) half_bits h[8], l[8];
-        *reinterpret_cast<u32x4_t*>(h) = *reinterpret_cast<const u32x4_t*>(p.add.hi + cell);
-        if (PLANES == 2 || KIND != kSquare) *reinterpret_cast<u32x4_t*>(l) = *reinterpret_cast<const u32x4_t*>(p.add.lo + cell);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float old = PLANES == 2 || KIND != kSquare ? half_to_f32(h[q]) + half_to_f32(l[q]) : half_to_f32(h[q]);
-          v[q] = __builtin_fmaf(old, p.of_add, v[q]);
+        for (int q = 0; q < 2; ++q) {
+          const f32x4_t w = *reinterpret_cast<const f32x4_t*>(at + 4 * q);
+          v[4 * q] = w[0] * p.of_product; v[4 * q + 1] = w[1] * p.of_product; v[4 * q + 2] = w[2] * p.of_product; v[4 * q + 3] = w[3] * p.of_product;
         }
-      }
-      if constexpr (KIND == kLast) {
-        if (!p.tall) store_last(p, e, pr + r, pc + c, v);
-      } else {
-        alignas(16) half_bits h[8], l[8];
+        if constexpr (ADDS) {
+          alignas(16) half_bits h[8], l[8];
+          *reinterpret_cast<u32x4_t*>(h) = add_hi[i & AHEAD][t];
+          if constexpr (ADDS_LO) *reinterpret_cast<u32x4_t*>(l) = add_lo[i & AHEAD][t];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) split(v[q], &h[q], &l[q]);
-        *reinterpret_cast<u32x4_t*>(p.to.hi + cell) = *reinterpret_cast<const u32x4_t*>(h);
-        if (PLANES == 2 || KIND == kApply) *reinterpret_cast<u32x4_t*>(p.to.lo + cell) = *reinterpret_cast<const u32x4_t*>(l);
-      }
-      if (turned) {
+          for (int q = 0; q < 8; ++q) v[q] = __builtin_fmaf(ADDS_LO ? half_to_f32(h[q]) + half_to_f32(l[q]) : half_to_f32(h[q]), p.of_add, v[q]);
+        }
+        if constexpr (KIND == kLast) {
+          if (!p.tall) store_last(p, e, pr + t * STEP + own_r, pc + own_c, v);
+        } else {
+          const long long cell = own + (long long)(i * 32 + t * STEP) * p.to.cols;
+          alignas(16) half_bits h[8], l[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) at[q] = v[q];
+          for (int q = 0; q < 8; ++q) split(v[q], &h[q], &l[q]);
+          *reinterpret_cast<u32x4_t*>(p.to.hi + cell) = *reinterpret_cast<const u32x4_t*>(h);
+          if (PLANES == 2 || KIND == kApply) *reinterpret_cast<u32x4_t*>(p.to.lo + cell) = *reinterpret_cast<const u32x4_t*>(l);
+        }
+        if (turned) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) *reinterpret_cast<f32x4_t*>(at + 4 * q) = f32x4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        }
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -239,7 +270,7 @@ __global__ __launch_bounds__(kOrthoThreads, 1) void ortho_product_kernel(OrthoSt
         if constexpr (KIND == kLast) {
           store_last(p, e, pc + c, pr + r, v);
         } else {
-          const long long cell = e * p.to.rows * p.to.cols + (long long)(pc + c) * p.to.cols + pr + r;
+          const long long cell = matrix + (long long)(pc + c) * p.to.cols + pr + r;
           alignas(16) half_bits h[8], l[8];
 #pragma unroll
           for (int q = 0; q < 8; ++q) split(v[q], &h[q], &l[q]);
@@ -266,14 +297,15 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_divide_kernel(const T* __
 template <int BM, int KIND, int PLANES>
 int launch_product(hipStream_t s, OrthoStep p) {
   constexpr bool SYMMETRIC = KIND == kGram || KIND == kSquare;
-  constexpr int LDS = W4Cfg<BM, BM, true, SYMMETRIC, BM == 256 ? 5 : 4, true>::LDS_BYTES;
+  typedef typename OrthoTile<BM, SYMMETRIC>::C C;
+  constexpr int LDS = C::LDS_BYTES;
   auto kern = ortho_product_kernel<BM, KIND, PLANES>;
   if (LDS > 64 * 1024) {
     const int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (rc != hipSuccess) return rc;
   }
-  p.tiles_r = (p.left.rows + BM - 1) / BM;
-  p.tiles_c = SYMMETRIC ? p.tiles_r : (p.right.cols + BM - 1) / BM;
+  p.tiles_r = (p.left.rows + C::BM - 1) / C::BM;
+  p.tiles_c = SYMMETRIC ? p.tiles_r : (p.right.cols + C::BN - 1) / C::BN;
   p.per_matrix = SYMMETRIC ? p.tiles_r * (p.tiles_r + 1) / 2 : p.tiles_r * p.tiles_c;
   hipLaunchKernelGGL(kern, dim3((unsigned)xcd_padded_grid(p.g * p.per_matrix)), dim3(kOrthoThreads), LDS, s, p);
   return (int)hipGetLastError();
