@@ -8,8 +8,10 @@
 // eleven bits instead of eight at the same rate.  What the tiles add up is fp32.
 //   16-bit G:  X is held in two numbers, hi + lo, of which the products take hi; A and B in one.  Along the small singular values of X
 //              every step multiplies what is there by a = 3.4, the rounding of X included, until after five steps it has grown 485 times:
-//              of an update of low rank X in one number left 2 % of noise, in two less than 0.1 %.  Products of hi alone cost next to
-//              nothing of that, since B is small along small singular values.
+//              of an update of low rank X in one number left 2 % of noise, in two 0.1 %.  Products of hi alone cost next to nothing of
+//              that, since B is small along small singular values.  lo is a byte, the residue times 32 in e4m3: its four bits behind hi's
+//              eleven are all that pays (sixteen of them left 0.1 % too), and X is most of what is moved.  X before the last step, whose
+//              rounding grows once, has none.
 //   float32 G: everything in two numbers and every product in three, hi hi + hi lo + lo hi: 22 bits, as accurate as float32 products.
 #include "rd_elem.h"
 #include "rd_gemm_w4.h"
@@ -52,51 +54,116 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_norm_kernel(const T* __re
   if (threadIdx.x == 0) partial[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
-__device__ __forceinline__ void split(float v, half_bits* hi, half_bits* lo) {
-  const f16_t h = (f16_t)v;
-  *hi = __builtin_bit_cast(half_bits, h);
-  *lo = __builtin_bit_cast(half_bits, (f16_t)(v - (float)h));
-}
 __device__ __forceinline__ float half_to_f32(half_bits b) { return (float)__builtin_bit_cast(f16_t, b); }
+// Eight numbers as hi, and what hi leaves: as float16 (TWO), or times 32 as e4m3 bytes.  Numbers stay below 2^15, so the residue below 8.
+constexpr float kByteUnit = 32.f;
+__device__ __forceinline__ u32x4_t high_of(const float (&v)[8], float (&rest)[8]) {
+  alignas(16) half_bits h[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const f16_t t = (f16_t)v[q];
+    h[q] = __builtin_bit_cast(half_bits, t);
+    rest[q] = v[q] - (float)t;
+  }
+  return *reinterpret_cast<const u32x4_t*>(h);
+}
+template <bool TWO>
+__device__ __forceinline__ void store_low(void* lo, long long cell, const float (&rest)[8]) {
+  if constexpr (TWO) {
+    float none[8];
+    *reinterpret_cast<u32x4_t*>(static_cast<half_bits*>(lo) + cell) = high_of(rest, none);
+  } else {
+    u32x2_t w;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int d = __builtin_amdgcn_cvt_pk_fp8_f32(rest[4 * h] * kByteUnit, rest[4 * h + 1] * kByteUnit, 0, false);
+      w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(rest[4 * h + 2] * kByteUnit, rest[4 * h + 3] * kByteUnit, d, true);
+    }
+    *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(lo) + cell) = w;
+  }
+}
+template <bool TWO> struct LowOf { typedef u32x2_t type; };
+template <> struct LowOf<true> { typedef u32x4_t type; };
+// v += hi + lo, times `by`
+__device__ __forceinline__ void add_high(float (&v)[8], u32x4_t hi, float by) {
+  alignas(16) half_bits h[8];
+  *reinterpret_cast<u32x4_t*>(h) = hi;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = __builtin_fmaf(half_to_f32(h[q]), by, v[q]);
+}
+__device__ __forceinline__ void add_low(float (&v)[8], u32x4_t lo, float by) { add_high(v, lo, by); }
+__device__ __forceinline__ void add_low(float (&v)[8], u32x2_t lo, float by) {
+  by *= 1 / kByteUnit;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo[h], true);
+    v[4 * h] = __builtin_fmaf(a[0], by, v[4 * h]); v[4 * h + 1] = __builtin_fmaf(a[1], by, v[4 * h + 1]);
+    v[4 * h + 2] = __builtin_fmaf(b[0], by, v[4 * h + 2]); v[4 * h + 3] = __builtin_fmaf(b[1], by, v[4 * h + 3]);
+  }
+}
+
+// The sum of a matrix's squares, by every wave for itself, in the same order.
+__device__ __forceinline__ double sum_of(const double* __restrict__ partial, int chunks) {
+  double sum = 0;
+  for (int i = threadIdx.x & 63; i < chunks; i += 64) sum += partial[i];
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  return sum;
+}
 
 // X = G / (norm + eps), 64 x 64 numbers of the padded X per work-group; `tall`: X is the transpose of G.
 template <class T>
 __global__ __launch_bounds__(kOrthoThreads) void ortho_start_kernel(const T* __restrict__ G, const double* __restrict__ partial, int chunks, half_bits* __restrict__ hi,
-                                                                    half_bits* __restrict__ lo, int k, int n, int rp, int cp, bool tall, double eps, float factor) {
+                                                                    void* __restrict__ lo, int k, int n, int rp, int cp, bool tall, double eps, float factor) {
   __shared__ float tile[64][65];
   const int across = cp / 64, down = rp / 64;
   const long long e = blockIdx.x / (across * down);
   const int in_matrix = (int)(blockIdx.x - e * across * down), r0 = in_matrix / across * 64, c0 = in_matrix % across * 64;
-  double sum = 0;
-  for (int i = 0; i < chunks; ++i) sum += partial[e * chunks + i];
-  const float by = (float)((double)factor / (sqrt(sum) + eps + (sum - sum)));  // (NaN for a sum that is no number)
   const T* g = G + e * k * n;
-  const int x = threadIdx.x & 63, y0 = threadIdx.x >> 6;
-  // read along the rows of G
-  const int gr = tall ? c0 : r0, gc = tall ? r0 : c0;
+  // eight neighbours of a row of G to a thread, twice
+  const int gr = tall ? c0 : r0, gc = tall ? r0 : c0, x = threadIdx.x % 8 * 8;
+  float v[2][8];
 #pragma unroll
-  for (int y = y0; y < 64; y += 4) {
-    const int r = gr + y, c = gc + x;
-    const float v = r < k && c < n ? to_f32<T>(g[(long long)r * n + c]) * by : 0.f;
-    if (tall) tile[x][y] = v; else tile[y][x] = v;
+  for (int h = 0; h < 2; ++h) {
+    const int r = gr + threadIdx.x / 8 + 32 * h, c = gc + x;
+    if (r < k && c + 8 <= n) {
+      alignas(16) T in[8];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(in) / 16; ++i) reinterpret_cast<u32x4_t*>(in)[i] = load_any<u32x4_t>(g + (long long)r * n + c + i * (16 / sizeof(T)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[h][i] = to_f32<T>(in[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[h][i] = r < k && c + i < n ? to_f32<T>(g[(long long)r * n + c + i]) : 0.f;
+    }
   }
+  const double sum = sum_of(partial + e * chunks, chunks);
+  const float by = (float)((double)factor / (sqrt(sum) + eps + (sum - sum)));  // (NaN for a sum that is no number)
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int y = threadIdx.x / 8 + 32 * h;
+      if (tall) tile[x + i][y] = v[h][i] * by; else tile[y][x + i] = v[h][i] * by;
+    }
   __syncthreads();
-  const long long base = e * rp * cp + (long long)r0 * cp + c0;
 #pragma unroll
   for (int i = threadIdx.x; i < 64 * 8; i += kOrthoThreads) {
     const int r = i / 8, c = i % 8 * 8;
-    alignas(16) half_bits h[8], l[8];
+    const long long cell = e * rp * cp + (long long)(r0 + r) * cp + c0 + c;
+    float w[8], rest[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) split(tile[r][c + j], &h[j], &l[j]);
-    *reinterpret_cast<u32x4_t*>(hi + base + (long long)r * cp + c) = *reinterpret_cast<const u32x4_t*>(h);
-    *reinterpret_cast<u32x4_t*>(lo + base + (long long)r * cp + c) = *reinterpret_cast<const u32x4_t*>(l);
+    for (int j = 0; j < 8; ++j) w[j] = tile[r][c + j];
+    *reinterpret_cast<u32x4_t*>(hi + cell) = high_of(w, rest);
+    if (lo) store_low<sizeof(T) == 4>(lo, cell, rest);
   }
 }
 
 // ---- products --------------------------------------------------------------------------------------------------------------
-// Two planes of padded matrices [rows][cols].
+// Two planes of padded matrices [rows][cols]; no lo: one.
 struct Planes {
-  half_bits *hi, *lo;
+  half_bits* hi;
+  void* lo;
   int rows, cols;
 };
 enum OrthoKind { kGram, kSquare, kApply, kLast };
@@ -179,8 +246,8 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
 #pragma unroll 1
   for (int term = 0; term < (PLANES == 2 ? 3 : 1); ++term) {
-    const half_bits* a = (term == 2 ? p.left.lo : p.left.hi) + left;
-    const half_bits* b = (term == 1 ? p.right.lo : p.right.hi) + right;
+    const half_bits* a = (term == 2 ? static_cast<const half_bits*>(p.left.lo) : p.left.hi) + left;
+    const half_bits* b = (term == 1 ? static_cast<const half_bits*>(p.right.lo) : p.right.hi) + right;
     if (live) w4_kloop<C, true>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
     else w4_kloop<C, false>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
   }
@@ -192,13 +259,15 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
   float* patch = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
   static_assert(C::NW * 32 * PITCH * 4 <= C::LDS_BYTES, "patches");
   constexpr int PER_ROW = C::WN / 8, STEP = 64 / PER_ROW, ITER = 32 / STEP;
-  constexpr bool ADDS = KIND != kGram, ADDS_LO = ADDS && (PLANES == 2 || KIND != kSquare);
+  constexpr bool TWO = PLANES == 2, ADDS = KIND != kGram, ADDS_LO = ADDS && (TWO || KIND == kApply);  // (X before the last step has no bytes)
+  typedef typename LowOf<TWO>::type Low;
   const bool turned = SYMMETRIC ? ti != tj : KIND == kLast && p.tall;
   const int own_r = lane / PER_ROW, own_c = lane % PER_ROW * 8, pc = c0 + wn * C::WN;
   const bool inside = pc + own_c < p.to.cols;
   const long long matrix = e * p.to.rows * p.to.cols, own = matrix + (long long)(r0 + wm * C::WM + own_r) * p.to.cols + pc + own_c;
   constexpr int AHEAD = SYMMETRIC ? 1 : 0;  // (the sums of the others leave no registers for two; the other work-group fills the wait)
-  u32x4_t add_hi[AHEAD + 1][ADDS ? ITER : 1], add_lo[AHEAD + 1][ADDS_LO ? ITER : 1];
+  u32x4_t add_hi[AHEAD + 1][ADDS ? ITER : 1];
+  Low add_lo[AHEAD + 1][ADDS_LO ? ITER : 1];
   auto request = [&](int i) {
     if constexpr (ADDS) {
       if (!inside || r0 + wm * C::WM + i * 32 >= p.left.rows) return;
@@ -206,7 +275,7 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
       for (int t = 0; t < ITER; ++t) {
         const long long cell = own + (long long)(i * 32 + t * STEP) * p.to.cols;
         add_hi[i & AHEAD][t] = *reinterpret_cast<const u32x4_t*>(p.add.hi + cell);
-        if constexpr (ADDS_LO) add_lo[i & AHEAD][t] = *reinterpret_cast<const u32x4_t*>(p.add.lo + cell);
+        if constexpr (ADDS_LO) add_lo[i & AHEAD][t] = *reinterpret_cast<const Low*>(static_cast<const char*>(p.add.lo) + cell * (int)(sizeof(Low) / 8));
       }
     }
   };
@@ -236,21 +305,16 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
           v[4 * q] = w[0] * p.of_product; v[4 * q + 1] = w[1] * p.of_product; v[4 * q + 2] = w[2] * p.of_product; v[4 * q + 3] = w[3] * p.of_product;
         }
         if constexpr (ADDS) {
-          alignas(16) half_bits h[8], l[8];
-          *reinterpret_cast<u32x4_t*>(h) = add_hi[i & AHEAD][t];
-          if constexpr (ADDS_LO) *reinterpret_cast<u32x4_t*>(l) = add_lo[i & AHEAD][t];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] = __builtin_fmaf(ADDS_LO ? half_to_f32(h[q]) + half_to_f32(l[q]) : half_to_f32(h[q]), p.of_add, v[q]);
+          add_high(v, add_hi[i & AHEAD][t], p.of_add);
+          if constexpr (ADDS_LO) add_low(v, add_lo[i & AHEAD][t], p.of_add);
         }
         if constexpr (KIND == kLast) {
           if (!p.tall) store_last(p, e, pr + t * STEP + own_r, pc + own_c, v);
         } else {
           const long long cell = own + (long long)(i * 32 + t * STEP) * p.to.cols;
-          alignas(16) half_bits h[8], l[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) split(v[q], &h[q], &l[q]);
-          *reinterpret_cast<u32x4_t*>(p.to.hi + cell) = *reinterpret_cast<const u32x4_t*>(h);
-          if (PLANES == 2 || KIND == kApply) *reinterpret_cast<u32x4_t*>(p.to.lo + cell) = *reinterpret_cast<const u32x4_t*>(l);
+          float rest[8];
+          *reinterpret_cast<u32x4_t*>(p.to.hi + cell) = high_of(v, rest);
+          if (TWO || (KIND == kApply && p.to.lo)) store_low<TWO>(p.to.lo, cell, rest);
         }
         if (turned) {
 #pragma unroll
@@ -271,11 +335,9 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
           store_last(p, e, pc + c, pr + r, v);
         } else {
           const long long cell = matrix + (long long)(pc + c) * p.to.cols + pr + r;
-          alignas(16) half_bits h[8], l[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) split(v[q], &h[q], &l[q]);
-          *reinterpret_cast<u32x4_t*>(p.to.hi + cell) = *reinterpret_cast<const u32x4_t*>(h);
-          if (PLANES == 2) *reinterpret_cast<u32x4_t*>(p.to.lo + cell) = *reinterpret_cast<const u32x4_t*>(l);
+          float rest[8];
+          *reinterpret_cast<u32x4_t*>(p.to.hi + cell) = high_of(v, rest);
+          if constexpr (TWO) store_low<TWO>(p.to.lo, cell, rest);
         }
       }
       __builtin_amdgcn_wave_barrier();
@@ -288,8 +350,7 @@ template <class T>
 __global__ __launch_bounds__(kOrthoThreads) void ortho_divide_kernel(const T* __restrict__ G, const double* __restrict__ partial, T* __restrict__ out, long long size,
                                                                      int chunks, double eps, double scale) {
   const long long e = blockIdx.x / chunks, first = (blockIdx.x - e * chunks) * (long long)kOrthoChunk;
-  double sum = 0;
-  for (int i = 0; i < chunks; ++i) sum += partial[e * chunks + i];
+  const double sum = sum_of(partial + e * chunks, chunks);
   const float by = (float)(scale / (sqrt(sum) + eps + (sum - sum)));
   for (long long i = first + threadIdx.x; i < size && i < first + kOrthoChunk; i += kOrthoThreads) out[e * size + i] = from_f32<T>(to_f32<T>(G[e * size + i]) * by);
 }
@@ -318,7 +379,7 @@ int launch_product(hipStream_t s, const OrthoStep& p, bool large, bool two) {
 
 struct OrthoSizes {
   int rp, cp, chunks;
-  size_t norm, x, square;  // bytes of the sums of squares, of one plane of X, and of one of A
+  size_t norm, x, bytes, square;  // bytes of the sums of squares, of one plane of X and one of its bytes, and of one of A
 };
 size_t up(size_t b) { return (b + 255) / 256 * 256; }
 OrthoSizes sizes_of(int g, int k, int n) {
@@ -329,6 +390,7 @@ OrthoSizes sizes_of(int g, int k, int n) {
   z.chunks = (int)(((long long)k * n + kOrthoChunk - 1) / kOrthoChunk);
   z.norm = up((size_t)g * z.chunks * sizeof(double));
   z.x = up((size_t)g * z.rp * z.cp * 2);
+  z.bytes = up((size_t)g * z.rp * z.cp);
   z.square = up((size_t)g * z.rp * z.rp * 2);
   return z;
 }
@@ -362,14 +424,13 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
   char* ws = static_cast<char*>(p.workspace);
   double* partial = reinterpret_cast<double*>(ws);
   ws += z.norm;
-  auto planes = [&](int rows, int cols, size_t bytes, bool lo) {
-    Planes q{reinterpret_cast<half_bits*>(ws), nullptr, rows, cols};
-    ws += bytes;
-    if (lo) { q.lo = reinterpret_cast<half_bits*>(ws); ws += bytes; }
+  auto planes = [&](int rows, int cols, size_t bytes, size_t lo) {
+    Planes q{reinterpret_cast<half_bits*>(ws), lo ? ws + bytes : nullptr, rows, cols};
+    ws += bytes + lo;
     return q;
   };
-  Planes X[2] = {planes(z.rp, z.cp, z.x, true), planes(z.rp, z.cp, z.x, true)};
-  const Planes A = planes(z.rp, z.rp, z.square, two), B = planes(z.rp, z.rp, z.square, two);
+  Planes X[2] = {planes(z.rp, z.cp, z.x, two ? z.x : z.bytes), planes(z.rp, z.cp, z.x, two ? z.x : z.bytes)};
+  const Planes A = planes(z.rp, z.rp, z.square, two ? z.square : 0), B = planes(z.rp, z.rp, z.square, two ? z.square : 0);
   const long long size = (long long)p.k * p.n;
   hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3((unsigned)(p.g * z.chunks)), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, size, z.chunks);
   int rc = (int)hipGetLastError();
@@ -380,7 +441,7 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
   }
   double bound = 1;
   int ex = exponent_for(bound);
-  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3((unsigned)(p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, z.chunks, X[0].hi, X[0].lo,
+  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3((unsigned)(p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, z.chunks, X[0].hi, two || p.steps > 1 ? X[0].lo : nullptr,
                      p.k, p.n, z.rp, z.cp, tall, p.eps, (float)ldexp(1.0, ex));
   if ((rc = (int)hipGetLastError()) != hipSuccess) return rc;
   const bool large = z.rp > 128;
@@ -404,6 +465,7 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
     t.left = B;
     t.right = t.add = X[i & 1];
     t.to = X[(i + 1) & 1];
+    if (!two && i + 2 == p.steps) t.to.lo = nullptr;
     t.of_product = last ? (float)ldexp(p.scale, -eb - ex) : (float)ldexp(1.0, en - eb - ex);
     t.of_add = last ? (float)ldexp(a * p.scale, -ex) : (float)ldexp(a, en - ex);
     t.out = p.out; t.k = p.k; t.n = p.n; t.elem = p.elem; t.tall = tall;
@@ -418,7 +480,7 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
 
 size_t ortho_workspace_bytes(int g, int k, int n, int elem) {
   const OrthoSizes z = sizes_of(g, k, n);
-  return z.norm + 4 * z.x + (elem == 1 ? 4 : 2) * z.square;
+  return z.norm + 2 * z.x + 2 * (elem == 1 ? z.x : z.bytes) + (elem == 1 ? 4 : 2) * z.square;
 }
 
 bool ortho_grid_fits(int g, int k, int n) {

@@ -332,7 +332,7 @@ int rd_gmm_float8(void* stream, const void* x, const float* x_scales, const void
  *   A = X X',  B = b A + c A A,  X = a X + B X        (on the transpose where k > n)
  * and out [g, k, n] = scale * X, of G's type.  With coefficients such as (3.4445, -4.7750, 2.0315), five times, the singular values
  * come out between 0.7 and 1.2, whatever they were from |G|_F / 500 on.  The norm is a 64-bit sum; sums of products are fp32.  For
- * 16-bit G products are of float16 numbers, with X held in 22 bits: results are off by 2e-3 of their norm (up to 8e-3
+ * 16-bit G products are of float16 numbers, with X held in 15 bits: results are off by 2e-3 of their norm (up to 8e-3
  * where there are few rows or columns, whose roundings do not average out).  For float32 every
  * product is of 22-bit numbers, as accurate as float32 products.  An infinity or NaN makes its matrix NaN; a matrix of zeros stays 0.
  * steps 0..32; coefficients: host, [steps][3], finite, such that no singular value from 0 to 1 is led beyond 1024; eps >= 0 and scale

@@ -27,30 +27,29 @@ def by_singular_values(G, coefficients, eps=1e-7):
 
 
 def rounded(G, coefficients, two, eps=1e-7, rng=None):
-    """The iteration with the roundings of the kernels' design and no others: X in two float16 numbers, hi + lo, A and B in one, products
-    of hi alone; with ``two`` all in two numbers and products hi hi + hi lo + lo hi.  Numbers are scaled so that float16's range plays
-    no part.  With ``rng`` every rounding is a random one of up to half a step instead."""
-    def split(x, planes):
-        if rng is not None:
-            fine = x * (1 + 2.0 ** -22 * rng.uniform(-1, 1, x.shape)) if planes else x
-            hi = fine * (1 + 2.0 ** -11 * rng.uniform(-1, 1, x.shape))
-            return (hi, fine - hi) if planes else (hi, 0 * hi)
-        top = np.abs(x).max()
-        unit = 2.0 ** (14 - np.frexp(top)[1]) if top else 1.0
-        hi = (x * unit).astype(np.float16).astype(np.float64)
-        lo = (x * unit - hi).astype(np.float16).astype(np.float64) if planes else 0 * hi
-        return hi / unit, lo / unit
+    """The iteration with the roundings of the kernels' design and no others: X in a float16 number and, but before the last step, the
+    next four bits of what that leaves, A and B in one float16 number, products of X's first number; with ``two`` all in two float16
+    numbers and products hi hi + hi lo + lo hi.  Numbers are scaled so that float16's range plays no part.  With ``rng`` every rounding is
+    a random one of up to half a step instead."""
+    def leading(x, bits):
+        unit = 2.0 ** (np.frexp(np.where(x == 0, 1.0, x))[1] - bits)
+        return x * (1 + 2.0 ** -bits * rng.uniform(-1, 1, x.shape)) if rng is not None else np.round(x / unit) * unit
+
+    def split(x, bits):
+        hi = leading(x, 11)
+        return hi, leading(x - hi, bits) if bits else 0 * hi
 
     def product(p, q):
         return p[0] @ q[0] + (p[0] @ q[1] + p[1] @ q[0] if two else 0)
 
     G = np.asarray(G, np.float64)
     X = G if G.shape[0] <= G.shape[1] else G.T
-    X = split(X / (np.sqrt((X * X).sum()) + eps), True)
+    X = split(X / (np.sqrt((X * X).sum()) + eps), 11 if two else 4 if len(coefficients) > 1 else 0)
     for i, (a, b, c) in enumerate(coefficients):
-        A = split(product(X, (X[0].T, X[1].T)), two)
-        B = split(b * (A[0] + A[1]) + c * product(A, A), two)
+        A = split(product(X, (X[0].T, X[1].T)), 11 if two else 0)
+        B = split(b * (A[0] + A[1]) + c * product(A, A), 11 if two else 0)
         Y = a * (X[0] + X[1]) + product(B, X)
-        X = split(Y, True) if i + 1 < len(coefficients) else (Y, 0 * Y)
+        left = len(coefficients) - 1 - i
+        X = split(Y, 11 if two else 4 if left > 1 else 0) if left else (Y, 0 * Y)
     X = X[0] + X[1]
     return X if G.shape[0] <= G.shape[1] else X.T
