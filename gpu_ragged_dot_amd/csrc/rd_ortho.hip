@@ -200,12 +200,71 @@ __device__ __forceinline__ void store_last(const OrthoStep& p, long long e, int 
 }
 
 // Tiles of the products.  Of the symmetric ones they are square; of the others, whose contraction is short and whose results are read and
-// written in two numbers, large ones are 128 x 256, two work-groups to a compute unit: one multiplies while the other stores.
+// written in two numbers, large ones are 128 x 256, two work-groups to a compute unit.
+template <bool SYMMETRIC>
+struct OrthoSmall {  // 64 x 64, a wave 32 x 32 of it, in slabs of 64
+  static constexpr bool HALF = true, SMALL = true;
+  static constexpr int BM = 64, BN = 64, BK = 64, STAGES = 5, NW = 4, WM = 32, WN = 32, TM = 1, TN = 1;
+  static constexpr int A_BYTES = BM * BK * 2, STAGE_BYTES = 2 * A_BYTES, LDS_BYTES = STAGES * STAGE_BYTES;
+  typedef DldsLoader<BM, BK, NW, true> LdA;
+  typedef DldsLoader<BN, BK, NW, SYMMETRIC> LdB;
+  typedef DldsFragReader<BM, BK, TM, true> FragA;
+  typedef DldsFragReader<BN, BK, TN, SYMMETRIC> FragB;
+};
 template <int BM, bool SYMMETRIC>
 struct OrthoTile {
   static constexpr int ROWS = !SYMMETRIC && BM == 256 ? 128 : BM, GROUPS = ROWS == 256 ? 1 : 2;
   typedef W4Cfg<ROWS, BM, true, SYMMETRIC, ROWS == 256 ? 5 : BM == 256 ? 3 : 4, true> C;
 };
+template <bool SYMMETRIC>
+struct OrthoTile<64, SYMMETRIC> {
+  static constexpr int GROUPS = 2;
+  typedef OrthoSmall<SYMMETRIC> C;
+};
+
+// The small tile's K loop: what bounds it is how long the first slabs are on their way, so up to four are, and little else.
+template <class C>
+__device__ __forceinline__ void small_kloop(const half_bits* a, int lda, int rows, const half_bits* b, int ldb, int cols, int klen, unsigned char* smem, int wave, int lane,
+                                            f32x16_t (&acc)[1][1]) {
+  typename C::LdA la;
+  typename C::LdB lb;
+  la.init(a, lda, rows, klen, wave, lane);
+  lb.init(b, ldb, cols, klen, wave, lane);
+  typename C::FragA fra;
+  typename C::FragB frb;
+  fra.init((wave >> 1) * C::WM, lane);
+  frb.init((wave & 1) * C::WN, lane);
+  const int nk = klen / C::BK;  // (padded matrices)
+  constexpr int L = C::LdA::PER + C::LdB::PER;
+  auto issue = [&](int step) {
+    unsigned char* st = smem + (step % C::STAGES) * C::STAGE_BYTES;
+    __amdgpu_buffer_rsrc_t ra = la.resource(), rb = lb.resource();
+#pragma unroll
+    for (int q = 0; q < C::LdA::PER; ++q) la.template issue<false>(ra, st, wave, q, 0, 0);
+#pragma unroll
+    for (int q = 0; q < C::LdB::PER; ++q) lb.template issue<false>(rb, st + C::A_BYTES, wave, q, 0, 0);
+    la.advance();
+    lb.advance();
+  };
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s)
+    if (s < nk) issue(s);
+  for (int kt = 0; kt < nk; ++kt) {
+    if (kt + C::STAGES - 2 < nk) wait_vmcnt<(C::STAGES - 2) * L>(); else wait_vmcnt<0>();
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();  // slab kt is in LDS, and slab kt - 1 is no longer being read
+    __builtin_amdgcn_sched_barrier(0);
+    if (kt + C::STAGES - 1 < nk) issue(kt + C::STAGES - 1);
+    const unsigned char* st = smem + (kt % C::STAGES) * C::STAGE_BYTES;
+#pragma unroll
+    for (int ks = 0; ks < C::BK / 16; ++ks) acc[0][0] = mfma_32x32x16<true>(frb.read(st + C::A_BYTES, 0, ks), fra.read(st, 0, ks), acc[0][0]);
+  }
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();  // the ring is no longer read by any wave
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 template <int BM, bool SYMMETRIC>
 constexpr int ortho_groups = OrthoTile<BM, SYMMETRIC>::GROUPS;
@@ -248,7 +307,8 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
   for (int term = 0; term < (PLANES == 2 ? 3 : 1); ++term) {
     const half_bits* a = (term == 2 ? static_cast<const half_bits*>(p.left.lo) : p.left.hi) + left;
     const half_bits* b = (term == 1 ? static_cast<const half_bits*>(p.right.lo) : p.right.hi) + right;
-    if (live) w4_kloop<C, true>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
+    if constexpr (BM == 64) small_kloop<C>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
+    else if (live) w4_kloop<C, true>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
     else w4_kloop<C, false>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
   }
   if (!live) return;
@@ -355,6 +415,22 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_divide_kernel(const T* __
   for (long long i = first + threadIdx.x; i < size && i < first + kOrthoChunk; i += kOrthoThreads) out[e * size + i] = from_f32<T>(to_f32<T>(G[e * size + i]) * by);
 }
 
+// Which tiles: the least time by rounds of what the device holds, 256 compute units of one or two work-groups, in tiles of 128 x 128.  As
+// measured, a unit takes 1.35 times as long per number in tiles of 128 x 128, whose operands' reads of LDS bound it, 1.2 times in those of
+// 128 x 256, 1.9 times in those of 64 x 64, and a work-group alone on it 0.7 times as long as two.  us, all products in tiles of 64 | 128 | 256, bf16: 4 of 256 x 512 83 | 127 | 213; 1 of 768 x 768 141 | 191 | 361; 1
+// of 2048 x 2048 500 | 343 | 634; 16 of 768 x 2048 817 | 583 | 653; 12 of 1515 x 1001 872 | 595 | 656; 1 of 4096 x 4096 3266 | 1948 |
+// 1503; 128 of 768 x 2048 7704 | 4963 | 4216.
+int tile_for(bool symmetric, int g, int rows, int cols) {
+  const auto time = [&](int r, int c, int groups, double slow) {
+    const long long down = (rows + r - 1) / r, across = (cols + c - 1) / c, tiles = g * (symmetric ? down * (down + 1) / 2 : down * across);
+    const double each = slow * r * c / (128.0 * 128.0);
+    const int rest = (int)(tiles % (256 * groups));
+    return (tiles / (256 * groups) * groups + (rest == 0 ? 0 : groups == 1 ? 1 : rest <= 256 ? 1.4 : 2)) * each;
+  };
+  const double large = symmetric ? time(256, 256, 1, 1) : time(128, 256, 2, 1.2), middle = time(128, 128, 2, 1.35), small = time(64, 64, 2, 1.9);
+  return large <= middle && large <= small ? 256 : middle <= small ? 128 : 64;
+}
+
 template <int BM, int KIND, int PLANES>
 int launch_product(hipStream_t s, OrthoStep p) {
   constexpr bool SYMMETRIC = KIND == kGram || KIND == kSquare;
@@ -372,9 +448,12 @@ int launch_product(hipStream_t s, OrthoStep p) {
   return (int)hipGetLastError();
 }
 template <int KIND>
-int launch_product(hipStream_t s, const OrthoStep& p, bool large, bool two) {
-  if (large) return two ? launch_product<256, KIND, 2>(s, p) : launch_product<256, KIND, 1>(s, p);
-  return two ? launch_product<128, KIND, 2>(s, p) : launch_product<128, KIND, 1>(s, p);
+int launch_product(hipStream_t s, const OrthoStep& p, bool two) {
+  switch (tile_for(KIND == kGram || KIND == kSquare, p.g, p.left.rows, p.right.cols)) {
+    case 256: return two ? launch_product<256, KIND, 2>(s, p) : launch_product<256, KIND, 1>(s, p);
+    case 128: return two ? launch_product<128, KIND, 2>(s, p) : launch_product<128, KIND, 1>(s, p);
+    default: return two ? launch_product<64, KIND, 2>(s, p) : launch_product<64, KIND, 1>(s, p);
+  }
 }
 
 struct OrthoSizes {
@@ -444,7 +523,6 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
   hipLaunchKernelGGL((ortho_start_kernel<T>), dim3((unsigned)(p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, z.chunks, X[0].hi, two || p.steps > 1 ? X[0].lo : nullptr,
                      p.k, p.n, z.rp, z.cp, tall, p.eps, (float)ldexp(1.0, ex));
   if ((rc = (int)hipGetLastError()) != hipSuccess) return rc;
-  const bool large = z.rp > 128;
   for (int i = 0; i < p.steps; ++i) {
     const double a = p.coefficients[3 * i], b = p.coefficients[3 * i + 1], c = p.coefficients[3 * i + 2];
     const int ea = exponent_for(bound * bound), eb = exponent_for(largest_square(bound * bound, b, c));
@@ -453,12 +531,12 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
     t.left = t.right = X[i & 1];
     t.to = A;
     t.of_product = (float)ldexp(1.0, ea - 2 * ex);
-    if ((rc = launch_product<kGram>(s, t, large, two)) != hipSuccess) return rc;
+    if ((rc = launch_product<kGram>(s, t, two)) != hipSuccess) return rc;
     t.left = t.right = t.add = A;
     t.to = B;
     t.of_product = (float)ldexp(c, eb - 2 * ea);
     t.of_add = (float)ldexp(b, eb - ea);
-    if ((rc = launch_product<kSquare>(s, t, large, two)) != hipSuccess) return rc;
+    if ((rc = launch_product<kSquare>(s, t, two)) != hipSuccess) return rc;
     const bool last = i + 1 == p.steps;
     const double next = largest(bound, a, b, c);
     const int en = exponent_for(next);
@@ -469,7 +547,7 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
     t.of_product = last ? (float)ldexp(p.scale, -eb - ex) : (float)ldexp(1.0, en - eb - ex);
     t.of_add = last ? (float)ldexp(a * p.scale, -ex) : (float)ldexp(a, en - ex);
     t.out = p.out; t.k = p.k; t.n = p.n; t.elem = p.elem; t.tall = tall;
-    if ((rc = last ? launch_product<kLast>(s, t, large, two) : launch_product<kApply>(s, t, large, two)) != hipSuccess) return rc;
+    if ((rc = last ? launch_product<kLast>(s, t, two) : launch_product<kApply>(s, t, two)) != hipSuccess) return rc;
     bound = next;
     ex = en;
   }
