@@ -417,7 +417,7 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_divide_kernel(const T* __
 
 // Which tiles: the least time by rounds of what the device holds, 256 compute units of one or two work-groups, in tiles of 128 x 128.  As
 // measured, a unit takes 1.35 times as long per number in tiles of 128 x 128, whose operands' reads of LDS bound it, 1.2 times in those of
-// 128 x 256, 1.9 times in those of 64 x 64, and a work-group alone on it 0.7 times as long as two.  us, all products in tiles of 64 | 128 | 256, bf16: 4 of 256 x 512 83 | 127 | 213; 1 of 768 x 768 141 | 191 | 361; 1
+// 128 x 256, 2.3 times in those of 64 x 64, and a work-group alone on it 0.7 times as long as two.  us, all products in tiles of 64 | 128 | 256, bf16: 4 of 256 x 512 83 | 127 | 213; 1 of 768 x 768 141 | 191 | 361; 1
 // of 2048 x 2048 500 | 343 | 634; 16 of 768 x 2048 817 | 583 | 653; 12 of 1515 x 1001 872 | 595 | 656; 1 of 4096 x 4096 3266 | 1948 |
 // 1503; 128 of 768 x 2048 7704 | 4963 | 4216.
 int tile_for(bool symmetric, int g, int rows, int cols) {
@@ -427,7 +427,7 @@ int tile_for(bool symmetric, int g, int rows, int cols) {
     const int rest = (int)(tiles % (256 * groups));
     return (tiles / (256 * groups) * groups + (rest == 0 ? 0 : groups == 1 ? 1 : rest <= 256 ? 1.4 : 2)) * each;
   };
-  const double large = symmetric ? time(256, 256, 1, 1) : time(128, 256, 2, 1.2), middle = time(128, 128, 2, 1.35), small = time(64, 64, 2, 1.9);
+  const double large = symmetric ? time(256, 256, 1, 1) : time(128, 256, 2, 1.2), middle = time(128, 128, 2, 1.35), small = time(64, 64, 2, 2.3);
   return large <= middle && large <= small ? 256 : middle <= small ? 128 : 64;
 }
 
