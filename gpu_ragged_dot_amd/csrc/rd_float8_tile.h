@@ -29,7 +29,7 @@ struct F8Loader {
   static_assert(ROWS % (RPI * NW) == 0 && PER >= 1, "slab does not split evenly over the waves");
   static __host__ __device__ constexpr int swizzle(int r) { return KMAJOR ? (r >> 1) & 7 : CPR >= 16 ? (r & 7) << 1 : CPR == 8 ? r & 7 : (r >> 1) & 3; }
   const uint8_t* base;
-  int records, step;  // bytes still addressable from base, and from one slab to the next
+  int records, step;  // bytes of the tile's window, and from one slab to the next
   int voff[PER];
   // lim: live rows (K-major) or columns in memory (MN-major, a multiple of 16); `blocks` slabs
   __host__ __device__ __forceinline__ void init(const uint8_t* p, int ld, int lim, int blocks, int wave, int lane) {
@@ -42,12 +42,13 @@ struct F8Loader {
       voff[j] = (KMAJOR ? r < lim : c * 16 < lim) ? r * ld + c * 16 : kOobOffset;
     }
   }
-  __device__ __forceinline__ void issue(unsigned char* lds, int wave) {
+  // Loads first, first + by, .. of a wave for slab `at`.
+  __device__ __forceinline__ void issue(unsigned char* lds, int wave, int at, int first = 0, int by = 1) const {
     __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, __builtin_amdgcn_readfirstlane(records), kBufferFlags);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_ptr)(lds + (wave + NW * j) * 1024), 16, voff[j], 0, 0, 0);
+    for (int j = 0; j < PER; ++j)
+      if (j % by == first) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_ptr)(lds + (wave + NW * j) * 1024), 16, voff[j], __builtin_amdgcn_readfirstlane(at * step), 0, 0);
   }
-  __host__ __device__ __forceinline__ void advance() { base += step; records -= step; }
 };
 
 // Fragments of v_mfma_f32_16x16x128_f8f6f4: lane l feeds row / column (l & 15) and the 32 contraction bytes 32 (l >> 4) .. + 31.
@@ -156,9 +157,6 @@ __device__ __forceinline__ void float8_store(const f32x4_t (&acc)[C::TM][C::TN],
   }
 }
 
-#ifndef V_FIRST
-#define V_FIRST 2
-#endif
 // What the K loops share: a wave's part of a tile and its operands' ways to LDS and out of it.
 template <class C>
 struct F8Wave {
@@ -189,16 +187,21 @@ struct F8Wave {
     scale_at = (wm * C::WM + (lane & 15)) * 16;
     col_scale = (const __attribute__((address_space(4))) float*)(live ? t.b_scales + (wn * C::WN / kF8Block) * t.b_column : t.b_scales);
   }
-  // The wave's share of slab `step`, and of the rows' scales of four blocks beside the first of them: 16 bytes a lane, 64 rows a wave.
-  __device__ __forceinline__ void issue(int step) {
-    unsigned char* st = smem + (step % C::STAGES) * C::STAGE_BYTES;
+  // The wave's share of slab `step`: of B, with the rows' scales of four blocks beside the first of them (16 bytes a lane, 64 rows a
+  // wave), and of A, HALF 0 or 1 of its loads, or (2) all.
+  __device__ __forceinline__ void issue_b(int step) const {
     if ((step & 3) == 0 && wave < (C::BM + 63) / 64)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(scale_rsrc, (lds_void_ptr)(smem + C::RING_BYTES + ((step >> 2) & 1) * C::SCALE_BYTES + wave * 1024), 16,
                                                scale_off >= 0 ? scale_off + step * 4 : kOobOffset, 0, 0, 0);
-    la.issue(st, wave);
-    lb.issue(st + C::A_BYTES, wave);
-    la.advance();
-    lb.advance();
+    lb.issue(smem + (step % C::STAGES) * C::STAGE_BYTES + C::A_BYTES, wave, step);
+  }
+  template <int HALF>
+  __device__ __forceinline__ void issue_a(int step) const {
+    la.issue(smem + (step % C::STAGES) * C::STAGE_BYTES, wave, step, HALF == 2 ? 0 : HALF, HALF == 2 ? 1 : 2);
+  }
+  __device__ __forceinline__ void issue(int step) const {
+    issue_b(step);
+    issue_a<2>(step);
   }
   __device__ __forceinline__ const unsigned char* slab(int step) const { return smem + (step % C::STAGES) * C::STAGE_BYTES; }
   // A lane's scale of its row in each of four pieces of sixteen rows, 4 h .. 4 h + 3 of the wave's, times w.  A lane reads that of one of the
@@ -261,25 +264,29 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, int b_block, 
 }
 
 // Two groups of four waves, one of each per SIMD, half a period apart: while one reads the fragments of half of its rows (memory phase),
-// the other multiplies (compute phase); a barrier ends every phase, four phases a slab.  In phases, group 0 reads slab t in 4 t and
-// 4 t + 2 and multiplies in 4 t + 1 and 4 t + 3, group 1 a phase later.  Slab t - 1 was read last in phase 4 t - 1, so both groups
-// request slab t + 1 in phase 4 t, group 1 amid its multiplications, and wait for it in phase 4 t + 3: nearly a slab's time on its way.
+// the other multiplies (compute phase); a barrier ends every phase, four phases a slab.  In phases, group 0 reads slab t in 4 t (the
+// weights' fragments, and the first half of its rows, the rest of it while it multiplies) and 4 t + 2 and multiplies in 4 t + 1 and 4 t +
+// 3, group 1 a phase later.  Loads are requested in memory phases, in one order, once both groups have read what they replace: the weights of slab t + 2 from phase 4 t + 2 on, the rows' first halves from 4 t
+// + 3, their second halves from 4 t + 4 on.  Of group 0 those are 4 t + 2, 4 t + 4 and 4 t + 4, of group 1 4 t + 3, 4 t + 3 and 4 t + 5;
+// the first two are wanted from phase 4 t + 8 on and the last from 4 t + 10.  A wave waits for its own at the ends of phases 4 t + 1
+// (second halves of slab t) and 4 t + 3 (the rest of slab t + 1), with eight loads on their way behind them, group 0 six in the latter.
+// 8192 x 7168 x 2048 in 32 groups, trans_rhs: 208 us, with all loads requested in phase 4 t and awaited in 4 t + 3 225.
+//
+// What bounds it: the longest of the phases that read.  16384 x 4096 x 14336 in 8 groups takes 950 us with trans_rhs (2.0 PFLOP/s) and
+// 1030 without; without its multiply-adds 8 % less, without its loads 15 %, without its reads of LDS 5 to 20 %, at any number of loads in
+// flight the same.  The same product without scales, whose sums stay where the matrix cores keep them: 840 and 785.
 // Inner sums enter the accumulators four instructions later, those of a phase's last row piece at the start of the next compute phase.
 template <class C>
 __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int b_block, f32x4_t (&acc)[C::TM][C::TN]) {
-  static_assert(C::NW == 8 && C::WAVES_M == 2 && C::STAGES == 2 && C::TM == 8, "two groups of four waves, four row pieces a phase");
+  static_assert(C::NW == 8 && C::WAVES_M == 2 && C::STAGES == 2 && C::TM == 8 && C::LdA::PER == 4 && C::LdB::PER == 4,
+                "two groups of four waves, four row pieces a phase; loads 0 and 2 of A hold the waves' first 64 rows");
+  constexpr int FIRST = 2;  // row pieces read before a slab's first compute phase
   const int group = u.wave >> 2;
   i32x8_t fa[4], fb[C::TN];
   float factor[4], carried = 0.f;
   f32x4_t part[2][C::TN];
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) part[1][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  constexpr int L = C::LdA::PER + C::LdB::PER;
-
-  u.issue(0);
-  if (nk > 1) { u.issue(1); wait_vmcnt<L>(); } else wait_vmcnt<0>();
-  phase_barrier();
-  if (group == 1) phase_barrier();
 
   auto read = [&](int kt, auto half, float w) {
     constexpr int H = decltype(half)::value;
@@ -289,14 +296,14 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int 
       for (int j = 0; j < C::TN; ++j) fb[j] = u.frb.read(ra + C::A_BYTES, j);
     }
 #pragma unroll
-    for (int i = 0; i < (H == 0 ? V_FIRST : 4); ++i) fa[i] = u.fra.read(ra, 4 * H + i);
+    for (int i = 0; i < (H == 0 ? FIRST : 4); ++i) fa[i] = u.fra.read(ra, 4 * H + i);
     u.factors(kt, H, w, factor);
   };
   auto multiply = [&](int kt, auto half) {
     constexpr int H = decltype(half)::value;
     if constexpr (H == 0) {
 #pragma unroll
-      for (int i = V_FIRST; i < 4; ++i) fa[i] = u.fra.read(u.slab(kt), i);
+      for (int i = FIRST; i < 4; ++i) fa[i] = u.fra.read(u.slab(kt), i);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -304,34 +311,51 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int 
       for (int j = 0; j < C::TN; ++j) {
         part[i & 1][j] = float8_part(fb[j], fa[i]);
         float8_add(acc[(4 * H + i + 7) & 7][j], part[(i + 1) & 1][j], i == 0 ? carried : factor[i == 0 ? 0 : i - 1]);
-#ifndef V_NOSB
         __builtin_amdgcn_sched_barrier(0);
-#endif
       }
     }
     carried = factor[3];
   };
+  auto wait = [&](bool steady) { if (steady) wait_vmcnt<8>(); else wait_vmcnt<0>(); };
+
+  u.issue_b(0);
+  u.template issue_a<0>(0);
+  u.template issue_a<1>(0);
+  if (nk > 1) u.issue_b(1);
+  if (group == 1 && nk > 1) u.template issue_a<0>(1);
+  if (nk > 1) wait_vmcnt<6>(); else wait_vmcnt<0>();  // (group 1 waits for two loads more than it has to)
+  phase_barrier();
+  if (group == 1) phase_barrier();
   typedef std::integral_constant<int, 0> First;
   typedef std::integral_constant<int, 1> Second;
   for (int kt = 0; kt < nk; ++kt) {
+    const bool next = kt + 1 < nk, after = kt + 2 < nk;
     const float w = u.live ? u.col_scale[(long long)kt * b_block] : 0.f;
     if (u.live) read(kt, First(), w);
-    if (group == 0 && kt > 0 && kt + 1 < nk) u.issue(kt + 1);
+    if (next) {
+      if (group == 0) u.template issue_a<0>(kt + 1);
+      u.template issue_a<1>(kt + 1);
+    }
+    if (group == 1) wait(next);
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     phase_barrier();
     __builtin_amdgcn_s_setprio(1);
     if (u.live) multiply(kt, First());
     __builtin_amdgcn_s_setprio(0);
+    if (group == 0) wait(next);
     phase_barrier();
     if (u.live) read(kt, Second(), w);
-    if (group == 1) wait_vmcnt<0>();
+    if (after) {
+      u.issue_b(kt + 2);
+      if (group == 1) u.template issue_a<0>(kt + 2);
+    }
+    if (group == 1) wait(after);
     __builtin_amdgcn_s_waitcnt(0xc07f);
     phase_barrier();
-    if (group == 1 && kt + 2 < nk) u.issue(kt + 2);
     __builtin_amdgcn_s_setprio(1);
     if (u.live) multiply(kt, Second());
     __builtin_amdgcn_s_setprio(0);
-    if (group == 0) wait_vmcnt<0>();
+    if (group == 0) { if (after) wait_vmcnt<6>(); else wait_vmcnt<0>(); }
     phase_barrier();
   }
   if (group == 0) phase_barrier();
