@@ -118,6 +118,14 @@ EXPORTS = (
     "rd_int4_pack",
     "rd_gmm_int4_workspace_bytes",
     "rd_gmm_int4",
+    "rd_float8_rows",
+    "rd_float8_weights",
+    "rd_float8_values",
+    "rd_moe_dispatch_float8",
+    "rd_moe_swiglu_float8",
+    "rd_gmm_float8",
+    "rd_orthogonalize_workspace_bytes",
+    "rd_orthogonalize",
 )
 
 
