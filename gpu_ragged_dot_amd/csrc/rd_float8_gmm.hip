@@ -3,15 +3,14 @@
 #include "rd_float8_tile.h"
 #include "rd_int4_rows.h"
 
+#include <math.h>
+
 namespace rd {
 
 namespace {
 
 constexpr int kF8ZeroRows = 64;  // rows that a work-group looks after which multiplies nothing
-#ifndef V_BAND
-#define V_BAND 8
-#endif
-constexpr int kF8Band = V_BAND;       // row tiles of a band of the walk
+constexpr int kF8Band = 8;       // row tiles of a band of the walk
 
 constexpr int larger(int a, int b) { return a > b ? a : b; }
 
@@ -27,6 +26,19 @@ struct F8Tall {
     if (t.rows <= 64) float8_tile<C64>(t, y, ldy, elem, smem);
     else if (t.rows <= 128) float8_tile<C128>(t, y, ldy, elem, smem);
     else float8_tile<C256>(t, y, ldy, elem, smem);
+  }
+};
+template <bool B_KMAJOR>
+struct F8Middle {
+  static constexpr int BM = 128, BN = 128, NT = 256, WAVES = 2;
+  typedef F8TileCfg<128, 128, 2, 2, 2, B_KMAJOR> C128;
+  typedef F8TileCfg<64, 128, 1, 4, 3, B_KMAJOR> C64;
+  typedef F8TileCfg<32, 128, 1, 4, 3, B_KMAJOR> C32;
+  static constexpr int LDS_BYTES = larger(C128::LDS_BYTES, larger(C64::LDS_BYTES, C32::LDS_BYTES));
+  static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
+    if (t.rows <= 32) float8_tile<C32>(t, y, ldy, elem, smem);
+    else if (t.rows <= 64) float8_tile<C64>(t, y, ldy, elem, smem);
+    else float8_tile<C128>(t, y, ldy, elem, smem);
   }
 };
 template <bool B_KMAJOR>
@@ -88,30 +100,46 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void gmm_float8_kernel(F8Problem p
   S::run(t, static_cast<char*>(p.y) + ((size_t)tile.first * p.n + c0) * size, p.n, p.elem, smem);
 }
 
-// A mean of at most 64 rows to a group: tiles of 64 rows, two work-groups to a compute unit.
-bool few_rows(const F8Problem& p) { return p.m <= 64ll * p.g; }
+// Which tiles, by rounds of what the device holds, if the rows are spread evenly and each of several groups has half a tile over: 256 tiles of
+// 256 x 256 take 1 (of at most 128 rows 0.65), 512 of 128 x 128, two to a compute unit, 0.75, and 512 of 64 x 128 0.5; half a round of
+// those 0.6 of it.  Groups of 32 rows and less have the least tiles, which run on 32 rows.
+//
+// us of 64 | 128 | 256 rows, trans_rhs: 8 groups of 128 x 2048 x 2048 16 | 18 | 33; of 256 rows 27 | 22 | 34; of 512 38 | 36 | 36; of
+// 1024 64 | 54 | 68; 1 of 500 x 4096 x 4096 22 | 29 | 60; 128 of 64 x 2048 x 768 44 | 42 | 47; 32 of 256 x 1024 x 1024 26 | 22 | 23; 32
+// of 128 x 7168 x 2048 159 | 155 | 119; 8 of 256 x 4096 x 14336 233 | 207 | 197; 4 of 1024 x 4096 x 4096 117 | 97 | 120.
+int height_for(const F8Problem& p) {
+  const double rows = (double)p.m / p.g;
+  if (rows <= 32) return 64;
+  const auto time = [&](int h, int bn, int held, double round) {
+    const double per_group = p.g == 1 ? ceil(rows / h) : rows / h + 0.5, tiles = p.g_local * (per_group > 1 ? per_group : 1) * ((p.n + bn - 1) / bn);
+    const double whole = floor(tiles / held), rest = tiles - whole * held;
+    return round * (whole + (rest <= 0 ? 0 : rest <= 256 && held > 256 ? 0.6 : 1));
+  };
+  const double tall = time(256, 256, 256, rows <= 128 ? 0.65 : 1), middle = time(128, 128, 512, 0.75), few = time(64, 128, 512, 0.5);
+  return tall <= middle && tall <= few ? 256 : middle <= few ? 128 : 64;
+}
 
 struct F8Grid {
-  int col_tiles;
+  int height, col_tiles;
   long long whole, all;
 };
 F8Grid grid_of(const F8Problem& p) {
-  const int bm = few_rows(p) ? 64 : 256, bn = few_rows(p) ? 128 : 256;
   F8Grid g;
+  g.height = height_for(p);
+  const int bn = g.height == 256 ? 256 : 128;
   g.col_tiles = (p.n + bn - 1) / bn;
-  g.whole = ((p.m / bm + imin(p.g_local, p.m)) * (long long)g.col_tiles + 7) / 8 * 8;
+  g.whole = ((p.m / g.height + imin(p.g_local, p.m)) * (long long)g.col_tiles + 7) / 8 * 8;
   g.all = g.whole + (p.m + kF8ZeroRows - 1) / kF8ZeroRows;
   return g;
 }
 
 template <template <bool> class S, bool B_KMAJOR>
-int launch_t(hipStream_t s, const F8Problem& p) {
+int launch_t(hipStream_t s, const F8Problem& p, const F8Grid& g) {
   auto kern = gmm_float8_kernel<S<B_KMAJOR>, B_KMAJOR>;
   if (S<B_KMAJOR>::LDS_BYTES > 64 * 1024) {
     const int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, S<B_KMAJOR>::LDS_BYTES);
     if (rc != hipSuccess) return rc;
   }
-  const F8Grid g = grid_of(p);
   hipLaunchKernelGGL(kern, dim3((unsigned)g.all), dim3(S<B_KMAJOR>::NT), S<B_KMAJOR>::LDS_BYTES, s, p, g.col_tiles, (int)g.whole);
   return (int)hipGetLastError();
 }
@@ -121,8 +149,10 @@ int launch_t(hipStream_t s, const F8Problem& p) {
 bool float8_grid_fits(const F8Problem& p) { return grid_of(p).all < (1ll << 31) / 512; }
 
 int launch_gmm_float8(hipStream_t s, const F8Problem& p) {
-  if (few_rows(p)) return p.trans_rhs ? launch_t<F8Few, true>(s, p) : launch_t<F8Few, false>(s, p);
-  return p.trans_rhs ? launch_t<F8Tall, true>(s, p) : launch_t<F8Tall, false>(s, p);
+  const F8Grid g = grid_of(p);
+  if (g.height == 64) return p.trans_rhs ? launch_t<F8Few, true>(s, p, g) : launch_t<F8Few, false>(s, p, g);
+  if (g.height == 128) return p.trans_rhs ? launch_t<F8Middle, true>(s, p, g) : launch_t<F8Middle, false>(s, p, g);
+  return p.trans_rhs ? launch_t<F8Tall, true>(s, p, g) : launch_t<F8Tall, false>(s, p, g);
 }
 
 }  // namespace rd

@@ -93,9 +93,10 @@ struct F8TileCfg {
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 16, TN = WN / 16;
   static constexpr int A_BYTES = BM * kF8Block, B_BYTES = BN * kF8Block, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int SCALE_BYTES = (BM + 63) / 64 * 1024;  // a row's scales of four blocks, as a wave loads them
+  static constexpr int SCALE_SETS = (STAGES + 2) / 4 + 1;  // of four blocks: that of slab kt + STAGES - 1 is not the one that slab kt reads
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int EPI_PITCH = WN * 4 + 16, EPI_BYTES = NW * 16 * EPI_PITCH;
-  static constexpr int USED_BYTES = RING_BYTES + 2 * SCALE_BYTES;
+  static constexpr int USED_BYTES = RING_BYTES + SCALE_SETS * SCALE_BYTES;
   static constexpr int LDS_BYTES = USED_BYTES > EPI_BYTES ? USED_BYTES : EPI_BYTES;
   typedef F8Loader<BM, NW, true> LdA;
   typedef F8Loader<BN, NW, B_KMAJOR> LdB;
@@ -191,7 +192,7 @@ struct F8Wave {
   // wave), and of A, HALF 0 or 1 of its loads, or (2) all.
   __device__ __forceinline__ void issue_b(int step) const {
     if ((step & 3) == 0 && wave < (C::BM + 63) / 64)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(scale_rsrc, (lds_void_ptr)(smem + C::RING_BYTES + ((step >> 2) & 1) * C::SCALE_BYTES + wave * 1024), 16,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(scale_rsrc, (lds_void_ptr)(smem + C::RING_BYTES + (step >> 2) % C::SCALE_SETS * C::SCALE_BYTES + wave * 1024), 16,
                                                scale_off >= 0 ? scale_off + step * 4 : kOobOffset, 0, 0, 0);
     lb.issue(smem + (step % C::STAGES) * C::STAGE_BYTES + C::A_BYTES, wave, step);
   }
@@ -207,7 +208,7 @@ struct F8Wave {
   // A lane's scale of its row in each of four pieces of sixteen rows, 4 h .. 4 h + 3 of the wave's, times w.  A lane reads that of one of the
   // 64 rows, and halves and quarters of the wave trade theirs (four reads of LDS take as long as two of a fragment).
   __device__ __forceinline__ void factors(int step, int h, float w, float (&factor)[4]) const {
-    const unsigned char* at = smem + C::RING_BYTES + ((step >> 2) & 1) * C::SCALE_BYTES + (step & 3) * 4;
+    const unsigned char* at = smem + C::RING_BYTES + (step >> 2) % C::SCALE_SETS * C::SCALE_BYTES + (step & 3) * 4;
     const uint32_t s = __builtin_bit_cast(uint32_t, *reinterpret_cast<const float*>(at + (wm * C::WM + 64 * h + lane) * 16) * w);
     const auto half = __builtin_amdgcn_permlane32_swap(s, s, false, false);
     const auto low = __builtin_amdgcn_permlane16_swap(half[0], half[0], false, false), high = __builtin_amdgcn_permlane16_swap(half[1], half[1], false, false);
@@ -216,7 +217,7 @@ struct F8Wave {
     for (int i = 0; i < 4; ++i) factor[i] = __builtin_bit_cast(float, got[i]);
   }
   __device__ __forceinline__ float row_scale(int step, int tile) const {
-    return *reinterpret_cast<const float*>(smem + C::RING_BYTES + ((step >> 2) & 1) * C::SCALE_BYTES + (step & 3) * 4 + scale_at + tile * 256);
+    return *reinterpret_cast<const float*>(smem + C::RING_BYTES + (step >> 2) % C::SCALE_SETS * C::SCALE_BYTES + (step & 3) * 4 + scale_at + tile * 256);
   }
 };
 
@@ -266,8 +267,8 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, int b_block, 
 // Two groups of four waves, one of each per SIMD, half a period apart: while one reads the fragments of half of its rows (memory phase),
 // the other multiplies (compute phase); a barrier ends every phase, four phases a slab.  In phases, group 0 reads slab t in 4 t (the
 // weights' fragments, and the first half of its rows, the rest of it while it multiplies) and 4 t + 2 and multiplies in 4 t + 1 and 4 t +
-// 3, group 1 a phase later.  Loads are requested in memory phases, in one order, once both groups have read what they replace: the weights of slab t + 2 from phase 4 t + 2 on, the rows' first halves from 4 t
-// + 3, their second halves from 4 t + 4 on.  Of group 0 those are 4 t + 2, 4 t + 4 and 4 t + 4, of group 1 4 t + 3, 4 t + 3 and 4 t + 5;
+// 3, group 1 a phase later.  Loads are requested in memory phases, in one order, once both groups have read what they replace: the
+// weights of slab t + 2 from phase 4 t + 2 on, the rows' first halves from 4 t + 3, their second halves from 4 t + 4 on.  Of group 0 those are 4 t + 2, 4 t + 4 and 4 t + 4, of group 1 4 t + 3, 4 t + 3 and 4 t + 5;
 // the first two are wanted from phase 4 t + 8 on and the last from 4 t + 10.  A wave waits for its own at the ends of phases 4 t + 1
 // (second halves of slab t) and 4 t + 3 (the rest of slab t + 1), with eight loads on their way behind them, group 0 six in the latter.
 // 8192 x 7168 x 2048 in 32 groups, trans_rhs: 208 us, with all loads requested in phase 4 t and awaited in 4 t + 3 225.

@@ -195,6 +195,21 @@ def test_product(m, k, n, sizes, trans):
         _check_product(m, k, n, sizes, trans, dtype, pow2=i == 1, held=i != 2, seed=i)
 
 
+# Launches large enough for tiles of 128 x 128 (the first three) and of 256 x 256, with tiles of every height left over, contractions
+# of one block, of few and of more than the rings of slabs and scales hold.
+FILLED = [(2500, 1300, 2304, [700, 129, 0, 65, 33, 1, 1000, 500]), (1500, 130, 2500, [257, 31, 200, 640, 128, 96, 140]),
+          (3900, 700, 1100, [130] * 10 + [0, 1, 400, 63] * 5), (2600, 700, 4100, [900, 300, 1, 0, 256, 64, 700]),
+          (2600, 1156, 2100, [130, 127, 128, 0, 257, 1, 64, 65, 500, 17] * 2), (5000, 100, 2100, [513, 300, 200, 1000, 40, 700, 0, 1500, 129, 255])]
+
+
+@pytest.mark.parametrize("trans", [False, True], ids=["nn", "nt"])
+@pytest.mark.parametrize("m,k,n,sizes", FILLED)
+def test_product_that_fills_the_device(m, k, n, sizes, trans):
+    print(f"product {m} {k} {n} {len(sizes)} groups trans={trans}", flush=True)
+    for i, dtype in enumerate(TYPES.values()):
+        _check_product(m, k, n, sizes, trans, dtype, pow2=i == 1, held=i != 2, seed=i)
+
+
 def test_no_rows_no_columns_no_contraction():
     gs = torch.tensor([2, 0], dtype=torch.int32, device="cuda")
     for m, k, n in ((0, 64, 32), (4, 0, 32), (4, 64, 0)):
