@@ -12,7 +12,7 @@
 //              that, since B is small along small singular values.  lo is a byte, the residue times 32 in e4m3: its four bits behind hi's
 //              eleven are all that pays (sixteen of them left 0.1 % too), and X is most of what is moved.  X before the last step, whose
 //              rounding grows once, has none.
-//   float32 G: everything in two numbers and every product in three, hi hi + hi lo + lo hi: 22 bits, as accurate as float32 products.
+//   float32 G: everything in two numbers and every product in three, lo hi + hi lo + hi hi: 22 bits, as accurate as float32 products.
 #include "rd_elem.h"
 #include "rd_gemm_w4.h"
 #include "rd_ortho.h"
@@ -269,7 +269,12 @@ __device__ __forceinline__ void small_kloop(const half_bits* a, int lda, int row
 template <int BM, bool SYMMETRIC>
 constexpr int ortho_groups = OrthoTile<BM, SYMMETRIC>::GROUPS;
 
-// PLANES 2: hi hi + hi lo + lo hi.
+// PLANES 2: lo hi + hi lo + hi hi, the largest last, so that the small ones are added to small sums.  In tiles of 64 and 128 each goes in
+// pieces of the contraction whose sums start from zero: one sum of all was rounded once per sixteen indices and product where it was
+// largest, and a long contraction of few rows lost more than float32 products do (1 x 32 x 4000: 8.0e-6 of the result, in pieces of 1024
+// 1.9e-6, float32 products 2.1e-6; 2048 x 2048: 3.4e-6, 1.0e-6, 3.6e-6).  Pieces of 512 give no more there and cost 5 % of 12 x 1515 x
+// 1001 instead of 2.  Tiles of 256 have no registers for a second sum, and enough rows for other roundings to outweigh this one.
+constexpr int kOrthoPiece = 1024;
 template <int BM, int KIND, int PLANES>
 __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || KIND == kSquare>)) void ortho_product_kernel(OrthoStep p) {
   constexpr bool SYMMETRIC = KIND == kGram || KIND == kSquare;
@@ -303,13 +308,45 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
     for (int j = 0; j < C::TN; ++j)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+  auto product = [&](const half_bits* a, const half_bits* b, int len) {
+    if constexpr (BM == 64) small_kloop<C>(a, p.left.cols, rows, b, p.right.cols, cols, len, smem, wave, lane, acc);
+    else if (live) w4_kloop<C, true>(a, p.left.cols, rows, b, p.right.cols, cols, len, smem, wave, lane, acc);
+    else w4_kloop<C, false>(a, p.left.cols, rows, b, p.right.cols, cols, len, smem, wave, lane, acc);
+  };
+  constexpr bool PIECES = PLANES == 2 && BM < 256;
+  f32x16_t sum[PIECES ? C::TM : 1][PIECES ? C::TN : 1];
+  if constexpr (PIECES) {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) sum[i][j] = acc[i][j];
+  }
 #pragma unroll 1
-  for (int term = 0; term < (PLANES == 2 ? 3 : 1); ++term) {
-    const half_bits* a = (term == 2 ? static_cast<const half_bits*>(p.left.lo) : p.left.hi) + left;
+  for (int term = PLANES == 2 ? 0 : 2; term < 3; ++term) {
+    const half_bits* a = (term == 0 ? static_cast<const half_bits*>(p.left.lo) : p.left.hi) + left;
     const half_bits* b = (term == 1 ? static_cast<const half_bits*>(p.right.lo) : p.right.hi) + right;
-    if constexpr (BM == 64) small_kloop<C>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
-    else if (live) w4_kloop<C, true>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
-    else w4_kloop<C, false>(a, p.left.cols, rows, b, p.right.cols, cols, klen, smem, wave, lane, acc);
+    if constexpr (!PIECES) product(a, b, klen);
+    else {
+#pragma unroll 1
+      for (int at = 0; at < klen; at += kOrthoPiece) {
+        product(a + at, b + (SYMMETRIC ? at : (long long)at * p.right.cols), imin(kOrthoPiece, klen - at));
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              sum[i][j][v] += acc[i][j][v];
+              acc[i][j][v] = 0.f;
+            }
+      }
+    }
+  }
+  if constexpr (PIECES) {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) acc[i][j] = sum[i][j];
   }
   if (!live) return;
 
@@ -417,9 +454,9 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_divide_kernel(const T* __
 
 // Which tiles: the least time by rounds of what the device holds, 256 compute units of one or two work-groups, in tiles of 128 x 128.  As
 // measured, a unit takes 1.35 times as long per number in tiles of 128 x 128, whose operands' reads of LDS bound it, 1.2 times in those of
-// 128 x 256, 2.3 times in those of 64 x 64, and a work-group alone on it 0.7 times as long as two.  us, all products in tiles of 64 | 128 | 256, bf16: 4 of 256 x 512 83 | 127 | 213; 1 of 768 x 768 141 | 191 | 361; 1
-// of 2048 x 2048 500 | 343 | 634; 16 of 768 x 2048 817 | 583 | 653; 12 of 1515 x 1001 872 | 595 | 656; 1 of 4096 x 4096 3266 | 1948 |
-// 1503; 128 of 768 x 2048 7704 | 4963 | 4216.
+// 128 x 256, 2.3 times in those of 64 x 64, and a work-group alone on it 0.7 times as long as two.  us, all products in tiles of 64 | 128 |
+// 256, bf16: 4 of 256 x 512 83 | 127 | 213; 1 of 768 x 768 141 | 191 | 361; 1 of 2048 x 2048 500 | 343 | 634; 16 of 768 x 2048 817 | 583
+// | 653; 12 of 1515 x 1001 872 | 595 | 656; 1 of 4096 x 4096 3266 | 1948 | 1503; 128 of 768 x 2048 7704 | 4963 | 4216.
 int tile_for(bool symmetric, int g, int rows, int cols) {
   const auto time = [&](int r, int c, int groups, double slow) {
     const long long down = (rows + r - 1) / r, across = (cols + c - 1) / c, tiles = g * (symmetric ? down * (down + 1) / 2 : down * across);

@@ -149,6 +149,26 @@ def test_refusals():
         rd.orthogonalize(G.clone().requires_grad_())
 
 
+@pytest.mark.parametrize("g,k,n", [(1, 32, 4000), (30, 40, 100), (2, 2048, 128), (1, 100, 8000), (1, 1024, 1500), (64, 512, 1280)])
+def test_float32_is_as_accurate_as_float32_products(g, k, n):
+    """Long contractions of few rows, one of more than a piece of the sums, and tiles of each size; float32 products of the vendor's
+    library in the formulas, whose roundings are others of the same size: three times what they are off by."""
+    print(f"accuracy {g} x {k} x {n}", flush=True)
+    G = torch.randn(g, k, n, generator=torch.Generator().manual_seed(k)).cuda()
+
+    def iterate(X):
+        X = X if k <= n else X.transpose(1, 2).contiguous()
+        X = X / (X.flatten(1).norm(dim=1)[:, None, None] + 1e-7)
+        for a, b, c in [COEFFICIENTS] * 5:
+            A = torch.bmm(X, X.transpose(1, 2).contiguous())
+            X = a * X + torch.bmm(b * A + c * torch.bmm(A, A), X)
+        return X if k <= n else X.transpose(1, 2)
+
+    ref = iterate(G.double())
+    off, plain = (float((y.double() - ref).norm() / ref.norm()) for y in (rd.orthogonalize(G), iterate(G)))
+    assert off <= 3 * plain, f"off by {off:.2e}, float32 products by {plain:.2e}"
+
+
 def test_captured_and_replayed():
     G = torch.randn(3, 200, 150, device="cuda").bfloat16()
     side = torch.cuda.Stream()
