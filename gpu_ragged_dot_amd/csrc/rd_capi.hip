@@ -1330,7 +1330,7 @@ static int check_float8(const void* codes, const void* scales, long long rows, i
   if (rows < 0 || cols < 0 || cols > rd::kF8MaxDim) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape: %lld rows of %d", rows, cols);
   const int rc = check_moe(0, 1, 0, dtype);
   if (rc != RD_OK) return rc;
-  if (rows * rd::float8_scale_pitch(cols) >= (1ll << 28) || rows * ((cols + 7) / 8) >= (1ll << 32))
+  if (rows * rd::float8_scale_pitch(cols) >= (1ll << 28) || rows * ((cols + 7) / 8) > (1ll << 32) - 256)
     return fail(RD_ERR_UNSUPPORTED, "%lld rows of %d are more blocks than a launch has work-groups for", rows, cols);
   if (rows > 0 && cols > 0 && (!codes || !scales || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) != 0))
     return fail(RD_ERR_INVALID_ARGUMENT, "the codes or scales are null or not 16-byte aligned");
@@ -1387,7 +1387,7 @@ int rd_float8_values(void* stream, const void* codes, const float* scales, void*
   if (rc == RD_OK) rc = check_moe(0, 1, 0, dtype);
   if (rc != RD_OK || a == 0 || b == 0) return rc;
   if (!out) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
-  if ((long long)g * a * ((b + 7) / 8) >= (1ll << 32)) return fail(RD_ERR_UNSUPPORTED, "%d matrices of %d x %d are more than a launch has work-groups for", g, a, b);
+  if ((long long)g * a * ((b + 7) / 8) > (1ll << 32) - 256) return fail(RD_ERR_UNSUPPORTED, "%d matrices of %d x %d are more than a launch has work-groups for", g, a, b);
   rc = rd::launch_float8_values((hipStream_t)stream, codes, scales, out, g, a, b, height, moe_elem(dtype));
   return rc == hipSuccess ? RD_OK : hip_fail(rc, "float8_values launch");
 }

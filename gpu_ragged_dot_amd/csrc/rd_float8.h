@@ -8,7 +8,7 @@
 // get near the least numbers of 32 bits.  In memory (the block counts of k and n are ceil(k / 128) and ceil(n / 128)):
 //   rows     codes [m][128 blocks], scales float32 [m][float8_scale_pitch(k)]
 //   weights  codes [g][128 blocks(a)][128 blocks(b)], scales float32 [g][blocks(a)][blocks(b)]; [a, b] is [k, n], or [n, k]
-// Codes of the padding are 0.  So every row of codes starts on a line of 128 bytes and no contraction has a tail.
+// Codes of the padding are 0, NaN in a block that is NaN.  So every row of codes starts on a line of 128 bytes and no contraction has a tail.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stddef.h>

@@ -749,9 +749,9 @@ Tensor gmm_held(const Held& x, const Held& A, const Tensor& gs_, int64_t k, int6
 
 // A product's operands: numbers, or (codes defined) numbers held as float8 already.
 struct Float8Call : torch::CustomClassHolder {
-  bool trans = false, pow2 = false;
-  int64_t g_first = -1, k = 0, n = 0;
-  at::ScalarType type = at::kBFloat16;
+  bool trans = false, pow2 = false, wants_x = false, wants_A = false;
+  int64_t g_first = -1, g_local = 0, k = 0, n = 0;
+  at::ScalarType type = at::kBFloat16, x_type = at::kBFloat16;
   Held x, A;
 };
 Tensor float8_product(const Float8Call& c, const Tensor& x, const Tensor& gs, const Held& A) {
@@ -764,7 +764,9 @@ struct Float8Node : torch::autograd::Function<Float8Node> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& A, const Tensor& gs, const c10::intrusive_ptr<Float8Call>& c) {
     const Tensor sizes = sizes_on(gs, x.device());
     const Held w = A ? quantize_weights_of(*A, c->pow2) : c->A;
-    ctx->save_for_backward({x, w.codes, w.scales, sizes});
+    // (each only where a gradient is made of it: x for dA, the weights for dx)
+    ctx->save_for_backward({c->wants_A ? x : Tensor(), c->wants_x ? w.codes : Tensor(), c->wants_x ? w.scales : Tensor(), sizes});
+    c->g_local = w.codes.size(0);
     ctx->saved_data["call"] = c10::IValue::make_capsule(c);
     return float8_product(*c, x, sizes, w);
   }
@@ -774,16 +776,16 @@ struct Float8Node : torch::autograd::Function<Float8Node> {
       const auto call = ctx->saved_data["call"].toCapsule();
       const Float8Call& c = *static_cast<Float8Call*>(call.get());
       const Tensor &x = saved[0], &gs = saved[3];
-      check_devices(x, grads[0]);
+      check_devices(gs, grads[0]);
       const Tensor dy = grads[0].contiguous();
       Tensor dx, dA;
-      if (ctx->needs_input_grad(0))
-        dx = gmm_held(quantize_rows_of(dy, c.pow2), {saved[1], saved[2]}, gs, c.n, c.k, !c.trans, c.g_first, x.scalar_type());
-      if (!c.A.codes.defined() && ctx->needs_input_grad(1)) {  // (given as numbers, not as codes)
+      if (c.wants_x && ctx->needs_input_grad(0))
+        dx = gmm_held(quantize_rows_of(dy, c.pow2), {saved[1], saved[2]}, gs, c.n, c.k, !c.trans, c.g_first, c.x_type);
+      if (c.wants_A && ctx->needs_input_grad(1)) {
         Call t;
         t.code = rows_code(x); t.g_first = c.g_first;
         const Tensor d = dy.to(x.scalar_type());
-        dA = c.trans ? tgmm_forward(d, x, gs, t, 2, saved[1].size(0)) : tgmm_forward(x, d, gs, t, 2, saved[1].size(0));
+        dA = c.trans ? tgmm_forward(d, x, gs, t, 2, c.g_local) : tgmm_forward(x, d, gs, t, 2, c.g_local);
       }
       return {dx, dA, Tensor(), Tensor()};
     });
@@ -819,6 +821,8 @@ Tensor gmm_float8(const std::optional<Tensor>& x_, const std::optional<Tensor>& 
   TORCH_CHECK_NOT_IMPLEMENTED(x.defined() || !wants_A, "the gradient of the weights needs the rows themselves, not rows held as float8");
   const Tensor& on = x.defined() ? x : c->x.codes;
   check_devices(on, A.defined() ? A : c->A.codes);
+  c->wants_x = wants_x; c->wants_A = wants_A;
+  if (x.defined()) c->x_type = x.scalar_type();
   if (wants_x || wants_A) return Float8Node::apply(x, A.defined() ? std::optional<Tensor>(A) : std::nullopt, gs, c);
   return float8_product(*c, x, gs, A.defined() ? quantize_weights_of(A, pow2) : c->A);
 }

@@ -25,13 +25,13 @@ __all__ = ["Float8Rows", "Float8Weights", "quantize_rows", "quantize_weights", "
 
 
 class Float8Rows(NamedTuple):
-    codes: torch.Tensor   # float8_e4m3fn [m, 128 ceil(k / 128)], 0 past k
+    codes: torch.Tensor   # float8_e4m3fn [m, 128 ceil(k / 128)], 0 past k (NaN in a block that is NaN)
     scales: torch.Tensor  # float32 [m, ceil(k / 128) rounded up to a multiple of 4]
     k: int
 
 
 class Float8Weights(NamedTuple):
-    codes: torch.Tensor   # float8_e4m3fn [g, rows, cols], both rounded up to multiples of 128, 0 in the padding
+    codes: torch.Tensor   # float8_e4m3fn [g, rows, cols], both rounded up to multiples of 128, 0 in the padding (the same)
     scales: torch.Tensor  # float32 [g, rows / 128, cols / 128]
     rows: int             # of a matrix: k, or n where the products are called with trans_rhs
     cols: int

@@ -303,7 +303,7 @@ int rd_gmm_int4(void* stream, const void* x, const void* codes, const void* scal
  *       a NaN or an infinity;   q = e4m3fn(float32(x / s)), both roundings to nearest even.
  *   rows:    codes [m][K], scales float32 [m][S], K = 128 ceil(k / 128), S = ceil(k / 128) rounded up to a multiple of 4;
  *   weights: codes [g][A][B], scales float32 [g][A / 128][B / 128], A and B the sizes a and b rounded up to multiples of 128.
- * Codes and scales of the padding are 0; codes are 16-byte aligned, and so are the rows' scales.
+ * Codes and scales of the padding are 0 (codes NaN in a block that is NaN); codes are 16-byte aligned, and so are the rows' scales.
  *   rd_float8_rows:    x [rows, k] (RD_DTYPE_BF16, RD_DTYPE_F32 or RD_DTYPE_F16).  rd_float8_values gives numbers back, q s rounded
  *                      once: height 1 for rows (g = 1), 128 for weights.
  *   rd_float8_weights: [g, a, b].

@@ -110,6 +110,30 @@ def test_steps_of_training():
                 p -= (0.02 * update).to(p.dtype)
 
 
+def test_a_gradient_keeps_only_what_it_reads():
+    """Of weights held as float8 only dx is made, which needs no rows: they may be written over, and are not kept."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    leaf = torch.randn(50, 256, generator=gen, device="cuda").bfloat16().requires_grad_()
+    w = rd.quantize_weights(torch.randn(2, 256, 128, generator=gen, device="cuda").bfloat16())
+    gs, dy = torch.tensor([20, 25], dtype=torch.int32, device="cuda"), torch.randn(50, 128, generator=gen, device="cuda").bfloat16()
+    x = leaf * 1
+    y = rd.ragged_dot_float8(x, w, gs)
+    want = rd.ragged_dot_float8(dy, w, gs, trans_rhs=True)
+    x.detach().zero_()
+    with torch.no_grad():
+        x.zero_()
+    got, = torch.autograd.grad(y, leaf, dy)
+    assert torch.equal(got, want)
+    kept = []
+    A = torch.randn(2, 256, 128, generator=gen, device="cuda").bfloat16().requires_grad_()
+    for rows, weights in ((leaf, A), (leaf, w), (leaf.detach(), A)):
+        before = torch.cuda.memory_allocated()
+        y = rd.ragged_dot_float8(rows, weights, gs)
+        kept.append(torch.cuda.memory_allocated() - before)
+        del y
+    assert kept[0] > kept[1] and kept[0] > kept[2]
+
+
 def test_two_calls_at_once_on_two_streams():
     """Nothing that a call writes is another's."""
     shapes = [(700, 512, 640), (90, 256, 1000)]
