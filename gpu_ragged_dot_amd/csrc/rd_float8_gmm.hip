@@ -52,6 +52,17 @@ struct F8Few {
     else float8_tile<C64>(t, y, ldy, elem, smem);
   }
 };
+template <bool B_KMAJOR>
+struct F8Narrow {  // a compute unit's LDS full of slabs on their way
+  static constexpr int BM = 64, BN = 64, NT = 256, WAVES = 1;
+  typedef F8TileCfg<64, 64, 1, 4, 8, B_KMAJOR> C64;
+  typedef F8TileCfg<32, 64, 1, 4, 10, B_KMAJOR> C32;
+  static constexpr int LDS_BYTES = larger(C64::LDS_BYTES, C32::LDS_BYTES);
+  static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
+    if (t.rows <= 32) float8_tile<C32>(t, y, ldy, elem, smem);
+    else float8_tile<C64>(t, y, ldy, elem, smem);
+  }
+};
 
 // Work-groups [0, whole): a tile each; those behind them: rows, of which they zero what is no row of a group that the weights hold.
 template <class S, bool B_KMAJOR>
@@ -119,16 +130,27 @@ int height_for(const F8Problem& p) {
   return tall <= middle && tall <= few ? 256 : middle <= few ? 128 : 64;
 }
 
+// Launches of at most so many tiles of 64 x 128 take 64 columns: more work-groups, and as many slabs on their way as LDS holds.  us, 128 | 64
+// columns, trans_rhs: 1 x 4096 x 4096 17.6 | 15.2; 33 rows in 4 groups x 7168 x 2048 28.0 | 24.8; 8 in 256 x 7168 x 2048 30.4 | 28.0 (without
+// trans_rhs 59.8 | 41.8).  Of more tiles 64 columns have twice the rounds: 32 rows in 128 x 2048 x 768 11.6 | 19.5.
+constexpr int kF8FewTiles = 128;
 struct F8Grid {
-  int height, col_tiles;
+  int height, width, col_tiles;
   long long whole, all;
 };
 F8Grid grid_of(const F8Problem& p) {
   F8Grid g;
   g.height = height_for(p);
-  const int bn = g.height == 256 ? 256 : 128;
-  g.col_tiles = (p.n + bn - 1) / bn;
-  g.whole = ((p.m / g.height + imin(p.g_local, p.m)) * (long long)g.col_tiles + 7) / 8 * 8;
+  const auto tiles = [&] {
+    g.col_tiles = (p.n + g.width - 1) / g.width;
+    g.whole = ((p.m / g.height + imin(p.g_local, p.m)) * (long long)g.col_tiles + 7) / 8 * 8;
+  };
+  g.width = g.height == 256 ? 256 : 128;
+  tiles();
+  if (g.height == 64 && g.whole <= kF8FewTiles) {
+    g.width = 64;
+    tiles();
+  }
   g.all = g.whole + (p.m + kF8ZeroRows - 1) / kF8ZeroRows;
   return g;
 }
@@ -150,6 +172,7 @@ bool float8_grid_fits(const F8Problem& p) { return grid_of(p).all < (1ll << 31) 
 
 int launch_gmm_float8(hipStream_t s, const F8Problem& p) {
   const F8Grid g = grid_of(p);
+  if (g.width == 64) return p.trans_rhs ? launch_t<F8Narrow, true>(s, p, g) : launch_t<F8Narrow, false>(s, p, g);
   if (g.height == 64) return p.trans_rhs ? launch_t<F8Few, true>(s, p, g) : launch_t<F8Few, false>(s, p, g);
   if (g.height == 128) return p.trans_rhs ? launch_t<F8Middle, true>(s, p, g) : launch_t<F8Middle, false>(s, p, g);
   return p.trans_rhs ? launch_t<F8Tall, true>(s, p, g) : launch_t<F8Tall, false>(s, p, g);

@@ -169,7 +169,9 @@ struct F8Wave {
   F8Reader16<C::BN, C::TN, C::B_KMAJOR> frb;
   __amdgpu_buffer_rsrc_t scale_rsrc;
   int scale_off, scale_at;
-  const __attribute__((address_space(4))) float* col_scale;  // (read through the scalar cache: no vector load to wait for)
+  const __attribute__((address_space(4))) float* col_scale;  // the wave's columns' of the first block
+  int b_block, blocks;
+  float held;  // (MN-major B) a lane's of the 64 blocks that the current one is among
   unsigned char* smem;
 
   __device__ __forceinline__ void init(const F8Tile& t, unsigned char* smem_) {
@@ -187,6 +189,24 @@ struct F8Wave {
     scale_off = row < t.rows ? row * t.ldas * 4 : -1;
     scale_at = (wm * C::WM + (lane & 15)) * 16;
     col_scale = (const __attribute__((address_space(4))) float*)(live ? t.b_scales + (wn * C::WN / kF8Block) * t.b_column : t.b_scales);
+    b_block = t.b_block; blocks = t.blocks;
+    held = 0.f;
+    if constexpr (!C::B_KMAJOR) hold(0);
+  }
+  // The columns' scale of a block.  Those of [n, k] weights are neighbours, read through the scalar cache.  Of [k, n] weights each is in a line
+  // of its own, which a scalar load per slab would wait for: a lane loads one of 64 blocks (8 groups of 2 x 14336 x 4096 150 -> 121
+  // us; 2048 x 4096 x 14336 with the rows' quantisation 1089 -> 1056).
+  __device__ __forceinline__ void hold(int first) {
+    if (first + lane < blocks) held = static_cast<const float*>((const void*)col_scale)[(long long)(first + lane) * b_block];
+  }
+  __device__ __forceinline__ void held_is_there() { asm volatile("" : "+v"(held)); }  // (waited for here, and not at every use in the loop)
+  __device__ __forceinline__ float column_scale(int step) {
+    if constexpr (C::B_KMAJOR) return col_scale[step];
+    if ((step & 63) == 0 && step > 0) {
+      hold(step);
+      held_is_there();
+    }
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), step & 63));
   }
   // The wave's share of slab `step`: of B, with the rows' scales of four blocks beside the first of them (16 bytes a lane, 64 rows a
   // wave), and of A, HALF 0 or 1 of its loads, or (2) all.
@@ -236,10 +256,11 @@ __device__ __forceinline__ void phase_barrier() {
 
 // A barrier per slab, several slabs on their way: tiles of few rows, which wait for their weights.
 template <class C>
-__device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, int b_block, f32x4_t (&acc)[C::TM][C::TN]) {
+__device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc)[C::TM][C::TN]) {
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s)
     if (s < nk) u.issue(s);
+  if constexpr (!C::B_KMAJOR) u.held_is_there();
   constexpr int L = C::LdA::PER + C::LdB::PER;
   for (int kt = 0; kt < nk; ++kt) {
     // (a load of scales makes a wave wait for no less)
@@ -248,7 +269,7 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, int b_block, 
     phase_barrier();  // slab kt is in LDS, and slab kt - 1 is no longer being read
     if (kt + C::STAGES - 1 < nk) u.issue(kt + C::STAGES - 1);
     if (u.live) {
-      const float w = u.col_scale[(long long)kt * b_block];
+      const float w = u.column_scale(kt);
       const unsigned char* ra = u.slab(kt);
       i32x8_t fb[C::TN];
 #pragma unroll
@@ -278,7 +299,7 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, int b_block, 
 // flight the same.  The same product without scales, whose sums stay where the matrix cores keep them: 840 and 785.
 // Inner sums enter the accumulators four instructions later, those of a phase's last row piece at the start of the next compute phase.
 template <class C>
-__device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int b_block, f32x4_t (&acc)[C::TM][C::TN]) {
+__device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x4_t (&acc)[C::TM][C::TN]) {
   static_assert(C::NW == 8 && C::WAVES_M == 2 && C::STAGES == 2 && C::TM == 8 && C::LdA::PER == 4 && C::LdB::PER == 4,
                 "two groups of four waves, four row pieces a phase; loads 0 and 2 of A hold the waves' first 64 rows");
   constexpr int FIRST = 2;  // row pieces read before a slab's first compute phase
@@ -324,6 +345,7 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int 
   u.template issue_a<1>(0);
   if (nk > 1) u.issue_b(1);
   if (group == 1 && nk > 1) u.template issue_a<0>(1);
+  if constexpr (!C::B_KMAJOR) u.held_is_there();
   if (nk > 1) wait_vmcnt<6>(); else wait_vmcnt<0>();  // (group 1 waits for two loads more than it has to)
   phase_barrier();
   if (group == 1) phase_barrier();
@@ -331,7 +353,7 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, int 
   typedef std::integral_constant<int, 1> Second;
   for (int kt = 0; kt < nk; ++kt) {
     const bool next = kt + 1 < nk, after = kt + 2 < nk;
-    const float w = u.live ? u.col_scale[(long long)kt * b_block] : 0.f;
+    const float w = u.live ? u.column_scale(kt) : 0.f;
     if (u.live) read(kt, First(), w);
     if (next) {
       if (group == 0) u.template issue_a<0>(kt + 1);
@@ -374,8 +396,8 @@ __device__ __forceinline__ void float8_tile(const F8Tile& t, void* y, int ldy, i
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   if (t.blocks > 0) {
-    if constexpr (C::PINGPONG) float8_kloop_pingpong<C>(u, t.blocks, t.b_block, acc);
-    else float8_kloop<C>(u, t.blocks, t.b_block, acc);
+    if constexpr (C::PINGPONG) float8_kloop_pingpong<C>(u, t.blocks, acc);
+    else float8_kloop<C>(u, t.blocks, acc);
   }
   __builtin_amdgcn_s_waitcnt(0xc07f);
   phase_barrier();  // the ring is no longer read by any wave

@@ -51,9 +51,9 @@ static bool check_all() {
     for (int more : {0, 1, 7}) {
       for (int lim : {1, 15, 16, T / 2, T / 2 + 1, T - 1, T})
         if (!check<T, NW, true>(lim, 128 * (blocks + more), blocks)) return false;
-      if constexpr (T >= 128)
-        for (int lim : {128, T})
-          if (!check<T, NW, false>(lim, 128 * (T / 128 + more), blocks)) return false;
+      if constexpr (T >= 64)
+        for (int lim : {T < 128 ? T : 128, T})
+          if (!check<T, NW, false>(lim, 128 * ((T + 127) / 128 + more), blocks)) return false;
     }
   return true;
 }
