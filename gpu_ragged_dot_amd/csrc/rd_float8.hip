@@ -95,7 +95,7 @@ __device__ __forceinline__ void row_block(const T* __restrict__ row, int k, int 
 }
 
 // A work-group takes kF8Groups neighbouring (row, block) items; blocks past the last one of a row are the padding of its scales.
-// 32768 x 7168 and 32768 x 2048 bf16: 175 us together, 5.2 TB/s; behind the gated activation, 32768 x 2048 bf16: 72 us, 4.7 TB/s.
+// 32768 x 7168 and 32768 x 2048 bf16: 175 us together, 5.2 TB/s; behind the gated activation, 32768 x 2048 bf16: 70 us, 4.8 TB/s.
 template <class T, bool SWIGLU>
 __global__ __launch_bounds__(kF8Threads) void float8_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, float* __restrict__ scales,
                                                                  long long items, int k, bool pow2) {
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kF8Threads) void float8_dispatch_kernel(const T* __
   }
 }
 
-// A work-group to a block of 128 x 128: sixteen lanes to a row, eight rows to a thread.  256 x 7168 x 2048 bf16: 2150 us, 5.2 TB/s.
+// A work-group to a block of 128 x 128: sixteen lanes to a row, eight rows to a thread.  256 x 7168 x 2048 bf16: 2140 us, 5.3 TB/s.
 template <class T>
 __global__ __launch_bounds__(kF8Threads) void float8_weights_kernel(const T* __restrict__ A, uint8_t* __restrict__ codes, float* __restrict__ scales,
                                                                     int a, int b, bool pow2) {

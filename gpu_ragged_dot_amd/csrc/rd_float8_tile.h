@@ -295,7 +295,7 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc
 // 8192 x 7168 x 2048 in 32 groups, trans_rhs: 208 us, with all loads requested in phase 4 t and awaited in 4 t + 3 225.
 //
 // What bounds it: the longest of the phases that read.  16384 x 4096 x 14336 in 8 groups takes 950 us with trans_rhs (2.0 PFLOP/s) and
-// 1030 without; without its multiply-adds 8 % less, without its loads 15 %, without its reads of LDS 5 to 20 %, at any number of loads in
+// 1010 without; without its multiply-adds 8 % less, without its loads 15 %, without its reads of LDS 5 to 20 %, at any number of loads in
 // flight the same.  The same product without scales, whose sums stay where the matrix cores keep them: 840 and 785.
 // Inner sums enter the accumulators four instructions later, those of a phase's last row piece at the start of the next compute phase.
 template <class C>
