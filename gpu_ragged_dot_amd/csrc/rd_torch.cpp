@@ -759,7 +759,8 @@ Tensor float8_product(const Float8Call& c, const Tensor& x, const Tensor& gs, co
 }
 
 // Straight through: the gradient of the product of what the operands are held as, taken for that of the operands themselves.  dx is a
-// product of the same kind, on the cotangent's rows in 8 bits and the weights that the forward product used; dA the 16- or 32-bit product.
+// product of the same kind, on the cotangent's rows in 8 bits and the weights that the forward product used; dA the 16- or 32-bit product
+// of the rows and the cotangent as they are, rounded once.
 struct Float8Node : torch::autograd::Function<Float8Node> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& A, const Tensor& gs, const c10::intrusive_ptr<Float8Call>& c) {
     const Tensor sizes = sizes_on(gs, x.device());
@@ -782,10 +783,12 @@ struct Float8Node : torch::autograd::Function<Float8Node> {
       if (c.wants_x && ctx->needs_input_grad(0))
         dx = gmm_held(quantize_rows_of(dy, c.pow2), {saved[1], saved[2]}, gs, c.n, c.k, !c.trans, c.g_first, c.x_type);
       if (c.wants_A && ctx->needs_input_grad(1)) {
+        // (of two types neither holds the other's numbers; float32 holds both)
+        const at::ScalarType type = dy.scalar_type() == x.scalar_type() ? x.scalar_type() : at::kFloat;
+        const Tensor d = dy.to(type), rows = x.to(type);
         Call t;
-        t.code = rows_code(x); t.g_first = c.g_first;
-        const Tensor d = dy.to(x.scalar_type());
-        dA = c.trans ? tgmm_forward(d, x, gs, t, 2, c.g_local) : tgmm_forward(x, d, gs, t, 2, c.g_local);
+        t.code = rows_code(rows); t.g_first = c.g_first;
+        dA = (c.trans ? tgmm_forward(d, rows, gs, t, 2, c.g_local) : tgmm_forward(rows, d, gs, t, 2, c.g_local)).to(x.scalar_type());
       }
       return {dx, dA, Tensor(), Tensor()};
     });

@@ -91,7 +91,8 @@ def ragged_dot_float8(x: Union[torch.Tensor, Float8Rows], A: Union[torch.Tensor,
     rows held as float8.  ``group_offset`` as in ``gmm``.
 
     Differentiable by operands that are tensors, straight through the quantisation: ``dx`` is the product of the output's gradient,
-    quantised too, with the same float8 weights, ``dA`` that of ``trans_ragged_dot`` on ``x`` and the gradient as they are."""
+    quantised too, with the same float8 weights, ``dA`` that of ``trans_ragged_dot`` on ``x`` and the gradient as they are: in float32
+    where ``out_dtype`` is not the type of ``x``, and rounded once."""
     if out_dtype is None:
         out_dtype = torch.bfloat16 if isinstance(x, Float8Rows) else x.dtype
     if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
