@@ -23,9 +23,9 @@ struct F8Tall {
   typedef F8TileCfg<64, 256, 2, 4, 3, B_KMAJOR> C64;
   static constexpr int LDS_BYTES = larger(C256::LDS_BYTES, larger(C128::LDS_BYTES, C64::LDS_BYTES));
   static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
-    if (t.rows <= 64) float8_tile<C64>(t, y, ldy, elem, smem);
-    else if (t.rows <= 128) float8_tile<C128>(t, y, ldy, elem, smem);
-    else float8_tile<C256>(t, y, ldy, elem, smem);
+    const bool again = t.rows <= 64 ? float8_tile<C64>(t, y, ldy, elem, smem) : t.rows <= 128 ? float8_tile<C128>(t, y, ldy, elem, smem)
+                                                                                             : float8_tile<C256>(t, y, ldy, elem, smem);
+    if (again) float8_tile_any_scale<C64>(t, y, ldy, elem, smem);
   }
 };
 template <bool B_KMAJOR>
@@ -36,9 +36,9 @@ struct F8Middle {
   typedef F8TileCfg<32, 128, 1, 4, 3, B_KMAJOR> C32;
   static constexpr int LDS_BYTES = larger(C128::LDS_BYTES, larger(C64::LDS_BYTES, C32::LDS_BYTES));
   static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
-    if (t.rows <= 32) float8_tile<C32>(t, y, ldy, elem, smem);
-    else if (t.rows <= 64) float8_tile<C64>(t, y, ldy, elem, smem);
-    else float8_tile<C128>(t, y, ldy, elem, smem);
+    const bool again = t.rows <= 32 ? float8_tile<C32>(t, y, ldy, elem, smem) : t.rows <= 64 ? float8_tile<C64>(t, y, ldy, elem, smem)
+                                                                                            : float8_tile<C128>(t, y, ldy, elem, smem);
+    if (again) float8_tile_any_scale<C32>(t, y, ldy, elem, smem);
   }
 };
 template <bool B_KMAJOR>
@@ -48,8 +48,8 @@ struct F8Few {
   typedef F8TileCfg<32, 128, 1, 4, 3, B_KMAJOR> C32;
   static constexpr int LDS_BYTES = larger(C64::LDS_BYTES, C32::LDS_BYTES);
   static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
-    if (t.rows <= 32) float8_tile<C32>(t, y, ldy, elem, smem);
-    else float8_tile<C64>(t, y, ldy, elem, smem);
+    const bool again = t.rows <= 32 ? float8_tile<C32>(t, y, ldy, elem, smem) : float8_tile<C64>(t, y, ldy, elem, smem);
+    if (again) float8_tile_any_scale<C32>(t, y, ldy, elem, smem);
   }
 };
 template <bool B_KMAJOR>
@@ -59,8 +59,8 @@ struct F8Narrow {  // a compute unit's LDS full of slabs on their way
   typedef F8TileCfg<32, 64, 1, 4, 10, B_KMAJOR> C32;
   static constexpr int LDS_BYTES = larger(C64::LDS_BYTES, C32::LDS_BYTES);
   static __device__ __forceinline__ void run(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
-    if (t.rows <= 32) float8_tile<C32>(t, y, ldy, elem, smem);
-    else float8_tile<C64>(t, y, ldy, elem, smem);
+    const bool again = t.rows <= 32 ? float8_tile<C32>(t, y, ldy, elem, smem) : float8_tile<C64>(t, y, ldy, elem, smem);
+    if (again) float8_tile_any_scale<C32>(t, y, ldy, elem, smem);
   }
 };
 

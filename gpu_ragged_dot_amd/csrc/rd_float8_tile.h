@@ -9,7 +9,15 @@
 //
 // The sums must lie in registers that the vector unit reads, of which a wave has 256 whatever its SIMD has left: eight waves of
 // 128 x 64 hold a tile of 256 x 256 in 128 of them each, beside the weights' fragments of a slab (32), two row pieces in turn (16) and
-// two sets of inner sums.  (Four waves of 128 x 128 with 32x32x64 instructions kept the sums in the accumulation registers and
+// two sets of inner sums.
+//
+// sx sw may be beyond float32, or lose bits below its least normal number, where what a block adds does neither (inner sums are 0, or between
+// 2^-18 and 2^25).  The K loops look at the products of scales, and a tile that meets such a one is computed again, in the least tiles of
+// its columns, by a loop that multiplies its inner sums twice (float8_tile_any_scale()); products that are normal numbers give the same bits
+// there.  Looking takes 2 % of a decoding step (64 rows in 128 groups x 2048 x 768: 17.4 -> 17.75 us), and nothing of large products; a
+// second multiplication everywhere would be as many again as the fused ones.
+//
+// (Four waves of 128 x 128 with 32x32x64 instructions kept the sums in the accumulation registers and
 // moved each there and back: 2.1 ms for 16384 x 4096 x 14336 in 8 groups.)
 #pragma once
 #include "rd_elem.h"
@@ -97,7 +105,9 @@ struct F8TileCfg {
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int EPI_PITCH = WN * 4 + 16, EPI_BYTES = NW * 16 * EPI_PITCH;
   static constexpr int USED_BYTES = RING_BYTES + SCALE_SETS * SCALE_BYTES;
-  static constexpr int LDS_BYTES = USED_BYTES > EPI_BYTES ? USED_BYTES : EPI_BYTES;
+  static constexpr int FLAGS_AT = USED_BYTES > EPI_BYTES ? USED_BYTES : EPI_BYTES;  // an int per wave
+  static constexpr int LDS_BYTES = FLAGS_AT + NW * 4;
+  static constexpr bool ALIKE = WAVES_M == 1 && BN <= kF8Block;  // all waves multiply by the same scales
   typedef F8Loader<BM, NW, true> LdA;
   typedef F8Loader<BN, NW, B_KMAJOR> LdB;
   static_assert(WN <= kF8Block && kF8Block % WN == 0, "a wave's columns lie in one block of the weights");
@@ -172,6 +182,8 @@ struct F8Wave {
   const __attribute__((address_space(4))) float* col_scale;  // the wave's columns' of the first block
   int b_block, blocks;
   float held;  // (MN-major B) a lane's of the 64 blocks that the current one is among
+  float kept;  // a lane's scale of the rows that are multiplied next
+  unsigned long long beyond;  // lanes that have met a product of scales that is no normal number
   unsigned char* smem;
 
   __device__ __forceinline__ void init(const F8Tile& t, unsigned char* smem_) {
@@ -191,7 +203,13 @@ struct F8Wave {
     col_scale = (const __attribute__((address_space(4))) float*)(live ? t.b_scales + (wn * C::WN / kF8Block) * t.b_column : t.b_scales);
     b_block = t.b_block; blocks = t.blocks;
     held = 0.f;
+    beyond = 0;
     if constexpr (!C::B_KMAJOR) hold(0);
+  }
+  // Lanes whose product of scales is infinite, subnormal or 0 where the scales are not 0 (NaN is what a NaN makes of a block); w is the wave's.
+  static __device__ __forceinline__ unsigned long long out_of_range(float row, float w, float product) {
+    const int classes = (__builtin_bit_cast(uint32_t, w) << 1) != 0 ? 0x2f4 : 0;
+    return __builtin_amdgcn_ballot_w64((row != 0.f) & __builtin_amdgcn_classf(product, classes));
   }
   // The columns' scale of a block.  Those of [n, k] weights are neighbours, read through the scalar cache.  Of [k, n] weights each is in a line
   // of its own, which a scalar load per slab would wait for: a lane loads one of 64 blocks (8 groups of 2 x 14336 x 4096 150 -> 121
@@ -227,9 +245,11 @@ struct F8Wave {
   __device__ __forceinline__ const unsigned char* slab(int step) const { return smem + (step % C::STAGES) * C::STAGE_BYTES; }
   // A lane's scale of its row in each of four pieces of sixteen rows, 4 h .. 4 h + 3 of the wave's, times w.  A lane reads that of one of the
   // 64 rows, and halves and quarters of the wave trade theirs (four reads of LDS take as long as two of a fragment).
-  __device__ __forceinline__ void factors(int step, int h, float w, float (&factor)[4]) const {
+  __device__ __forceinline__ void factors(int step, int h, float w, float (&factor)[4]) {
     const unsigned char* at = smem + C::RING_BYTES + (step >> 2) % C::SCALE_SETS * C::SCALE_BYTES + (step & 3) * 4;
-    const uint32_t s = __builtin_bit_cast(uint32_t, *reinterpret_cast<const float*>(at + (wm * C::WM + 64 * h + lane) * 16) * w);
+    const float row = *reinterpret_cast<const float*>(at + (wm * C::WM + 64 * h + lane) * 16), product = row * w;
+    kept = row;
+    const uint32_t s = __builtin_bit_cast(uint32_t, product);
     const auto half = __builtin_amdgcn_permlane32_swap(s, s, false, false);
     const auto low = __builtin_amdgcn_permlane16_swap(half[0], half[0], false, false), high = __builtin_amdgcn_permlane16_swap(half[1], half[1], false, false);
     const uint32_t got[4] = {low[0], low[1], high[0], high[1]};  // (a bit cast of a vector's element itself would read element 0)
@@ -254,8 +274,10 @@ __device__ __forceinline__ void phase_barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// A barrier per slab, several slabs on their way: tiles of few rows, which wait for their weights.
-template <class C>
+// A barrier per slab, several slabs on their way: tiles of few rows, which wait for their weights.  ANY_SCALE: an inner sum is multiplied by
+// half of the powers of two of its scales and then, as it is added, by the other half and what is left of the scales, between 1/4 and 1.
+// The first is exact wherever the result is a normal number.  (Powers beyond 2^250 make any sum but 0 infinite.)
+template <class C, bool ANY_SCALE>
 __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc)[C::TM][C::TN]) {
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s)
@@ -277,9 +299,30 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc
 #pragma unroll
       for (int i = 0; i < C::TM; ++i) {
         const i32x8_t fa = u.fra.read(ra, i);
-        const float factor = u.row_scale(kt, i) * w;
+        const float row = u.row_scale(kt, i);
+        float factor = row * w;
+        const unsigned long long beyond = u.out_of_range(row, w, factor);
+        if constexpr (ANY_SCALE) {
+          float before = 1.f;
+          if (beyond >> u.lane & 1) {
+            const int e = imin(__builtin_amdgcn_frexp_expf(row) + __builtin_amdgcn_frexp_expf(w), 250);
+            before = __builtin_ldexpf(1.f, e - (e >> 1));
+            factor = __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(row) * __builtin_amdgcn_frexp_mantf(w), e >> 1);
+          }
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j) float8_add(acc[i][j], float8_part(fb[j], fa), factor);
+          for (int j = 0; j < C::TN; ++j) float8_add(acc[i][j], float8_part(fb[j], fa) * before, factor);
+        } else {
+          u.beyond |= beyond;
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) float8_add(acc[i][j], float8_part(fb[j], fa), factor);
+        }
+      }
+    } else if constexpr (C::ALIKE && !ANY_SCALE) {  // looks as the others do, and so comes to what they come to
+      const float w = u.column_scale(kt);
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const float row = u.row_scale(kt, i);
+        u.beyond |= u.out_of_range(row, w, row * w);
       }
     }
   }
@@ -321,7 +364,7 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x
     for (int i = 0; i < (H == 0 ? FIRST : 4); ++i) fa[i] = u.fra.read(ra, 4 * H + i);
     u.factors(kt, H, w, factor);
   };
-  auto multiply = [&](int kt, auto half) {
+  auto multiply = [&](int kt, auto half, float wk) {
     constexpr int H = decltype(half)::value;
     if constexpr (H == 0) {
 #pragma unroll
@@ -333,6 +376,8 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x
       for (int j = 0; j < C::TN; ++j) {
         part[i & 1][j] = float8_part(fb[j], fa[i]);
         float8_add(acc[(4 * H + i + 7) & 7][j], part[(i + 1) & 1][j], i == 0 ? carried : factor[i == 0 ? 0 : i - 1]);
+        // (here, between products: behind the reads, which bound the loop, it took 6 % of 16384 x 4096 x 14336, and at the end of the phase 1 %)
+        if (i == 1 && j == 2) u.beyond |= u.out_of_range(u.kept, wk, u.kept * wk);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -363,7 +408,7 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     phase_barrier();
     __builtin_amdgcn_s_setprio(1);
-    if (u.live) multiply(kt, First());
+    if (u.live) multiply(kt, First(), w);
     __builtin_amdgcn_s_setprio(0);
     if (group == 0) wait(next);
     phase_barrier();
@@ -376,7 +421,7 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x
     __builtin_amdgcn_s_waitcnt(0xc07f);
     phase_barrier();
     __builtin_amdgcn_s_setprio(1);
-    if (u.live) multiply(kt, Second());
+    if (u.live) multiply(kt, Second(), w);
     __builtin_amdgcn_s_setprio(0);
     if (group == 0) { if (after) wait_vmcnt<6>(); else wait_vmcnt<0>(); }
     phase_barrier();
@@ -386,8 +431,9 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x
   for (int j = 0; j < C::TN; ++j) float8_add(acc[7][j], part[1][j], carried);
 }
 
-template <class C>
-__device__ __forceinline__ void float8_tile(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
+// Returns whether scales were met whose product is no normal number: the tile is then not written.  ANY_SCALE: takes all, and writes.
+template <class C, bool ANY_SCALE = false>
+__device__ __forceinline__ bool float8_tile(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
   F8Wave<C> u;
   u.init(t, smem);
   f32x4_t acc[C::TM][C::TN];
@@ -396,15 +442,37 @@ __device__ __forceinline__ void float8_tile(const F8Tile& t, void* y, int ldy, i
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   if (t.blocks > 0) {
-    if constexpr (C::PINGPONG) float8_kloop_pingpong<C>(u, t.blocks, acc);
-    else float8_kloop<C>(u, t.blocks, acc);
+    if constexpr (C::PINGPONG && !ANY_SCALE) float8_kloop_pingpong<C>(u, t.blocks, acc);
+    else float8_kloop<C, ANY_SCALE>(u, t.blocks, acc);
+  }
+  int* flags = reinterpret_cast<int*>(smem + C::FLAGS_AT);
+  if constexpr (!ANY_SCALE && !C::ALIKE) {
+    if (u.lane == 0) flags[u.wave] = u.beyond != 0;
   }
   __builtin_amdgcn_s_waitcnt(0xc07f);
   phase_barrier();  // the ring is no longer read by any wave
-  if (!u.live) return;
+  if constexpr (!ANY_SCALE) {
+    if (C::ALIKE ? u.beyond != 0 : __ballot(flags[u.lane % C::NW] != 0) != 0) return true;  // (in all waves)
+  }
+  if (!u.live) return false;
   if (elem == 1) float8_store<C, float>(acc, u.wm, u.wn, u.wave, u.lane, t.rows, t.cols, static_cast<float*>(y), ldy, smem);
   else if (elem == 2) float8_store<C, f16_t>(acc, u.wm, u.wn, u.wave, u.lane, t.rows, t.cols, static_cast<f16_t*>(y), ldy, smem);
   else float8_store<C, bf16_bits>(acc, u.wm, u.wn, u.wave, u.lane, t.rows, t.cols, static_cast<bf16_bits*>(y), ldy, smem);
+  return false;
+}
+
+// The tile again, whatever its scales, C::BM rows at a time.
+template <class C>
+__device__ __forceinline__ void float8_tile_any_scale(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
+  for (int first = 0; first < t.rows; first += C::BM) {
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    phase_barrier();  // what the waves read of LDS before is no longer wanted
+    F8Tile part = t;
+    part.a += (size_t)first * t.lda;
+    part.a_scales += (size_t)first * t.ldas;
+    part.rows = imin(t.rows - first, C::BM);
+    float8_tile<C, true>(part, static_cast<char*>(y) + (size_t)first * ldy * (elem == 1 ? 4 : 2), ldy, elem, smem);
+  }
 }
 
 }  // namespace rd
