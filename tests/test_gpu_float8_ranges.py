@@ -1,4 +1,4 @@
-"""The product on float8 with scales anywhere in float32's range, against 64 bits."""
+"""The product on float8 with scales anywhere in float32's range, and contractions of more than 64 blocks, against 64 bits."""
 
 import numpy as np
 import pytest
@@ -81,3 +81,39 @@ def test_scales_that_are_no_numbers_or_zero(trans):
     same[[3, 40, 50]] = False
     same[:30, :128] = False
     assert torch.equal(y[same], want[same])
+
+
+def _uneven(shape, axis, exponents, seed):
+    """Normal numbers whose blocks of 128 along ``axis`` differ by powers of two."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    by = torch.from_numpy(np.exp2(exponents)).cuda().float().repeat_interleave(128)[:shape[axis]]
+    return torch.randn(shape, generator=gen, device="cuda") * by.view([-1 if i == axis else 1 for i in range(len(shape))])
+
+
+@launches
+@pytest.mark.parametrize("k", [8193, 8320, 14336])
+def test_contractions_of_more_than_64_blocks(m, n, sizes, k):
+    """Weights [k, n], whose columns' scales are held 64 blocks at a time.  The scales differ from block to block by powers of two, the rows'
+    the other way round, so that every block counts alike and the scale of another one would show."""
+    print(f"long {m} x {k} x {n} {len(sizes)} groups", flush=True)
+    exponents = np.random.default_rng(k).integers(-12, 13, -(-k // 128)).astype(np.float64)
+    x, A = _uneven((m, k), 1, -exponents, 1), _uneven((len(sizes), k, n), 1, exponents, 2)
+    q, w = rd.quantize_rows(x), rd.quantize_weights(A)
+    y = rd.ragged_dot_float8(q, w, torch.tensor(sizes, dtype=torch.int32, device="cuda"), out_dtype=torch.float32)
+    ref, mag = _products(rd.dequantize(q, torch.float32).double(), rd.dequantize(w, torch.float32).double(), sizes, False)
+    # of eight products at most seven lose 2^-13 of the largest of them: less than 2^-10 of their sum; then fp32 sums
+    assert ((y.double() - ref).abs() <= (2.0 ** -10 + k * 2.0 ** -24) * mag).all()
+
+
+@pytest.mark.parametrize("m,sizes", [(6, [2, 4]), (300, [100, 200]), (1500, [1500])])
+def test_gradient_of_rows_over_more_than_64_blocks(m, sizes):
+    """Weights [n, k] of n beyond 8192: the rows' gradient is a product on them as [k, n]."""
+    k, n = 300, 9000
+    print(f"long gradient {m}", flush=True)
+    exponents = np.random.default_rng(n).integers(-12, 13, -(-n // 128)).astype(np.float64)
+    x = torch.randn(m, k, device="cuda").requires_grad_()
+    A, dy = _uneven((len(sizes), n, k), 1, exponents, 3), _uneven((m, n), 1, -exponents, 4)
+    w, gs = rd.quantize_weights(A), torch.tensor(sizes, dtype=torch.int32, device="cuda")
+    dx, = torch.autograd.grad(rd.ragged_dot_float8(x, w, gs, trans_rhs=True), x, dy)
+    ref, mag = _products(rd.dequantize(rd.quantize_rows(dy), torch.float32).double(), rd.dequantize(w, torch.float32).double(), sizes, False)
+    assert ((dx.double() - ref).abs() <= (2.0 ** -10 + n * 2.0 ** -24) * mag).all()
