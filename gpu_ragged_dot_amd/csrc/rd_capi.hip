@@ -1330,7 +1330,7 @@ static int check_float8(const void* codes, const void* scales, long long rows, i
   if (rows < 0 || cols < 0 || cols > rd::kF8MaxDim) return fail(RD_ERR_INVALID_ARGUMENT, "bad shape: %lld rows of %d", rows, cols);
   const int rc = check_moe(0, 1, 0, dtype);
   if (rc != RD_OK) return rc;
-  if (rows * rd::float8_scale_pitch(cols) >= (1ll << 28) || rows * ((cols + 7) / 8) > (1ll << 32) - 256)
+  if (rows * rd::float8_scale_pitch(cols) > (1ll << 28) - 16 || rows * ((cols + 7) / 8) > (1ll << 32) - 256)
     return fail(RD_ERR_UNSUPPORTED, "%lld rows of %d are more blocks than a launch has work-groups for", rows, cols);
   if (rows > 0 && cols > 0 && (!codes || !scales || ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) != 0))
     return fail(RD_ERR_INVALID_ARGUMENT, "the codes or scales are null or not 16-byte aligned");
