@@ -518,14 +518,16 @@ OrthoSizes sizes_of(int g, int k, int n) {
   return z;
 }
 
-// The largest |q(x)| for 0 <= x <= limit, of x p(x x) = a x + b x^3 + c x^5 or of b x + c x^2: at the end or where the derivative is 0.
+// The largest |q(x)| for 0 <= x <= limit, of x p(x x) = a x + b x^3 + c x^5 or of b x + c x^2: at the end or where the derivative is 0.  The
+// roots of a + 3 b y + 5 c y^2, y = x^2, without differences of what is nearly alike: h = -(3 b + sign(b) sqrt(9 b^2 - 20 a c)) gives the
+// one as h / (10 c) and the other as 2 a / h, which is the cubic's where c is next to nothing.
 double largest(double limit, double a, double b, double c) {
-  double top = 0;
-  auto see = [&](double x) { if (x >= 0 && x <= limit) top = fmax(top, fabs(x * (a + x * x * (b + x * x * c)))); };
-  see(limit);
-  const double d = 9 * b * b - 20 * a * c;  // a + 3 b y + 5 c y^2 = 0, y = x^2
-  if (c != 0 && d >= 0) { see(sqrt(fmax(0.0, (-3 * b + sqrt(d)) / (10 * c)))); see(sqrt(fmax(0.0, (-3 * b - sqrt(d)) / (10 * c)))); }
-  else if (b != 0) see(sqrt(fmax(0.0, -a / (3 * b))));
+  const auto value = [&](double x) { return fabs(x * (a + x * x * (b + x * x * c))); };
+  double top = value(limit);
+  const double unit = fmax(fmax(fabs(a), fabs(b)), fabs(c));  // (squares of coefficients beyond 1e154)
+  const double h = -(3 * (b / unit) + copysign(sqrt(9 * (b / unit) * (b / unit) - 20 * (a / unit) * (c / unit)), b));
+  for (const double y : {h / (10 * (c / unit)), 2 * (a / unit) / h})
+    if (y >= 0 && sqrt(y) <= limit) top = fmax(top, value(sqrt(y)));  // (no roots: y is no number)
   return top;
 }
 double largest_square(double limit, double b, double c) {

@@ -1,0 +1,39 @@
+"""Orthogonalised updates of any size of numbers, rank and coefficients, against 64 bits and relative to the result."""
+
+import numpy as np
+import pytest
+import torch
+
+import gpu_ragged_dot_amd as rd
+from gpu_ragged_dot_amd.ortho import COEFFICIENTS
+from oracle import ortho_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+HALF_ULP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+types = pytest.mark.parametrize("dtype", list(TYPES.values()), ids=list(TYPES))
+wide_types = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])  # with eight bits of exponent
+
+
+def _np(t):
+    return t.double().cpu().numpy()
+
+
+def _randn(*shape, seed=0):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
+
+
+def _relative(got, ref):
+    return np.linalg.norm(_np(got) - ref) / np.linalg.norm(ref)
+
+
+@types
+def test_a_nearly_cubic_step(dtype):
+    """c so small that the largest value lies where the cubic's does, at 3^-1/2, where all singular values are; what the next step's numbers
+    are multiplied with follows from it."""
+    G = torch.eye(3, 5)[None].repeat(2, 1, 1).to(dtype).cuda()
+    for c in (1e-20, -1e-20, 1e-300, 0.0):
+        out = rd.orthogonalize(G, steps=2, coefficients=[(3.0, -3.0, c), (1.0, 0.0, 0.0)], eps=0.0)
+        # 2 / 3^1/2 on the diagonal.  Two steps: roundings of X, A and B, each of 22 or 11 bits, times 3 at most
+        assert ((out.double() - G.double() * 2 / 3 ** 0.5).abs() <= (2.0 ** -18 if dtype == torch.float32 else 2.0 ** -7) + 2 * HALF_ULP[dtype]).all()
