@@ -1434,7 +1434,7 @@ int rd_orthogonalize(void* stream, const void* G, void* out, int g, int k, int n
     return fail(RD_ERR_INVALID_ARGUMENT, "no spec, no coefficients, or steps outside 0..%d", rd::kOrthoMaxSteps);
   for (int i = 0; i < 3 * spec->steps; ++i)
     if (!(spec->coefficients[i] - spec->coefficients[i] == 0)) return fail(RD_ERR_INVALID_ARGUMENT, "coefficients must be finite");
-  if (!(spec->eps >= 0) || !(spec->eps - spec->eps == 0) || !(spec->scale - spec->scale == 0)) return fail(RD_ERR_INVALID_ARGUMENT, "eps must be finite and not negative, scale finite");
+  if (!(spec->eps >= 0) || !(spec->eps - spec->eps == 0) || !((float)spec->scale - (float)spec->scale == 0)) return fail(RD_ERR_INVALID_ARGUMENT, "eps must be finite and not negative, scale a finite float32");
   if (!(rd::ortho_growth(spec->steps, spec->coefficients) <= 1024))
     return fail(RD_ERR_INVALID_ARGUMENT, "these coefficients lead singular values beyond 1024: the iteration does not converge");
   if (g == 0 || k == 0 || n == 0) return RD_OK;

@@ -173,6 +173,7 @@ struct OrthoStep {
   Planes left, right;  // operands: the product is left right' (kGram, kSquare), or left right
   Planes add, to;      // result = of_product * product + of_add * add (kGram: no second term)
   float of_product, of_add;
+  float scale;         // kLast: of the result
   int g, tiles_r, tiles_c, per_matrix;
   // kLast: the numbers themselves, [k][n]
   void* out;
@@ -412,7 +413,9 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
           add_high(v, add_hi[i & AHEAD][t], p.of_add);
           if constexpr (ADDS_LO) add_low(v, add_lo[i & AHEAD][t], p.of_add);
         }
-        if constexpr (KIND == kLast) {
+        if constexpr (KIND == kLast) {  // (apart from the others' factors, with which a small scale would be less than a normal number)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] *= p.scale;
           if (!p.tall) store_last(p, e, pr + t * STEP + own_r, pc + own_c, v);
         } else {
           const long long cell = own + (long long)(i * 32 + t * STEP) * p.to.cols;
@@ -455,8 +458,8 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_divide_kernel(const T* __
                                                                      int chunks, double eps, double scale) {
   const long long e = blockIdx.x / chunks, first = (blockIdx.x - e * chunks) * (long long)kOrthoChunk;
   const double sum = sum_of(partial + e * chunks, chunks);
-  const float by = (float)(scale / (sqrt(sum) + eps + (sum - sum)));
-  for (long long i = first + threadIdx.x; i < size && i < first + kOrthoChunk; i += kOrthoThreads) out[e * size + i] = from_f32<T>(to_f32<T>(G[e * size + i]) * by);
+  const double by = scale / (sqrt(sum) + eps + (sum - sum));
+  for (long long i = first + threadIdx.x; i < size && i < first + kOrthoChunk; i += kOrthoThreads) out[e * size + i] = from_f32<T>((float)(to_f32<T>(G[e * size + i]) * by));
 }
 
 // Which tiles: the least time by rounds of what the device holds, 256 compute units of one or two work-groups, in tiles of 128 x 128.  As
@@ -590,8 +593,9 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
     t.right = t.add = X[i & 1];
     t.to = X[(i + 1) & 1];
     if (!two && i + 2 == p.steps) t.to.lo = nullptr;
-    t.of_product = last ? (float)ldexp(p.scale, -eb - ex) : (float)ldexp(1.0, en - eb - ex);
-    t.of_add = last ? (float)ldexp(a * p.scale, -ex) : (float)ldexp(a, en - ex);
+    t.of_product = (float)ldexp(1.0, (last ? 0 : en) - eb - ex);
+    t.of_add = (float)ldexp(a, (last ? 0 : en) - ex);
+    t.scale = (float)p.scale;
     t.out = p.out; t.k = p.k; t.n = p.n; t.elem = p.elem; t.tall = tall;
     if ((rc = last ? launch_product<kLast>(s, t, two) : launch_product<kApply>(s, t, two)) != hipSuccess) return rc;
     bound = next;

@@ -37,3 +37,16 @@ def test_a_nearly_cubic_step(dtype):
         out = rd.orthogonalize(G, steps=2, coefficients=[(3.0, -3.0, c), (1.0, 0.0, 0.0)], eps=0.0)
         # 2 / 3^1/2 on the diagonal.  Two steps: roundings of X, A and B, each of 22 or 11 bits, times 3 at most
         assert ((out.double() - G.double() * 2 / 3 ** 0.5).abs() <= (2.0 ** -18 if dtype == torch.float32 else 2.0 ** -7) + 2 * HALF_ULP[dtype]).all()
+
+
+def test_scales_of_any_size():
+    for shape, steps in (((60, 100), 5), ((100, 60), 5), ((60, 100), 1), ((60, 100), 0)):
+        G = _randn(*shape, seed=6).cuda()
+        base = rd.orthogonalize(G, steps=steps)
+        base[base.abs() < 2.0 ** -8] = 0
+        for power in (-116, -60, 60, 116):
+            got = rd.orthogonalize(G, steps=steps, scale=2.0 ** power)
+            got[base == 0] = 0
+            assert torch.equal(got, base * 2.0 ** power)
+    with pytest.raises(RuntimeError, match="scale"):
+        rd.orthogonalize(G, scale=1e39)

@@ -25,3 +25,8 @@ def test_growth_of_nearly_cubic_steps():
         assert _call([(1e200, -1e200, c)]) == INVALID and b"converge" in lib.rd_last_error(), c
     assert _call([(0.0, 0.0, 2000.0)]) == INVALID and _call([(0.0, 0.0, 1000.0)], g=0) == 0
     assert _call([(0.0, -2000.0, 0.0)]) == INVALID and _call([(0.0, 0.0, 0.0)], g=0) == 0
+
+
+def test_scale_is_a_float32():
+    assert _call([(1.0, 0.0, 0.0)], scale=1e39) == INVALID and b"scale" in lib.rd_last_error()
+    assert _call([(1.0, 0.0, 0.0)], scale=-3e38, g=0) == 0
