@@ -111,6 +111,8 @@ __device__ __forceinline__ double sum_of(const double* __restrict__ partial, int
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
   return sum;
 }
+// 1 / (norm + eps) of a sum of squares; NaN for one that is no number; of zeros, which stay 0 whatever eps, 0.
+__device__ __forceinline__ double reciprocal_norm(double sum, double eps) { return sum == 0 ? 0. : 1 / (sqrt(sum) + eps + (sum - sum)); }
 
 // X = G / (norm + eps), 64 x 64 numbers of the padded X per work-group; `tall`: X is the transpose of G.
 // Memory: 128 x 2048 x 768 bf16 192 us, 5.2 TB/s.
@@ -139,14 +141,16 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_start_kernel(const T* __r
       for (int i = 0; i < 8; ++i) v[h][i] = r < k && c + i < n ? to_f32<T>(g[(long long)r * n + c + i]) : 0.f;
     }
   }
-  const double sum = sum_of(partial + e * chunks, chunks);
-  const float by = (float)((double)factor / (sqrt(sum) + eps + (sum - sum)));  // (NaN for a sum that is no number)
+  // a power of two and a number between 1/2 and 1: the factor of small norms is beyond float32
+  int power;
+  const float by = (float)frexp(reciprocal_norm(sum_of(partial + e * chunks, chunks), eps) * factor, &power);
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int y = threadIdx.x / 8 + 32 * h;
-      if (tall) tile[x + i][y] = v[h][i] * by; else tile[y][x + i] = v[h][i] * by;
+      const float w = __builtin_ldexpf(v[h][i], power) * by;
+      if (tall) tile[x + i][y] = w; else tile[y][x + i] = w;
     }
   __syncthreads();
 #pragma unroll
@@ -457,8 +461,7 @@ template <class T>
 __global__ __launch_bounds__(kOrthoThreads) void ortho_divide_kernel(const T* __restrict__ G, const double* __restrict__ partial, T* __restrict__ out, long long size,
                                                                      int chunks, double eps, double scale) {
   const long long e = blockIdx.x / chunks, first = (blockIdx.x - e * chunks) * (long long)kOrthoChunk;
-  const double sum = sum_of(partial + e * chunks, chunks);
-  const double by = scale / (sqrt(sum) + eps + (sum - sum));
+  const double by = scale * reciprocal_norm(sum_of(partial + e * chunks, chunks), eps);
   for (long long i = first + threadIdx.x; i < size && i < first + kOrthoChunk; i += kOrthoThreads) out[e * size + i] = from_f32<T>((float)(to_f32<T>(G[e * size + i]) * by));
 }
 

@@ -29,6 +29,28 @@ def _relative(got, ref):
 
 
 @types
+@pytest.mark.parametrize("steps", [0, 1, 5])
+def test_zeros_stay_zeros_without_eps(steps, dtype):
+    """Such as the gradient of an expert that saw no token, among others."""
+    G = _randn(3, 70, 200).to(dtype).cuda()
+    G[1] = 0
+    out = rd.orthogonalize(G, steps=steps, eps=0.0)
+    assert not out[1].any()
+    for e in (0, 2):
+        assert torch.equal(out[e], rd.orthogonalize(G[e], steps=steps, eps=0.0)) and out[e].isfinite().all()
+
+
+@wide_types
+@pytest.mark.parametrize("power", [-120, -100, 100])
+def test_without_eps_a_power_of_two_changes_nothing(power, dtype):
+    for shape in ((70, 200), (200, 70)):
+        G = _randn(*shape, seed=1).to(dtype).cuda()
+        G[G.abs() < 2.0 ** -5] = 0  # (what stays a normal number)
+        for steps in (0, 1, 5):
+            assert torch.equal(rd.orthogonalize(G * 2.0 ** power, steps=steps, eps=0.0), rd.orthogonalize(G, steps=steps, eps=0.0))
+
+
+@types
 def test_a_nearly_cubic_step(dtype):
     """c so small that the largest value lies where the cubic's does, at 3^-1/2, where all singular values are; what the next step's numbers
     are multiplied with follows from it."""
