@@ -3,8 +3,8 @@
 // with X the smaller side down (G or its transpose), which drives the singular values of X towards one.  Three products of matrices
 // per step, of which the first two are symmetric: their tiles on and below the diagonal are computed, and written twice.
 //
-// Numbers are float16 times a power of two per step and matrix kind that the growth of the singular values allows (|X|, |A| and |B|
-// are bounded by polynomials of it), so that 2^15 is reached and 2^-29 of it still has all eleven bits.  float16 and not bfloat16:
+// Numbers are float16 times a power of two per matrix, step and kind that the growth of the singular values allows (|X|, |A| and |B|
+// are bounded by polynomials of it, from |G|_F / (|G|_F + eps) on), so that 2^15 is reached and 2^-29 of it still has all eleven bits.  float16 and not bfloat16:
 // eleven bits instead of eight at the same rate.  What the tiles add up is fp32.
 //   16-bit G:  X is held in two numbers, hi + lo, of which the products take hi; A and B in one.  Along the small singular values of X
 //              every step multiplies what is there by a = 3.4, the rounding of X included, until after five steps it has grown 485 times:
@@ -113,17 +113,96 @@ __device__ __forceinline__ double sum_of(const double* __restrict__ partial, int
 }
 // 1 / (norm + eps) of a sum of squares; NaN for one that is no number; of zeros, which stay 0 whatever eps, 0.
 __device__ __forceinline__ double reciprocal_norm(double sum, double eps) { return sum == 0 ? 0. : 1 / (sqrt(sum) + eps + (sum - sum)); }
+// What the singular values of X = G / (norm + eps) are below.
+__device__ __forceinline__ double bound_of(double sum, double eps) { return sum > 0 ? sqrt(sum) * reciprocal_norm(sum, eps) : 1; }
+
+// ---- bounds of the singular values ------------------------------------------------------------------------------------------
+// A step's coefficients with what the host finds out: the places x where the derivative of q(x) = a x + b x^3 + c x^5 is 0, y of that of
+// b y + c y^2, and the magnitudes there (places that there are not: beyond every limit).
+struct OrthoTriple {
+  double a, b, c, extreme[2], value[2], vertex, vertex_value;
+};
+struct OrthoTriples {
+  OrthoTriple step[kOrthoMaxSteps];
+  int steps;
+};
+__host__ __device__ inline double value_at(const OrthoTriple& t, double x) { return fabs(x * (t.a + x * x * (t.b + x * x * t.c))); }
+// The largest |q(x)| for 0 <= x <= limit: at the end or where the derivative is 0; and |b y + c y^2| up to y = limit.
+__host__ __device__ inline double largest(const OrthoTriple& t, double limit) {
+  const double first = t.extreme[0] <= limit ? t.value[0] : 0, second = t.extreme[1] <= limit ? t.value[1] : 0;
+  return fmax(value_at(t, limit), fmax(first, second));
+}
+__host__ __device__ inline double largest_square(const OrthoTriple& t, double limit) {
+  return fmax(fabs(limit * (t.b + limit * t.c)), t.vertex <= limit ? t.vertex_value : 0);
+}
+// The power of two that takes numbers up to `top` to 2^15 at most, with room for what roundings add; and keeps factors normal numbers.
+__host__ __device__ inline int exponent_for(double top) {
+  int e;
+  frexp(top * 1.01, &e);
+  return top > 0 && 15 - e < 100 ? 15 - e : 100;
+}
+// The roots of a + 3 b y + 5 c y^2, y = x^2, without differences of what is nearly alike: h = -(3 b + sign(b) sqrt(9 b^2 - 20 a c)) gives the
+// one as h / (10 c) and the other as 2 a / h, which is the cubic's where c is next to nothing.
+OrthoTriple triple_of(double a, double b, double c) {
+  OrthoTriple t{a, b, c, {HUGE_VAL, HUGE_VAL}, {0, 0}, HUGE_VAL, 0};
+  const double unit = fmax(fmax(fabs(a), fabs(b)), fabs(c));  // (squares of coefficients beyond 1e154)
+  const double h = -(3 * (b / unit) + copysign(sqrt(9 * (b / unit) * (b / unit) - 20 * (a / unit) * (c / unit)), b));
+  const double y[2] = {h / (10 * (c / unit)), 2 * (a / unit) / h};
+  for (int i = 0; i < 2; ++i)
+    if (y[i] >= 0) {  // (no roots: y is no number)
+      t.extreme[i] = sqrt(y[i]);
+      t.value[i] = value_at(t, t.extreme[i]);
+    }
+  if (-b / (2 * c) >= 0) {
+    t.vertex = -b / (2 * c);
+    t.vertex_value = fabs(t.vertex * (b / 2));
+  }
+  return t;
+}
+OrthoTriples triples_of(int steps, const double* coefficients) {
+  OrthoTriples t;
+  t.steps = steps;
+  for (int i = 0; i < steps; ++i) t.step[i] = triple_of(coefficients[3 * i], coefficients[3 * i + 1], coefficients[3 * i + 2]);
+  return t;
+}
+
+// What a product multiplies its sums and what it adds by, and the last one its result.
+struct OrthoFactors {
+  float of_product, of_add, unit, none;
+};
+// Of the three products of a step whose singular values start below `bound`.
+__device__ __forceinline__ void factors_of(const OrthoTriple& t, double bound, bool last, OrthoFactors* __restrict__ to) {
+  const int ex = exponent_for(bound), ea = exponent_for(bound * bound), eb = exponent_for(largest_square(t, bound * bound)), en = exponent_for(largest(t, bound));
+  to[0] = {(float)ldexp(1., ea - 2 * ex), 0.f, 1.f, 0.f};
+  to[1] = {(float)ldexp(t.c, eb - 2 * ea), (float)ldexp(t.b, eb - ea), 1.f, 0.f};
+  // (the last one's unit apart: together they would be less than normal numbers where singular values are small)
+  to[2] = last ? OrthoFactors{(float)ldexp(1., -eb), (float)t.a, (float)ldexp(1., -ex), 0.f}
+               : OrthoFactors{(float)ldexp(1., en - eb - ex), (float)ldexp(t.a, en - ex), 1.f, 0.f};
+}
 
 // X = G / (norm + eps), 64 x 64 numbers of the padded X per work-group; `tall`: X is the transpose of G.
-// Memory: 128 x 2048 x 768 bf16 192 us, 5.2 TB/s.
+// Memory: 128 x 2048 x 768 bf16 192 us, 5.2 TB/s.  The first g work-groups work out the factors of a matrix each, a lane those of a step
+// (4 x 256 x 512: 4.5 us; in the first work-group of the matrix's tiles 5.7).
 template <class T>
 __global__ __launch_bounds__(kOrthoThreads) void ortho_start_kernel(const T* __restrict__ G, const double* __restrict__ partial, int chunks, half_bits* __restrict__ hi,
-                                                                    void* __restrict__ lo, int k, int n, int rp, int cp, bool tall, double eps, float factor) {
+                                                                    void* __restrict__ lo, int g, int k, int n, int rp, int cp, bool tall, double eps, OrthoTriples triples,
+                                                                    OrthoFactors* __restrict__ factors) {
   __shared__ float tile[64][65];
-  const int across = cp / 64, down = rp / 64;
-  const long long e = blockIdx.x / (across * down);
-  const int in_matrix = (int)(blockIdx.x - e * across * down), r0 = in_matrix / across * 64, c0 = in_matrix % across * 64;
-  const T* g = G + e * k * n;
+  if ((int)blockIdx.x < g) {
+    const double sum = sum_of(partial + (long long)blockIdx.x * chunks, chunks);
+    double bound = bound_of(sum, eps), own = bound;
+    for (int i = 0; i < triples.steps; ++i) {
+      if (i == (int)threadIdx.x) own = bound;
+      bound = largest(triples.step[i], bound);
+    }
+    if ((int)threadIdx.x < triples.steps)
+      factors_of(triples.step[threadIdx.x], own, (int)threadIdx.x + 1 == triples.steps, factors + ((long long)blockIdx.x * triples.steps + threadIdx.x) * 3);
+    return;
+  }
+  const int block = (int)blockIdx.x - g, across = cp / 64, down = rp / 64;
+  const long long e = block / (across * down);
+  const int in_matrix = (int)(block - e * across * down), r0 = in_matrix / across * 64, c0 = in_matrix % across * 64;
+  const T* from = G + e * k * n;
   // eight neighbours of a row of G to a thread, twice
   const int gr = tall ? c0 : r0, gc = tall ? r0 : c0, x = threadIdx.x % 8 * 8;
   float v[2][8];
@@ -133,17 +212,18 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_start_kernel(const T* __r
     if (r < k && c + 8 <= n) {
       alignas(16) T in[8];
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(in) / 16; ++i) reinterpret_cast<u32x4_t*>(in)[i] = load_any<u32x4_t>(g + (long long)r * n + c + i * (16 / sizeof(T)));
+      for (int i = 0; i < (int)sizeof(in) / 16; ++i) reinterpret_cast<u32x4_t*>(in)[i] = load_any<u32x4_t>(from + (long long)r * n + c + i * (16 / sizeof(T)));
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[h][i] = to_f32<T>(in[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[h][i] = r < k && c + i < n ? to_f32<T>(g[(long long)r * n + c + i]) : 0.f;
+      for (int i = 0; i < 8; ++i) v[h][i] = r < k && c + i < n ? to_f32<T>(from[(long long)r * n + c + i]) : 0.f;
     }
   }
+  const double sum = sum_of(partial + e * chunks, chunks);
   // a power of two and a number between 1/2 and 1: the factor of small norms is beyond float32
   int power;
-  const float by = (float)frexp(reciprocal_norm(sum_of(partial + e * chunks, chunks), eps) * factor, &power);
+  const float by = (float)frexp(ldexp(reciprocal_norm(sum, eps), exponent_for(bound_of(sum, eps))), &power);
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -175,9 +255,10 @@ struct Planes {
 enum OrthoKind { kGram, kSquare, kApply, kLast };
 struct OrthoStep {
   Planes left, right;  // operands: the product is left right' (kGram, kSquare), or left right
-  Planes add, to;      // result = of_product * product + of_add * add (kGram: no second term)
-  float of_product, of_add;
-  float scale;         // kLast: of the result
+  Planes add, to;      // result = of_product * product + of_add * add (kGram: no second term), of the matrix's factors, kLast: times unit and scale
+  const OrthoFactors* factors;  // of the first matrix; those of the next one are `stride` behind it
+  int stride;
+  float scale;
   int g, tiles_r, tiles_c, per_matrix;
   // kLast: the numbers themselves, [k][n]
   void* out;
@@ -313,6 +394,8 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
   const bool live = wm * C::WM < rows && wn * C::WN < cols;
 
+  // one to a lane, on their way with the first slabs (a scalar load's result would be waited for in front of them, or behind the K loop)
+  const float factors = reinterpret_cast<const float*>(p.factors + e * p.stride)[lane & 3];
   f32x16_t acc[C::TM][C::TN];
 #pragma unroll
   for (int i = 0; i < C::TM; ++i)
@@ -361,6 +444,8 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
       for (int j = 0; j < C::TN; ++j) acc[i][j] = sum[i][j];
   }
   if (!live) return;
+  const auto factor = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, factors), i)); };
+  const OrthoFactors by = {factor(0), factor(1), factor(2), 0.f};
 
   // by way of LDS, 32 rows of the wave's columns at a time, for eight neighbours of a row to a lane, or of a column; what is added is
   // requested before, a piece ahead where registers allow
@@ -411,15 +496,15 @@ __global__ __launch_bounds__(kOrthoThreads, (ortho_groups<BM, KIND == kGram || K
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const f32x4_t w = *reinterpret_cast<const f32x4_t*>(at + 4 * q);
-          v[4 * q] = w[0] * p.of_product; v[4 * q + 1] = w[1] * p.of_product; v[4 * q + 2] = w[2] * p.of_product; v[4 * q + 3] = w[3] * p.of_product;
+          v[4 * q] = w[0] * by.of_product; v[4 * q + 1] = w[1] * by.of_product; v[4 * q + 2] = w[2] * by.of_product; v[4 * q + 3] = w[3] * by.of_product;
         }
         if constexpr (ADDS) {
-          add_high(v, add_hi[i & AHEAD][t], p.of_add);
-          if constexpr (ADDS_LO) add_low(v, add_lo[i & AHEAD][t], p.of_add);
+          add_high(v, add_hi[i & AHEAD][t], by.of_add);
+          if constexpr (ADDS_LO) add_low(v, add_lo[i & AHEAD][t], by.of_add);
         }
-        if constexpr (KIND == kLast) {  // (apart from the others' factors, with which a small scale would be less than a normal number)
+        if constexpr (KIND == kLast) {  // (one after the other: together they may be less than a normal number)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] *= p.scale;
+          for (int q = 0; q < 8; ++q) v[q] = v[q] * by.unit * p.scale;
           if (!p.tall) store_last(p, e, pr + t * STEP + own_r, pc + own_c, v);
         } else {
           const long long cell = own + (long long)(i * 32 + t * STEP) * p.to.cols;
@@ -508,7 +593,7 @@ int launch_product(hipStream_t s, const OrthoStep& p, bool two) {
 
 struct OrthoSizes {
   int rp, cp, chunks;
-  size_t norm, x, bytes, square;  // bytes of the sums of squares, of one plane of X and one of its bytes, and of one of A
+  size_t norm, factors, x, bytes, square;  // bytes of the sums of squares, of the products' factors, of one plane of X and one of its bytes, and of one of A
 };
 size_t up(size_t b) { return (b + 255) / 256 * 256; }
 OrthoSizes sizes_of(int g, int k, int n) {
@@ -518,34 +603,11 @@ OrthoSizes sizes_of(int g, int k, int n) {
   z.cp = (c + kOrthoPad - 1) / kOrthoPad * kOrthoPad;
   z.chunks = (int)(((long long)k * n + kOrthoChunk - 1) / kOrthoChunk);
   z.norm = up((size_t)g * z.chunks * sizeof(double));
+  z.factors = up((size_t)g * kOrthoMaxSteps * 3 * sizeof(OrthoFactors));
   z.x = up((size_t)g * z.rp * z.cp * 2);
   z.bytes = up((size_t)g * z.rp * z.cp);
   z.square = up((size_t)g * z.rp * z.rp * 2);
   return z;
-}
-
-// The largest |q(x)| for 0 <= x <= limit, of x p(x x) = a x + b x^3 + c x^5 or of b x + c x^2: at the end or where the derivative is 0.  The
-// roots of a + 3 b y + 5 c y^2, y = x^2, without differences of what is nearly alike: h = -(3 b + sign(b) sqrt(9 b^2 - 20 a c)) gives the
-// one as h / (10 c) and the other as 2 a / h, which is the cubic's where c is next to nothing.
-double largest(double limit, double a, double b, double c) {
-  const auto value = [&](double x) { return fabs(x * (a + x * x * (b + x * x * c))); };
-  double top = value(limit);
-  const double unit = fmax(fmax(fabs(a), fabs(b)), fabs(c));  // (squares of coefficients beyond 1e154)
-  const double h = -(3 * (b / unit) + copysign(sqrt(9 * (b / unit) * (b / unit) - 20 * (a / unit) * (c / unit)), b));
-  for (const double y : {h / (10 * (c / unit)), 2 * (a / unit) / h})
-    if (y >= 0 && sqrt(y) <= limit) top = fmax(top, value(sqrt(y)));  // (no roots: y is no number)
-  return top;
-}
-double largest_square(double limit, double b, double c) {
-  double top = fabs(limit * (b + limit * c));
-  if (c != 0 && -b / (2 * c) >= 0 && -b / (2 * c) <= limit) top = fmax(top, b * b / (4 * fabs(c)));
-  return top;
-}
-// The power of two that takes numbers up to `top` to 2^15 at most, with room for what roundings add.
-int exponent_for(double top) {
-  int e;
-  frexp(fmax(top * 1.01, 0x1p-9), &e);
-  return 15 - e;
 }
 
 template <class T>
@@ -555,6 +617,8 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
   char* ws = static_cast<char*>(p.workspace);
   double* partial = reinterpret_cast<double*>(ws);
   ws += z.norm;
+  OrthoFactors* factors = reinterpret_cast<OrthoFactors*>(ws);
+  ws += z.factors;
   auto planes = [&](int rows, int cols, size_t bytes, size_t lo) {
     Planes q{reinterpret_cast<half_bits*>(ws), lo ? ws + bytes : nullptr, rows, cols};
     ws += bytes + lo;
@@ -570,39 +634,28 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
     hipLaunchKernelGGL((ortho_divide_kernel<T>), dim3((unsigned)(p.g * z.chunks)), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, (T*)p.out, size, z.chunks, p.eps, p.scale);
     return (int)hipGetLastError();
   }
-  double bound = 1;
-  int ex = exponent_for(bound);
-  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3((unsigned)(p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, z.chunks, X[0].hi, two || p.steps > 1 ? X[0].lo : nullptr,
-                     p.k, p.n, z.rp, z.cp, tall, p.eps, (float)ldexp(1.0, ex));
+  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3((unsigned)(p.g + p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, z.chunks, X[0].hi,
+                     two || p.steps > 1 ? X[0].lo : nullptr, p.g, p.k, p.n, z.rp, z.cp, tall, p.eps, triples_of(p.steps, p.coefficients), factors);
   if ((rc = (int)hipGetLastError()) != hipSuccess) return rc;
+  OrthoStep t{};
+  t.g = p.g; t.stride = 3 * p.steps;
+  t.out = p.out; t.k = p.k; t.n = p.n; t.elem = p.elem; t.tall = tall; t.scale = (float)p.scale;
   for (int i = 0; i < p.steps; ++i) {
-    const double a = p.coefficients[3 * i], b = p.coefficients[3 * i + 1], c = p.coefficients[3 * i + 2];
-    const int ea = exponent_for(bound * bound), eb = exponent_for(largest_square(bound * bound, b, c));
-    OrthoStep t{};
-    t.g = p.g;
+    t.factors = factors + 3 * i;
     t.left = t.right = X[i & 1];
     t.to = A;
-    t.of_product = (float)ldexp(1.0, ea - 2 * ex);
     if ((rc = launch_product<kGram>(s, t, two)) != hipSuccess) return rc;
+    ++t.factors;
     t.left = t.right = t.add = A;
     t.to = B;
-    t.of_product = (float)ldexp(c, eb - 2 * ea);
-    t.of_add = (float)ldexp(b, eb - ea);
     if ((rc = launch_product<kSquare>(s, t, two)) != hipSuccess) return rc;
+    ++t.factors;
     const bool last = i + 1 == p.steps;
-    const double next = largest(bound, a, b, c);
-    const int en = exponent_for(next);
     t.left = B;
     t.right = t.add = X[i & 1];
     t.to = X[(i + 1) & 1];
     if (!two && i + 2 == p.steps) t.to.lo = nullptr;
-    t.of_product = (float)ldexp(1.0, (last ? 0 : en) - eb - ex);
-    t.of_add = (float)ldexp(a, (last ? 0 : en) - ex);
-    t.scale = (float)p.scale;
-    t.out = p.out; t.k = p.k; t.n = p.n; t.elem = p.elem; t.tall = tall;
     if ((rc = last ? launch_product<kLast>(s, t, two) : launch_product<kApply>(s, t, two)) != hipSuccess) return rc;
-    bound = next;
-    ex = en;
   }
   return hipSuccess;
 }
@@ -611,7 +664,7 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
 
 size_t ortho_workspace_bytes(int g, int k, int n, int elem) {
   const OrthoSizes z = sizes_of(g, k, n);
-  return z.norm + 2 * z.x + 2 * (elem == 1 ? z.x : z.bytes) + (elem == 1 ? 4 : 2) * z.square;
+  return z.norm + z.factors + 2 * z.x + 2 * (elem == 1 ? z.x : z.bytes) + (elem == 1 ? 4 : 2) * z.square;
 }
 
 bool ortho_grid_fits(int g, int k, int n) {
@@ -624,7 +677,7 @@ bool ortho_grid_fits(int g, int k, int n) {
 double ortho_growth(int steps, const double* coefficients) {
   double bound = 1, top = 1;
   for (int i = 0; i < steps; ++i) {
-    bound = largest(bound, coefficients[3 * i], coefficients[3 * i + 1], coefficients[3 * i + 2]);
+    bound = largest(triple_of(coefficients[3 * i], coefficients[3 * i + 1], coefficients[3 * i + 2]), bound);
     top = fmax(top, bound);
   }
   return top;

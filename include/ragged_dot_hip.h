@@ -334,7 +334,8 @@ int rd_gmm_float8(void* stream, const void* x, const float* x_scales, const void
  * come out between 0.7 and 1.2, whatever they were from |G|_F / 500 on.  The norm is a 64-bit sum; sums of products are fp32.  For
  * 16-bit G products are of float16 numbers, with X held in 15 bits: results are off by 2e-3 of their norm (up to 8e-3
  * where there are few rows or columns, whose roundings do not average out).  For float32 every
- * product is of 22-bit numbers, as accurate as float32 products.  An infinity or NaN makes its matrix NaN; a matrix of zeros stays 0.
+ * product is of 22-bit numbers, as accurate as float32 products.  Both also where |G|_F is far below eps (down to 1e-25 of it) or
+ * coefficients make X small.  An infinity or NaN makes its matrix NaN; a matrix of zeros stays 0.
  * steps 0..32; coefficients: host, [steps][3], finite, such that no singular value from 0 to 1 is led beyond 1024; eps >= 0 finite,
  * scale a finite float32.  g, k, n >= 1 with a padded matrix below 2^30 numbers, and what a launch has of work-groups (RD_ERR_UNSUPPORTED beyond).
  * Workspace: rd_orthogonalize_workspace_bytes() bytes, 256-byte aligned, for X twice, A and B.  G and out do not overlap, or are the same. */

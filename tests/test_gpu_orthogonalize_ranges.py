@@ -28,6 +28,11 @@ def _relative(got, ref):
     return np.linalg.norm(_np(got) - ref) / np.linalg.norm(ref)
 
 
+# One rounding of X to what it is held in, relative: 22 bits for float32; 15 for 16-bit numbers, 11 before the last step.  Where the
+# iteration is linear, all directions grow alike and the roundings of up to eight steps add up as they are.
+LINEAR = {torch.float32: 8 * 2.0 ** -22, torch.bfloat16: 8 * 2.0 ** -15 + 2.0 ** -11, torch.float16: 8 * 2.0 ** -15 + 2.0 ** -11}
+
+
 @types
 @pytest.mark.parametrize("steps", [0, 1, 5])
 def test_zeros_stay_zeros_without_eps(steps, dtype):
@@ -48,6 +53,35 @@ def test_without_eps_a_power_of_two_changes_nothing(power, dtype):
         G[G.abs() < 2.0 ** -5] = 0  # (what stays a normal number)
         for steps in (0, 1, 5):
             assert torch.equal(rd.orthogonalize(G * 2.0 ** power, steps=steps, eps=0.0), rd.orthogonalize(G, steps=steps, eps=0.0))
+
+
+@wide_types
+@pytest.mark.parametrize("size", [1e-11, 1e-13, 1e-15, 1e-18, 1e-25])
+def test_norms_far_below_eps(size, dtype):
+    """X starts at |G| / eps and every step multiplies it by a."""
+    G = _randn(70, 80, seed=2)
+    G = (G * (size / G.norm())).to(dtype).cuda()
+    ref = oracle.orthogonalize(_np(G), [COEFFICIENTS] * 5)
+    assert _relative(rd.orthogonalize(G), ref) <= LINEAR[dtype] + HALF_ULP[dtype]
+
+
+@wide_types
+@pytest.mark.parametrize("a,steps", [(0.01, 8), (2.0 ** -9, 5), (0.25, 8)])
+def test_coefficients_that_shrink(a, steps, dtype):
+    G = _randn(130, 90, seed=3).to(dtype).cuda()
+    for triple in ((a, 0.0, 0.0), (a, -0.1 * a, 0.0)):
+        ref = oracle.orthogonalize(_np(G), [triple] * steps)
+        assert _relative(rd.orthogonalize(G, steps=steps, coefficients=triple), ref) <= LINEAR[dtype] + HALF_ULP[dtype]
+
+
+def test_norms_of_every_size_in_one_stack():
+    G = _randn(6, 100, 140, seed=4)
+    G *= torch.tensor([1.0, 1e-9, 1e-20, 0.0, 1e12, 1e-6])[:, None, None]
+    for dtype in (torch.float32, torch.bfloat16):
+        H = G.to(dtype).cuda()
+        out = rd.orthogonalize(H)
+        for e in range(len(G)):
+            assert torch.equal(rd.orthogonalize(H[e]), out[e])
 
 
 @types
