@@ -125,6 +125,7 @@ EXPORTS = (
     "rd_moe_swiglu_float8",
     "rd_gmm_float8",
     "rd_orthogonalize_workspace_bytes",
+    "rd_orthogonalize_spec_workspace_bytes",
     "rd_orthogonalize",
 )
 
@@ -215,6 +216,8 @@ def _load() -> ctypes.CDLL:
     lib.rd_gmm_float8.restype = i
     lib.rd_orthogonalize_workspace_bytes.argtypes = [i, i, i, i]
     lib.rd_orthogonalize_workspace_bytes.restype = sz
+    lib.rd_orthogonalize_spec_workspace_bytes.argtypes = [i, i, i, ctypes.POINTER(OrthoSpec), i]
+    lib.rd_orthogonalize_spec_workspace_bytes.restype = sz
     lib.rd_orthogonalize.argtypes = [vp, vp, vp, i, i, i, ctypes.POINTER(OrthoSpec), i, vp, sz]
     lib.rd_orthogonalize.restype = i
     return lib

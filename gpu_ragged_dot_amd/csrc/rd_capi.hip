@@ -1421,15 +1421,7 @@ static int check_ortho(int g, int k, int n, int dtype) {
   return RD_OK;
 }
 
-size_t rd_orthogonalize_workspace_bytes(int g, int k, int n, int dtype) {
-  if (check_ortho(g, k, n, dtype) != RD_OK || g == 0 || k == 0 || n == 0) return 0;
-  return align_up(rd::ortho_workspace_bytes(g, k, n, moe_elem(dtype)), 256);
-}
-
-int rd_orthogonalize(void* stream, const void* G, void* out, int g, int k, int n, const rd_ortho_spec* spec, int dtype, void* workspace,
-                     size_t workspace_bytes) {
-  int rc = check_ortho(g, k, n, dtype);
-  if (rc != RD_OK) return rc;
+static int check_ortho_spec(const rd_ortho_spec* spec) {
   if (!spec || spec->steps < 0 || spec->steps > rd::kOrthoMaxSteps || (spec->steps > 0 && !spec->coefficients))
     return fail(RD_ERR_INVALID_ARGUMENT, "no spec, no coefficients, or steps outside 0..%d", rd::kOrthoMaxSteps);
   for (int i = 0; i < 3 * spec->steps; ++i)
@@ -1437,9 +1429,26 @@ int rd_orthogonalize(void* stream, const void* G, void* out, int g, int k, int n
   if (!(spec->eps >= 0) || !(spec->eps - spec->eps == 0) || !((float)spec->scale - (float)spec->scale == 0)) return fail(RD_ERR_INVALID_ARGUMENT, "eps must be finite and not negative, scale a finite float32");
   if (!(rd::ortho_growth(spec->steps, spec->coefficients) <= 1024))
     return fail(RD_ERR_INVALID_ARGUMENT, "these coefficients lead singular values beyond 1024: the iteration does not converge");
-  if (g == 0 || k == 0 || n == 0) return RD_OK;
+  return RD_OK;
+}
+
+size_t rd_orthogonalize_workspace_bytes(int g, int k, int n, int dtype) {
+  if (check_ortho(g, k, n, dtype) != RD_OK || g == 0 || k == 0 || n == 0) return 0;
+  return align_up(rd::ortho_workspace_bytes(g, k, n, true), 256);
+}
+
+size_t rd_orthogonalize_spec_workspace_bytes(int g, int k, int n, const rd_ortho_spec* spec, int dtype) {
+  if (check_ortho(g, k, n, dtype) != RD_OK || check_ortho_spec(spec) != RD_OK || g == 0 || k == 0 || n == 0) return 0;
+  return align_up(rd::ortho_workspace_bytes(g, k, n, moe_elem(dtype) == 1 || rd::ortho_in_two(spec->steps, spec->coefficients)), 256);
+}
+
+int rd_orthogonalize(void* stream, const void* G, void* out, int g, int k, int n, const rd_ortho_spec* spec, int dtype, void* workspace,
+                     size_t workspace_bytes) {
+  int rc = check_ortho(g, k, n, dtype);
+  if (rc == RD_OK) rc = check_ortho_spec(spec);
+  if (rc != RD_OK || g == 0 || k == 0 || n == 0) return rc;
   if (!G || !out) return fail(RD_ERR_INVALID_ARGUMENT, "null pointer argument");
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || workspace_bytes < rd_orthogonalize_workspace_bytes(g, k, n, dtype))
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || workspace_bytes < rd_orthogonalize_spec_workspace_bytes(g, k, n, spec, dtype))
     return fail(RD_ERR_WORKSPACE, "workspace too small or misaligned");
   const rd::OrthoProblem p = {G, out, g, k, n, moe_elem(dtype), spec->steps, spec->coefficients, spec->eps, spec->scale, workspace};
   rc = rd::launch_orthogonalize((hipStream_t)stream, p);

@@ -7,6 +7,9 @@
 namespace rd {
 
 constexpr int kOrthoMaxSteps = 32;
+// Roundings of X in 15 bits, of 256 x 512 of rank 2, grown by 485 (five steps of a = 3.4445): 1.9e-3 of the result, by 1670: 7.6e-3, by
+// 19816: 8.7e-2.
+constexpr double kOrthoMostGrown = 2048;
 constexpr int kOrthoPad = 64;  // matrices are padded to multiples of this inside
 
 struct OrthoProblem {
@@ -20,7 +23,9 @@ struct OrthoProblem {
   void* workspace;
 };
 
-size_t ortho_workspace_bytes(int g, int k, int n, int elem);
+size_t ortho_workspace_bytes(int g, int k, int n, bool two);
+// whether numbers of 16-bit matrices are held in two float16 numbers, as those of float32 ones are
+bool ortho_in_two(int steps, const double* coefficients);
 bool ortho_grid_fits(int g, int k, int n);
 // the largest singular value that the iteration can lead to from values up to 1
 double ortho_growth(int steps, const double* coefficients);

@@ -13,6 +13,9 @@
 //              eleven are all that pays (sixteen of them left 0.1 % too), and X is most of what is moved.  X before the last step, whose
 //              rounding grows once, has none.
 //   float32 G: everything in two numbers and every product in three, lo hi + hi lo + hi hi: 22 bits, as accurate as float32 products.
+//   16-bit G whose coefficients make the small singular values, and with them the roundings, grow more than 2048 times: as float32 G, for 2.4
+//              times the time.  Of 256 x 512 of rank 4 eight steps of a = 3.4445 (19816 times) left 3.4e-2 of noise in the numbers above, ten
+//              0.39, in these 5e-4 and 5e-3.
 #include "rd_elem.h"
 #include "rd_gemm_w4.h"
 #include "rd_ortho.h"
@@ -183,7 +186,7 @@ __device__ __forceinline__ void factors_of(const OrthoTriple& t, double bound, b
 // X = G / (norm + eps), 64 x 64 numbers of the padded X per work-group; `tall`: X is the transpose of G.
 // Memory: 128 x 2048 x 768 bf16 192 us, 5.2 TB/s.  The first g work-groups work out the factors of a matrix each, a lane those of a step
 // (4 x 256 x 512: 4.5 us; in the first work-group of the matrix's tiles 5.7).
-template <class T>
+template <class T, bool TWO>
 __global__ __launch_bounds__(kOrthoThreads) void ortho_start_kernel(const T* __restrict__ G, const double* __restrict__ partial, int chunks, half_bits* __restrict__ hi,
                                                                     void* __restrict__ lo, int g, int k, int n, int rp, int cp, bool tall, double eps, OrthoTriples triples,
                                                                     OrthoFactors* __restrict__ factors) {
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(kOrthoThreads) void ortho_start_kernel(const T* __r
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = tile[r][c + j];
     *reinterpret_cast<u32x4_t*>(hi + cell) = high_of(w, rest);
-    if (lo) store_low<sizeof(T) == 4>(lo, cell, rest);
+    if (lo) store_low<TWO>(lo, cell, rest);
   }
 }
 
@@ -613,7 +616,7 @@ OrthoSizes sizes_of(int g, int k, int n) {
 template <class T>
 int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
   const OrthoSizes z = sizes_of(p.g, p.k, p.n);
-  const bool two = sizeof(T) == 4, tall = p.k > p.n;
+  const bool two = p.elem == 1 || ortho_in_two(p.steps, p.coefficients), tall = p.k > p.n;
   char* ws = static_cast<char*>(p.workspace);
   double* partial = reinterpret_cast<double*>(ws);
   ws += z.norm;
@@ -634,8 +637,8 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
     hipLaunchKernelGGL((ortho_divide_kernel<T>), dim3((unsigned)(p.g * z.chunks)), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, (T*)p.out, size, z.chunks, p.eps, p.scale);
     return (int)hipGetLastError();
   }
-  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3((unsigned)(p.g + p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, z.chunks, X[0].hi,
-                     two || p.steps > 1 ? X[0].lo : nullptr, p.g, p.k, p.n, z.rp, z.cp, tall, p.eps, triples_of(p.steps, p.coefficients), factors);
+  hipLaunchKernelGGL((two ? ortho_start_kernel<T, true> : ortho_start_kernel<T, sizeof(T) == 4>), dim3((unsigned)(p.g + p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s,
+                     (const T*)p.G, partial, z.chunks, X[0].hi, two || p.steps > 1 ? X[0].lo : nullptr, p.g, p.k, p.n, z.rp, z.cp, tall, p.eps, triples_of(p.steps, p.coefficients), factors);
   if ((rc = (int)hipGetLastError()) != hipSuccess) return rc;
   OrthoStep t{};
   t.g = p.g; t.stride = 3 * p.steps;
@@ -662,9 +665,19 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
 
 }  // namespace
 
-size_t ortho_workspace_bytes(int g, int k, int n, int elem) {
+size_t ortho_workspace_bytes(int g, int k, int n, bool two) {
   const OrthoSizes z = sizes_of(g, k, n);
-  return z.norm + z.factors + 2 * z.x + 2 * (elem == 1 ? z.x : z.bytes) + (elem == 1 ? 4 : 2) * z.square;
+  return z.norm + z.factors + 2 * z.x + 2 * (two ? z.x : z.bytes) + (two ? 4 : 2) * z.square;
+}
+
+bool ortho_in_two(int steps, const double* coefficients) {
+  double bound = 1, grown = 1;  // the most that what was rounded so far has grown: X by 1 at the start and by its size before each step
+  for (int i = 0; i < steps; ++i) {
+    const double a = coefficients[3 * i];
+    grown = fmax(grown, bound) * fabs(a);
+    bound = largest(triple_of(a, coefficients[3 * i + 1], coefficients[3 * i + 2]), bound);
+  }
+  return grown > kOrthoMostGrown;
 }
 
 bool ortho_grid_fits(int g, int k, int n) {

@@ -843,9 +843,9 @@ Tensor orthogonalize(const Tensor& G_, const std::vector<double>& coefficients, 
   const at::Device dev = G.device();
   const c10::DeviceGuard guard(dev);
   Tensor out = empty_on(G.sizes(), G.scalar_type(), dev);
-  const size_t bytes = rd_orthogonalize_workspace_bytes((int)g, (int)k, (int)n, code);
-  const Tensor ws = scratch(bytes, dev);
   const rd_ortho_spec spec{(int)(coefficients.size() / 3), coefficients.data(), eps, scale};
+  const size_t bytes = rd_orthogonalize_spec_workspace_bytes((int)g, (int)k, (int)n, &spec, code);
+  const Tensor ws = scratch(bytes, dev);
   check(rd_orthogonalize(stream_of(dev), G.const_data_ptr(), out.mutable_data_ptr(), (int)g, (int)k, (int)n, &spec, code, ws.mutable_data_ptr(), bytes));
   return out;
 }

@@ -106,3 +106,50 @@ def test_scales_of_any_size():
             assert torch.equal(got, base * 2.0 ** power)
     with pytest.raises(RuntimeError, match="scale"):
         rd.orthogonalize(G, scale=1e39)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("k,n,rank", [(256, 512, 4), (512, 256, 1), (64, 64, 2)])
+@pytest.mark.parametrize("steps", [8, 10])
+def test_many_steps_on_low_rank(steps, k, n, rank, dtype):
+    """The gradient of an expert that saw few tokens, exact in 16 bits.  What a step rounds in directions that it leaves empty is multiplied by
+    a = 3.4445 in every later one.  Numbers of 22 bits: X is off by 2^-22 of its norm at the start, and by less than three times that in all
+    steps together, weighted with what is left to grow; the norm is at least 0.7: 2^-20 a^steps of the result.  (Numbers of 11 and 15 bits
+    leave 0.04 to 0.09 of noise at eight steps, 0.4 to 1 at ten.)"""
+    rng = np.random.default_rng(rank)
+    G = rng.integers(-2, 3, (k, rank)) @ rng.integers(-2, 3, (rank, n)) if rank > 1 else np.outer(rng.integers(1, 8, k), rng.integers(-7, 8, n))
+    t = torch.from_numpy(G).to(dtype).cuda()
+    assert np.array_equal(_np(t), G)
+    ref = oracle.orthogonalize(G, [COEFFICIENTS] * steps)
+    assert _relative(rd.orthogonalize(t, steps=steps), ref) <= 2.0 ** -20 * COEFFICIENTS[0] ** steps + HALF_ULP[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("steps,most", [(5, 8e-3), (6, 1e-2)])
+def test_few_steps_on_low_rank(steps, most, dtype):
+    """What the header promises for matrices of few rows, columns or directions."""
+    for k, n, rank in ((256, 512, 1), (64, 64, 1), (512, 100, 2), (256, 512, 4)):
+        rng = np.random.default_rng(rank)
+        G = rng.integers(-2, 3, (k, rank)) @ rng.integers(-2, 3, (rank, n)) if rank > 1 else np.outer(rng.integers(1, 8, k), rng.integers(-7, 8, n))
+        t = torch.from_numpy(G).to(dtype).cuda()
+        assert _relative(rd.orthogonalize(t, steps=steps), oracle.orthogonalize(G, [COEFFICIENTS] * steps)) <= most + HALF_ULP[dtype]
+
+
+def test_a_workspace_of_one_spec_does():
+    """Stacks of 16-bit matrices, few steps and many, in the bytes that the C entry asks for and no more."""
+    import ctypes
+
+    from gpu_ragged_dot_amd import _capi
+
+    G = _randn(3, 200, 150, seed=8).bfloat16().cuda()
+    for steps in (5, 8):
+        flat = (ctypes.c_double * (3 * steps))(*(COEFFICIENTS * steps))
+        spec = _capi.OrthoSpec(steps, flat, 1e-7, 1.0)
+        need = _capi.lib.rd_orthogonalize_spec_workspace_bytes(3, 200, 150, ctypes.byref(spec), _capi.RD_DTYPE_BF16)
+        whole = torch.full((need + 512,), 77, dtype=torch.uint8, device="cuda")
+        out = torch.empty_like(G)
+        at = -whole.data_ptr() % 256
+        status = _capi.lib.rd_orthogonalize(torch.cuda.current_stream().cuda_stream, G.data_ptr(), out.data_ptr(), 3, 200, 150, ctypes.byref(spec),
+                                            _capi.RD_DTYPE_BF16, whole.data_ptr() + at, need)
+        assert status == 0 and torch.equal(out, rd.orthogonalize(G, steps=steps))
+        assert (whole[:at] == 77).all() and (whole[at + need:] == 77).all()

@@ -1,12 +1,12 @@
-"""What the orthogonalised update refuses, on the host alone."""
+"""What the orthogonalised update refuses and how much memory it asks for, on the host alone."""
 
 import ctypes
 
 from gpu_ragged_dot_amd import _capi
 
 lib = _capi.lib
-INVALID = -1
-F32 = _capi.RD_DTYPE_F32
+INVALID, WORKSPACE = -1, -3
+BF16, F32, F16 = _capi.RD_DTYPE_BF16, _capi.RD_DTYPE_F32, _capi.RD_DTYPE_F16
 HERE = ctypes.addressof(ctypes.create_string_buffer(4096)) // 256 * 256 + 256  # an address that is never read
 
 
@@ -30,3 +30,25 @@ def test_growth_of_nearly_cubic_steps():
 def test_scale_is_a_float32():
     assert _call([(1.0, 0.0, 0.0)], scale=1e39) == INVALID and b"scale" in lib.rd_last_error()
     assert _call([(1.0, 0.0, 0.0)], scale=-3e38, g=0) == 0
+
+
+def _bytes(triples, dtype, g=3, k=200, n=150):
+    flat = (ctypes.c_double * (3 * len(triples)))(*(v for t in triples for v in t))
+    s = _capi.OrthoSpec(len(triples), flat, 1e-7, 1.0)
+    return lib.rd_orthogonalize_spec_workspace_bytes(g, k, n, ctypes.byref(s), dtype)
+
+
+def test_workspace_follows_from_the_growth_of_roundings():
+    """16-bit matrices in 15 bits up to 2048 times, and in two numbers beyond."""
+    steep, slow, flat = (3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (0.5, 0.0, 0.0)
+    for dtype in (BF16, F16):
+        few, most = _bytes([steep] * 5, dtype), lib.rd_orthogonalize_workspace_bytes(3, 200, 150, dtype)
+        assert 0 < few < most == _bytes([steep] * 5, F32) == lib.rd_orthogonalize_workspace_bytes(3, 200, 150, F32)
+        for triples, want in (([steep] * 6, few), ([steep] * 7, most), ([slow] * 18, few), ([slow] * 19, most), ([flat] * 10 + [steep] * 6, few),
+                              ([steep] * 6 + [flat] * 10, few), ([flat] + [steep] * 8, most),
+                              ([flat] * 10 + [steep] * 7, few), ([], few)):  # (before the last: 2^-10 of X is what is rounded, and grows 5752 times)
+            assert _bytes(triples, dtype) == want, triples
+            assert _call(triples, dtype, g=3, k=200, n=150, ws_bytes=want - 256) == WORKSPACE
+    assert _bytes([(30.0, 0.0, 0.0)] * 3, BF16) == 0 and b"converge" in lib.rd_last_error()
+    assert lib.rd_orthogonalize_spec_workspace_bytes(3, 200, 150, None, BF16) == 0
+    assert _bytes([steep], BF16, k=1 << 30) == 0 and _bytes([steep], BF16, g=0) == 0
