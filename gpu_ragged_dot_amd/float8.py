@@ -55,7 +55,8 @@ def quantize_weights(A: torch.Tensor, *, pow2: bool = False) -> Float8Weights:
 
 def pack_float8(codes: torch.Tensor, scales: torch.Tensor) -> Float8Weights:
     """Weights as a checkpoint holds them: e4m3fn ``codes`` ``[g, a, b]`` and ``scales`` ``[g, ceil(a / 128), ceil(b / 128)]``, what a
-    code is multiplied with.  Codes are copied only where ``a`` or ``b`` is no multiple of 128."""
+    code is multiplied with.  Codes are copied only where ``a`` or ``b`` is no multiple of 128, or where they are not contiguous
+    or not at a 16-byte address."""
     assert codes.ndim == 3, f"but {codes.ndim=}"
     if codes.dtype != torch.float8_e4m3fn:
         raise TypeError(f"unsupported dtype {codes.dtype}; codes are float8_e4m3fn")
@@ -70,7 +71,10 @@ def pack_float8(codes: torch.Tensor, scales: torch.Tensor) -> Float8Weights:
         whole = torch.zeros((g, 128 * down, 128 * across), dtype=torch.uint8, device=codes.device)
         whole[:, :a, :b] = codes.view(torch.uint8)
         codes = whole.view(torch.float8_e4m3fn)
-    return Float8Weights(codes.contiguous(), scales.float().contiguous(), a, b)
+    codes = codes.contiguous()
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
+    return Float8Weights(codes, scales.float().contiguous(), a, b)
 
 
 def dequantize(held: Union[Float8Rows, Float8Weights], dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
