@@ -79,8 +79,8 @@ struct F8FragReader {
     return i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
   }
 };
-// MN-major slab [BK][ROW_BYTES], chunk c of contraction row kk at position c ^ ((kk & 3) << 2), of rows of 128 bytes c ^ ((kk & 1) << 2)
-// (the loader of an MN-major bf16 slab): four 8-bit transposing reads (ds_read_b64_tr_b8) of 8 contraction rows each.  In one such read a 16-lane
+// MN-major slab [BK][ROW_BYTES], chunk c of contraction row kk at position c ^ ((kk & 3) << 2) (the loader of an MN-major
+// bf16 slab): four 8-bit transposing reads (ds_read_b64_tr_b8) of 8 contraction rows each.  In one such read a 16-lane
 // group fetches an 8 x 16 byte block - lane i supplies the address of row (i >> 1), bytes 8 (i & 1) .. + 7 - and lane i
 // receives the 8 contraction-consecutive bytes of column i.
 template <int ROW_BYTES, int TILES>
@@ -89,7 +89,7 @@ struct F8FragReaderT {
   __device__ __forceinline__ void init(int col0, int lane) {
     const int q = lane >> 4, i = lane & 15;
     const int row = 32 * (q >> 1) + (i >> 1);
-    const int s = ((i >> 1) & (ROW_BYTES >= 256 ? 3 : ROW_BYTES / 64 - 1)) << 2;
+    const int s = ((i >> 1) & 3) << 2;
 #pragma unroll
     for (int j = 0; j < TILES; ++j) {
       const int chunk = ((col0 >> 4) + 2 * j + (q & 1)) ^ s;
