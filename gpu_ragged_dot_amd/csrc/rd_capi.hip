@@ -1439,7 +1439,7 @@ size_t rd_orthogonalize_workspace_bytes(int g, int k, int n, int dtype) {
 
 size_t rd_orthogonalize_spec_workspace_bytes(int g, int k, int n, const rd_ortho_spec* spec, int dtype) {
   if (check_ortho(g, k, n, dtype) != RD_OK || check_ortho_spec(spec) != RD_OK || g == 0 || k == 0 || n == 0) return 0;
-  return align_up(rd::ortho_workspace_bytes(g, k, n, moe_elem(dtype) == 1 || rd::ortho_in_two(spec->steps, spec->coefficients)), 256);
+  return align_up(rd::ortho_workspace_bytes(g, k, n, rd::ortho_in_two(moe_elem(dtype), spec->steps, spec->coefficients)), 256);
 }
 
 int rd_orthogonalize(void* stream, const void* G, void* out, int g, int k, int n, const rd_ortho_spec* spec, int dtype, void* workspace,

@@ -24,8 +24,8 @@ struct OrthoProblem {
 };
 
 size_t ortho_workspace_bytes(int g, int k, int n, bool two);
-// whether numbers of 16-bit matrices are held in two float16 numbers, as those of float32 ones are
-bool ortho_in_two(int steps, const double* coefficients);
+// whether numbers are held in two float16 numbers: not those of bfloat16 matrices, unless their roundings grow too far
+bool ortho_in_two(int elem, int steps, const double* coefficients);
 bool ortho_grid_fits(int g, int k, int n);
 // the largest singular value that the iteration can lead to from values up to 1
 double ortho_growth(int steps, const double* coefficients);

@@ -6,21 +6,23 @@
 // Numbers are float16 times a power of two per matrix, step and kind that the growth of the singular values allows (|X|, |A| and |B|
 // are bounded by polynomials of it, from |G|_F / (|G|_F + eps) on), so that 2^15 is reached and 2^-29 of it still has all eleven bits.  float16 and not bfloat16:
 // eleven bits instead of eight at the same rate.  What the tiles add up is fp32.
-//   16-bit G:  X is held in two numbers, hi + lo, of which the products take hi; A and B in one.  Along the small singular values of X
+//   bfloat16 G: X is held in two numbers, hi + lo, of which the products take hi; A and B in one.  Along the small singular values of X
 //              every step multiplies what is there by a = 3.4, the rounding of X included, until after five steps it has grown 485 times:
 //              of an update of low rank X in one number left 2 % of noise, in two 0.1 %.  Products of hi alone cost next to nothing of
 //              that, since B is small along small singular values.  lo is a byte, the residue times 32 in e4m3: its four bits behind hi's
 //              eleven are all that pays (sixteen of them left 0.1 % too), and X is most of what is moved.  X before the last step, whose
 //              rounding grows once, has none.
 //   float32 G: everything in two numbers and every product in three, lo hi + hi lo + hi hi: 22 bits, as accurate as float32 products.
-//   16-bit G whose coefficients make the small singular values, and with them the roundings, grow more than 2048 times: as float32 G, for 2.4
-//              times the time.  Of 256 x 512 of rank 4 eight steps of a = 3.4445 (19816 times) left 3.4e-2 of noise in the numbers above, ten
+//   float16 G: as float32 G, for 2.4 times the time of bfloat16: products of eleven bits were off by 1.4e-3 to 2.3e-3, five times what the
+//              rounding of the result is.
+//   bfloat16 G whose coefficients make the small singular values, and with them the roundings, grow more than 2048 times: as float32 G.  Of 256 x 512 of rank 4 eight steps of a = 3.4445 (19816 times) left 3.4e-2 of noise in the numbers above, ten
 //              0.39, in these 5e-4 and 5e-3.
 #include "rd_elem.h"
 #include "rd_gemm_w4.h"
 #include "rd_ortho.h"
 
 #include <math.h>
+#include <type_traits>
 
 namespace rd {
 
@@ -616,7 +618,7 @@ OrthoSizes sizes_of(int g, int k, int n) {
 template <class T>
 int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
   const OrthoSizes z = sizes_of(p.g, p.k, p.n);
-  const bool two = p.elem == 1 || ortho_in_two(p.steps, p.coefficients), tall = p.k > p.n;
+  const bool two = ortho_in_two(p.elem, p.steps, p.coefficients), tall = p.k > p.n;
   char* ws = static_cast<char*>(p.workspace);
   double* partial = reinterpret_cast<double*>(ws);
   ws += z.norm;
@@ -637,7 +639,7 @@ int orthogonalize_t(hipStream_t s, const OrthoProblem& p) {
     hipLaunchKernelGGL((ortho_divide_kernel<T>), dim3((unsigned)(p.g * z.chunks)), dim3(kOrthoThreads), 0, s, (const T*)p.G, partial, (T*)p.out, size, z.chunks, p.eps, p.scale);
     return (int)hipGetLastError();
   }
-  hipLaunchKernelGGL((two ? ortho_start_kernel<T, true> : ortho_start_kernel<T, sizeof(T) == 4>), dim3((unsigned)(p.g + p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s,
+  hipLaunchKernelGGL((two ? ortho_start_kernel<T, true> : ortho_start_kernel<T, !std::is_same<T, bf16_bits>::value>), dim3((unsigned)(p.g + p.g * (z.rp / 64) * (z.cp / 64))), dim3(kOrthoThreads), 0, s,
                      (const T*)p.G, partial, z.chunks, X[0].hi, two || p.steps > 1 ? X[0].lo : nullptr, p.g, p.k, p.n, z.rp, z.cp, tall, p.eps, triples_of(p.steps, p.coefficients), factors);
   if ((rc = (int)hipGetLastError()) != hipSuccess) return rc;
   OrthoStep t{};
@@ -670,7 +672,8 @@ size_t ortho_workspace_bytes(int g, int k, int n, bool two) {
   return z.norm + z.factors + 2 * z.x + 2 * (two ? z.x : z.bytes) + (two ? 4 : 2) * z.square;
 }
 
-bool ortho_in_two(int steps, const double* coefficients) {
+bool ortho_in_two(int elem, int steps, const double* coefficients) {
+  if (elem != 0) return true;
   double bound = 1, grown = 1;  // the most that what was rounded so far has grown: X by 1 at the start and by its size before each step
   for (int i = 0; i < steps; ++i) {
     const double a = coefficients[3 * i];

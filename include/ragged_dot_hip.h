@@ -332,16 +332,17 @@ int rd_gmm_float8(void* stream, const void* x, const float* x_scales, const void
  *   A = X X',  B = b A + c A A,  X = a X + B X        (on the transpose where k > n)
  * and out [g, k, n] = scale * X, of G's type.  With coefficients such as (3.4445, -4.7750, 2.0315), five times, the singular values
  * come out between 0.7 and 1.2, whatever they were from |G|_F / 500 on.  The norm is a 64-bit sum; sums of products are fp32.  For
- * 16-bit G products are of float16 numbers, with X held in 15 bits: results are off by 2e-3 of their norm after five such steps and by 3e-3
+ * bfloat16 G products are of float16 numbers, with X held in 15 bits: results are off by 2e-3 of their norm after five such steps and by 3e-3
  * after six (up to 8e-3 and 1e-2 where there are few rows, columns or directions, whose roundings do not average out).  Roundings in
  * directions that G leaves empty are multiplied by a in every later step, by 485 in five and by 1670 in six; with coefficients that
- * multiply them by more than 2048, 16-bit G is iterated as float32 is, for 2.4 times the time.  For float32 every product is of 22-bit numbers, as accurate as float32
- * products: 2^-20 of the norm at most, times what the coefficients multiply roundings by.  Both also where |G|_F is far below eps (down to 1e-25 of it) or
+ * multiply them by more than 2048, bfloat16 G is iterated as the others are, for 2.4 times the time.  For float32 and float16 G every product is
+ * of 22-bit numbers, as accurate as float32 products: 2^-20 of the norm at most, times what the coefficients multiply roundings by, before
+ * the result is rounded.  Both also where |G|_F is far below eps (down to 1e-25 of it) or
  * coefficients make X small.  An infinity or NaN makes its matrix NaN; a matrix of zeros stays 0.
  * steps 0..32; coefficients: host, [steps][3], finite, such that no singular value from 0 to 1 is led beyond 1024; eps >= 0 finite,
  * scale a finite float32.  g, k, n >= 1 with a padded matrix below 2^30 numbers, and what a launch has of work-groups (RD_ERR_UNSUPPORTED beyond).
  * Workspace, 256-byte aligned, for X twice, A and B: rd_orthogonalize_workspace_bytes() bytes do for any spec,
- * rd_orthogonalize_spec_workspace_bytes() for one (0 if it is refused): for 16-bit G and few steps 6 to 8 bytes for each number instead of 8 to 16.  G and out do not overlap, or are the same. */
+ * rd_orthogonalize_spec_workspace_bytes() for one (0 if it is refused): for bfloat16 G and few steps 6 to 8 bytes for each number instead of 8 to 16.  G and out do not overlap, or are the same. */
 typedef struct rd_ortho_spec {
   int steps;
   const double* coefficients; /* host */

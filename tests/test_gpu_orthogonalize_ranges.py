@@ -28,9 +28,9 @@ def _relative(got, ref):
     return np.linalg.norm(_np(got) - ref) / np.linalg.norm(ref)
 
 
-# One rounding of X to what it is held in, relative: 22 bits for float32; 15 for 16-bit numbers, 11 before the last step.  Where the
+# One rounding of X to what it is held in, relative: 22 bits for float32; 15 for bfloat16, 11 before the last step.  Where the
 # iteration is linear, all directions grow alike and the roundings of up to eight steps add up as they are.
-LINEAR = {torch.float32: 8 * 2.0 ** -22, torch.bfloat16: 8 * 2.0 ** -15 + 2.0 ** -11, torch.float16: 8 * 2.0 ** -15 + 2.0 ** -11}
+LINEAR = {torch.float32: 8 * 2.0 ** -22, torch.bfloat16: 8 * 2.0 ** -15 + 2.0 ** -11}
 
 
 @types
@@ -153,3 +153,15 @@ def test_a_workspace_of_one_spec_does():
                                             _capi.RD_DTYPE_BF16, whole.data_ptr() + at, need)
         assert status == 0 and torch.equal(out, rd.orthogonalize(G, steps=steps))
         assert (whole[:at] == 77).all() and (whole[at + need:] == 77).all()
+
+
+@pytest.mark.parametrize("k,n", [(8, 300), (64, 64), (256, 512), (515, 100), (1024, 768)])
+@pytest.mark.parametrize("rank", [None, 5])
+def test_float16_results_are_off_by_their_own_rounding(rank, k, n):
+    """Eleven bits of a result are not to be had from products of eleven: 2^-20 of the result for each time that the coefficients multiply
+    roundings, which numbers of 22 bits leave at most, and half a step of float16."""
+    G = _randn(k, n, seed=9) if rank is None else _randn(k, rank, seed=9) @ _randn(rank, n, seed=10)
+    G = G.half().cuda()
+    ref = oracle.orthogonalize(_np(G), [COEFFICIENTS] * 5)
+    got = rd.orthogonalize(G)
+    assert _relative(got, ref) <= 2.0 ** -20 * COEFFICIENTS[0] ** 5 + HALF_ULP[torch.float16]

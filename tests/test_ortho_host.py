@@ -39,16 +39,16 @@ def _bytes(triples, dtype, g=3, k=200, n=150):
 
 
 def test_workspace_follows_from_the_growth_of_roundings():
-    """16-bit matrices in 15 bits up to 2048 times, and in two numbers beyond."""
+    """bfloat16 matrices in 15 bits up to 2048 times, and in two numbers beyond; the others in two always."""
     steep, slow, flat = (3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (0.5, 0.0, 0.0)
-    for dtype in (BF16, F16):
-        few, most = _bytes([steep] * 5, dtype), lib.rd_orthogonalize_workspace_bytes(3, 200, 150, dtype)
-        assert 0 < few < most == _bytes([steep] * 5, F32) == lib.rd_orthogonalize_workspace_bytes(3, 200, 150, F32)
-        for triples, want in (([steep] * 6, few), ([steep] * 7, most), ([slow] * 18, few), ([slow] * 19, most), ([flat] * 10 + [steep] * 6, few),
-                              ([steep] * 6 + [flat] * 10, few), ([flat] + [steep] * 8, most),
-                              ([flat] * 10 + [steep] * 7, few), ([], few)):  # (before the last: 2^-10 of X is what is rounded, and grows 5752 times)
-            assert _bytes(triples, dtype) == want, triples
-            assert _call(triples, dtype, g=3, k=200, n=150, ws_bytes=want - 256) == WORKSPACE
+    assert _bytes([steep] * 5, F16) == _bytes([steep] * 5, F32) == lib.rd_orthogonalize_workspace_bytes(3, 200, 150, F16)
+    few, most = _bytes([steep] * 5, BF16), lib.rd_orthogonalize_workspace_bytes(3, 200, 150, BF16)
+    assert 0 < few < most == _bytes([steep] * 5, F32) == lib.rd_orthogonalize_workspace_bytes(3, 200, 150, F32)
+    for triples, want in (([steep] * 6, few), ([steep] * 7, most), ([slow] * 18, few), ([slow] * 19, most), ([flat] * 10 + [steep] * 6, few),
+                          ([steep] * 6 + [flat] * 10, few), ([flat] + [steep] * 8, most),
+                          ([flat] * 10 + [steep] * 7, few), ([], few)):  # (before the last: 2^-10 of X is what is rounded, and grows 5752 times)
+        assert _bytes(triples, BF16) == want, triples
+        assert _call(triples, BF16, g=3, k=200, n=150, ws_bytes=want - 256) == WORKSPACE
     assert _bytes([(30.0, 0.0, 0.0)] * 3, BF16) == 0 and b"converge" in lib.rd_last_error()
     assert lib.rd_orthogonalize_spec_workspace_bytes(3, 200, 150, None, BF16) == 0
     assert _bytes([steep], BF16, k=1 << 30) == 0 and _bytes([steep], BF16, g=0) == 0
