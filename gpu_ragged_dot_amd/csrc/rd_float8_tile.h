@@ -12,10 +12,10 @@
 // two sets of inner sums.
 //
 // sx sw may be beyond float32, or lose bits below its least normal number, where what a block adds does neither (inner sums are 0, or between
-// 2^-18 and 2^25).  The K loops look at the products of scales, and a tile that meets such a one is computed again, in the least tiles of
-// its columns, by a loop that multiplies its inner sums twice (float8_tile_any_scale()); products that are normal numbers give the same bits
-// there.  Looking takes 2 % of a decoding step (64 rows in 128 groups x 2048 x 768: 17.4 -> 17.75 us), and nothing of large products; a
-// second multiplication everywhere would be as many again as the fused ones.
+// 2^-18 and 2^25).  The K loops look at the scales, and a tile that meets such a pair is computed again, in the least tiles of its columns,
+// by a loop that multiplies its inner sums twice (float8_tile_any_scale()); products that are normal numbers give the same bits there.
+// Looking takes 2 % of a decoding step (64 rows in 128 groups x 2048 x 768: 17.35 -> 17.85 us), 5 % of 1 x 4096 x 4096 (15.2 -> 16.0), and
+// next to nothing of large products; a second multiplication everywhere would be as many again as the fused ones.
 //
 // (Four waves of 128 x 128 with 32x32x64 instructions kept the sums in the accumulation registers and
 // moved each there and back: 2.1 ms for 16384 x 4096 x 14336 in 8 groups.)
@@ -107,10 +107,10 @@ struct F8TileCfg {
   static constexpr int USED_BYTES = RING_BYTES + SCALE_SETS * SCALE_BYTES;
   static constexpr int FLAGS_AT = USED_BYTES > EPI_BYTES ? USED_BYTES : EPI_BYTES;  // an int per wave
   static constexpr int LDS_BYTES = FLAGS_AT + NW * 4;
-  static constexpr bool ALIKE = WAVES_M == 1 && BN <= kF8Block;  // all waves multiply by the same scales
   typedef F8Loader<BM, NW, true> LdA;
   typedef F8Loader<BN, NW, B_KMAJOR> LdB;
   static_assert(WN <= kF8Block && kF8Block % WN == 0, "a wave's columns lie in one block of the weights");
+  static_assert(PINGPONG || WM <= 64, "a wave has a lane for each of its rows' scales");
   static_assert(STAGES >= 2 && LDS_BYTES <= 160 * 1024, "LDS budget");
 };
 
@@ -168,6 +168,23 @@ __device__ __forceinline__ void float8_store(const f32x4_t (&acc)[C::TM][C::TN],
   }
 }
 
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t umin(uint32_t a, uint32_t b) { return a < b ? a : b; }
+// The largest and least scales that a lane has met, as bits, of which 0 counts as none.  (Negative ones and NaN are among the largest.)
+struct F8Scales {
+  uint32_t most = 0, less = ~0u;  // (the least less 1)
+  __device__ __forceinline__ void see(uint32_t bits) {
+    most = umax(most, bits);
+    less = umin(less, bits - 1);
+  }
+};
+// Whether the product of two of them may be no normal number, in any lane.
+__device__ __forceinline__ bool may_leave_range(const F8Scales& rows, const F8Scales& columns) {
+  const auto number = [](uint32_t bits) { return __builtin_bit_cast(float, bits); };
+  const bool inside = number(rows.most) * number(columns.most) <= 0x1.fffffep127f && number(rows.less + 1) * number(columns.less + 1) >= 0x1p-126f;
+  return __ballot(rows.most != 0 && columns.most != 0 && !inside) != 0;
+}
+
 // What the K loops share: a wave's part of a tile and its operands' ways to LDS and out of it.
 template <class C>
 struct F8Wave {
@@ -182,8 +199,7 @@ struct F8Wave {
   const __attribute__((address_space(4))) float* col_scale;  // the wave's columns' of the first block
   int b_block, blocks;
   float held;  // (MN-major B) a lane's of the 64 blocks that the current one is among
-  float kept;  // a lane's scale of the rows that are multiplied next
-  unsigned long long beyond;  // lanes that have met a product of scales that is no normal number
+  float kept;  // (alternating phases) a lane's scale of the rows that are multiplied next
   unsigned char* smem;
 
   __device__ __forceinline__ void init(const F8Tile& t, unsigned char* smem_) {
@@ -203,13 +219,7 @@ struct F8Wave {
     col_scale = (const __attribute__((address_space(4))) float*)(live ? t.b_scales + (wn * C::WN / kF8Block) * t.b_column : t.b_scales);
     b_block = t.b_block; blocks = t.blocks;
     held = 0.f;
-    beyond = 0;
     if constexpr (!C::B_KMAJOR) hold(0);
-  }
-  // Lanes whose product of scales is infinite, subnormal or 0 where the scales are not 0 (NaN is what a NaN makes of a block); w is the wave's.
-  static __device__ __forceinline__ unsigned long long out_of_range(float row, float w, float product) {
-    const int classes = (__builtin_bit_cast(uint32_t, w) << 1) != 0 ? 0x2f4 : 0;
-    return __builtin_amdgcn_ballot_w64((row != 0.f) & __builtin_amdgcn_classf(product, classes));
   }
   // The columns' scale of a block.  Those of [n, k] weights are neighbours, read through the scalar cache.  Of [k, n] weights each is in a line
   // of its own, which a scalar load per slab would wait for: a lane loads one of 64 blocks (8 groups of 2 x 14336 x 4096 150 -> 121
@@ -256,11 +266,16 @@ struct F8Wave {
 #pragma unroll
     for (int i = 0; i < 4; ++i) factor[i] = __builtin_bit_cast(float, got[i]);
   }
+  // Of the wave's rows (64 at most), one to a lane, in the four blocks from `step` on.
+  __device__ __forceinline__ u32x4_t row_scales(int step) const {
+    return *reinterpret_cast<const u32x4_t*>(smem + C::RING_BYTES + (step >> 2) % C::SCALE_SETS * C::SCALE_BYTES + (wm * C::WM + lane % C::WM) * 16);
+  }
   __device__ __forceinline__ float row_scale(int step, int tile) const {
     return *reinterpret_cast<const float*>(smem + C::RING_BYTES + (step >> 2) % C::SCALE_SETS * C::SCALE_BYTES + (step & 3) * 4 + scale_at + tile * 256);
   }
 };
 
+constexpr int kNoNormalNumber = 0x2f4;  // v_cmp_class: infinite, subnormal or 0, but not NaN, which is what a NaN makes of a block
 __device__ __forceinline__ f32x4_t float8_part(const i32x8_t& b, const i32x8_t& a) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
 }
@@ -277,12 +292,17 @@ __device__ __forceinline__ void phase_barrier() {
 // A barrier per slab, several slabs on their way: tiles of few rows, which wait for their weights.  ANY_SCALE: an inner sum is multiplied by
 // half of the powers of two of its scales and then, as it is added, by the other half and what is left of the scales, between 1/4 and 1.
 // The first is exact wherever the result is a normal number.  (Powers beyond 2^250 make any sum but 0 infinite.)
+// Returns whether scales were met whose product may be no normal number, by the largest and the least of the rows, looked at where those of
+// four blocks have come to LDS together, and of the columns, which are in scalar registers.  (A look at every product made 1 x 4096 x
+// 4096 17.8 us: the vector and the scalar unit wait for each other.  The columns' scales as a load of 64 blocks before the first slabs:
+// 16.5, since the compiler waits for it, and so for slabs, in front of the loop.)
 template <class C, bool ANY_SCALE>
-__device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc)[C::TM][C::TN]) {
+__device__ __forceinline__ bool float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc)[C::TM][C::TN]) {
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s)
     if (s < nk) u.issue(s);
   if constexpr (!C::B_KMAJOR) u.held_is_there();
+  F8Scales rows, columns;
   constexpr int L = C::LdA::PER + C::LdB::PER;
   for (int kt = 0; kt < nk; ++kt) {
     // (a load of scales makes a wave wait for no less)
@@ -290,8 +310,11 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     phase_barrier();  // slab kt is in LDS, and slab kt - 1 is no longer being read
     if (kt + C::STAGES - 1 < nk) u.issue(kt + C::STAGES - 1);
+    u32x4_t four = {0, 0, 0, 0};
+    if (!ANY_SCALE && (kt & 3) == 0) four = u.row_scales(kt);
     if (u.live) {
       const float w = u.column_scale(kt);
+      if constexpr (!ANY_SCALE) columns.see(__builtin_bit_cast(uint32_t, w));
       const unsigned char* ra = u.slab(kt);
       i32x8_t fb[C::TN];
 #pragma unroll
@@ -301,10 +324,9 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc
         const i32x8_t fa = u.fra.read(ra, i);
         const float row = u.row_scale(kt, i);
         float factor = row * w;
-        const unsigned long long beyond = u.out_of_range(row, w, factor);
         if constexpr (ANY_SCALE) {
           float before = 1.f;
-          if (beyond >> u.lane & 1) {
+          if (row != 0.f && w != 0.f && __builtin_amdgcn_classf(factor, kNoNormalNumber)) {
             const int e = imin(__builtin_amdgcn_frexp_expf(row) + __builtin_amdgcn_frexp_expf(w), 250);
             before = __builtin_ldexpf(1.f, e - (e >> 1));
             factor = __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(row) * __builtin_amdgcn_frexp_mantf(w), e >> 1);
@@ -312,20 +334,20 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc
 #pragma unroll
           for (int j = 0; j < C::TN; ++j) float8_add(acc[i][j], float8_part(fb[j], fa) * before, factor);
         } else {
-          u.beyond |= beyond;
 #pragma unroll
           for (int j = 0; j < C::TN; ++j) float8_add(acc[i][j], float8_part(fb[j], fa), factor);
         }
       }
-    } else if constexpr (C::ALIKE && !ANY_SCALE) {  // looks as the others do, and so comes to what they come to
-      const float w = u.column_scale(kt);
+    }
+    if constexpr (!ANY_SCALE) {
+      if ((kt & 3) == 0) {
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) {
-        const float row = u.row_scale(kt, i);
-        u.beyond |= u.out_of_range(row, w, row * w);
+        for (int i = 0; i < 4; ++i) rows.see(four[i]);
       }
     }
   }
+  if constexpr (ANY_SCALE) return false;
+  return may_leave_range(rows, columns);
 }
 
 // Two groups of four waves, one of each per SIMD, half a period apart: while one reads the fragments of half of its rows (memory phase),
@@ -342,13 +364,14 @@ __device__ __forceinline__ void float8_kloop(F8Wave<C>& u, int nk, f32x4_t (&acc
 // flight the same.  The same product without scales, whose sums stay where the matrix cores keep them: 840 and 785.
 // Inner sums enter the accumulators four instructions later, those of a phase's last row piece at the start of the next compute phase.
 template <class C>
-__device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x4_t (&acc)[C::TM][C::TN]) {
+__device__ __forceinline__ bool float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x4_t (&acc)[C::TM][C::TN]) {
   static_assert(C::NW == 8 && C::WAVES_M == 2 && C::STAGES == 2 && C::TM == 8 && C::LdA::PER == 4 && C::LdB::PER == 4,
                 "two groups of four waves, four row pieces a phase; loads 0 and 2 of A hold the waves' first 64 rows");
   constexpr int FIRST = 2;  // row pieces read before a slab's first compute phase
   const int group = u.wave >> 2;
   i32x8_t fa[4], fb[C::TN];
   float factor[4], carried = 0.f;
+  unsigned long long beyond = 0;  // lanes that have met a product of scales that is no normal number
   f32x4_t part[2][C::TN];
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) part[1][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -377,7 +400,9 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x
         part[i & 1][j] = float8_part(fb[j], fa[i]);
         float8_add(acc[(4 * H + i + 7) & 7][j], part[(i + 1) & 1][j], i == 0 ? carried : factor[i == 0 ? 0 : i - 1]);
         // (here, between products: behind the reads, which bound the loop, it took 6 % of 16384 x 4096 x 14336, and at the end of the phase 1 %)
-        if (i == 1 && j == 2) u.beyond |= u.out_of_range(u.kept, wk, u.kept * wk);
+        if (i == 1 && j == 2)
+          beyond |= __builtin_amdgcn_ballot_w64(u.kept != 0.f) &
+                    __builtin_amdgcn_ballot_w64(__builtin_amdgcn_classf(u.kept * wk, (__builtin_bit_cast(uint32_t, wk) << 1) != 0 ? kNoNormalNumber : 0));
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -429,9 +454,10 @@ __device__ __forceinline__ void float8_kloop_pingpong(F8Wave<C>& u, int nk, f32x
   if (group == 0) phase_barrier();
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) float8_add(acc[7][j], part[1][j], carried);
+  return beyond != 0;
 }
 
-// Returns whether scales were met whose product is no normal number: the tile is then not written.  ANY_SCALE: takes all, and writes.
+// Returns whether scales were met whose product may be no normal number: the tile is then not written.  ANY_SCALE: takes all, and writes.
 template <class C, bool ANY_SCALE = false>
 __device__ __forceinline__ bool float8_tile(const F8Tile& t, void* y, int ldy, int elem, unsigned char* smem) {
   F8Wave<C> u;
@@ -441,18 +467,19 @@ __device__ __forceinline__ bool float8_tile(const F8Tile& t, void* y, int ldy, i
   for (int i = 0; i < C::TM; ++i)
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  bool met = false;
   if (t.blocks > 0) {
-    if constexpr (C::PINGPONG && !ANY_SCALE) float8_kloop_pingpong<C>(u, t.blocks, acc);
-    else float8_kloop<C, ANY_SCALE>(u, t.blocks, acc);
+    if constexpr (C::PINGPONG && !ANY_SCALE) met = float8_kloop_pingpong<C>(u, t.blocks, acc);
+    else met = float8_kloop<C, ANY_SCALE>(u, t.blocks, acc);
   }
   int* flags = reinterpret_cast<int*>(smem + C::FLAGS_AT);
-  if constexpr (!ANY_SCALE && !C::ALIKE) {
-    if (u.lane == 0) flags[u.wave] = u.beyond != 0;
+  if constexpr (!ANY_SCALE) {
+    if (u.lane == 0) flags[u.wave] = met;
   }
   __builtin_amdgcn_s_waitcnt(0xc07f);
   phase_barrier();  // the ring is no longer read by any wave
   if constexpr (!ANY_SCALE) {
-    if (C::ALIKE ? u.beyond != 0 : __ballot(flags[u.lane % C::NW] != 0) != 0) return true;  // (in all waves)
+    if (__ballot(flags[u.lane % C::NW] != 0) != 0) return true;  // (in all waves)
   }
   if (!u.live) return false;
   if (elem == 1) float8_store<C, float>(acc, u.wm, u.wn, u.wave, u.lane, t.rows, t.cols, static_cast<float*>(y), ldy, smem);
