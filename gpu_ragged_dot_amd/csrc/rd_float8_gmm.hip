@@ -115,9 +115,9 @@ __global__ __launch_bounds__(S::NT, S::WAVES) void gmm_float8_kernel(F8Problem p
 // 256 x 256 take 1 (of at most 128 rows 0.65), 512 of 128 x 128, two to a compute unit, 0.75, and 512 of 64 x 128 0.5; half a round of
 // those 0.6 of it.  Groups of 32 rows and less have the least tiles, which run on 32 rows.
 //
-// us of 64 | 128 | 256 rows, trans_rhs: 8 groups of 128 x 2048 x 2048 16 | 18 | 33; of 256 rows 27 | 22 | 34; of 512 38 | 36 | 36; of
-// 1024 64 | 54 | 68; 1 of 500 x 4096 x 4096 22 | 29 | 60; 128 of 64 x 2048 x 768 44 | 42 | 47; 32 of 256 x 1024 x 1024 26 | 22 | 23; 32
-// of 128 x 7168 x 2048 159 | 155 | 119; 8 of 256 x 4096 x 14336 233 | 207 | 197; 4 of 1024 x 4096 x 4096 117 | 97 | 120.
+// us of 64 | 128 | 256 rows, trans_rhs, of rows dealt out at random: 8 groups of 128 x 2048 x 2048 17 | 19 | 33; of 256 rows 28 | 23 | 35; of
+// 512 40 | 37 | 36; of 1024 66 | 56 | 67; 1 of 500 x 4096 x 4096 22 | 30 | 59; 128 of 64 x 2048 x 768 44 | 44 | 49; 32 of 256 x 1024 x
+// 1024 26 | 25 | 23; 32 of 128 x 7168 x 2048 165 | 164 | 124; 8 of 256 x 4096 x 14336 230 | 197 | 196; 4 of 1024 x 4096 x 4096 115 | 100 | 120.
 int height_for(const F8Problem& p) {
   const double rows = (double)p.m / p.g;
   if (rows <= 32) return 64;
@@ -131,8 +131,9 @@ int height_for(const F8Problem& p) {
 }
 
 // Launches of at most so many tiles of 64 x 128 take 64 columns: more work-groups, and as many slabs on their way as LDS holds.  us, 128 | 64
-// columns, trans_rhs: 1 x 4096 x 4096 17.6 | 15.2; 33 rows in 4 groups x 7168 x 2048 28.0 | 24.8; 8 in 256 x 7168 x 2048 30.4 | 28.0 (without
-// trans_rhs 59.8 | 41.8).  Of more tiles 64 columns have twice the rounds: 32 rows in 128 x 2048 x 768 11.6 | 19.5.
+// columns, trans_rhs: 1 x 4096 x 4096 19.5 | 16.2; 33 rows in 4 groups x 7168 x 2048 31.4 | 26.4; 8 in 256 x 7168 x 2048 33.7 | 29.3 (without
+// trans_rhs 46.9 | 41.8).  Of more tiles 64 columns have twice the rounds: 32 rows in 128 x 2048 x 768 11.6 | 19.5 (before tiles looked
+// at their scales).
 constexpr int kF8FewTiles = 128;
 struct F8Grid {
   int height, width, col_tiles;
